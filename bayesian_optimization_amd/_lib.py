@@ -18,6 +18,8 @@ KERNEL_RBF, KERNEL_MATERN52 = 0, 1
 VARIANT_V4, VARIANT_SINGLE, VARIANT_M3 = 0, 1, 3
 ACQ_EI, ACQ_UCB, ACQ_PI = 0, 1, 2
 INCUMBENT_MAX_MU, INCUMBENT_MAX_Y, INCUMBENT_GIVEN = 0, 1, 2
+TYPE_F64, TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2, 3
+ACT_SILU, ACT_GELU = 0, 1
 
 
 class Timings(C.Structure):
@@ -44,6 +46,7 @@ class StateDesc(C.Structure):
 _dp = C.POINTER(C.c_double)
 _i64p = C.POINTER(C.c_int64)
 _i32p = C.POINTER(C.c_int32)
+_vp, _i64 = C.c_void_p, C.c_int64
 
 # name -> (restype, argtypes); every symbol include/gpbo.h declares
 SIGNATURES = {
@@ -111,6 +114,22 @@ SIGNATURES = {
     'gpbo_multi_append_acquire': (C.c_int, [C.c_void_p, _dp, C.c_double, C.c_int32, C.c_double, C.c_int32, C.c_double, _dp, _i64p, _dp]),
     'gpbo_multi_lml_batch': (C.c_int, [C.c_void_p, _dp, _dp, C.c_int64, C.c_int32, _dp, _dp, C.c_int32, C.c_int32, _dp, _dp, _i32p]),
     'gpbo_multi_last_distribute': (C.c_int, [C.c_void_p, _dp, _dp]),
+    'gpbo_multi_draw': (C.c_int, [C.c_void_p, _dp, C.c_int64, C.c_double, C.c_int64, C.c_double, C.c_double, _i64p, _dp]),
+    'gpbo_draw': (C.c_int, [C.c_void_p, _dp, C.c_int64, C.c_double, C.c_int64, C.c_double, C.c_double, _i64p, _dp]),
+    'gpbo_lml_inputs': (C.c_int, [C.c_void_p, _dp, _dp, C.c_int64, C.c_int32, _dp, C.c_double, C.c_int32, _dp, _dp, _dp]),
+    'gpbo_layernorm': (C.c_int, [C.c_int32, _vp, C.c_int32, _vp, _i64, _i64, _i64, _vp, _vp, C.c_double, _vp, _i64, _vp, _vp]),
+    'gpbo_layernorm_backward_workspace': (_i64, [C.c_int32, _i64, _i64]),
+    'gpbo_layernorm_backward': (C.c_int, [C.c_int32, _vp, C.c_int32, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp,
+                                          _vp, _i64]),
+    'gpbo_gated_workspace': (_i64, [C.c_int32, _i64, _i64, _i64]),
+    'gpbo_gated': (C.c_int, [C.c_int32, _vp, C.c_int32, C.c_int32, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp,
+                             _i64]),
+    'gpbo_gated_backward_workspace': (_i64, [C.c_int32, _i64, _i64, _i64]),
+    'gpbo_gated_backward': (C.c_int, [C.c_int32, _vp, C.c_int32, C.c_int32, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp,
+                                      _vp, _i64, _vp, _vp, _i64, _vp, _i64]),
+    'gpbo_draw_static_workspace': (_i64, [C.c_int32, _i64, _i64, _i64]),
+    'gpbo_draw_static': (C.c_int, [C.c_int32, _vp, C.c_int32, _vp, _i64, _i64, _i64, _vp, _i64, C.c_double, _i64, C.c_double, C.c_double,
+                                   _vp, _vp, _vp, _vp, _i64]),
     'gpbo_set_chunk': (C.c_int, [C.c_void_p, C.c_int64]),
     'gpbo_selftest_gemm': (C.c_int, [C.c_void_p, C.c_int32, _dp, _dp]),
 }

@@ -94,6 +94,8 @@ struct gpbo_ctx {
     size_t lb_xraw_cap = 0, lb_b_cap = 0, lb_bd_cap = 0;
     double* lane_gpart = nullptr;
     size_t lane_gpart_cap = 0;
+    double *lane_gx = nullptr, *lane_gxout = nullptr;      // input gradient: per-block sums, result
+    size_t lane_gx_cap = 0, lane_gxout_cap = 0;
     LmlSlot* lane_slot = nullptr;
     hipGraphExec_t lane_graph = nullptr;
     std::vector<int64_t> lane_graph_key;
@@ -121,6 +123,8 @@ struct gpbo_ctx {
     double *acq_pv = nullptr, *bmax = nullptr;   // per-workgroup partials: fused acquisition/argmax, max(mu) of the append sweep
     long* acq_pi = nullptr;
     bool have_posterior = false;
+    char* draw_buf = nullptr;   // gpbo_draw: uniform numbers, results and scratch, kept between calls
+    size_t draw_cap = 0;
     bool have_acq = false;      // acq holds the acquisition values of the current posterior
 
     // chunk scratch
@@ -489,13 +493,20 @@ int launch_trsv(gpbo_ctx* ctx, const double* L, double eps_val, const double* ep
     return GPBO_OK;
 }
 
+// Zeros by a kernel, not by a memset: these launches may be captured into a graph, where memset nodes are not reliable on
+// replay.  count is even (every buffer cleared here is a multiple of 128 doubles or of GRAD_D).
+void launch_clear(hipStream_t st, double* p, size_t count) {
+    const size_t pairs = count / 2;
+    hipLaunchKernelGGL(k_clear, dim3((unsigned)std::min<size_t>((pairs + 255) / 256, 8192)), dim3(256), 0, st, reinterpret_cast<double2*>(p), pairs);
+}
+
 // W = inv(L): diagonal blocks from Dinv, then log2(nb) doubling levels
 int launch_inverse(gpbo_ctx* ctx, const double* L, double* W, double* T) {
     Scope s(ctx, T_INV);
     const long ld = ctx->n_pad;
     const int nb = (int)ctx->nb;
     const unsigned S = (unsigned)ctx->batch;
-    HIPCHK(hipMemsetAsync(W, 0, (size_t)ctx->n_pad * ctx->n_pad * S * sizeof(double), ctx->stream));
+    launch_clear(ctx->stream, W, (size_t)ctx->n_pad * ctx->n_pad * S);
     hipLaunchKernelGGL(k_inv_copy_diag, dim3(nb, 1, S), dim3(256), 0, ctx->stream, W, ld, (const double*)ctx->Dinv, ctx->bs);
     static const long inv_half_max = getenv("GPBO_INV_HALF_MAX") ? atol(getenv("GPBO_INV_HALF_MAX")) : 1024;
     for (int sb = 1; sb < nb; sb *= 2) {
@@ -977,6 +988,40 @@ int acquire_enqueue(gpbo_ctx* ctx, int acq, double kappa, int mode, double incum
     return GPBO_OK;
 }
 
+// Draws from m scores on ctx's GPU (gpbo_draw; the joint array of several contexts): uniform numbers up, results down, one
+// synchronisation.
+int draw_impl(gpbo_ctx* ctx, const double* scores, int64_t m, const double* u, int64_t draws, double temperature, int64_t top_k,
+              double top_p, double min_p, int64_t* index_out, double* logp_out) {
+    if (!u || !index_out) BADARG("draw: null input or output");
+    if (draws < 1 || draws > INT32_MAX) BADARG("draw: need 1 <= draws < 2^31");
+    if (!(temperature >= 0.0) || !std::isfinite(temperature)) BADARG("draw: temperature must be finite and >= 0");
+    if (top_k < 0) BADARG("draw: top_k must be >= 0");
+    if (!(top_p >= 0.0 && top_p <= 1.0) || !(min_p >= 0.0 && min_p <= 1.0)) BADARG("draw: top_p and min_p must lie in [0, 1]");
+    const int64_t need = gpbo_draw_static_workspace(GPBO_TYPE_F64, 1, m, draws);
+    if (need < 0) BADARG("draw: at most 2^28 candidates");
+    HIPCHK(hipSetDevice(ctx->device));
+    const size_t part = (size_t)round_up(draws * 8, 256), bytes = 3 * part + (size_t)need;
+    if (ctx->draw_cap < bytes) {
+        if (ctx->draw_buf) hipFree(ctx->draw_buf);
+        ctx->draw_buf = nullptr;
+        ctx->draw_cap = 0;
+        HIPCHK(hipMalloc((void**)&ctx->draw_buf, bytes));
+        ctx->draw_cap = bytes;
+    }
+    double *du = (double*)ctx->draw_buf, *dl = (double*)(ctx->draw_buf + 2 * part);
+    int64_t* di = (int64_t*)(ctx->draw_buf + part);
+    HIPCHK(hipMemcpyAsync(du, u, (size_t)draws * 8, hipMemcpyHostToDevice, ctx->stream));
+    if (gpbo_draw_static(ctx->device, ctx->stream, GPBO_TYPE_F64, scores, m, 1, m, du, draws, temperature, top_k, top_p, min_p, nullptr,
+                         di, dl, ctx->draw_buf + 3 * part, need) != GPBO_OK) {
+        ctx->err = "draw: launch failed";
+        return GPBO_ERR_HIP;
+    }
+    HIPCHK(hipMemcpyAsync(index_out, di, (size_t)draws * 8, hipMemcpyDeviceToHost, ctx->stream));
+    if (logp_out) HIPCHK(hipMemcpyAsync(logp_out, dl, (size_t)draws * 8, hipMemcpyDeviceToHost, ctx->stream));
+    HIPCHK(hipStreamSynchronize(ctx->stream));
+    return GPBO_OK;
+}
+
 struct StepResult {      // what one synchronisation brings back
     double par[8];
     double mu_max, best;
@@ -1199,7 +1244,7 @@ void gpbo_destroy(gpbo_ctx* ctx) {
     if (ctx->sm_host) hipHostFree(ctx->sm_host);
     if (ctx->lane_graph) hipGraphExecDestroy(ctx->lane_graph);
     for (void* p : {(void*)ctx->lb_xraw, (void*)ctx->lb_th, (void*)ctx->lb_sg, (void*)ctx->lb_nll, (void*)ctx->lb_grad,
-                    (void*)ctx->lb_info, (void*)ctx->lane_gpart, (void*)ctx->lane_slot})
+                    (void*)ctx->lb_info, (void*)ctx->lane_gpart, (void*)ctx->lane_slot, (void*)ctx->lane_gx, (void*)ctx->lane_gxout, (void*)ctx->draw_buf})
         if (p) hipFree(p);
     if (ctx->stream) hipStreamDestroy(ctx->stream);
     delete ctx;
@@ -2082,8 +2127,10 @@ int gpbo_reserve_appends(gpbo_ctx* ctx, int64_t max_appends) {
     return GPBO_OK;
 }
 
-int gpbo_lml_batch(gpbo_ctx* ctx, const double* X, const double* y, int64_t n, int32_t d, const double* thetas,
-                   const double* sigmas, int32_t B, int32_t kernel, double* nll_out, double* grad_out, int32_t* status_out) {
+// gradx_out (n, d), with B = 1 only: the gradient w.r.t. the inputs too (grad_out is then given)
+static int lml_batch_impl(gpbo_ctx* ctx, const double* X, const double* y, int64_t n, int32_t d, const double* thetas,
+                          const double* sigmas, int32_t B, int32_t kernel, double* nll_out, double* grad_out, int32_t* status_out,
+                          double* gradx_out) {
     if (!ctx) return GPBO_ERR_BAD_ARG;
     if (!X || !y || !thetas || !sigmas || !nll_out) BADARG("lml_batch: null input");
     if (n <= 0 || d <= 0 || d > MAX_D || B <= 0) BADARG("lml_batch: need n >= 1, 1 <= d <= 32, B >= 1");
@@ -2105,7 +2152,8 @@ int gpbo_lml_batch(gpbo_ctx* ctx, const double* X, const double* y, int64_t n, i
         // one persistent device workspace, one upload, one launch, one download:
         //   in : [Xraw d*128][y 128][thetas B*d][sigmas B]      out: [nll B][grad B*d][info B (as doubles)]
         const size_t n_in = (size_t)d * PB + PB + (size_t)B * d + B;
-        const size_t n_out = (size_t)B + (size_t)B * d + B;
+        const size_t n_gx = gradx_out ? (size_t)n * d : 0;
+        const size_t n_out = (size_t)B + (size_t)B * d + B + n_gx;
         if (ctx->sm_cap < n_in + n_out) {
             if (ctx->sm_buf) hipFree(ctx->sm_buf);
             if (ctx->sm_host) hipHostFree(ctx->sm_host);
@@ -2132,16 +2180,17 @@ int gpbo_lml_batch(gpbo_ctx* ctx, const double* X, const double* y, int64_t n, i
         double* dnll = ctx->sm_buf + n_in;
         double* dgrad = dnll + B;
         int* dinfo = reinterpret_cast<int*>(dgrad + (size_t)B * d);
+        double* dgx = dgrad + (size_t)B * d + B;
         const auto t0 = std::chrono::steady_clock::now();
         HIPCHK(hipMemcpyAsync(ctx->sm_buf, h, n_in * 8, hipMemcpyHostToDevice, ctx->stream));
+        auto launch_small = [&](auto k, int threads) {
+            hipLaunchKernelGGL(k, dim3((unsigned)B), dim3(threads), 0, ctx->stream, (const double*)dX, (int)PB, (const double*)dy, (int)n,
+                               (int)d, (const double*)dth, (const double*)dsg, (int)kernel, grad_out ? 1 : 0, dnll, dgrad, dinfo, dgx);
+        };
         if (n > small_wide_min())
-            hipLaunchKernelGGL(k_lml_small<true>, dim3((unsigned)B), dim3(SMALL_WIDE_THREADS), 0, ctx->stream, (const double*)dX, (int)PB,
-                               (const double*)dy, (int)n, (int)d, (const double*)dth, (const double*)dsg, (int)kernel, grad_out ? 1 : 0,
-                               dnll, dgrad, dinfo);
+            gradx_out ? launch_small(k_lml_small<true, true>, SMALL_WIDE_THREADS) : launch_small(k_lml_small<true, false>, SMALL_WIDE_THREADS);
         else
-            hipLaunchKernelGGL(k_lml_small<false>, dim3((unsigned)B), dim3(POTRF_THREADS), 0, ctx->stream, (const double*)dX, (int)PB,
-                               (const double*)dy, (int)n, (int)d, (const double*)dth, (const double*)dsg, (int)kernel, grad_out ? 1 : 0,
-                               dnll, dgrad, dinfo);
+            gradx_out ? launch_small(k_lml_small<false, true>, POTRF_THREADS) : launch_small(k_lml_small<false, false>, POTRF_THREADS);
         HIPCHK(hipGetLastError());
         HIPCHK(hipMemcpyAsync(h + n_in, dnll, n_out * 8, hipMemcpyDeviceToHost, ctx->stream));
         HIPCHK(hipStreamSynchronize(ctx->stream));
@@ -2158,6 +2207,7 @@ int gpbo_lml_batch(gpbo_ctx* ctx, const double* X, const double* y, int64_t n, i
             if (grad_out)
                 for (int t = 0; t < d; ++t) grad_out[(size_t)b * d + t] = bad ? NAN : ograd[(size_t)b * d + t];
         }
+        if (gradx_out) memcpy(gradx_out, ograd + (size_t)B * d + B, n_gx * 8);
         return GPBO_OK;
     }
 
@@ -2310,6 +2360,22 @@ int gpbo_lml_batch(gpbo_ctx* ctx, const double* X, const double* y, int64_t n, i
             c->lane_gpart_cap = (size_t)ntiles * GRAD_D * S;
             c->alloc_gen += 1;
         }
+        auto grow = [&](double** p, size_t* cap, size_t need) -> hipError_t {
+            if (*cap >= need) return hipSuccess;
+            if (*p) hipFree(*p);
+            *p = nullptr;
+            *cap = 0;
+            const hipError_t e = hipMalloc((void**)p, need * 8);
+            if (e == hipSuccess) {
+                *cap = need;
+                c->alloc_gen += 1;
+            }
+            return e;
+        };
+        if (gradx_out) {
+            LCHK(grow(&c->lane_gx, &c->lane_gx_cap, (size_t)nb * d * n_pad));
+            LCHK(grow(&c->lane_gxout, &c->lane_gxout_cap, (size_t)n * d));
+        }
     }
     {
         // one staged upload: the d padded coordinate rows, then the padded y as row d; the slots' copies of y are
@@ -2342,10 +2408,19 @@ int gpbo_lml_batch(gpbo_ctx* ctx, const double* X, const double* y, int64_t n, i
         if (grad_out) {
             st = launch_inverse(c, c->bufA, c->bufW, c->bufB);
             if (st != GPBO_OK) return st;
-            if (hipMemsetAsync(c->lane_gpart, 0, (size_t)ntiles * GRAD_D * 8 * S, c->stream) != hipSuccess) return GPBO_ERR_HIP;
-            hipLaunchKernelGGL(k_lml_grad_tiles, dim3((unsigned)(nb * (nb + 1) / 2), 1, S), dim3(GEMM_THREADS), 0, c->stream,
-                               (const double*)c->bufW, (long)n_pad, (const double*)c->Xts, (int)n, (int)n_pad, (int)d,
-                               (const double*)c->alpha1, (const double*)c->params, c->lane_gpart, nb, (int)kernel, c->bs);
+            launch_clear(c->stream, c->lane_gpart, (size_t)ntiles * GRAD_D * S);
+            auto launch_grad = [&](auto k) {
+                hipLaunchKernelGGL(k, dim3((unsigned)(nb * (nb + 1) / 2), 1, S), dim3(GEMM_THREADS), 0, c->stream, (const double*)c->bufW,
+                                   (long)n_pad, (const double*)c->Xts, (int)n, (int)n_pad, (int)d, (const double*)c->alpha1,
+                                   (const double*)c->params, c->lane_gpart, c->lane_gx, nb, (int)kernel, c->bs);
+            };
+            if (gradx_out) {
+                launch_grad(k_lml_grad_tiles<true>);
+                hipLaunchKernelGGL(k_lml_inputs_store, dim3((unsigned)((n + 255) / 256), (unsigned)d), dim3(256), 0, c->stream,
+                                   (const double*)c->lane_gx, (const double*)c->params, (int)n, (int)n_pad, (int)d, nb, c->lane_gxout);
+            } else {
+                launch_grad(k_lml_grad_tiles<false>);
+            }
         }
         hipLaunchKernelGGL(k_lml_store, dim3(1, 1, S), dim3(256), 0, c->stream, (const double*)c->params, (const LmlSlot*)c->lane_slot,
                            (const double*)c->lane_gpart, ntiles, (int)d, grad_out ? 1 : 0, ctx->lb_nll, ctx->lb_grad, ctx->lb_info, c->bs);
@@ -2355,7 +2430,7 @@ int gpbo_lml_batch(gpbo_ctx* ctx, const double* X, const double* y, int64_t n, i
         const std::vector<int64_t> key = {n, n_pad, d, kernel, grad_out ? 1 : 0, (int64_t)(intptr_t)ctx->lb_xraw,
                                           (int64_t)(intptr_t)ctx->lb_nll, (int64_t)(intptr_t)ctx->lb_grad,
                                           (int64_t)(intptr_t)ctx->lb_info, (int64_t)(intptr_t)ctx->lb_th,
-                                          (int64_t)(intptr_t)ctx->lb_sg, 0};
+                                          (int64_t)(intptr_t)ctx->lb_sg, gradx_out ? 1 : 0, 0};
         for (int l = 0; l < lanes; ++l) {
             gpbo_ctx* c = lane[l];
             std::vector<int64_t> k = key;
@@ -2413,6 +2488,7 @@ int gpbo_lml_batch(gpbo_ctx* ctx, const double* X, const double* y, int64_t n, i
     LCHK(hipMemcpy(nll_out, ctx->lb_nll, (size_t)B * 8, hipMemcpyDeviceToHost));
     if (grad_out) LCHK(hipMemcpy(grad_out, ctx->lb_grad, (size_t)B * d * 8, hipMemcpyDeviceToHost));
     LCHK(hipMemcpy(hinfo.data(), ctx->lb_info, (size_t)B * sizeof(int), hipMemcpyDeviceToHost));
+    if (gradx_out) LCHK(hipMemcpy(gradx_out, lane[0]->lane_gxout, (size_t)n * d * 8, hipMemcpyDeviceToHost));
 #undef LCHK
     ctx->tm.fit_total_ms = wall_ms;      // host wall time of the whole sweep (several streams run concurrently)
     ctx->tm.chol_count = B;
@@ -2423,6 +2499,34 @@ int gpbo_lml_batch(gpbo_ctx* ctx, const double* X, const double* y, int64_t n, i
         if (bad) nll_out[b] = NAN;
     }
     return GPBO_OK;
+}
+
+int gpbo_lml_batch(gpbo_ctx* ctx, const double* X, const double* y, int64_t n, int32_t d, const double* thetas,
+                   const double* sigmas, int32_t B, int32_t kernel, double* nll_out, double* grad_out, int32_t* status_out) {
+    return lml_batch_impl(ctx, X, y, n, d, thetas, sigmas, B, kernel, nll_out, grad_out, status_out, nullptr);
+}
+
+int gpbo_lml_inputs(gpbo_ctx* ctx, const double* X, const double* y, int64_t n, int32_t d, const double* theta, double sigmaY,
+                    int32_t kernel, double* nll_out, double* grad_out, double* gradx_out) {
+    if (!ctx) return GPBO_ERR_BAD_ARG;
+    if (!gradx_out) BADARG("lml_inputs: null output");
+    if (d < 1 || d > GRAD_D) BADARG("lml_inputs: need 1 <= d <= 16");
+    double own_grad[GRAD_D];
+    int32_t status = GPBO_OK;
+    CHK(lml_batch_impl(ctx, X, y, n, d, theta, &sigmaY, 1, kernel, nll_out, grad_out ? grad_out : own_grad, &status, gradx_out));
+    if (status == GPBO_ERR_NOT_PD) {
+        for (int t = 0; grad_out && t < d; ++t) grad_out[t] = NAN;
+        for (int64_t i = 0; i < n * d; ++i) gradx_out[i] = NAN;
+        ctx->err = "lml_inputs: the covariance matrix is not positive definite";
+    }
+    return status;
+}
+
+int gpbo_draw(gpbo_ctx* ctx, const double* u, int64_t draws, double temperature, int64_t top_k, double top_p, double min_p,
+              int64_t* index_out, double* logp_out) {
+    if (!ctx) return GPBO_ERR_BAD_ARG;
+    if (!ctx->have_posterior || !ctx->have_acq) BADARG("draw: no acquisition values for the current posterior (call gpbo_acquire first)");
+    return draw_impl(ctx, ctx->acq, ctx->m, u, draws, temperature, top_k, top_p, min_p, index_out, logp_out);
 }
 
 }  // extern "C"

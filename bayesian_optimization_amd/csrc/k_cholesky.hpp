@@ -570,4 +570,8 @@ __global__ __launch_bounds__(256) void k_zero_upper(double* __restrict__ A, int 
     if (i < n_pad && j < n_pad && j > i) A[(long)i * n_pad + j] = 0.0;
 }
 
+__global__ __launch_bounds__(256) void k_clear(double2* __restrict__ p, size_t pairs) {
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < pairs; i += (size_t)gridDim.x * 256) p[i] = make_double2(0.0, 0.0);
+}
+
 }  // namespace gpbo

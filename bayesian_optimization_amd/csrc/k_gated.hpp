@@ -1,0 +1,324 @@
+// Gated unit: h = act(x Wg^T) * (x Wu^T), forward and backward.
+//   g = x Wg^T, u = x Wu^T;  silu: act(g) = g / (1 + exp(-g)),  gelu: act(g) = g Phi(g)
+//   dg = dh u act'(g), du = dh act(g);  dx = dg Wg + du Wu;  dWg = dg^T x, dWu = du^T x
+// Four products' worth of matrix work forward (two projections), eight back.  Both projections of a tile are formed by the
+// same workgroup from one staged tile of x, so the activation and the product are an epilogue on the accumulators and g, u
+// never go to memory unless the caller keeps them for the backward pass.  Sums are held in 32 bits, and so are the kept g and
+// u: rounded to 16 bits they would put two more roundings of the same size under every gradient.  h is rounded once, and dg and
+// du once each, to the type of x: they are operands of the matrix instructions.
+#pragma once
+
+#include "static_ops.hpp"
+
+namespace gpbo_static {
+
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
+
+// One 16-byte fragment a lane: row lane % 16 of the operand, elements (lane / 16) * N .. + N of a slab of 4 N along the
+// contraction (N = 8 in 16 bits: one 16x16x32 instruction; N = 4 in 32 bits: four 16x16x4 instructions, which take element i
+// of every lane -- the contraction index is permuted, in both operands alike).
+// D: row (lane / 16) * 4 + r comes from the first operand, column lane % 16 from the second.
+template <typename T>
+__device__ __forceinline__ f32x4 mma(const uint4& a, const uint4& b, f32x4 c);
+template <>
+__device__ __forceinline__ f32x4 mma<bf16>(const uint4& a, const uint4& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x4 mma<f16>(const uint4& a, const uint4& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x4 mma<float>(const uint4& a, const uint4& b, f32x4 c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.x), __uint_as_float(b.x), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.y), __uint_as_float(b.y), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.z), __uint_as_float(b.z), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.w), __uint_as_float(b.w), c, 0, 0, 0);
+}
+
+// act(g) and act'(g).  silu through the logistic function, whose exponential saturates to 0 or infinity with the right limit;
+// gelu through erfc, which keeps the far negative tail that 1 + erf loses.
+__device__ __forceinline__ void activation(float g, int act, float& a, float& da) {
+    if (act == GPBO_ACT_SILU) {
+        const float s = 1.0f / (1.0f + expf(-g));
+        a = g * s;
+        da = s + a * (1.0f - s);
+    } else {
+        const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
+        a = g * cdf;
+        da = cdf + g * (0.39894228040143268f * expf(-0.5f * g * g));
+    }
+}
+__device__ __forceinline__ float activate(float g, int act) {
+    float a, da;
+    activation(g, act, a, da);
+    return a;
+}
+
+// A product's operand: element (row, k) at p + row * sr + k * sk, one of the two strides 1.
+struct Operand {
+    const void* p;
+    int64_t sr, sk;
+};
+
+constexpr int GATED_FWD = 0;      // a[0] b[0] and a[0] b[1] side by side, epilogue act(.) * (.)
+constexpr int GATED_SUM = 1;      // a[0] b[0] + a[1] b[1]
+constexpr int GATED_PAIR = 2;     // a[z] b[0] to out[z], z = 0, 1
+
+struct GatedArgs {
+    Operand a[2], b[2];
+    int64_t m, n, k;              // out is (m, n), k the contraction (of each part)
+    void* out[2];
+    int64_t os;                   // row stride of out
+    float *keep_g, *keep_u;       // (m, n) contiguous, or null
+    int act, splits;
+    float* part;                  // splits > 1: [z][split][m][n] sums in 32 bits
+};
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Tile kernel for every shape, stride and alignment: 64 x 64 outputs, 4 waves of 32 x 32, 128 bytes of contraction a step,
+// staged through registers (guarded at every edge) into LDS.  Slot (row, chunk) of a staged tile lives at chunk ^ (row & 7):
+// the 16 rows that one fragment read touches then fall into different banks.
+constexpr int TB = 64, STEP_BYTES = 128;
+
+template <typename T, bool KC>
+struct TileLoad {
+    static constexpr int V = 16 / sizeof(T), KS = STEP_BYTES / sizeof(T);
+    static constexpr int PACKS = TB * KS / V / 256;
+    Pack<T> r[PACKS];
+    __device__ __forceinline__ void load(const Operand& o, int64_t row0, int64_t rows, int64_t k0, int64_t k1) {
+        const T* p = (const T*)o.p;
+#pragma unroll
+        for (int i = 0; i < PACKS; ++i) {
+            const int id = threadIdx.x + i * 256;
+            if constexpr (KC) {
+                const int64_t row = row0 + id / 8, k = k0 + (id % 8) * V;
+                if (row < rows && k + V <= k1) r[i] = load_pack(p + row * o.sr + k);
+                else
+#pragma unroll
+                    for (int j = 0; j < V; ++j) r[i].v[j] = (row < rows && k + j < k1) ? p[row * o.sr + k + j] : from_float<T>(0.0f);
+            } else {
+                const int64_t row = row0 + (id % (TB / V)) * V, k = k0 + id / (TB / V);
+                if (k < k1 && row + V <= rows) r[i] = load_pack(p + k * o.sk + row);
+                else
+#pragma unroll
+                    for (int j = 0; j < V; ++j) r[i].v[j] = (k < k1 && row + j < rows) ? p[k * o.sk + row + j] : from_float<T>(0.0f);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(uint4* lds) const {
+#pragma unroll
+        for (int i = 0; i < PACKS; ++i) {
+            const int id = threadIdx.x + i * 256;
+            if constexpr (KC) {
+                const int row = id / 8, c = id % 8;
+                lds[row * 8 + (c ^ (row & 7))] = __builtin_bit_cast(uint4, r[i]);
+            } else {
+                const int row = (id % (TB / V)) * V, k = id / (TB / V);
+                T* l = reinterpret_cast<T*>(lds);
+#pragma unroll
+                for (int j = 0; j < V; ++j) l[((row + j) * 8 + ((k / V) ^ ((row + j) & 7))) * V + k % V] = r[i].v[j];
+            }
+        }
+    }
+};
+
+template <typename T, int MODE, bool AKC, bool BKC>
+__global__ __launch_bounds__(256) void k_gated_tile(GatedArgs g) {
+    constexpr int KS = STEP_BYTES / sizeof(T), NB = MODE == GATED_FWD ? 2 : 1;
+    __shared__ uint4 la[TB * 8], lb[NB][TB * 8];
+    const int64_t nt = (g.n + TB - 1) / TB;
+    const int64_t row0 = (int64_t)(blockIdx.x / nt) * TB, col0 = (int64_t)(blockIdx.x % nt) * TB;
+    const int z = MODE == GATED_PAIR ? blockIdx.z : 0, split = blockIdx.y;
+    const int64_t per = ((g.k + g.splits - 1) / g.splits + KS - 1) / KS * KS;
+    const int64_t kb = min(split * per, g.k), ke = min(kb + per, g.k);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wr = (wave >> 1) * 32, wc = (wave & 1) * 32;
+    f32x4 acc[NB][2][2];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) acc[b][i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int64_t steps1 = (ke - kb + KS - 1) / KS, steps = MODE == GATED_SUM ? 2 * steps1 : steps1;
+    TileLoad<T, AKC> ta;
+    TileLoad<T, BKC> tb[NB];
+    auto fetch = [&](int64_t s) {
+        const int part = MODE == GATED_SUM && s >= steps1;
+        const int64_t k0 = kb + (s - (part ? steps1 : 0)) * KS;
+        ta.load(g.a[MODE == GATED_PAIR ? z : part], row0, g.m, k0, ke);
+        tb[0].load(g.b[part], col0, g.n, k0, ke);
+        if constexpr (NB == 2) tb[1].load(g.b[1], col0, g.n, k0, ke);
+    };
+    if (steps > 0) fetch(0);
+    for (int64_t s = 0; s < steps; ++s) {
+        ta.store(la);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) tb[b].store(lb[b]);
+        __syncthreads();
+        if (s + 1 < steps) fetch(s + 1);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            uint4 fa[2], fb[NB][2];
+            const int c = kk * 4 + (lane >> 4);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = wr + i * 16 + (lane & 15);
+                fa[i] = la[r * 8 + (c ^ (r & 7))];
+                const int q = wc + i * 16 + (lane & 15);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) fb[b][i] = lb[b][q * 8 + (c ^ (q & 7))];
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) acc[b][i][j] = mma<T>(fb[b][j], fa[i], acc[b][i][j]);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int64_t row = row0 + wr + i * 16 + (lane & 15), col = col0 + wc + j * 16 + (lane >> 4) * 4;
+            if (row >= g.m) continue;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (col + r >= g.n) continue;
+                if constexpr (MODE == GATED_FWD) {
+                    const float gv = acc[0][i][j][r], uv = acc[NB - 1][i][j][r];
+                    ((T*)g.out[0])[row * g.os + col + r] = from_float<T>(activate(gv, g.act) * uv);
+                    if (g.keep_g) {
+                        g.keep_g[row * g.n + col + r] = gv;
+                        g.keep_u[row * g.n + col + r] = uv;
+                    }
+                } else {
+                    const float v = acc[0][i][j][r];
+                    if (g.splits > 1) g.part[(((int64_t)z * g.splits + split) * g.m + row) * g.n + col + r] = v;
+                    else ((T*)g.out[z])[row * g.os + col + r] = from_float<T>(v);
+                }
+            }
+        }
+}
+
+// The split sums of one output, added in split order.
+template <typename T>
+__global__ __launch_bounds__(256) void k_gated_join(GatedArgs g) {
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, z = blockIdx.y;
+    if (e >= g.m * g.n) return;
+    const float* p = g.part + z * g.splits * g.m * g.n + e;
+    float v = 0.0f;
+    for (int s = 0; s < g.splits; ++s) v += p[(int64_t)s * g.m * g.n];
+    ((T*)g.out[z])[e / g.n * g.os + e % g.n] = from_float<T>(v);
+}
+
+// dg = dh u act'(g), du = dh act(g).
+template <typename T>
+__global__ __launch_bounds__(256) void k_gated_slopes(const T* __restrict__ dh, int64_t dhs, const float* __restrict__ kg,
+                                                      const float* __restrict__ ku, int64_t m, int64_t n, int act, T* __restrict__ dg,
+                                                      T* __restrict__ du) {
+    constexpr int V = Pack<T>::N;
+    const int64_t packs = (n + V - 1) / V;
+    for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < m * packs; id += (int64_t)gridDim.x * 256) {
+        const int64_t row = id / packs, c = (id % packs) * V;
+        const int64_t e = row * n + c;
+        const T* d = dh + row * dhs + c;
+        const int len = (int)min((int64_t)V, n - c);
+        Pack<T> pd, og, ou;
+        float gv[V], uv[V];
+        if (len == V) {
+            pd = load_pack(d);
+            __builtin_memcpy(gv, kg + e, sizeof(gv));
+            __builtin_memcpy(uv, ku + e, sizeof(uv));
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                pd.v[i] = i < len ? d[i] : from_float<T>(0.0f);
+                gv[i] = i < len ? kg[e + i] : 0.0f;
+                uv[i] = i < len ? ku[e + i] : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float a, da;
+            activation(gv[i], act, a, da);
+            og.v[i] = from_float<T>(to_float(pd.v[i]) * uv[i] * da);
+            ou.v[i] = from_float<T>(to_float(pd.v[i]) * a);
+        }
+        if (len == V) {
+            store_pack(dg + e, og);
+            store_pack(du + e, ou);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (i < len) dg[e + i] = og.v[i], du[e + i] = ou.v[i];
+        }
+    }
+}
+
+// Pieces of the contraction for a product of few tiles: up to two workgroups a CU, at least 4 steps each.
+inline int gated_splits(int64_t tiles, int64_t k, int64_t step) {
+    if (tiles >= 256) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(512, tiles), k / (4 * step)));
+}
+
+struct GatedPlan {
+    int64_t slopes_bytes, part_bytes;
+    int splits_x, splits_w;
+};
+template <typename T>
+GatedPlan gated_plan(int64_t m, int64_t k, int64_t h) {
+    constexpr int KS = STEP_BYTES / sizeof(T);
+    GatedPlan p{};
+    p.slopes_bytes = round_up(m * h * (int64_t)sizeof(T), 256);
+    p.splits_x = gated_splits(ceil_div(m, TB) * ceil_div(k, TB), h, KS);
+    p.splits_w = gated_splits(2 * ceil_div(h, TB) * ceil_div(k, TB), m, KS);
+    p.part_bytes = std::max<int64_t>(p.splits_x > 1 ? p.splits_x * m * k * 4 : 0, p.splits_w > 1 ? 2 * p.splits_w * h * k * 4 : 0);
+    return p;
+}
+
+template <typename T>
+hipError_t gated_forward(hipStream_t st, const GatedArgs& g) {
+    const int64_t tiles = ceil_div(g.m, TB) * ceil_div(g.n, TB);
+    hipLaunchKernelGGL((k_gated_tile<T, GATED_FWD, true, true>), dim3((unsigned)tiles), dim3(256), 0, st, g);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const void* x, int64_t xs, const void* wg, const void* wu, int64_t ws,
+                          const float* kg, const float* ku, int64_t m, int64_t k, int64_t h, int act, void* dx, int64_t dxs, void* dwg,
+                          void* dwu, int64_t dws, char* work) {
+    const GatedPlan p = gated_plan<T>(m, k, h);
+    T *dg = (T*)work, *du = (T*)(work + p.slopes_bytes);
+    float* part = (float*)(work + 2 * p.slopes_bytes);
+    const int64_t packs = m * ceil_div(h, Pack<T>::N);
+    if (m > 0)
+        hipLaunchKernelGGL(k_gated_slopes<T>, dim3((unsigned)std::min<int64_t>(ceil_div(packs, 256), 8192)), dim3(256), 0, st, (const T*)dh, dhs,
+                           kg, ku, m, h, act, dg, du);
+    if (dx && m > 0) {
+        GatedArgs g{};
+        g.a[0] = {dg, h, 1}, g.a[1] = {du, h, 1};
+        g.b[0] = {wg, 1, ws}, g.b[1] = {wu, 1, ws};
+        g.m = m, g.n = k, g.k = h, g.out[0] = dx, g.os = dxs, g.splits = p.splits_x, g.part = part;
+        hipLaunchKernelGGL((k_gated_tile<T, GATED_SUM, true, false>), dim3((unsigned)(ceil_div(m, TB) * ceil_div(k, TB)), (unsigned)g.splits),
+                           dim3(256), 0, st, g);
+        if (g.splits > 1) hipLaunchKernelGGL(k_gated_join<T>, dim3((unsigned)ceil_div(m * k, 256), 1), dim3(256), 0, st, g);
+    }
+    if (dwg) {
+        GatedArgs g{};
+        g.a[0] = {dg, 1, h}, g.a[1] = {du, 1, h};
+        g.b[0] = g.b[1] = {x, 1, xs};
+        g.m = h, g.n = k, g.k = m, g.out[0] = dwg, g.out[1] = dwu, g.os = dws, g.splits = p.splits_w, g.part = part;
+        hipLaunchKernelGGL((k_gated_tile<T, GATED_PAIR, false, false>), dim3((unsigned)(ceil_div(h, TB) * ceil_div(k, TB)), (unsigned)g.splits, 2),
+                           dim3(256), 0, st, g);
+        if (g.splits > 1) hipLaunchKernelGGL(k_gated_join<T>, dim3((unsigned)ceil_div(h * k, 256), 2), dim3(256), 0, st, g);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace gpbo_static

@@ -25,12 +25,18 @@ __global__ __launch_bounds__(256) void k_setup_setting(const double* __restrict_
 // One workgroup = one lower tile (jb >= kb) of Kinv on the MFMA tile engine, reduced against dK_t
 // in the epilogue without ever storing Kinv.  gpart[(jb*nb + kb)*GRAD_D + t] = sum_tile c_jk q_t K0_jk
 // (x2 for off-diagonal tiles); the caller zero-fills gpart.
+// GX: the gradient w.r.t. the inputs as well.  With F as above, dK_jk / dx_jt = -F_jk (x_jt - x_kt) / theta_t^2, so
+//   d(-logL)/dx_jt = (1 / theta_t) sum_k c_jk F_jk (xs_jt - xs_kt),   xs = x / theta.
+// A tile (jb, kb) adds to the rows of block jb and, by symmetry, to those of block kb: each sum goes to a slot of its own,
+// gx[(o*d + t)*n_pad + row] with o the OTHER block of the tile, and k_lml_inputs_store adds the nb slots in order (no atomics).
 constexpr int GRAD_D = 16;
+template <bool GX>
 __global__ __launch_bounds__(GEMM_THREADS, 2) void k_lml_grad_tiles(const double* __restrict__ W, long ld,
                                                                     const double* __restrict__ Xts, int n, int n_pad, int d,
                                                                     const double* __restrict__ alpha1,
                                                                     const double* __restrict__ params,
-                                                                    double* __restrict__ gpart, int nb, int kernel, BatchStride bs) {
+                                                                    double* __restrict__ gpart, double* __restrict__ gx, int nb,
+                                                                    int kernel, BatchStride bs) {
     W += blockIdx.z * bs.mat;
     Xts += blockIdx.z * bs.xts;
     alpha1 += blockIdx.z * bs.vec;
@@ -101,6 +107,54 @@ __global__ __launch_bounds__(GEMM_THREADS, 2) void k_lml_grad_tiles(const double
     if (tid < GRAD_D)
         gpart[((long)jb * nb + kb) * GRAD_D + tid] =
             (tid < d) ? wgt * (red[tid] + red[GRAD_D + tid] + red[2 * GRAD_D + tid] + red[3 * GRAD_D + tid]) : 0.0;
+    if constexpr (GX) {
+        double* rr = red + 4 * GRAD_D;         // [2][128] row sums of the two column halves
+        double* rc = rr + 2 * PB;              // [2][128] column sums of the two row halves
+        static_assert(2 * GRAD_D * PB + 2 * PB + 4 * GRAD_D + 4 * PB <= GEMM_LDS_DOUBLES, "the sums fit behind the coordinates");
+        const int wrow = (tid >> 7) & 1, wcol = (tid >> 6) & 1, lane = tid & 63;
+        for (int t = 0; t < d; ++t) {
+            double xkt[4], cs[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+            for (int tb = 0; tb < 4; ++tb) xkt[tb] = xk[t * PB + acc_col(tb)];
+#pragma unroll
+            for (int ta = 0; ta < 4; ++ta)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = acc_row(ta, r);
+                    const double xjt = xj[t * PB + row];
+                    double rs = 0.0;
+#pragma unroll
+                    for (int tb = 0; tb < 4; ++tb) {
+                        const double v = acc[ta][tb][r] * (xjt - xkt[tb]);
+                        rs += v;
+                        cs[tb] -= v;
+                    }
+                    for (int o = 8; o > 0; o >>= 1) rs += __shfl_xor(rs, o);
+                    if ((lane & 15) == 0) rr[wcol * PB + row] = rs;
+                }
+#pragma unroll
+            for (int tb = 0; tb < 4; ++tb) {
+                cs[tb] += __shfl_xor(cs[tb], 16);
+                cs[tb] += __shfl_xor(cs[tb], 32);
+                if (lane < 16) rc[wrow * PB + acc_col(tb)] = cs[tb];
+            }
+            __syncthreads();
+            const int i = tid & (PB - 1);
+            if (tid < PB) gx[((long)kb * d + t) * n_pad + jb * PB + i] = rr[i] + rr[PB + i];
+            else if (jb != kb) gx[((long)jb * d + t) * n_pad + kb * PB + i] = rc[i] + rc[PB + i];
+            __syncthreads();
+        }
+    }
+}
+
+// out[i*d + t] = (1/theta_t) * sum over the nb slots of k_lml_grad_tiles<true>
+__global__ __launch_bounds__(256) void k_lml_inputs_store(const double* __restrict__ gx, const double* __restrict__ params, int n,
+                                                          int n_pad, int d, int nb, double* __restrict__ out) {
+    const int i = blockIdx.x * 256 + threadIdx.x, t = blockIdx.y;
+    if (i >= n) return;
+    double s = 0.0;
+    for (int o = 0; o < nb; ++o) s += gx[((long)o * d + t) * n_pad + i];
+    out[(long)i * d + t] = s * params[P_INVTHETA + t];
 }
 
 // Whole -logL (+ gradient) evaluation of ONE hyper-parameter setting in ONE workgroup, for n <= 128: covariance
@@ -162,9 +216,9 @@ __device__ __forceinline__ void lml_small_build(const SmallLds& m, int n, int d,
 }
 
 // everything after the inverse: W out of the packed block, z, alpha, the scalars, Kinv = W^T W tile by tile, gradient sums
-template <int TS, int TG>
+template <int TS, int TG, bool GX>
 __device__ __forceinline__ void lml_small_finish(const SmallLds& m, int n, int d, const double* th, int kernel, int want_grad,
-                                                 int fail, double* out_nll, double* out_grad, int* out_info) {
+                                                 int fail, double* out_nll, double* out_grad, int* out_info, double* out_gx) {
     constexpr int MS = TG * TS;                // rows and columns covered by the register tiles
     constexpr int NW = TG * TG / 64;           // waves
     const int tid = threadIdx.x, tr = tid / TG, tc = tid % TG;
@@ -281,12 +335,35 @@ __device__ __forceinline__ void lml_small_finish(const SmallLds& m, int n, int d
             sum += (m.red[w * GRAD_D + tid] + m.red[(w + 1) * GRAD_D + tid]) + (m.red[(w + 2) * GRAD_D + tid] + m.red[(w + 3) * GRAD_D + tid]);
         out_grad[tid] = bad ? NAN : -0.5 * sum * (1.0 / th[tid]);
     }
+    if constexpr (GX) {                        // the whole symmetric c F in LDS (W is no longer read), then one sum a thread
+        __syncthreads();
+        if (lower) {
+            const double unwgt = (tr == tc) ? 1.0 : 0.5;
+#pragma unroll
+            for (int rr = 0; rr < TS; ++rr)
+#pragma unroll
+                for (int cc = 0; cc < TS; ++cc) {
+                    const double c = a[rr][cc] * unwgt;
+                    Wl[(tr * TS + rr) * SMALL_WP + tc * TS + cc] = c;
+                    Wl[(tc * TS + cc) * SMALL_WP + tr * TS + rr] = c;
+                }
+        }
+        __syncthreads();
+        for (int e = tid; e < n * d; e += TG * TG) {
+            const int i = e / d, t = e - i * d;
+            const double xi = m.xs[t * PB + i];
+            double s = 0.0;
+            for (int k = 0; k < n; ++k) s = fma(Wl[k * SMALL_WP + i], xi - m.xs[t * PB + k], s);
+            out_gx[e] = bad ? NAN : s * (1.0 / th[t]);
+        }
+    }
 }
 
-template <bool WIDE>
+template <bool WIDE, bool GX = false>
 __device__ __forceinline__ void lml_small_body(double* __restrict__ lds, const double* __restrict__ Xraw, int xpitch,
                                                const double* __restrict__ y, int n, int d, const double* th, double sg, int kernel,
-                                               int want_grad, double* out_nll, double* out_grad, int* out_info) {
+                                               int want_grad, double* out_nll, double* out_grad, int* out_info,
+                                               double* out_gx = nullptr) {
     const SmallLds m(lds);
     const int tid = threadIdx.x;
     const double eps = (sg == 0.0) ? 1e-15 * (double)n : sg * sg;
@@ -314,23 +391,23 @@ __device__ __forceinline__ void lml_small_body(double* __restrict__ lds, const d
     if (tid < n) m.dg[tid] = m.Wl[tri_off(tid) + tid];
     __syncthreads();                           // diag L is saved before the inverse overwrites it
     trinv128_mfma(m.Wl, Wi8, Tbuf, ntl);
-    if (WIDE && n > 64) lml_small_finish<4, 32>(m, n, d, th, kernel, want_grad, fail, out_nll, out_grad, out_info);
-    else if (WIDE) lml_small_finish<2, 32>(m, n, d, th, kernel, want_grad, fail, out_nll, out_grad, out_info);
-    else if (n <= 32) lml_small_finish<2, 16>(m, n, d, th, kernel, want_grad, fail, out_nll, out_grad, out_info);
-    else lml_small_finish<4, 16>(m, n, d, th, kernel, want_grad, fail, out_nll, out_grad, out_info);
+    if (WIDE && n > 64) lml_small_finish<4, 32, GX>(m, n, d, th, kernel, want_grad, fail, out_nll, out_grad, out_info, out_gx);
+    else if (WIDE) lml_small_finish<2, 32, GX>(m, n, d, th, kernel, want_grad, fail, out_nll, out_grad, out_info, out_gx);
+    else if (n <= 32) lml_small_finish<2, 16, GX>(m, n, d, th, kernel, want_grad, fail, out_nll, out_grad, out_info, out_gx);
+    else lml_small_finish<4, 16, GX>(m, n, d, th, kernel, want_grad, fail, out_nll, out_grad, out_info, out_gx);
 }
 
-template <bool WIDE>
+template <bool WIDE, bool GX>
 __global__ __launch_bounds__(WIDE ? SMALL_WIDE_THREADS : POTRF_THREADS) void k_lml_small(const double* __restrict__ Xraw, int xpitch,
                                                              const double* __restrict__ y, int n, int d,
                                                              const double* __restrict__ thetas,
                                                              const double* __restrict__ sigmas, int kernel, int want_grad,
                                                              double* __restrict__ out_nll, double* __restrict__ out_grad,
-                                                             int* __restrict__ out_info) {
+                                                             int* __restrict__ out_info, double* __restrict__ out_gx) {
     __shared__ double lds[SMALL_LDS_DOUBLES];
     const int b = blockIdx.x;
-    lml_small_body<WIDE>(lds, Xraw, xpitch, y, n, d, thetas + (long)b * d, sigmas[b], kernel, want_grad, out_nll + b,
-                   out_grad + (long)b * d, out_info + b);
+    lml_small_body<WIDE, GX>(lds, Xraw, xpitch, y, n, d, thetas + (long)b * d, sigmas[b], kernel, want_grad, out_nll + b,
+                             out_grad + (long)b * d, out_info + b, GX ? out_gx + (long)b * n * d : nullptr);
 }
 
 // The reference's descent on -logL (conj_gradient_descent, BayesOpt_v4.ipynb:31-87, steprule other than 'backtrack') for

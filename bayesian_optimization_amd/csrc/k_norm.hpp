@@ -1,0 +1,436 @@
+// Layer norm of the rows of a matrix, forward and backward.
+//   mu = mean(x), rstd = 1 / sqrt(mean((x - mu)^2) + eps), xh = (x - mu) rstd, y = xh w + b
+//   g = dy w;  dx = rstd (g - mean(g) - xh mean(g xh));  dw = sum over rows of dy xh;  db = sum over rows of dy
+// Bound by memory: forward reads x and writes y, backward reads x and dy and writes dx, a dozen operations an element.  So
+// a row is read once and stays in registers: the centred second moment is taken from there (two sums, no cancellation, all
+// in 32 bits), TPR threads share a row in 16-byte packs, and a workgroup walks over rows with weight and bias (and, going
+// back, the column sums of dw and db) in registers too.  The column sums of every row group go to the workspace and are
+// added by a second launch in a fixed order: no atomics, the same bits every time.
+#pragma once
+
+#include "static_ops.hpp"
+
+namespace gpbo_static {
+
+// Sum over the TPR threads of a row (TPR <= 64: part of a wave; above: the whole workgroup through LDS, two slots so that one
+// barrier a sum is enough as long as consecutive sums alternate the slot).
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* lds) {
+    if constexpr (TPR <= 64) {
+#pragma unroll
+        for (int o = TPR / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+        return v;
+    } else {
+        v = wave_sum(v);
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) lds[wave] = v;
+        __syncthreads();
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < TPR / 64; ++i) s += lds[i];
+        return s;
+    }
+}
+
+// Pack c of a row of `cols` elements.  The last pack of a row whose length is no multiple of N is moved back so that it ends
+// with the row: it is loaded and stored whole, its first `dup` elements are the pack before's (left out of sums, stored twice
+// with the same value).  Rows shorter than one pack go element by element.
+template <typename T>
+struct Span {
+    static constexpr int V = Pack<T>::N;
+    int64_t e;
+    int dup, len;                              // elements dup .. len are this pack's own; len 0: behind the row's end
+    __device__ __forceinline__ Span(int64_t c, int64_t cols) {
+        const int64_t s = c * V;
+        e = s, dup = 0, len = s < cols ? V : 0;
+        if (s < cols && s + V > cols) {
+            if (cols >= V) e = cols - V, dup = (int)(s - e);
+            else len = (int)cols;
+        }
+    }
+    __device__ __forceinline__ bool own(int i) const { return i >= dup && i < len; }
+    __device__ __forceinline__ Pack<T> load(const T* row) const {
+        if (len == V) return load_pack(row + e);
+        Pack<T> r;
+#pragma unroll
+        for (int i = 0; i < V; ++i) r.v[i] = i < len ? row[e + i] : from_float<T>(0.0f);
+        return r;
+    }
+    __device__ __forceinline__ void store(T* row, const Pack<T>& p) const {
+        if (len == V) {
+            store_pack(row + e, p);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < len) row[e + i] = p.v[i];
+    }
+};
+
+struct NormArgs {
+    const void *x, *w, *b, *dy;
+    void *y, *dx;
+    int64_t rows, cols, xs, ys, dys, dxs;      // row strides in elements
+    float eps;
+    float *mean, *rstd;
+    float* part;                               // [groups][2][cols] column sums of dy xh and dy
+};
+
+// Rows of up to TPR * NCH packs.
+template <typename T, int TPR, int NCH>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_fwd(NormArgs a) {
+    constexpr int V = Pack<T>::N, BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR;
+    __shared__ float lds[2][16];
+    const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
+    const T *w = (const T*)a.w, *b = (const T*)a.b;
+    const int cols = (int)a.cols;
+    Pack<T> pw[NCH], pb[NCH];
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+        const Span<T> sp(lane + k * TPR, cols);
+        if (w) pw[k] = sp.load(w);
+        if (b) pb[k] = sp.load(b);
+    }
+    const float inv = 1.0f / (float)cols;
+    // the trip count is the same for all threads of a workgroup: row sums of wide rows hold barriers
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
+        const int64_t r = r0 + group;
+        const bool on = r < a.rows;
+        const T* x = (const T*)a.x + (on ? r : 0) * a.xs;
+        Pack<T> px[NCH];
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) px[k] = Span<T>(lane + k * TPR, cols).load(x);
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            const Span<T> sp(lane + k * TPR, cols);
+#pragma unroll
+            for (int i = 0; i < V; ++i) s += sp.own(i) ? to_float(px[k].v[i]) : 0.0f;
+        }
+        const float mu = row_sum<TPR>(s, lds[0]) * inv;
+        float q = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            const Span<T> sp(lane + k * TPR, cols);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float d = to_float(px[k].v[i]) - mu;
+                q += sp.own(i) ? d * d : 0.0f;
+            }
+        }
+        const float rstd = 1.0f / sqrtf(row_sum<TPR>(q, lds[1]) * inv + a.eps);
+        if (!on) continue;                     // only where TPR <= 64: no barrier is skipped
+        T* y = (T*)a.y + r * a.ys;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            Pack<T> py;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float xh = (to_float(px[k].v[i]) - mu) * rstd;
+                py.v[i] = from_float<T>((w ? xh * to_float(pw[k].v[i]) : xh) + (b ? to_float(pb[k].v[i]) : 0.0f));
+            }
+            Span<T>(lane + k * TPR, cols).store(y, py);
+        }
+        if (lane == 0) {
+            if (a.mean) a.mean[r] = mu;
+            if (a.rstd) a.rstd[r] = rstd;
+        }
+    }
+}
+
+// Any length: one workgroup a row, three passes over it (the later ones from the caches).
+template <typename T>
+__global__ __launch_bounds__(1024) void k_norm_fwd_long(NormArgs a) {
+    constexpr int V = Pack<T>::N;
+    __shared__ float lds[2][16];
+    const int64_t chunks = (a.cols + V - 1) / V;
+    const float inv = 1.0f / (float)a.cols;
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T* x = (const T*)a.x + r * a.xs;
+        float s = 0.0f;
+        for (int64_t c = threadIdx.x; c < chunks; c += 1024) {
+            const Span<T> sp(c, a.cols);
+            const Pack<T> p = sp.load(x);
+            float t = 0.0f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) t += sp.own(i) ? to_float(p.v[i]) : 0.0f;
+            s += t;
+        }
+        const float mu = row_sum<1024>(s, lds[0]) * inv;
+        float q = 0.0f;
+        for (int64_t c = threadIdx.x; c < chunks; c += 1024) {
+            const Span<T> sp(c, a.cols);
+            const Pack<T> p = sp.load(x);
+            float t = 0.0f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float d = to_float(p.v[i]) - mu;
+                t += sp.own(i) ? d * d : 0.0f;
+            }
+            q += t;
+        }
+        const float rstd = 1.0f / sqrtf(row_sum<1024>(q, lds[1]) * inv + a.eps);
+        T* y = (T*)a.y + r * a.ys;
+        for (int64_t c = threadIdx.x; c < chunks; c += 1024) {
+            const Span<T> sp(c, a.cols);
+            const Pack<T> p = sp.load(x);
+            Pack<T> pw, pb, py;
+            if (a.w) pw = sp.load((const T*)a.w);
+            if (a.b) pb = sp.load((const T*)a.b);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float xh = (to_float(p.v[i]) - mu) * rstd;
+                py.v[i] = from_float<T>((a.w ? xh * to_float(pw.v[i]) : xh) + (a.b ? to_float(pb.v[i]) : 0.0f));
+            }
+            sp.store(y, py);
+        }
+        if (threadIdx.x == 0) {
+            if (a.mean) a.mean[r] = mu;
+            if (a.rstd) a.rstd[r] = rstd;
+        }
+    }
+}
+
+template <typename T, int TPR, int NCH>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_bwd(NormArgs a) {
+    constexpr int V = Pack<T>::N, BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR;
+    __shared__ float lds[4][16];
+    const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
+    const T* w = (const T*)a.w;
+    const int cols = (int)a.cols;
+    Pack<T> pw[NCH];
+    float aw[NCH][V], ab[NCH][V];
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+        if (w) pw[k] = Span<T>(lane + k * TPR, cols).load(w);
+#pragma unroll
+        for (int i = 0; i < V; ++i) aw[k][i] = ab[k][i] = 0.0f;
+    }
+    const float inv = 1.0f / (float)cols;
+    int par = 0;
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
+        const int64_t r = r0 + group;
+        const bool on = r < a.rows;
+        const int64_t rr = on ? r : 0;
+        const T* x = (const T*)a.x + rr * a.xs;
+        const T* dy = (const T*)a.dy + rr * a.dys;
+        Pack<T> px[NCH], pd[NCH];
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            const Span<T> sp(lane + k * TPR, cols);
+            px[k] = sp.load(x);
+            pd[k] = sp.load(dy);
+        }
+        const float mu = a.mean[rr], rstd = a.rstd[rr];
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            const Span<T> sp(lane + k * TPR, cols);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float xh = (to_float(px[k].v[i]) - mu) * rstd, d = to_float(pd[k].v[i]);
+                const float g = w ? d * to_float(pw[k].v[i]) : d;
+                s1 += sp.own(i) ? g : 0.0f;
+                s2 += sp.own(i) ? g * xh : 0.0f;
+                aw[k][i] += on ? d * xh : 0.0f;
+                ab[k][i] += on ? d : 0.0f;
+            }
+        }
+        const float m1 = row_sum<TPR>(s1, lds[par]) * inv, m2 = row_sum<TPR>(s2, lds[par + 1]) * inv;
+        par ^= 2;
+        if (!on) continue;
+        T* dx = (T*)a.dx + r * a.dxs;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            Pack<T> po;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float xh = (to_float(px[k].v[i]) - mu) * rstd, d = to_float(pd[k].v[i]);
+                const float g = w ? d * to_float(pw[k].v[i]) : d;
+                po.v[i] = from_float<T>(rstd * (g - m1 - xh * m2));
+            }
+            Span<T>(lane + k * TPR, cols).store(dx, po);
+        }
+    }
+    if (!a.part) return;
+    float* part = a.part + ((int64_t)blockIdx.x * RPB + group) * 2 * a.cols;
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+        const Span<T> sp(lane + k * TPR, cols);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (sp.own(i)) {
+                part[sp.e + i] = aw[k][i];
+                part[cols + sp.e + i] = ab[k][i];
+            }
+    }
+}
+
+// Any length: the row sums by one workgroup a row, dx in a second pass; dw and db by k_norm_bwd_long_cols.
+template <typename T>
+__global__ __launch_bounds__(1024) void k_norm_bwd_long(NormArgs a) {
+    constexpr int V = Pack<T>::N;
+    __shared__ float lds[4][16];
+    const int64_t chunks = (a.cols + V - 1) / V;
+    const float inv = 1.0f / (float)a.cols;
+    int par = 0;
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T* x = (const T*)a.x + r * a.xs;
+        const T* dy = (const T*)a.dy + r * a.dys;
+        const float mu = a.mean[r], rstd = a.rstd[r];
+        float s1 = 0.0f, s2 = 0.0f;
+        for (int64_t c = threadIdx.x; c < chunks; c += 1024) {
+            const Span<T> sp(c, a.cols);
+            const Pack<T> px = sp.load(x), pd = sp.load(dy);
+            Pack<T> pw;
+            if (a.w) pw = sp.load((const T*)a.w);
+            float t1 = 0.0f, t2 = 0.0f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                if (!sp.own(i)) continue;
+                const float g = a.w ? to_float(pd.v[i]) * to_float(pw.v[i]) : to_float(pd.v[i]);
+                t1 += g;
+                t2 += g * ((to_float(px.v[i]) - mu) * rstd);
+            }
+            s1 += t1;
+            s2 += t2;
+        }
+        const float m1 = row_sum<1024>(s1, lds[par]) * inv, m2 = row_sum<1024>(s2, lds[par + 1]) * inv;
+        par ^= 2;
+        T* dx = (T*)a.dx + r * a.dxs;
+        for (int64_t c = threadIdx.x; c < chunks; c += 1024) {
+            const Span<T> sp(c, a.cols);
+            const Pack<T> px = sp.load(x), pd = sp.load(dy);
+            Pack<T> pw, po;
+            if (a.w) pw = sp.load((const T*)a.w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float g = a.w ? to_float(pd.v[i]) * to_float(pw.v[i]) : to_float(pd.v[i]);
+                po.v[i] = from_float<T>(rstd * (g - m1 - (to_float(px.v[i]) - mu) * rstd * m2));
+            }
+            sp.store(dx, po);
+        }
+    }
+}
+
+// Column sums of rows too long for registers: a workgroup takes 256 packs' columns and every gridDim.y-th row.
+template <typename T>
+__global__ __launch_bounds__(256) void k_norm_bwd_long_cols(NormArgs a) {
+    constexpr int V = Pack<T>::N;
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c * V >= a.cols) return;
+    const Span<T> sp(c, a.cols);
+    float aw[V], ab[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) aw[i] = ab[i] = 0.0f;
+    for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
+        const Pack<T> px = sp.load((const T*)a.x + r * a.xs), pd = sp.load((const T*)a.dy + r * a.dys);
+        const float mu = a.mean[r], rstd = a.rstd[r];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float d = to_float(pd.v[i]);
+            aw[i] += d * ((to_float(px.v[i]) - mu) * rstd);
+            ab[i] += d;
+        }
+    }
+    float* part = a.part + (int64_t)blockIdx.y * 2 * a.cols;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (sp.own(i)) {
+            part[sp.e + i] = aw[i];
+            part[a.cols + sp.e + i] = ab[i];
+        }
+}
+
+// dw (blockIdx.y = 0) and db (1): the groups' partial sums, 16 interleaved running sums a column joined in a fixed order.
+template <typename T>
+__global__ __launch_bounds__(1024) void k_norm_cols(const float* __restrict__ part, int groups, int64_t cols, T* __restrict__ dw,
+                                                    T* __restrict__ db) {
+    __shared__ float lds[16][64];
+    T* out = blockIdx.y ? db : dw;
+    if (!out) return;
+    const int cl = threadIdx.x & 63, s = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 64 + cl;
+    float v = 0.0f;
+    if (c < cols) {
+        const float* p = part + (int64_t)blockIdx.y * cols + c;
+#pragma unroll 8
+        for (int g = s; g < groups; g += 16) v += p[(int64_t)g * 2 * cols];
+    }
+    lds[s][cl] = v;
+    __syncthreads();
+    if (s == 0 && c < cols) {
+        float t = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t += lds[i][cl];
+        out[c] = from_float<T>(t);
+    }
+}
+
+// How a row length is laid out: threads a row and packs a thread (0 packs: the any-length kernels).
+struct NormPlan {
+    int tpr, nch;
+    int64_t grid, groups;
+};
+
+// Threads a row, by the packs it has.  8 threads up to 8 packs: eight short rows share a wave; a wave up to 128 packs: sums
+// without a barrier; a workgroup of 256 and of 1024 above, so that no thread holds more than 2 packs of x (and, going back,
+// 2 of dy and 16 column sums a pack; 4 packs spill): beyond 2048 packs the row does not fit and is read again.
+inline NormPlan norm_plan(int64_t rows, int64_t cols, int vec, bool backward) {
+    const int64_t packs = ceil_div(cols, vec);
+    NormPlan p{};
+    if (packs <= 8) p.tpr = 8, p.nch = 1;
+    else if (packs <= 128) p.tpr = 64, p.nch = packs <= 64 ? 1 : 2;
+    else if (packs <= 512) p.tpr = 256, p.nch = packs <= 256 ? 1 : 2;
+    else if (packs <= 2048) p.tpr = 1024, p.nch = packs <= 1024 ? 1 : 2;
+    else p.tpr = 1024, p.nch = 0;
+    const int64_t block = p.tpr > 256 ? p.tpr : 256, rpb = block / p.tpr;
+    // forward: as many workgroups as the card holds; backward: fewer, since each leaves column sums behind
+    const int64_t most = backward ? (p.tpr == 1024 ? 256 : p.tpr == 256 ? 1024 : 1024) : (p.tpr == 1024 ? 512 : 2048);
+    p.grid = std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, rpb), most));
+    if (backward && p.nch == 0) p.groups = std::max<int64_t>(1, std::min<int64_t>(rows, 64));
+    else p.groups = p.grid * rpb;
+    return p;
+}
+
+template <typename T>
+hipError_t norm_forward(hipStream_t st, const NormArgs& a) {
+    if (a.rows == 0) return hipSuccess;
+    const NormPlan p = norm_plan(a.rows, a.cols, Pack<T>::N, false);
+    const dim3 g((unsigned)p.grid), b256(256), b1024(1024);
+    if (p.nch == 0) hipLaunchKernelGGL(k_norm_fwd_long<T>, g, b1024, 0, st, a);
+    else if (p.tpr == 8) hipLaunchKernelGGL((k_norm_fwd<T, 8, 1>), g, b256, 0, st, a);
+    else if (p.tpr == 64 && p.nch == 1) hipLaunchKernelGGL((k_norm_fwd<T, 64, 1>), g, b256, 0, st, a);
+    else if (p.tpr == 64 && p.nch == 2) hipLaunchKernelGGL((k_norm_fwd<T, 64, 2>), g, b256, 0, st, a);
+    else if (p.tpr == 256 && p.nch == 1) hipLaunchKernelGGL((k_norm_fwd<T, 256, 1>), g, b256, 0, st, a);
+    else if (p.tpr == 256) hipLaunchKernelGGL((k_norm_fwd<T, 256, 2>), g, b256, 0, st, a);
+    else if (p.nch == 1) hipLaunchKernelGGL((k_norm_fwd<T, 1024, 1>), g, b1024, 0, st, a);
+    else hipLaunchKernelGGL((k_norm_fwd<T, 1024, 2>), g, b1024, 0, st, a);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t norm_backward(hipStream_t st, const NormArgs& a, void* dw, void* db) {
+    const NormPlan p = norm_plan(a.rows, a.cols, Pack<T>::N, true);
+    const dim3 g((unsigned)p.grid), b256(256), b1024(1024);
+    if (a.rows > 0) {
+        if (p.nch == 0) {
+            hipLaunchKernelGGL(k_norm_bwd_long<T>, g, b1024, 0, st, a);
+            if (a.part)
+                hipLaunchKernelGGL(k_norm_bwd_long_cols<T>, dim3((unsigned)ceil_div(ceil_div(a.cols, Pack<T>::N), 256), (unsigned)p.groups),
+                                   b256, 0, st, a);
+        } else if (p.tpr == 8) hipLaunchKernelGGL((k_norm_bwd<T, 8, 1>), g, b256, 0, st, a);
+        else if (p.tpr == 64 && p.nch == 1) hipLaunchKernelGGL((k_norm_bwd<T, 64, 1>), g, b256, 0, st, a);
+        else if (p.tpr == 64 && p.nch == 2) hipLaunchKernelGGL((k_norm_bwd<T, 64, 2>), g, b256, 0, st, a);
+        else if (p.tpr == 256 && p.nch == 1) hipLaunchKernelGGL((k_norm_bwd<T, 256, 1>), g, b256, 0, st, a);
+        else if (p.tpr == 256) hipLaunchKernelGGL((k_norm_bwd<T, 256, 2>), g, b256, 0, st, a);
+        else if (p.nch == 1) hipLaunchKernelGGL((k_norm_bwd<T, 1024, 1>), g, b1024, 0, st, a);
+        else hipLaunchKernelGGL((k_norm_bwd<T, 1024, 2>), g, b1024, 0, st, a);
+    }
+    if (dw || db)
+        hipLaunchKernelGGL(k_norm_cols<T>, dim3((unsigned)ceil_div(a.cols, 64), 2), b1024, 0, st, (const float*)a.part,
+                           a.rows > 0 ? (int)p.groups : 0, a.cols, (T*)dw, (T*)db);
+    return hipGetLastError();
+}
+
+}  // namespace gpbo_static

@@ -633,6 +633,43 @@ int gpbo_multi_lml_batch(gpbo_multi* mg, const double* X, const double* y, int64
     });
 }
 
+int gpbo_multi_draw(gpbo_multi* mg, const double* u, int64_t draws, double temperature, int64_t top_k, double top_p, double min_p,
+                    int64_t* index_out, double* logp_out) {
+    if (!mg) return GPBO_ERR_BAD_ARG;
+    const int N = (int)mg->ctx.size();
+    if (mg->poff.empty() || mg->poff[(size_t)N] <= 0) MBADARG("draw: no posterior (call gpbo_multi_posterior first)");
+    const int64_t m = mg->poff[(size_t)N];
+    for (int i = 0; i < N; ++i)
+        if (mg->poff[(size_t)i + 1] > mg->poff[(size_t)i] && (!mg->ctx[(size_t)i]->have_posterior || !mg->ctx[(size_t)i]->have_acq))
+            MBADARG("draw: no acquisition values for the current posterior (call gpbo_multi_acquire first)");
+    gpbo_ctx* c0 = mg->ctx[0];
+    int st;
+    if (c0->m == m && mg->poff[1] == m) {
+        st = gpbo_draw(c0, u, draws, temperature, top_k, top_p, min_p, index_out, logp_out);
+    } else {      // a draw needs all scores: the blocks' values side by side on context 0's GPU (every context is idle between calls)
+        if (m > ((int64_t)1 << 28)) MBADARG("draw: at most 2^28 candidates");
+        double* all = nullptr;
+        hipError_t e = hipSetDevice(c0->device);
+        if (e == hipSuccess) e = hipMalloc((void**)&all, (size_t)m * 8);
+        for (int i = 0; i < N && e == hipSuccess; ++i) {
+            const int64_t lo = mg->poff[(size_t)i], cnt = mg->poff[(size_t)i + 1] - lo;
+            if (cnt > 0) e = hipMemcpyPeerAsync(all + lo, c0->device, mg->ctx[(size_t)i]->acq, mg->ctx[(size_t)i]->device, (size_t)cnt * 8, c0->stream);
+        }
+        if (e == hipSuccess) {
+            st = draw_impl(c0, all, m, u, draws, temperature, top_k, top_p, min_p, index_out, logp_out);
+        } else {
+            c0->err = std::string("draw: gathering the scores: ") + hipGetErrorString(e);
+            st = GPBO_ERR_HIP;
+        }
+        if (all) {
+            (void)hipStreamSynchronize(c0->stream);
+            (void)hipFree(all);
+        }
+    }
+    if (st != GPBO_OK) mg->err = c0->err;
+    return st;
+}
+
 int gpbo_multi_last_distribute(gpbo_multi* mg, double* ms_out, double* bytes_out) {
     if (!mg) return GPBO_ERR_BAD_ARG;
     if (ms_out) *ms_out = mg->distribute_ms;

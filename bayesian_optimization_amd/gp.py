@@ -320,6 +320,23 @@ class GP:
                                              stat.ctypes.data_as(C.POINTER(C.c_int32))))
         return (nll, g, stat) if grad else (nll, stat)
 
+    def lml_inputs(self, xTrain, yTrain, theta, sigmaY, kernel=L.KERNEL_RBF):
+        """-logL of one setting, its gradient w.r.t. theta (d,) and w.r.t. the training inputs (n, d); d <= 16."""
+        X = _f64(xTrain, 2)
+        y = _f64(np.asarray(yTrain).reshape(-1), 1)
+        th = _f64(np.asarray(theta).reshape(-1), 1)
+        if y.shape[0] != X.shape[0] or th.shape[0] != X.shape[1]:
+            raise ValueError('xTrain has shape %s, yTrain %d entries, theta %d' % (X.shape, y.shape[0], th.shape[0]))
+        nll, g, gx = C.c_double(), np.empty(X.shape[1]), np.empty(X.shape)
+        self._check(self._lib.gpbo_lml_inputs(self._h, L.dptr(X), L.dptr(y), X.shape[0], X.shape[1], L.dptr(th), float(sigmaY), int(kernel),
+                                              C.byref(nll), L.dptr(g), L.dptr(gx)))
+        return nll.value, g, gx
+
+    def draw(self, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """One candidate index per uniform number in u, from softmax(acquisition / temperature) after acquire(): a batch of picks
+        where acquire() returns the single best one.  Settings as in draws.sample.  Returns (index int64, logp), both (len(u),)."""
+        return _draw(self, self._lib.gpbo_draw, u, temperature, top_k, top_p, min_p)
+
     def descent_small(self, xTrain, yTrain, W0, sigmaY, alpha, beta, norm, steprule, max_its, kernel=L.KERNEL_RBF):
         """The reference's descent on -logL for every row of W0, to the end on the device (n <= 128, d <= 16).
         norm: 0 'component', 1 'full', 2 raw gradient; steprule: 0 constant, 1 'diminishing', 2 'backtrack'.
@@ -360,6 +377,16 @@ class GP:
         err, r = C.c_double(), C.c_double()
         self._check(self._lib.gpbo_selftest_gemm(self._h, int(n), C.byref(err), C.byref(r) if rate else None))
         return (err.value, r.value) if rate else err.value
+
+
+def _draw(gp, fn, u, temperature, top_k, top_p, min_p):
+    u = _f64(np.asarray(u).reshape(-1), 1)
+    if top_k != int(top_k):
+        raise ValueError('top_k must be a whole number; got %r' % (top_k,))
+    index, logp = np.empty(u.shape[0], dtype=np.int64), np.empty(u.shape[0])
+    gp._check(fn(gp._h, L.dptr(u), u.shape[0], float(temperature), min(int(top_k), 1 << 62), float(top_p), float(min_p),
+                 index.ctypes.data_as(C.POINTER(C.c_int64)), L.dptr(logp)))
+    return index, logp
 
 
 class MultiGP:
@@ -624,6 +651,13 @@ class MultiGP:
 
     def descent_small(self, *args, **kwargs):
         return self.contexts[0].descent_small(*args, **kwargs)
+
+    def lml_inputs(self, *args, **kwargs):
+        return self.contexts[0].lml_inputs(*args, **kwargs)
+
+    def draw(self, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """As GP.draw, over the candidates of all contexts (global indices)."""
+        return _draw(self, self._lib.gpbo_multi_draw, u, temperature, top_k, top_p, min_p)
 
     def kriging_lml(self, *args, **kwargs):
         return self.contexts[0].kriging_lml(*args, **kwargs)

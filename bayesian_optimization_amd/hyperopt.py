@@ -336,3 +336,18 @@ def gpr_descent(xT, yT, deg, epsilon, alpha, beta, max_its, W0, fd_h=1e-6, devic
             w_hist[r].append(np.array([w[r]]))
             c_hist[r].append(cost[r])
     return w_hist, c_hist
+
+
+def lml_inputs(xTrain, yTrain, theta, sigmaY, kernel=0, device=None):
+    """-logL (mlefcn, BayesOpt_v4.ipynb:154-165), its gradient w.r.t. theta and w.r.t. the training inputs (n, d)."""
+    return _lml_gp(device).lml_inputs(xTrain, yTrain, theta, sigmaY, kernel)
+
+
+def lml_features(fmap, x, yTrain, theta, sigmaY, kernel=0, device=None):
+    """-logL of a GP on learned inputs z = fmap.forward(x), with its gradients w.r.t. theta (d,) and w.r.t. every parameter of
+    the map (a dict of tensors, and 'x'): one training step's worth.  x is a GPU tensor of the map's type; a setting whose
+    covariance matrix is not positive definite raises LinAlgError, as fit() does."""
+    import torch
+    z, saved = fmap.forward(x, keep=True)
+    nll, g_theta, g_z = lml_inputs(z.double().cpu().numpy(), yTrain, theta, sigmaY, kernel, device)
+    return nll, g_theta, fmap.backward(torch.from_numpy(g_z).to(device=x.device, dtype=torch.float32), saved)

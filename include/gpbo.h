@@ -51,6 +51,14 @@ extern "C" {
 #define GPBO_INCUMBENT_MAX_Y 1  /* max(yTrain), GP/GPFR.m:48 */
 #define GPBO_INCUMBENT_GIVEN 2  /* caller-supplied (multi-GPU: the all-reduced max) */
 
+/* Element types and activations of the operators on learned inputs and of the draws */
+#define GPBO_TYPE_F64 0
+#define GPBO_TYPE_F32 1
+#define GPBO_TYPE_BF16 2
+#define GPBO_TYPE_F16 3
+#define GPBO_ACT_SILU 0        /* g / (1 + exp(-g)) */
+#define GPBO_ACT_GELU 1        /* g Phi(g), Phi the normal distribution function */
+
 typedef struct gpbo_ctx gpbo_ctx;
 
 /* Milliseconds measured with HIP events on the context's own stream, for the most
@@ -347,8 +355,75 @@ int gpbo_multi_append_acquire(gpbo_multi* mg, const double* x_new, double y_new,
 /* The B settings are independent: context i evaluates a contiguous block of them, nothing is exchanged. */
 int gpbo_multi_lml_batch(gpbo_multi* mg, const double* X, const double* y, int64_t n, int32_t d, const double* thetas,
                          const double* sigmas, int32_t B, int32_t kernel, double* nll_out, double* grad_out, int32_t* status_out);
+/* gpbo_draw over all blocks (global indices): the scores are gathered on context 0's GPU, at most 2^28 of them. */
+int gpbo_multi_draw(gpbo_multi* mg, const double* u, int64_t draws, double temperature, int64_t top_k, double top_p, double min_p,
+                    int64_t* index_out, double* logp_out);
 /* Wall time (ms) and bytes moved by the model hand-over of the last gpbo_multi_fit / gpbo_multi_kriging_fit. */
 int gpbo_multi_last_distribute(gpbo_multi* mg, double* ms_out, double* bytes_out);
+
+/* ---- Operators on caller-owned device arrays: learned inputs in front of the covariance, draws behind the acquisition.
+ * No counterpart in the reference, whose inputs are the raw coordinates (BayesOpt_v4.ipynb:131-134) and whose pick is
+ * np.argmax (:647).  Like gpbo_acquire_static they need no context, allocate nothing, copy nothing to the host and do not
+ * synchronise: they only enqueue kernels on `stream` (a hipStream_t of `device`; NULL = its default stream), so they may be
+ * captured.  Every pointer is a DEVICE pointer; strides count elements between rows, elements of a row are contiguous, and an
+ * array needs no more alignment than its element type has.  Outputs must not overlap inputs or each other.  Scratch memory is
+ * the caller's: `workspace`, 256-byte aligned, of at least the bytes the function of the same name + _workspace returns
+ * (0: none needed, -1: bad arguments); calls that may run at the same time need one each.  The same arguments
+ * give the same bits every time.  Bad arguments return GPBO_ERR_BAD_ARG and launch nothing; the caller's current device is
+ * put back.  Sizes: rows of 1 .. 2^31 - 1 elements, up to 2^31 - 1 rows; element offsets are 64-bit. */
+
+/* Layer norm of x (rows, cols): mu = mean(x), rstd = 1 / sqrt(mean((x - mu)^2) + eps), y = (x - mu) rstd w + b.
+ * dtype: GPBO_TYPE_F32, _BF16 or _F16, the type of x, w, b and y; w, b (cols,) may be NULL (1 and 0).  mean_out, rstd_out
+ * (rows,) are float32 and may be NULL; the backward pass needs them.  Statistics are held in 32 bits. */
+int gpbo_layernorm(int32_t device, void* stream, int32_t dtype, const void* x, int64_t x_stride, int64_t rows, int64_t cols,
+                   const void* w, const void* b, double eps, void* y, int64_t y_stride, float* mean_out, float* rstd_out);
+/* Its backward pass: dx (rows, cols), dw and db (cols,; both may be NULL, then no workspace is needed). */
+int64_t gpbo_layernorm_backward_workspace(int32_t dtype, int64_t rows, int64_t cols);
+int gpbo_layernorm_backward(int32_t device, void* stream, int32_t dtype, const void* dy, int64_t dy_stride, const void* x,
+                            int64_t x_stride, int64_t rows, int64_t cols, const void* w, const float* mean, const float* rstd,
+                            void* dx, int64_t dx_stride, void* dw, void* db, void* workspace, int64_t workspace_bytes);
+
+/* Gated unit: h = act(x wg^T) * (x wu^T), x (rows, cols), wg and wu (hidden, cols) with one row stride, h (rows, hidden).
+ * dtype: GPBO_TYPE_F32, _BF16 or _F16 for all of these; sums in 32 bits.  keep_g, keep_u (rows, hidden; contiguous float32;
+ * both or neither): x wg^T and x wu^T, for the backward pass. */
+int64_t gpbo_gated_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_t hidden);
+int gpbo_gated(int32_t device, void* stream, int32_t dtype, int32_t act, const void* x, int64_t x_stride, int64_t rows,
+               int64_t cols, const void* wg, const void* wu, int64_t w_stride, int64_t hidden, void* h, int64_t h_stride,
+               float* keep_g, float* keep_u, void* workspace, int64_t workspace_bytes);
+/* Its backward pass from dh (rows, hidden) and the kept products: dx (rows, cols) and dwg, dwu (hidden, cols; one row
+ * stride).  dx may be NULL, and so may dwg and dwu together. */
+int64_t gpbo_gated_backward_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_t hidden);
+int gpbo_gated_backward(int32_t device, void* stream, int32_t dtype, int32_t act, const void* dh, int64_t dh_stride, const void* x,
+                        int64_t x_stride, int64_t rows, int64_t cols, const void* wg, const void* wu, int64_t w_stride,
+                        int64_t hidden, const float* keep_g, const float* keep_u, void* dx, int64_t dx_stride, void* dwg, void* dwu,
+                        int64_t dw_stride, void* workspace, int64_t workspace_bytes);
+
+/* Draws from rows of scores (rows, cols) of type dtype (any of the four) with given uniform numbers u (rows, draws), float64 in
+ * [0, 1) (others count as the nearest end).  Valid scores are neither NaN nor -inf.  w_i = exp((s_i - max) / temperature);
+ * ranked by falling score, rising index on ties.  Kept: the first top_k (0: all); of those w_i >= min_p (0: all); of those every
+ * position in front of which less than top_p of their mass lies (1: all), the first always.  A draw is the lowest kept index
+ * i with C_i > u Z, C the running sum of the kept weights in index order and Z their mass.  index_out (rows, draws) int64, -1
+ * in a row without a valid score; logp_out (rows, draws) float64 = log(w_i / Z), may be NULL, -inf where the index is -1.
+ * temperature = 0: the best score, lowest index, logp 0.  params (rows, 4) float64 {temperature, top_k, top_p, min_p} gives
+ * every row settings of its own (the scalars are then not read; numbers out of range count as the nearest end), or is NULL.
+ * cols may be up to 2^28 (268,435,456) as for gpbo_acquire_static. */
+int64_t gpbo_draw_static_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_t draws);
+int gpbo_draw_static(int32_t device, void* stream, int32_t dtype, const void* scores, int64_t score_stride, int64_t rows,
+                     int64_t cols, const double* u, int64_t draws, double temperature, int64_t top_k, double top_p, double min_p,
+                     const double* params, int64_t* index_out, double* logp_out, void* workspace, int64_t workspace_bytes);
+
+/* The same draw from the acquisition values the last gpbo_acquire stored: where the loop takes np.argmax(ei)
+ * (BayesOpt_v4.ipynb:647), a batch of `draws` candidates at once.  Host arrays; u (draws,), index_out (draws,), logp_out
+ * (draws,) or NULL.  GPBO_ERR_BAD_ARG when there are no acquisition values of the current posterior. */
+int gpbo_draw(gpbo_ctx* ctx, const double* u, int64_t draws, double temperature, int64_t top_k, double top_p, double min_p,
+              int64_t* index_out, double* logp_out);
+
+/* -logL of one setting (mlefcn, BayesOpt_v4.ipynb:154-165) with its gradient w.r.t. theta, as gpbo_lml_batch, and w.r.t. the
+ * training inputs, gradx_out (n, d): what a learned map in front of the covariance needs for its own backward pass (no
+ * counterpart in the reference, whose inputs are fixed).  d <= 16.  grad_out may be NULL.  GPBO_ERR_NOT_PD when K + eps is not
+ * positive definite.  Host arrays; the model, candidates and posterior of ctx are untouched. */
+int gpbo_lml_inputs(gpbo_ctx* ctx, const double* X, const double* y, int64_t n, int32_t d, const double* theta, double sigmaY,
+                    int32_t kernel, double* nll_out, double* grad_out, double* gradx_out);
 
 /* Tuning knob: candidates per posterior chunk (multiple of 128; 0 = default). */
 int gpbo_set_chunk(gpbo_ctx* ctx, int64_t chunk);
