@@ -263,7 +263,7 @@ __global__ __launch_bounds__(256) void k_gated_slopes(const T* __restrict__ dh, 
 
 // Pieces of the contraction for a product of few tiles: up to two workgroups a CU, at least 4 steps each.
 inline int gated_splits(int64_t tiles, int64_t k, int64_t step) {
-    if (tiles >= 256) return 1;
+    if (tiles < 1 || tiles >= 256) return 1;
     return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(512, tiles), k / (4 * step)));
 }
 

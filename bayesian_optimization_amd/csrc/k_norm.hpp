@@ -91,7 +91,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_fwd(NormArgs a) 
         if (w) pw[k] = sp.load(w);
         if (b) pb[k] = sp.load(b);
     }
-    const float inv = 1.0f / (float)cols;
+    const float n = (float)cols;
     // the trip count is the same for all threads of a workgroup: row sums of wide rows hold barriers
     for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
         const int64_t r = r0 + group;
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_fwd(NormArgs a) 
 #pragma unroll
             for (int i = 0; i < V; ++i) s += sp.own(i) ? to_float(px[k].v[i]) : 0.0f;
         }
-        const float mu = row_sum<TPR>(s, lds[0]) * inv;
+        const float mu = row_sum<TPR>(s, lds[0]) / n;
         float q = 0.0f;
 #pragma unroll
         for (int k = 0; k < NCH; ++k) {
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_fwd(NormArgs a) 
                 q += sp.own(i) ? d * d : 0.0f;
             }
         }
-        const float rstd = 1.0f / sqrtf(row_sum<TPR>(q, lds[1]) * inv + a.eps);
+        const float rstd = 1.0f / sqrtf(row_sum<TPR>(q, lds[1]) / n + a.eps);
         if (!on) continue;                     // only where TPR <= 64: no barrier is skipped
         T* y = (T*)a.y + r * a.ys;
 #pragma unroll
@@ -144,7 +144,7 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_long(NormArgs a) {
     constexpr int V = Pack<T>::N;
     __shared__ float lds[2][16];
     const int64_t chunks = (a.cols + V - 1) / V;
-    const float inv = 1.0f / (float)a.cols;
+    const float n = (float)a.cols;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T* x = (const T*)a.x + r * a.xs;
         float s = 0.0f;
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_long(NormArgs a) {
             for (int i = 0; i < V; ++i) t += sp.own(i) ? to_float(p.v[i]) : 0.0f;
             s += t;
         }
-        const float mu = row_sum<1024>(s, lds[0]) * inv;
+        const float mu = row_sum<1024>(s, lds[0]) / n;
         float q = 0.0f;
         for (int64_t c = threadIdx.x; c < chunks; c += 1024) {
             const Span<T> sp(c, a.cols);
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_long(NormArgs a) {
             }
             q += t;
         }
-        const float rstd = 1.0f / sqrtf(row_sum<1024>(q, lds[1]) * inv + a.eps);
+        const float rstd = 1.0f / sqrtf(row_sum<1024>(q, lds[1]) / n + a.eps);
         T* y = (T*)a.y + r * a.ys;
         for (int64_t c = threadIdx.x; c < chunks; c += 1024) {
             const Span<T> sp(c, a.cols);
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_bwd(NormArgs a) 
 #pragma unroll
         for (int i = 0; i < V; ++i) aw[k][i] = ab[k][i] = 0.0f;
     }
-    const float inv = 1.0f / (float)cols;
+    const float n = (float)cols;
     int par = 0;
     for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
         const int64_t r = r0 + group;
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_bwd(NormArgs a) 
                 ab[k][i] += on ? d : 0.0f;
             }
         }
-        const float m1 = row_sum<TPR>(s1, lds[par]) * inv, m2 = row_sum<TPR>(s2, lds[par + 1]) * inv;
+        const float m1 = row_sum<TPR>(s1, lds[par]) / n, m2 = row_sum<TPR>(s2, lds[par + 1]) / n;
         par ^= 2;
         if (!on) continue;
         T* dx = (T*)a.dx + r * a.dxs;
@@ -272,7 +272,7 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormArgs a) {
     constexpr int V = Pack<T>::N;
     __shared__ float lds[4][16];
     const int64_t chunks = (a.cols + V - 1) / V;
-    const float inv = 1.0f / (float)a.cols;
+    const float n = (float)a.cols;
     int par = 0;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T* x = (const T*)a.x + r * a.xs;
@@ -295,7 +295,7 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormArgs a) {
             s1 += t1;
             s2 += t2;
         }
-        const float m1 = row_sum<1024>(s1, lds[par]) * inv, m2 = row_sum<1024>(s2, lds[par + 1]) * inv;
+        const float m1 = row_sum<1024>(s1, lds[par]) / n, m2 = row_sum<1024>(s2, lds[par + 1]) / n;
         par ^= 2;
         T* dx = (T*)a.dx + r * a.dxs;
         for (int64_t c = threadIdx.x; c < chunks; c += 1024) {

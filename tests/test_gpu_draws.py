@@ -1,0 +1,268 @@
+"""GPU: draws from scores against a plain implementation in 64 bits (sort, cut, walk).
+
+An index may differ from the plain one only where u lies within the rounding of the running sums of a border: sums of n weights
+in 64 bits in any order are off by at most n 2^-53 of their total; anything else is a failure."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float64, torch.float32, torch.bfloat16, torch.float16]
+
+
+def kept_weights(s, temperature, top_k, top_p, min_p):
+    """Weights by index (0: not kept) and log weights of one row of float64 scores; None when nothing can be drawn."""
+    s = np.where(np.isnan(s), -np.inf, s)
+    top = s.max() if s.size else -np.inf
+    if top == -np.inf:
+        return None, None
+    with np.errstate(invalid='ignore'):
+        t = np.where(s == top, 0.0, (s - top) / temperature) if temperature > 0 else np.where(s == top, 0.0, -np.inf)
+    w = np.exp(t)
+    order = np.argsort(-s, kind='stable')
+    order = order[s[order] > -np.inf]
+    if temperature == 0 or top_p == 0:
+        order = order[:1]
+    if top_k > 0:
+        order = order[:top_k]
+    order = order[w[order] >= min_p]
+    mass = np.cumsum(w[order])
+    if top_p < 1:
+        keep = (mass - w[order]) < top_p * mass[-1]
+        keep[0] = True
+        order = order[keep]
+    out = np.zeros_like(w)
+    out[order] = w[order]
+    return out, t
+
+
+def check(scores, u, index, logp, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    S = scores.double().cpu().numpy()
+    U, index, logp = u.cpu().numpy(), index.cpu().numpy(), logp.cpu().numpy()
+    per_row = lambda v, r: float(v[r]) if isinstance(v, torch.Tensor) else v
+    for r in range(S.shape[0]):
+        w, t = kept_weights(S[r], per_row(temperature, r), int(per_row(top_k, r)), per_row(top_p, r), per_row(min_p, r))
+        if w is None:
+            assert (index[r] == -1).all() and (logp[r] == -np.inf).all(), r
+            continue
+        run = np.cumsum(w)
+        Z = run[-1]
+        at = np.searchsorted(run, np.clip(U[r], 0, None) * Z, side='right')
+        at = np.minimum(at, np.nonzero(w)[0][-1])
+        slack = S.shape[1] * 2.0 ** -53 * Z * 4
+        for q in np.nonzero(at != index[r])[0]:
+            i = index[r, q]
+            assert w[i] > 0, (r, q, 'not in the kept set', i, at[q])
+            assert run[i] - w[i] - slack <= U[r, q] * Z <= run[i] + slack, (r, q, i, at[q])
+        want = t[index[r]] - math.log(Z)
+        assert np.allclose(logp[r], want, rtol=1e-13, atol=S.shape[1] * 2.0 ** -52 + 1e-14), r
+
+
+def rand_scores(rows, cols, dtype, seed, scale=2.0):
+    g = torch.Generator(device='cuda').manual_seed(seed)
+    return (torch.randn(rows, cols, generator=g, device='cuda', dtype=torch.float64) * scale).to(dtype)
+
+
+def rand_u(rows, draws, seed):
+    g = torch.Generator(device='cuda').manual_seed(1000 + seed)
+    return torch.rand(rows, draws, generator=g, device='cuda', dtype=torch.float64)
+
+
+SETTINGS = [dict(), dict(temperature=0.3), dict(top_k=1), dict(top_k=7), dict(top_k=700, temperature=2.0), dict(top_k=5000, temperature=3.0), dict(top_p=0.5), dict(top_p=0.97, temperature=1.7),
+            dict(min_p=0.05), dict(top_k=40, top_p=0.9, min_p=0.01, temperature=0.8), dict(top_k=3000, top_p=0.8, min_p=1e-4, temperature=2.5), dict(temperature=0.0), dict(top_p=0.0),
+            dict(top_p=1e-9), dict(min_p=1.0), dict(top_k=1 << 40), dict(temperature=1e-300), dict(temperature=1e300)]
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('rows,cols', [(1, 1), (3, 2), (2, 63), (2, 64), (1, 400), (4, 1000), (2, 1024), (2, 1025), (3, 4097), (2, 65537), (1, 300001)])
+def test_draws_match_the_plain_form(dtype, rows, cols):
+    from bayesian_optimization_amd import draws
+    s, u = rand_scores(rows, cols, dtype, cols), rand_u(rows, 70, cols)
+    for st in SETTINGS:
+        check(s, u, *draws.sample(s, u, **st), **st)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('cols', [5, 900, 1500, 70001, 600011])
+def test_ties_rank_by_index(dtype, cols):
+    """Few distinct scores: the cut falls inside a group of equals, whose first few by index are kept."""
+    from bayesian_optimization_amd import draws
+    g = torch.Generator(device='cuda').manual_seed(cols)
+    s = torch.randint(-2, 3, (2, cols), generator=g, device='cuda').to(dtype)
+    s[1] = 0                           # all the same; -0 ranks with +0
+    s[1, ::2] = -0.0
+    u = rand_u(2, 50, cols)
+    for st in (dict(), dict(top_k=3), dict(top_k=cols // 3), dict(top_k=cols - 1), dict(top_p=0.3), dict(top_p=0.9), dict(top_k=max(1, cols // 2), top_p=0.6),
+               dict(min_p=0.1, top_p=0.7), dict(top_k=max(1, cols // 7), min_p=0.3, top_p=0.999)):
+        check(s, u, *draws.sample(s, u, **st), **st)
+
+
+@pytest.mark.parametrize('cols', [3, 300, 3000, 200003])
+def test_masked_scores_infinities_and_empty_rows(cols):
+    from bayesian_optimization_amd import draws
+    inf, nan = float('inf'), float('nan')
+    for dtype in TYPES:
+        s = rand_scores(7, cols, dtype, 5)
+        s[0] = -inf                    # nothing left
+        s[1] = nan
+        s[2, 1:] = -inf                # one left, the first
+        s[3, :-1] = nan                # one left, the last
+        s[4, cols // 2] = inf          # takes everything
+        s[5, ::2] = torch.finfo(dtype).min      # masked with the lowest number: valid, without weight
+        s[6, 0], s[6, cols - 1] = inf, inf
+        u = rand_u(7, 33, 6)
+        for st in (dict(), dict(temperature=0.0), dict(top_k=2), dict(top_p=0.5), dict(min_p=0.2), dict(top_k=max(2, cols - 1), top_p=0.9)):
+            index, logp = draws.sample(s, u, **st)
+            check(s, u, index, logp, **st)
+            assert bool((index[0] == -1).all()) and bool((index[1] == -1).all())
+            assert bool((index[2] == 0).all()) and bool((index[3] == cols - 1).all()) and bool((index[4] == cols // 2).all())
+
+
+def test_most_scores_zero_as_expected_improvement_has_them():
+    from bayesian_optimization_amd import draws
+    s = torch.zeros(1, 1 << 20, device='cuda', dtype=torch.float64)
+    g = torch.Generator(device='cuda').manual_seed(3)
+    at = torch.randint(0, 1 << 20, (1000,), generator=g, device='cuda')
+    s[0, at] = torch.rand(1000, generator=g, device='cuda', dtype=torch.float64)
+    u = rand_u(1, 95, 4)
+    for st in (dict(temperature=0.05), dict(temperature=0.05, top_p=0.5), dict(temperature=0.05, top_k=500), dict(temperature=0.05, top_k=5000, top_p=0.99), dict(temperature=1.0, top_p=0.9)):
+        check(s, u, *draws.sample(s, u, **st), **st)
+
+
+def test_settings_per_row():
+    from bayesian_optimization_amd import draws
+    rows = 6
+    for cols in (500, 20001):
+        s, u = rand_scores(rows, cols, torch.float32, 9), rand_u(rows, 20, 9)
+        st = dict(temperature=torch.tensor([0.5, 1, 2, 0, 1, 1], device='cuda'), top_k=torch.tensor([0, 5, 100, 3, 0, 2000], device='cuda'),
+                  top_p=torch.tensor([1.0, 0.9, 0.5, 1.0, 0.2, 0.99], device='cuda', dtype=torch.float64), min_p=0.001)
+        index, logp = draws.sample(s, u, **st)
+        check(s, u, index, logp, **st)
+        for r in range(rows):
+            one = {k: (v[r].item() if isinstance(v, torch.Tensor) else v) for k, v in st.items()}
+            i1, l1 = draws.sample(s[r:r + 1], u[r:r + 1], **one)
+            assert torch.equal(i1[0], index[r]) and torch.equal(l1[0], logp[r])
+
+
+def test_uniform_numbers_at_and_beyond_the_ends():
+    from bayesian_optimization_amd import draws
+    for cols in (300, 5000):
+        s = rand_scores(1, cols, torch.float64, 10)
+        s[0, :3], s[0, -2:] = -float('inf'), float('nan')
+        u = torch.tensor([[0.0, -1.0, float('nan'), 1.0, 2.0, float('inf'), 1 - 2.0 ** -53]], device='cuda', dtype=torch.float64)
+        index, _ = draws.sample(s, u)
+        assert index[0].tolist() == [3, 3, 3, cols - 3, cols - 3, cols - 3, cols - 3]
+
+
+def test_strided_rows_streams_and_graphs():
+    from bayesian_optimization_amd import draws
+    for cols, dtype in ((400, torch.float64), (30001, torch.bfloat16), (1 << 18, torch.float64)):
+        base = rand_scores(6, cols + 11, dtype, 11)
+        s = base[::2, 5:5 + cols]
+        u = rand_u(3, 9, 11)
+        st = dict(temperature=0.7, top_k=2000, top_p=0.9)
+        first = draws.sample(s, u, **st)
+        check(s, u, *first, **st)
+        assert all(torch.equal(a, b) for a, b in zip(first, draws.sample(s.contiguous(), u, **st)))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            again = draws.sample(s, u, **st)
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+        graph, graph2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = draws.sample(s, u, **st)
+        with torch.cuda.graph(graph2):
+            out2 = draws.sample(s, u, **st)
+        for i in range(4):
+            base.copy_(rand_scores(6, cols + 11, dtype, 20 + i))
+            u.copy_(rand_u(3, 9, 20 + i))
+            graph.replay()
+            graph2.replay()
+            torch.cuda.synchronize()
+            eager = draws.sample(s, u, **st)
+            check(s, u, *eager, **st)
+            assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(eager, out, out2))
+
+
+def test_many_rows_and_no_rows():
+    from bayesian_optimization_amd import draws
+    s, u = rand_scores(3000, 17, torch.float16, 12), rand_u(3000, 2, 12)
+    check(s, u, *draws.sample(s, u, top_p=0.8), top_p=0.8)
+    index, logp = draws.sample(s[:0], u[:0])
+    assert index.shape == (0, 2) and logp.shape == (0, 2)
+    index, logp = draws.sample(s, u[:, :0])
+    assert index.shape == (3000, 0)
+
+
+def test_the_longest_row():
+    """2^28 scores of float16: 512 MB; the best few are known."""
+    from bayesian_optimization_amd import draws
+    n = 1 << 28
+    s = torch.zeros(1, n, dtype=torch.float16, device='cuda')
+    at = [0, 12345, n // 2, n - 1]
+    s[0, at] = 200.0
+    u = torch.tensor([[0.1, 0.3, 0.6, 0.99]], device='cuda', dtype=torch.float64)
+    for st in (dict(), dict(top_k=4), dict(top_p=0.99), dict(min_p=0.5)):
+        index, logp = draws.sample(s, u, **st)
+        assert index[0].tolist() == at and np.allclose(logp.cpu().numpy(), math.log(0.25))
+    with pytest.raises(ValueError):
+        draws.sample(torch.zeros(1, 1, dtype=torch.float16, device='cuda').expand(1, n + 1).contiguous(), u)
+
+
+def test_refusals():
+    from bayesian_optimization_amd import draws
+    s, u = rand_scores(2, 10, torch.float32, 13), rand_u(2, 3, 13)
+    for bad in (dict(temperature=-1.0), dict(temperature=float('nan')), dict(temperature=float('inf')), dict(top_k=-1), dict(top_k=2.5), dict(top_p=1.5), dict(top_p=-0.1),
+                dict(min_p=2.0), dict(top_p=float('nan')), dict(top_k=torch.ones(3, device='cuda')), dict(top_p=torch.ones(2))):
+        with pytest.raises(ValueError):
+            draws.sample(s, u, **bad)
+    for a, b in ((s.t(), u), (s.int(), u), (s[0], u), (s, u.float()), (s, u[:1]), (s.cpu(), u), (s, u.cpu())):
+        with pytest.raises(ValueError):
+            draws.sample(a, b)
+
+
+def test_gp_draw_after_acquire(gp0):
+    import bayesian_optimization_amd as bo
+    rng = np.random.default_rng(1)
+    X = rng.random((50, 2))
+    y = np.sin(5 * X.sum(1))
+    Xs = rng.random((30000, 2))
+    u = rng.random(60)
+    gp0.fit(X, y, [0.3, 0.4], 0.05)
+    gp0.set_candidates(Xs)
+    gp0.posterior()
+    with pytest.raises(ValueError):
+        gp0.draw(u)                    # no acquisition values yet
+    best, _ = gp0.acquire()
+    ei = gp0.read(mu=False, var=False, acq=True)
+    st = dict(temperature=0.02, top_k=5000, top_p=0.95, min_p=1e-6)
+    index, logp = gp0.draw(u, **st)
+    T = lambda a: torch.from_numpy(np.asarray(a)[None]).cuda()
+    check(T(ei), T(u), T(index), T(logp), **st)
+    assert gp0.draw([0.5], temperature=0)[0][0] == best
+    for bad in (dict(temperature=-1), dict(top_k=-3), dict(top_k=1.5), dict(top_p=2), dict(min_p=-1), dict(temperature=float('nan'))):
+        with pytest.raises(ValueError):
+            gp0.draw(u, **bad)
+    with pytest.raises(ValueError):
+        gp0.draw([])
+    mg = bo.MultiGP([0, 0, 0])
+    mg.fit(X, y, [0.3, 0.4], 0.05)
+    mg.set_candidates(Xs)
+    mg.posterior()
+    with pytest.raises(ValueError):
+        mg.draw(u)
+    mg.acquire()
+    i3, l3 = mg.draw(u, **st)
+    assert (i3 == index).all() and (l3 == logp).all()
+    one = bo.MultiGP([0])
+    one.fit(X, y, [0.3, 0.4], 0.05)
+    one.set_candidates(Xs)
+    one.posterior()
+    one.acquire()
+    assert (one.draw(u, **st)[0] == index).all()
+    mg.close()
+    one.close()
