@@ -2,7 +2,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "k_gated.hpp"
+#include "k_gated_fast.hpp"
 #include "k_norm.hpp"
 
 using namespace gpbo_static;
@@ -72,7 +72,7 @@ int gpbo_layernorm_backward(int32_t device, void* stream, int32_t dtype, const v
 
 int64_t gpbo_gated_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_t hidden) {
     if (!is_float_type(dtype) || !matrix_ok(rows, cols, cols) || !matrix_ok(rows, hidden, hidden)) return -1;
-    return 0;
+    return by_type(dtype, [&](auto t) { return forward_plan<decltype(t)>(rows, cols, hidden).bytes(); });
 }
 
 int gpbo_gated(int32_t device, void* stream, int32_t dtype, int32_t act, const void* x, int64_t x_stride, int64_t rows,
@@ -89,15 +89,12 @@ int gpbo_gated(int32_t device, void* stream, int32_t dtype, int32_t act, const v
     GatedArgs g{};
     g.a[0] = {x, x_stride, 1}, g.b[0] = {wg, w_stride, 1}, g.b[1] = {wu, w_stride, 1};
     g.m = rows, g.n = hidden, g.k = cols, g.out[0] = h, g.os = h_stride, g.keep_g = keep_g, g.keep_u = keep_u, g.act = act, g.splits = 1;
-    return result(by_type(dtype, [&](auto t) { return gated_forward<decltype(t)>((hipStream_t)stream, g); }));
+    return result(by_type(dtype, [&](auto t) { return gated_forward<decltype(t)>((hipStream_t)stream, g, (char*)workspace); }));
 }
 
 int64_t gpbo_gated_backward_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_t hidden) {
     if (!is_float_type(dtype) || !matrix_ok(rows, cols, cols) || !matrix_ok(rows, hidden, hidden)) return -1;
-    return by_type(dtype, [&](auto t) {
-        const GatedPlan p = gated_plan<decltype(t)>(rows, cols, hidden);
-        return 2 * p.slopes_bytes + p.part_bytes;
-    });
+    return by_type(dtype, [&](auto t) { return backward_plan<decltype(t)>(rows, cols, hidden).bytes(); });
 }
 
 int gpbo_gated_backward(int32_t device, void* stream, int32_t dtype, int32_t act, const void* dh, int64_t dh_stride, const void* x,

@@ -267,58 +267,4 @@ inline int gated_splits(int64_t tiles, int64_t k, int64_t step) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(512, tiles), k / (4 * step)));
 }
 
-struct GatedPlan {
-    int64_t slopes_bytes, part_bytes;
-    int splits_x, splits_w;
-};
-template <typename T>
-GatedPlan gated_plan(int64_t m, int64_t k, int64_t h) {
-    constexpr int KS = STEP_BYTES / sizeof(T);
-    GatedPlan p{};
-    p.slopes_bytes = round_up(m * h * (int64_t)sizeof(T), 256);
-    p.splits_x = gated_splits(ceil_div(m, TB) * ceil_div(k, TB), h, KS);
-    p.splits_w = gated_splits(2 * ceil_div(h, TB) * ceil_div(k, TB), m, KS);
-    p.part_bytes = std::max<int64_t>(p.splits_x > 1 ? p.splits_x * m * k * 4 : 0, p.splits_w > 1 ? 2 * p.splits_w * h * k * 4 : 0);
-    return p;
-}
-
-template <typename T>
-hipError_t gated_forward(hipStream_t st, const GatedArgs& g) {
-    const int64_t tiles = ceil_div(g.m, TB) * ceil_div(g.n, TB);
-    hipLaunchKernelGGL((k_gated_tile<T, GATED_FWD, true, true>), dim3((unsigned)tiles), dim3(256), 0, st, g);
-    return hipGetLastError();
-}
-
-template <typename T>
-hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const void* x, int64_t xs, const void* wg, const void* wu, int64_t ws,
-                          const float* kg, const float* ku, int64_t m, int64_t k, int64_t h, int act, void* dx, int64_t dxs, void* dwg,
-                          void* dwu, int64_t dws, char* work) {
-    const GatedPlan p = gated_plan<T>(m, k, h);
-    T *dg = (T*)work, *du = (T*)(work + p.slopes_bytes);
-    float* part = (float*)(work + 2 * p.slopes_bytes);
-    const int64_t packs = m * ceil_div(h, Pack<T>::N);
-    if (m > 0)
-        hipLaunchKernelGGL(k_gated_slopes<T>, dim3((unsigned)std::min<int64_t>(ceil_div(packs, 256), 8192)), dim3(256), 0, st, (const T*)dh, dhs,
-                           kg, ku, m, h, act, dg, du);
-    if (dx && m > 0) {
-        GatedArgs g{};
-        g.a[0] = {dg, h, 1}, g.a[1] = {du, h, 1};
-        g.b[0] = {wg, 1, ws}, g.b[1] = {wu, 1, ws};
-        g.m = m, g.n = k, g.k = h, g.out[0] = dx, g.os = dxs, g.splits = p.splits_x, g.part = part;
-        hipLaunchKernelGGL((k_gated_tile<T, GATED_SUM, true, false>), dim3((unsigned)(ceil_div(m, TB) * ceil_div(k, TB)), (unsigned)g.splits),
-                           dim3(256), 0, st, g);
-        if (g.splits > 1) hipLaunchKernelGGL(k_gated_join<T>, dim3((unsigned)ceil_div(m * k, 256), 1), dim3(256), 0, st, g);
-    }
-    if (dwg) {
-        GatedArgs g{};
-        g.a[0] = {dg, 1, h}, g.a[1] = {du, 1, h};
-        g.b[0] = g.b[1] = {x, 1, xs};
-        g.m = h, g.n = k, g.k = m, g.out[0] = dwg, g.out[1] = dwu, g.os = dws, g.splits = p.splits_w, g.part = part;
-        hipLaunchKernelGGL((k_gated_tile<T, GATED_PAIR, false, false>), dim3((unsigned)(ceil_div(h, TB) * ceil_div(k, TB)), (unsigned)g.splits, 2),
-                           dim3(256), 0, st, g);
-        if (g.splits > 1) hipLaunchKernelGGL(k_gated_join<T>, dim3((unsigned)ceil_div(h * k, 256), 2), dim3(256), 0, st, g);
-    }
-    return hipGetLastError();
-}
-
 }  // namespace gpbo_static

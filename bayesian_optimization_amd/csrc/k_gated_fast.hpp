@@ -1,0 +1,430 @@
+// The gated unit's products on large operands: both operands contiguous along the contraction, in 128-byte steps, straight from
+// memory into LDS.
+#pragma once
+
+#include "k_gated.hpp"
+
+namespace gpbo_static {
+
+// Tile of BM x BN outputs by WM x WN waves; a step is 128 bytes of contraction of BM + BN rows.  The step after the current one
+// is on its way into the other LDS buffer (16 bytes a lane, no registers) while the current one is multiplied: one barrier a
+// step.  Row r of a step lies at 128 r, its 16-byte chunk c at slot c ^ (r & 7): a fragment read touches 16 rows, and without the
+// exchange all of them would start in the same bank; the loads do the exchange by the address each lane fetches from, since
+// their destination is fixed (wave base + 16 lane).
+template <typename T, int MODE, int BM, int BN, int WM, int WN>
+struct FastTile {
+    static constexpr int THREADS = 64 * WM * WN, KS = STEP_BYTES / sizeof(T);
+    static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;              // 16 x 16 fragments of a wave
+    static constexpr int LA = BM * 8 / THREADS, LB = BN * 8 / THREADS;      // 16-byte loads of a thread and step
+    static constexpr int COLS = MODE == GATED_FWD ? BN / 2 : BN;            // output columns of a tile
+};
+
+typedef __attribute__((address_space(3))) void* LdsPtr;
+
+// A tile's operand as a buffer: 16 bytes from byte `lane_offset + step_offset` behind p into LDS at `lds` + 16 lane.  Every offset is
+// in range by construction (rows behind the last repeat it), so the descriptor's bound is left open.
+__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t r, uint4* lds, uint32_t lane_offset, uint32_t step_offset) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)lds, 16, lane_offset, step_offset, 0, 0);
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, 0xffffffffu, 0x00020000);
+}
+
+// Workgroups of one XCD (consecutive ids go round the eight of them) take neighbouring tiles, GROUP tile rows at a time, so that
+// what one XCD works on shares rows of both operands in its L2.
+__device__ __forceinline__ void tile_of(uint32_t id, uint32_t tm, uint32_t tn, uint32_t& im, uint32_t& in) {
+    constexpr uint32_t XCDS = 8, GROUP = 8;
+    const uint32_t tiles = tm * tn, per = tiles / XCDS, rest = tiles % XCDS, x = id % XCDS;
+    const uint32_t t = x * per + min(x, rest) + id / XCDS;
+    const uint32_t band = t / (GROUP * tn), rows = min(GROUP, tm - band * GROUP), in_band = t - band * GROUP * tn;
+    im = __builtin_amdgcn_readfirstlane(band * GROUP + in_band % rows);      // the same in all lanes: divisions leave it in vector registers
+    in = __builtin_amdgcn_readfirstlane(in_band / rows);
+}
+
+template <typename T, int MODE, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, BM == 256 ? 1 : 2) void k_gated_fast(GatedArgs g) {
+    using F = FastTile<T, MODE, BM, BN, WM, WN>;
+    constexpr int FM = F::FM, FN = F::FN, KS = F::KS;
+    __shared__ uint4 buf0[(BM + BN) * 8], buf1[(BM + BN) * 8];
+    uint32_t im, in;
+    tile_of(blockIdx.x, (uint32_t)((g.m + BM - 1) / BM), (uint32_t)((g.n + F::COLS - 1) / F::COLS), im, in);
+    const int64_t row0 = (int64_t)im * BM, col0 = (int64_t)in * F::COLS;
+    const int z = MODE == GATED_PAIR ? blockIdx.z : 0, split = blockIdx.y;
+    const uint32_t all_steps = (uint32_t)(g.k / KS), per = (all_steps + g.splits - 1) / (uint32_t)g.splits;
+    const uint32_t s0 = __builtin_amdgcn_readfirstlane(min(split * per, all_steps));
+    const int steps1 = (int)__builtin_amdgcn_readfirstlane(min(s0 + per, all_steps) - s0), steps = MODE == GATED_SUM ? 2 * steps1 : steps1;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+
+    // what this thread loads of a step: byte offsets from the tile's first row
+    uint32_t oa[F::LA], ob[F::LB];
+    const int64_t sa = g.a[0].sr * (int64_t)sizeof(T), sb = g.b[0].sr * (int64_t)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < F::LA; ++i) {
+        const int r = (i * F::THREADS + tid) >> 3, c = (tid & 7) ^ (r & 7);
+        oa[i] = (uint32_t)(min((int64_t)r, g.m - 1 - row0) * sa + c * 16);
+    }
+#pragma unroll
+    for (int i = 0; i < F::LB; ++i) {
+        const int r = (i * F::THREADS + tid) >> 3, c = (tid & 7) ^ (r & 7);
+        const int q = MODE == GATED_FWD ? r % F::COLS : r;
+        ob[i] = (uint32_t)(min((int64_t)q, g.n - 1 - col0) * sb + c * 16);
+    }
+    const int64_t at_a = row0 * sa + (int64_t)s0 * STEP_BYTES, at_b = col0 * sb + (int64_t)s0 * STEP_BYTES;
+    const auto ra0 = buffer_of((const char*)(MODE == GATED_PAIR && z ? g.a[1].p : g.a[0].p) + at_a);
+    const auto ra1 = buffer_of((const char*)g.a[1].p + at_a);
+    const auto rb0 = buffer_of((const char*)g.b[0].p + at_b), rb1 = buffer_of((const char*)g.b[1].p + at_b);
+    auto fetch = [&](uint4* buf, int s) {
+        const bool second = MODE == GATED_SUM && s >= steps1;
+        const uint32_t k = (uint32_t)(s - (second ? steps1 : 0)) * STEP_BYTES;
+#pragma unroll
+        for (int i = 0; i < F::LA; ++i) load_lds(second ? ra1 : ra0, buf + i * F::THREADS + wave * 64, oa[i], k);
+#pragma unroll
+        for (int i = 0; i < F::LB; ++i) {
+            const bool up = MODE == GATED_FWD ? i * F::THREADS / 8 >= F::COLS : second;
+            load_lds(up ? rb1 : rb0, buf + BM * 8 + i * F::THREADS + wave * 64, ob[i], k);
+        }
+    };
+
+    f32x4 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    auto multiply = [&](const uint4* buf) {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            uint4 fa[FM], fb[FN];
+            const int c = (kk * 4 + (lane >> 4)) ^ (lane & 7);              // every fragment starts at a multiple of 8 rows
+            const uint4* pa = buf + (wm * FM * 16 + (lane & 15)) * 8 + c;
+            const uint4* pb = buf + (BM + (MODE == GATED_FWD ? wn * (FN / 2 * 16) : wn * FN * 16) + (lane & 15)) * 8 + c;
+#pragma unroll
+            for (int j = 0; j < FN; ++j) fb[j] = pb[MODE == GATED_FWD ? ((j >= FN / 2) * F::COLS + (j % (FN / 2)) * 16) * 8 : j * 16 * 8];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) fa[i] = pa[i * 16 * 8];
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = mma<T>(fb[j], fa[i], acc[i][j]);
+        }
+    };
+    if (steps > 0) {
+        fetch(buf0, 0);
+        __syncthreads();
+        int s = 0;
+        for (; s + 1 < steps; s += 2) {
+            fetch(buf1, s + 1);
+            __builtin_amdgcn_sched_barrier(0);       // the loads stay in front of the products that hide them
+            multiply(buf0);
+            __syncthreads();
+            fetch(buf0, min(s + 2, steps - 1));      // behind the last step: loaded again, not used
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(buf1);
+            __syncthreads();
+        }
+        if (s < steps) multiply(buf0);
+    }
+
+    // lane: row lane % 16 of a fragment, four neighbouring columns from (lane / 16) * 4 on
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int64_t row = row0 + wm * FM * 16 + i * 16 + (lane & 15);
+        if (row >= g.m) continue;
+#pragma unroll
+        for (int j = 0; j < (MODE == GATED_FWD ? FN / 2 : FN); ++j) {
+            const int64_t col = col0 + (MODE == GATED_FWD ? wn * (FN / 2 * 16) : wn * FN * 16) + j * 16 + (lane >> 4) * 4;
+            if (col >= g.n) continue;
+            const int len = (int)min((int64_t)4, g.n - col);
+            float v[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if constexpr (MODE == GATED_FWD) v[r] = activate(acc[i][j][r], g.act) * acc[i][j + FN / 2][r];
+                else v[r] = acc[i][j][r];
+            }
+            if (MODE != GATED_FWD && g.splits > 1) {
+                float* p = g.part + (((int64_t)z * g.splits + split) * g.m + row) * g.n + col;
+                if (len == 4) __builtin_memcpy(p, v, 16);
+                else
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (r < len) p[r] = v[r];
+                continue;
+            }
+            T o[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = from_float<T>(v[r]);
+            T* p = (T*)(z ? g.out[1] : g.out[0]) + row * g.os + col;
+            if (len == 4) __builtin_memcpy(p, o, sizeof(o));
+            else
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (r < len) p[r] = o[r];
+            if (MODE == GATED_FWD && g.keep_g) {
+                float *kg = g.keep_g + row * g.n + col, *ku = g.keep_u + row * g.n + col;
+                const f32x4 vg = acc[i][j], vu = acc[i][MODE == GATED_FWD ? j + FN / 2 : j];
+                if (len == 4) {
+                    __builtin_memcpy(kg, &vg, 16);
+                    __builtin_memcpy(ku, &vu, 16);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (r < len) kg[r] = vg[r], ku[r] = vu[r];
+                }
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Operands laid out for it.  Rows padded with zeros to whole steps.
+struct PackJob {
+    const void* src;
+    int64_t stride, rows, cols;   // source
+    void* dst;
+    int64_t pitch;                // elements of a destination row
+    int64_t blocks;               // tiles of 64 x 64
+};
+struct PackArgs {
+    PackJob job[3];
+    int count;
+};
+
+// dst[r][c] = src[r][c] (TRANSPOSE: dst[c][r] = src[r][c]), zero up to the pitch.
+template <typename T, bool TRANSPOSE>
+__global__ __launch_bounds__(256) void k_gated_pack(PackArgs a) {
+    int64_t id = blockIdx.x;
+    int which = 0;
+    while (which + 1 < a.count && id >= a.job[which].blocks) id -= a.job[which++].blocks;
+    const PackJob& jb = a.job[which];
+    __shared__ T tile[64][65];
+    const T* src = (const T*)jb.src;
+    T* dst = (T*)jb.dst;
+    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    // the grid covers the padded destination: destination columns are source columns, or (transposed) source rows
+    const int64_t tiles_c = TRANSPOSE ? (jb.cols + 63) / 64 : jb.pitch / 64;
+    const int64_t r0 = id / tiles_c * 64, c0 = id % tiles_c * 64;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int64_t r = r0 + ty + i * 4, c = c0 + tx;
+        const T v = r < jb.rows && c < jb.cols ? src[r * jb.stride + c] : from_float<T>(0.0f);
+        if constexpr (TRANSPOSE) tile[ty + i * 4][tx] = v;
+        else if (r < jb.rows) dst[r * jb.pitch + c] = v;
+    }
+    if constexpr (TRANSPOSE) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int64_t c = c0 + ty + i * 4, r = r0 + tx;      // pitch is a multiple of 64: r < pitch
+            if (c < jb.cols) dst[c * jb.pitch + r] = tile[tx][ty + i * 4];
+        }
+    }
+}
+
+// dg and du, row by row (pitch hp) and transposed (pitch mp), zero in the padding of both.
+template <typename T>
+__global__ __launch_bounds__(256) void k_gated_slopes_both(const T* __restrict__ dh, int64_t dhs, const float* __restrict__ kg,
+                                                           const float* __restrict__ ku, int64_t m, int64_t n, int act, T* __restrict__ dg,
+                                                           T* __restrict__ du, int64_t hp, T* __restrict__ dgt, T* __restrict__ dut, int64_t mp) {
+    __shared__ T tg[64][66], tu[64][66];
+    const int64_t tiles_c = hp / 64, r0 = blockIdx.x / tiles_c * 64, c0 = blockIdx.x % tiles_c * 64;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;      // four columns a thread, 16 rows a pass
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t r = r0 + ty + i * 16, c = c0 + tx * 4;
+        const int len = r < m ? (int)max((int64_t)0, min((int64_t)4, n - c)) : 0;
+        float gv[4] = {0.0f, 0.0f, 0.0f, 0.0f}, uv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        T dv[4], og[4], ou[4];
+        if (len == 4) {
+            __builtin_memcpy(gv, kg + r * n + c, 16);
+            __builtin_memcpy(uv, ku + r * n + c, 16);
+            __builtin_memcpy(dv, dh + r * dhs + c, sizeof(dv));
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                dv[k] = k < len ? dh[r * dhs + c + k] : from_float<T>(0.0f);
+                if (k < len) gv[k] = kg[r * n + c + k], uv[k] = ku[r * n + c + k];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float a, da;
+            activation(gv[k], act, a, da);
+            og[k] = from_float<T>(k < len ? to_float(dv[k]) * uv[k] * da : 0.0f);
+            ou[k] = from_float<T>(k < len ? to_float(dv[k]) * a : 0.0f);
+            tg[ty + i * 16][tx * 4 + k] = og[k];
+            tu[ty + i * 16][tx * 4 + k] = ou[k];
+        }
+        if (r < m) {
+            __builtin_memcpy(dg + r * hp + c, og, sizeof(og));
+            __builtin_memcpy(du + r * hp + c, ou, sizeof(ou));
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t c = c0 + ty + i * 16, r = r0 + tx * 4;
+        if (c >= n) continue;
+        T og[4], ou[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) og[k] = tg[tx * 4 + k][ty + i * 16], ou[k] = tu[tx * 4 + k][ty + i * 16];
+        __builtin_memcpy(dgt + c * mp + r, og, sizeof(og));
+        __builtin_memcpy(dut + c * mp + r, ou, sizeof(ou));
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Which kernels a call takes, and its workspace.
+
+inline bool aligned16(const void* p, int64_t stride, int64_t bytes) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * bytes % 16 == 0 && stride * bytes < (1 << 23);
+}
+
+struct ForwardPlan {
+    bool fast = false, pack = false;
+    int tile = 128;
+    int64_t kp = 0, x_bytes = 0, w_bytes = 0;
+    int64_t bytes() const { return pack ? x_bytes + 2 * w_bytes : 0; }
+};
+// The loads straight into LDS need whole steps and 16-byte rows.  A contraction that is no whole number of steps is packed into the
+// workspace first, which pays from some 2 GFLOP on; below, and for few tiles, the any-shape kernel starts sooner.
+template <typename T>
+ForwardPlan forward_plan(int64_t m, int64_t k, int64_t h) {
+    constexpr int KS = STEP_BYTES / sizeof(T);
+    ForwardPlan p;
+    p.kp = round_up(k, KS);
+    p.fast = m * h >= 128 * 64 * 64 && 4 * m * h * k >= (int64_t)1 << 31 && k * (int64_t)sizeof(T) < (1 << 23);
+    p.pack = p.fast && k % KS != 0;
+    if (ceil_div(m, 256) * ceil_div(h, 128) >= 256 && k >= 8 * KS) p.tile = 256;
+    p.x_bytes = round_up(m * p.kp * (int64_t)sizeof(T), 256);
+    p.w_bytes = round_up(h * p.kp * (int64_t)sizeof(T), 256);
+    return p;
+}
+
+template <typename T, int MODE>
+void launch_fast(hipStream_t st, const GatedArgs& g, int tile) {
+    const int zs = MODE == GATED_PAIR ? 2 : 1;
+    if (tile == 256)
+        hipLaunchKernelGGL((k_gated_fast<T, MODE, 256, 256, 2, 4>),
+                           dim3((unsigned)(ceil_div(g.m, 256) * ceil_div(g.n, MODE == GATED_FWD ? 128 : 256)), (unsigned)g.splits, zs), dim3(512), 0, st, g);
+    else
+        hipLaunchKernelGGL((k_gated_fast<T, MODE, 128, 128, 2, 2>),
+                           dim3((unsigned)(ceil_div(g.m, 128) * ceil_div(g.n, MODE == GATED_FWD ? 64 : 128)), (unsigned)g.splits, zs), dim3(256), 0, st, g);
+}
+
+template <typename T>
+hipError_t gated_forward(hipStream_t st, GatedArgs g, char* work) {
+    constexpr int KS = STEP_BYTES / sizeof(T);
+    const ForwardPlan p = forward_plan<T>(g.m, g.k, g.n);
+    const bool direct = aligned16(g.a[0].p, g.a[0].sr, sizeof(T)) && aligned16(g.b[0].p, g.b[0].sr, sizeof(T)) && aligned16(g.b[1].p, g.b[1].sr, sizeof(T));
+    if (p.fast && (p.pack || direct)) {
+        if (p.pack) {
+            PackArgs a{};
+            a.count = 3;
+            a.job[0] = {g.a[0].p, g.a[0].sr, g.m, g.k, work, p.kp, ceil_div(g.m, 64) * ceil_div(p.kp, 64)};
+            a.job[1] = {g.b[0].p, g.b[0].sr, g.n, g.k, work + p.x_bytes, p.kp, ceil_div(g.n, 64) * ceil_div(p.kp, 64)};
+            a.job[2] = {g.b[1].p, g.b[1].sr, g.n, g.k, work + p.x_bytes + p.w_bytes, p.kp, ceil_div(g.n, 64) * ceil_div(p.kp, 64)};
+            hipLaunchKernelGGL((k_gated_pack<T, false>), dim3((unsigned)(a.job[0].blocks + a.job[1].blocks + a.job[2].blocks)), dim3(256), 0, st, a);
+            g.a[0] = {a.job[0].dst, p.kp, 1}, g.b[0] = {a.job[1].dst, p.kp, 1}, g.b[1] = {a.job[2].dst, p.kp, 1};
+            g.k = p.kp;
+        }
+        static_assert(KS >= 32, "a step");
+        launch_fast<T, GATED_FWD>(st, g, p.tile);
+    } else {
+        const int64_t tiles = ceil_div(g.m, TB) * ceil_div(g.n, TB);
+        hipLaunchKernelGGL((k_gated_tile<T, GATED_FWD, true, true>), dim3((unsigned)tiles), dim3(256), 0, st, g);
+    }
+    return hipGetLastError();
+}
+
+// Backward.  Large: dg and du are written both ways round, x and the weights transposed, so that every product contracts along
+// rows; these copies are a few per cent of the products' time.
+struct BackwardPlan {
+    bool fast = false;
+    int tile_x = 128, tile_w = 128, splits_x = 1, splits_w = 1;
+    int64_t hp = 0, mp = 0;
+    int64_t d_bytes = 0, dt_bytes = 0, xt_bytes = 0, wt_bytes = 0, part_bytes = 0;
+    int64_t bytes() const { return 2 * d_bytes + 2 * dt_bytes + xt_bytes + 2 * wt_bytes + part_bytes; }
+};
+template <typename T>
+BackwardPlan backward_plan(int64_t m, int64_t k, int64_t h) {
+    constexpr int KS = STEP_BYTES / sizeof(T);
+    constexpr int64_t B = sizeof(T);
+    BackwardPlan p;
+    p.fast = m >= 128 && h >= 128 && k >= 64 && 8 * m * h * k >= (int64_t)1 << 32 && m * B < (1 << 23) && h * B < (1 << 23);
+    if (p.fast) {
+        p.hp = round_up(h, 64), p.mp = round_up(m, 64);
+        auto choose = [&](int64_t rows, int64_t cols, int64_t zs, int64_t steps, int& tile, int& splits) {
+            const int64_t t256 = zs * ceil_div(rows, 256) * ceil_div(cols, 256), t128 = zs * ceil_div(rows, 128) * ceil_div(cols, 128);
+            tile = t256 >= 256 ? 256 : 128;
+            splits = tile == 256 || t128 >= 256 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(512, t128), steps / 8));
+        };
+        choose(m, k, 1, p.hp / KS, p.tile_x, p.splits_x);
+        choose(h, k, 2, p.mp / KS, p.tile_w, p.splits_w);
+        p.d_bytes = round_up(m * p.hp * B, 256), p.dt_bytes = round_up(h * p.mp * B, 256);
+        p.xt_bytes = round_up(k * p.mp * B, 256), p.wt_bytes = round_up(k * p.hp * B, 256);
+    } else {
+        p.d_bytes = round_up(m * h * B, 256);
+        p.splits_x = gated_splits(ceil_div(m, TB) * ceil_div(k, TB), h, KS);
+        p.splits_w = gated_splits(2 * ceil_div(h, TB) * ceil_div(k, TB), m, KS);
+    }
+    p.part_bytes = std::max<int64_t>(p.splits_x > 1 ? p.splits_x * m * k * 4 : 0, p.splits_w > 1 ? 2 * p.splits_w * h * k * 4 : 0);
+    return p;
+}
+
+template <typename T>
+hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const void* x, int64_t xs, const void* wg, const void* wu, int64_t ws,
+                          const float* kg, const float* ku, int64_t m, int64_t k, int64_t h, int act, void* dx, int64_t dxs, void* dwg,
+                          void* dwu, int64_t dws, char* work) {
+    const BackwardPlan p = backward_plan<T>(m, k, h);
+    char* at = work;
+    auto take = [&](int64_t bytes) { char* r = at; at += bytes; return r; };
+    T *dg = (T*)take(p.d_bytes), *du = (T*)take(p.d_bytes), *dgt = (T*)take(p.dt_bytes), *dut = (T*)take(p.dt_bytes), *xt = (T*)take(p.xt_bytes),
+      *wgt = (T*)take(p.wt_bytes), *wut = (T*)take(p.wt_bytes);
+    float* part = (float*)take(p.part_bytes);
+    if (p.fast) {
+        hipLaunchKernelGGL(k_gated_slopes_both<T>, dim3((unsigned)(p.mp / 64 * (p.hp / 64))), dim3(256), 0, st, (const T*)dh, dhs, kg, ku, m, h, act,
+                           dg, du, p.hp, dgt, dut, p.mp);
+        PackArgs a{};
+        if (dwg) a.job[a.count++] = {x, xs, m, k, xt, p.mp, p.mp / 64 * ceil_div(k, 64)};
+        if (dx) {
+            a.job[a.count++] = {wg, ws, h, k, wgt, p.hp, p.hp / 64 * ceil_div(k, 64)};
+            a.job[a.count++] = {wu, ws, h, k, wut, p.hp, p.hp / 64 * ceil_div(k, 64)};
+        }
+        int64_t blocks = 0;
+        for (int i = 0; i < a.count; ++i) blocks += a.job[i].blocks;
+        if (blocks) hipLaunchKernelGGL((k_gated_pack<T, true>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    } else if (m > 0) {
+        const int64_t packs = m * ceil_div(h, Pack<T>::N);
+        hipLaunchKernelGGL(k_gated_slopes<T>, dim3((unsigned)std::min<int64_t>(ceil_div(packs, 256), 8192)), dim3(256), 0, st, (const T*)dh, dhs,
+                           kg, ku, m, h, act, dg, du);
+    }
+    if (dx && m > 0) {
+        GatedArgs g{};
+        g.m = m, g.n = k, g.out[0] = dx, g.os = dxs, g.splits = p.splits_x, g.part = part;
+        if (p.fast) {
+            g.a[0] = {dg, p.hp, 1}, g.a[1] = {du, p.hp, 1}, g.b[0] = {wgt, p.hp, 1}, g.b[1] = {wut, p.hp, 1}, g.k = p.hp;
+            launch_fast<T, GATED_SUM>(st, g, p.tile_x);
+        } else {
+            g.a[0] = {dg, h, 1}, g.a[1] = {du, h, 1}, g.b[0] = {wg, 1, ws}, g.b[1] = {wu, 1, ws}, g.k = h;
+            hipLaunchKernelGGL((k_gated_tile<T, GATED_SUM, true, false>), dim3((unsigned)(ceil_div(m, TB) * ceil_div(k, TB)), (unsigned)g.splits),
+                               dim3(256), 0, st, g);
+        }
+        if (g.splits > 1) hipLaunchKernelGGL(k_gated_join<T>, dim3((unsigned)ceil_div(m * k, 256), 1), dim3(256), 0, st, g);
+    }
+    if (dwg) {
+        GatedArgs g{};
+        g.m = h, g.n = k, g.out[0] = dwg, g.out[1] = dwu, g.os = dws, g.splits = p.splits_w, g.part = part;
+        if (p.fast) {
+            g.a[0] = {dgt, p.mp, 1}, g.a[1] = {dut, p.mp, 1}, g.b[0] = g.b[1] = {xt, p.mp, 1}, g.k = p.mp;
+            launch_fast<T, GATED_PAIR>(st, g, p.tile_w);
+        } else {
+            g.a[0] = {dg, 1, h}, g.a[1] = {du, 1, h}, g.b[0] = g.b[1] = {x, 1, xs}, g.k = m;
+            hipLaunchKernelGGL((k_gated_tile<T, GATED_PAIR, false, false>), dim3((unsigned)(ceil_div(h, TB) * ceil_div(k, TB)), (unsigned)g.splits, 2),
+                               dim3(256), 0, st, g);
+        }
+        if (g.splits > 1) hipLaunchKernelGGL(k_gated_join<T>, dim3((unsigned)ceil_div(h * k, 256), 2), dim3(256), 0, st, g);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace gpbo_static

@@ -178,6 +178,14 @@ def test_gated_unit_forward_and_backward(dtype, act, rows, cols, hidden):
     check_gated(dtype, act, rows, cols, hidden)
 
 
+# large enough for the kernels that load straight into LDS, both tile sizes, whole and broken steps, split contractions, edges
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('rows,cols,hidden', [(1100, 1024, 1000), (2050, 621, 777), (300, 4096, 1030), (128, 2048, 2111), (4100, 520, 2049), (2305, 1024, 4224), (20000, 64, 128),
+                                              (129, 8192, 640), (8200, 640, 1024)])
+def test_gated_unit_large(dtype, rows, cols, hidden):
+    check_gated(dtype, 'gelu' if rows % 2 else 'silu', rows, cols, hidden)
+
+
 def check_gated(dtype, act, rows, cols, hidden):
     from bayesian_optimization_amd import features
     x, dh = rand((rows, cols), dtype, 1), rand((rows, hidden), dtype, 2)
@@ -212,7 +220,7 @@ def check_gated(dtype, act, rows, cols, hidden):
 @pytest.mark.parametrize('dtype', TYPES)
 def test_gated_unit_takes_strided_and_unaligned_arrays(dtype):
     from bayesian_optimization_amd import features
-    for rows, cols, hidden in ((70, 129, 77), (300, 256, 384)):
+    for rows, cols, hidden in ((70, 129, 77), (300, 256, 384), (1030, 1000, 1100), (1030, 1024, 1100)):
         x = rand((2 * rows, cols + 9), dtype, 21)[::2, 3:3 + cols]
         wg, wu = (rand((hidden, cols + 5), dtype, s, 0.1)[:, 1:1 + cols] for s in (22, 23))
         dh = rand((rows, hidden + 3), dtype, 24)[:, 2:2 + hidden]
@@ -295,7 +303,7 @@ def test_gated_unit_offsets_past_32_bits():
 def test_operators_repeat_bit_for_bit_and_replay_from_a_graph(dtype):
     """Captured once, replayed on new inputs in the same buffers with eager work in between; every replay equals the eager call."""
     from bayesian_optimization_amd import features
-    for rows, cols, hidden in ((95, 621, 128), (512, 512, 256)):
+    for rows, cols, hidden in ((95, 621, 128), (512, 512, 256), (1100, 1000, 1024)):
         x, dh = rand((rows, cols), dtype, 61), rand((rows, hidden), dtype, 62)
         w, wg, wu = rand((cols,), dtype, 63), rand((hidden, cols), dtype, 64, 0.05), rand((hidden, cols), dtype, 65, 0.05)
 
