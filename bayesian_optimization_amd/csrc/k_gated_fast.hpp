@@ -201,14 +201,14 @@ __global__ __launch_bounds__(256) void k_gated_pack(PackArgs a) {
     T* dst = (T*)jb.dst;
     const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
     // the grid covers the padded destination: destination columns are source columns, or (transposed) source rows
-    const int64_t tiles_c = TRANSPOSE ? (jb.cols + 63) / 64 : jb.pitch / 64;
+    const int64_t tiles_c = ((TRANSPOSE ? jb.cols : jb.pitch) + 63) / 64;
     const int64_t r0 = id / tiles_c * 64, c0 = id % tiles_c * 64;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int64_t r = r0 + ty + i * 4, c = c0 + tx;
         const T v = r < jb.rows && c < jb.cols ? src[r * jb.stride + c] : from_float<T>(0.0f);
         if constexpr (TRANSPOSE) tile[ty + i * 4][tx] = v;
-        else if (r < jb.rows) dst[r * jb.pitch + c] = v;
+        else if (r < jb.rows && c < jb.pitch) dst[r * jb.pitch + c] = v;
     }
     if constexpr (TRANSPOSE) {
         __syncthreads();
