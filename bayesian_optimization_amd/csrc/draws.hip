@@ -14,7 +14,12 @@ extern "C" {
 
 int64_t gpbo_draw_static_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_t draws) {
     if (type_bytes(dtype) == 0 || rows < 0 || rows > MOST_ROWS || cols < 1 || cols > MOST_COLS || draws < 0 || draws > MOST_ROWS) return -1;
-    return 0;
+    switch (dtype) {
+        case GPBO_TYPE_F64: return draw_work_bytes<double>(rows, cols);
+        case GPBO_TYPE_F32: return draw_work_bytes<float>(rows, cols);
+        case GPBO_TYPE_BF16: return draw_work_bytes<bf16>(rows, cols);
+        default: return draw_work_bytes<f16>(rows, cols);
+    }
 }
 
 int gpbo_draw_static(int32_t device, void* stream, int32_t dtype, const void* scores, int64_t score_stride, int64_t rows,
@@ -37,10 +42,10 @@ int gpbo_draw_static(int32_t device, void* stream, int32_t dtype, const void* sc
     const hipStream_t st = (hipStream_t)stream;
     hipError_t e;
     switch (dtype) {
-        case GPBO_TYPE_F64: e = draw_rows<double>(st, a); break;
-        case GPBO_TYPE_F32: e = draw_rows<float>(st, a); break;
-        case GPBO_TYPE_BF16: e = draw_rows<bf16>(st, a); break;
-        default: e = draw_rows<f16>(st, a); break;
+        case GPBO_TYPE_F64: e = draw_rows<double>(st, a, (char*)workspace); break;
+        case GPBO_TYPE_F32: e = draw_rows<float>(st, a, (char*)workspace); break;
+        case GPBO_TYPE_BF16: e = draw_rows<bf16>(st, a, (char*)workspace); break;
+        default: e = draw_rows<f16>(st, a, (char*)workspace); break;
     }
     return e == hipSuccess ? GPBO_OK : GPBO_ERR_HIP;
 }

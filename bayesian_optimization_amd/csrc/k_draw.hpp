@@ -3,11 +3,15 @@
 //   rank: falling score, rising index on ties.  Kept: the first top_k; of those w_i >= min_p; of those position p as long as
 //   the mass in front of it is < top_p times their mass (the first always).
 //   pick(u): the lowest kept i, in index order, with C_i > u Z;  C the running sum of kept w, Z their mass;  logp = t_i - log Z.
-// No sort of the row: the kept set is { score > cut } plus the first few, by index, of those equal to the cut, and the cut is
-// found digit by digit.  A score's bits are mapped to an unsigned key of the same order; a histogram over 11 bits of it, counts
-// for top-k, masses for top-p, names the digit that holds the cut, until at most LIST keys are left to be ranked against each
-// other.  Counts are integers, and the masses of a histogram are integers too (two words of 35 bits behind the point each), so
-// that the order in which atomics arrive changes nothing; all other sums are in 64 bits in a fixed order.
+// No sort of the row: the kept set is { score > cut } plus the first few, by index, of those equal to the cut.  The cut is found by
+// histograms of 2048 bins, counts for top-k, masses for top-p: the first one linear in the score, which spreads what lies near
+// the best over many bins, the next ones of the integer range of keys that is left (a score's bits, mapped to an unsigned key of
+// the same order), until at most LIST keys remain to be ranked against each other; where that list holds all that can be kept,
+// the rest of the work is done on it alone.  Counts are integers, and so are the masses of a histogram (two words of 35 bits
+// each), so that the order in which atomics arrive changes nothing; all other sums are in 64 bits in a fixed order.
+// Bound by memory: a pass over the row per step, two to five of them, and by the exponential of every score of a top-p step.
+// Short rows: one workgroup a row does everything (k_draw_row).  Long rows: the same steps with many workgroups a row, one
+// launch a step, the state of a row in the workspace; the last workgroup to arrive at a step takes its decision.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -30,6 +34,11 @@ struct Score {
         const uint32_t b = __float_as_uint(f);
         return (b >> 31) ? ~b : (b | 0x80000000u);
     }
+    static __device__ __forceinline__ Key key_of(double v) {      // of the nearest 32-bit number
+        const float f = (float)v + 0.0f;
+        const uint32_t b = __float_as_uint(f);
+        return !(f > -INFINITY) ? 0 : (b >> 31) ? ~b : (b | 0x80000000u);
+    }
     static __device__ __forceinline__ double value(Key k) {
         return (double)__uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k);
     }
@@ -44,6 +53,7 @@ struct Score<double> {
         const uint64_t b = (uint64_t)__double_as_longlong(f);
         return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
     }
+    static __device__ __forceinline__ Key key_of(double v) { return key(v); }
     static __device__ __forceinline__ double value(Key k) {
         return __longlong_as_double((long long)((k >> 63) ? (k & 0x7fffffffffffffffull) : ~k));
     }
@@ -121,6 +131,60 @@ __device__ __forceinline__ V block_scan(V v, V* red, V& total) {
     return before + v;
 }
 
+// Where the search for the cut stands.  Lives in LDS (one workgroup a row) or in the workspace (many).
+enum { PHASE_TOPK = 0, PHASE_TOPP = 1, PHASE_PICK = 2, PHASE_DONE = 3 };
+template <typename T>
+struct DrawState {
+    using Key = typename Score<T>::Key;
+    Key top, bot;                 // best and lowest valid key
+    Key klo, khi;                 // the cut lies among keys klo .. khi (and in linear bin lin_bin, if lin == 2)
+    Key cut, floor_key;           // PHASE_TOPP: the cut of top-k, whose ties are one group below all other keys
+    double scale;                 // linear bins per score
+    double above, goal;           // PHASE_TOPP: mass above khi; mass to reach
+    double floor_mass;
+    long long rank;               // PHASE_TOPK: how many of klo .. khi are kept
+    long long count_above;        // keys above khi that may be kept
+    int phase, lin, lin_bin;      // lin: 0 no linear step, 1 this step is linear, 2 it has been
+    int gather, gather_all;       // this step collects the list; all keys from klo up, or klo .. khi only
+    uint32_t cut_ties, floor_ties, best_idx;
+    unsigned int n_list, ticket;
+};
+
+// What of a score counts in the present step; w is its weight (PHASE_TOPP).
+template <typename T>
+struct DrawStep {
+    using S = Score<T>;
+    using Key = typename S::Key;
+    Key top, klo, khi, floor_key;
+    double smax, scale, min_p, temperature;
+    int phase, lin, lin_bin, gather_all, shift;
+    __device__ __forceinline__ DrawStep(const DrawState<T>& st, const DrawRow& p)
+        : top(st.top), klo(st.klo), khi(st.khi), floor_key(st.floor_key), smax(S::value(st.top)), scale(st.scale), min_p(p.min_p),
+          temperature(p.temperature), phase(st.phase), lin(st.lin), lin_bin(st.lin_bin), gather_all(st.gather_all) {
+        const Key width = khi - klo;
+        const int bits = width == 0 ? 0 : S::BITS == 64 ? 64 - __clzll((long long)width) : 32 - __clz((int)width);
+        shift = bits > DIGIT ? bits - DIGIT : 0;
+    }
+    __device__ __forceinline__ int linear(Key k) const {
+        const double v = (smax - S::value(k)) * scale;
+        return v >= (double)(BINS - 1) ? BINS - 1 : (int)v;
+    }
+    __device__ __forceinline__ bool counts(Key k, double& w) const {
+        if (k < klo || k == 0 || (k > khi && !gather_all)) return false;
+        if (lin == 2) {
+            const int b = linear(k);
+            if (gather_all ? b > lin_bin : b != lin_bin) return false;
+        }
+        if (phase == PHASE_TOPP) {
+            if (k <= floor_key) return false;
+            w = exp(draw_t<T>(k, top, temperature));
+            return w >= min_p;
+        }
+        return true;
+    }
+    __device__ __forceinline__ int bin(Key k) const { return lin == 1 ? linear(k) : (int)((khi - k) >> shift); }
+};
+
 template <typename T>
 struct DrawLds {
     using Key = typename Score<T>::Key;
@@ -140,26 +204,235 @@ struct DrawLds {
             uint32_t ties[TILES];              // scores equal to the cut in front of a tile
         } t;
     };
+    DrawState<T> st;
     double red[32];
     unsigned long long red_u[32];
-    Key best_key[16];
-    uint32_t best_idx[16];
-    Key cut;
-    uint32_t cut_ties, n_list, pick_bin;
-    unsigned int bin_count;
-    double above, target;
-    long long rank_left;
+    Key red_k[2][16];
+    uint32_t red_i[16];
+    unsigned int bin, any_bin, last;
 };
 
-// Everything behind the list: n <= LIST (key, index) pairs in l.key, l.idx that hold every score that can be kept.
+// Every score of elements [begin, end) of a row, 16 bytes a load, the workgroup's threads side by side: f(key, index).
+template <typename T, typename F>
+__device__ __forceinline__ void each_score(const T* x, uint32_t begin, uint32_t end, F&& f) {
+    constexpr uint32_t V = Pack<T>::N;
+    const uint32_t packs = (end - begin) / V;
+    for (uint32_t c = threadIdx.x; c < packs; c += DRAW_THREADS) {
+        const Pack<T> p = load_pack(x + begin + c * V);
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i) f(Score<T>::key(p.v[i]), begin + c * V + i);
+    }
+    for (uint32_t i = begin + packs * V + threadIdx.x; i < end; i += DRAW_THREADS) f(Score<T>::key(x[i]), i);
+}
+
+// Best key with its lowest index, and lowest valid key, of [begin, end).
 template <typename T>
-__device__ void draw_from_list(DrawLds<T>& s, const DrawArgs& a, const DrawRow& p, int64_t row, int n, typename Score<T>::Key top) {
+__device__ void draw_extremes(DrawLds<T>& s, const T* x, uint32_t begin, uint32_t end, typename Score<T>::Key& top, typename Score<T>::Key& bot, uint32_t& idx) {
+    using Key = typename Score<T>::Key;
+    Key bk = 0, lk = ~(Key)0;
+    uint32_t bi = 0;
+    each_score(x, begin, end, [&](Key k, uint32_t i) {
+        if (k > bk) bk = k, bi = i;            // a thread meets its indices in rising order, up to the tail's
+        if (k != 0 && k < lk) lk = k;
+    });
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const Key k = __shfl_xor(bk, o), l = __shfl_xor(lk, o);
+        const uint32_t i = __shfl_xor(bi, o);
+        if (k > bk || (k == bk && i < bi)) bk = k, bi = i;
+        if (l < lk) lk = l;
+    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (lane == 0) s.red_k[0][wave] = bk, s.red_k[1][wave] = lk, s.red_i[wave] = bi;
+    __syncthreads();
+    top = 0, bot = ~(Key)0, idx = 0;
+    for (int i = 0; i < DRAW_THREADS / 64; ++i) {
+        const Key k = s.red_k[0][i];
+        if (k > top || (k == top && s.red_i[i] < idx)) top = k, idx = s.red_i[i];
+        if (s.red_k[1][i] < bot) bot = s.red_k[1][i];
+    }
+    __syncthreads();
+}
+
+// Nothing to choose: no valid score (index -1), or the best one.
+template <typename T>
+__device__ void draw_same(const DrawArgs& a, int64_t row, int64_t index, double logp) {
+    for (int64_t q = threadIdx.x; q < a.draws; q += DRAW_THREADS) {
+        a.index[row * a.draws + q] = index;
+        if (a.logp) a.logp[row * a.draws + q] = logp;
+    }
+}
+
+// Thread 0: the first step of a phase, or the next phase that has any.
+template <typename T>
+__device__ void draw_begin(DrawState<T>& st, const DrawRow& p, int phase) {
+    using S = Score<T>;
+    if (phase == PHASE_TOPK && p.top_k == 0) phase = PHASE_TOPP;
+    if (phase == PHASE_TOPP && !(p.top_p < 1.0)) phase = PHASE_PICK;
+    st.phase = phase;
+    if (phase >= PHASE_PICK) return;
+    st.klo = st.bot, st.khi = st.top;
+    st.above = st.goal = st.floor_mass = 0.0;
+    st.count_above = 0;
+    st.rank = p.top_k;
+    st.gather = st.gather_all = 0;
+    st.floor_key = 0, st.floor_ties = 0;
+    double span = S::value(st.top) - S::value(st.bot);
+    if (phase == PHASE_TOPP) {
+        st.floor_key = st.cut, st.floor_ties = st.cut_ties;
+        if (st.floor_ties) {
+            const double w = exp(draw_t<T>(st.floor_key, st.top, p.temperature));
+            if (w >= p.min_p) st.floor_mass = w * st.floor_ties;
+        }
+        span = fmin(span, 48.0 * p.temperature);      // e^-48: below what a histogram's fixed point resolves
+    }
+    st.scale = (double)(BINS - 1) / span;
+    st.lin = span > 0.0 && span < INFINITY && st.scale < INFINITY && st.scale > 0.0;
+}
+
+// A step's histogram over [begin, end) into LDS.  The last bin of the linear step, where all that lies far from the best falls, is
+// summed in registers: thousands of atomics on one address would take their turns.
+template <typename T>
+__device__ void draw_histogram(DrawLds<T>& s, const DrawStep<T>& d, const T* x, uint32_t begin, uint32_t end) {
+    using Key = typename Score<T>::Key;
+    for (int b = threadIdx.x; b < BINS; b += DRAW_THREADS) s.h.count[b] = 0, s.h.hi[b] = 0, s.h.lo[b] = 0;
+    __syncthreads();
+    unsigned int rest = 0;
+    unsigned long long rest_hi = 0, rest_lo = 0;
+    each_score(x, begin, end, [&](Key k, uint32_t) {
+        double w = 0.0;
+        if (!d.counts(k, w)) return;
+        const int b = d.bin(k);
+        unsigned long long hi = 0, lo = 0;
+        if (d.phase == PHASE_TOPP) to_fixed(w, hi, lo);
+        if (d.lin == 1 && b == BINS - 1) {
+            rest += 1, rest_hi += hi, rest_lo += lo;
+        } else {
+            atomicAdd(&s.h.count[b], 1u);
+            if (hi) atomicAdd(&s.h.hi[b], hi);
+            if (lo) atomicAdd(&s.h.lo[b], lo);
+        }
+    });
+    if (d.lin == 1) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            rest += __shfl_xor(rest, o);
+            rest_hi += __shfl_xor(rest_hi, o);
+            rest_lo += __shfl_xor(rest_lo, o);
+        }
+        if ((threadIdx.x & 63) == 0 && rest) {
+            atomicAdd(&s.h.count[BINS - 1], rest);
+            atomicAdd(&s.h.hi[BINS - 1], rest_hi);
+            atomicAdd(&s.h.lo[BINS - 1], rest_lo);
+        }
+    }
+    __syncthreads();
+}
+
+// The whole histogram of a step is in LDS: find the bin that holds the cut and move the state there.
+template <typename T>
+__device__ void draw_decide(DrawLds<T>& s, const DrawRow& p) {
+    using S = Score<T>;
+    using Key = typename S::Key;
+    const int tid = threadIdx.x, b0 = 2 * tid, b1 = b0 + 1;      // bins from the top down
+    DrawState<T>& st = s.st;
+    const DrawStep<T> d(st, p);
+    const bool first = st.lin == 1 || (st.lin == 0 && st.klo == st.bot && st.khi == st.top);
+    if (tid == 0) s.bin = 0xffffffffu, s.any_bin = 0;
+    const unsigned long long c0 = s.h.count[b0], c1 = s.h.count[b1];
+    unsigned long long all_c;
+    const unsigned long long run_c = block_scan(c0 + c1, s.red_u, all_c);      // up to and with this thread's bins
+    bool spare = false;
+    double m0 = 0.0, m1 = 0.0, run_m = 0.0, all_m = 0.0, goal = st.goal;
+    const double above = st.above;
+    const long long rank = st.rank;
+    if (st.phase == PHASE_TOPK) {
+        spare = first && all_c <= (unsigned long long)rank;                    // fewer valid scores than top_k: no cut
+        const long long before = (long long)(run_c - c0 - c1);
+        if (c0 && before < rank && before + (long long)c0 >= rank) s.bin = b0;
+        if (c1 && before + (long long)c0 < rank && before + (long long)(c0 + c1) >= rank) s.bin = b1;
+    } else {
+        m0 = from_fixed(s.h.hi[b0], s.h.lo[b0]), m1 = from_fixed(s.h.hi[b1], s.h.lo[b1]);
+        run_m = block_scan(m0 + m1, s.red, all_m);
+        if (first) goal = p.top_p * (all_m + st.floor_mass);
+        spare = first && !(all_m >= goal);                                     // all above the group of the top-k cut is kept
+        // the first bin with which the running mass reaches the goal; the last one in use if rounding leaves none
+        if (c1 && above + run_m >= goal) atomicMin(&s.bin, (unsigned)b1);
+        if (c0 && above + (run_m - m1) >= goal) atomicMin(&s.bin, (unsigned)b0);
+        if (c1) atomicMax(&s.any_bin, (unsigned)b1);
+        else if (c0) atomicMax(&s.any_bin, (unsigned)b0);
+    }
+    __syncthreads();
+    const unsigned bin = s.bin != 0xffffffffu ? s.bin : s.any_bin;
+    if (spare) {
+        if (tid == 0) {
+            if (st.phase == PHASE_TOPK) {
+                st.cut = 0, st.cut_ties = 0;
+                draw_begin(st, p, PHASE_TOPP);
+            } else {                           // of the group, as many as the mass still asks for
+                st.cut = st.floor_key;
+                st.cut_ties = 0;
+                if (st.floor_ties) {
+                    const double w = exp(draw_t<T>(st.floor_key, st.top, p.temperature));
+                    const double r = w > 0.0 ? ceil((goal - all_m) / w) : 0.0;
+                    st.cut_ties = (uint32_t)fmin(fmax(r, 0.0), (double)st.floor_ties);
+                }
+                st.phase = PHASE_PICK;
+            }
+        }
+    } else if (bin == (unsigned)b0 || bin == (unsigned)b1) {
+        const bool low = bin == (unsigned)b1;
+        const unsigned long long cnt = low ? c1 : c0, before_c = run_c - (low ? c1 : c0 + c1);
+        if (st.lin == 1) {
+            // keys that can fall into the bin: its ends, moved out by more than the rounding of either side
+            const double smax = S::value(st.top);
+            const double hi_s = smax - bin / st.scale * (1.0 - 1e-14), lo_s = smax - (bin + 1) / st.scale * (1.0 + 1e-14);
+            const Key kh = S::key_of(hi_s), kl = S::key_of(lo_s);
+            if (bin > 0 && kh != 0 && st.top - kh > 2) st.khi = kh + 2;
+            if (bin < BINS - 1 && kl != 0 && kl > st.bot && kl - st.bot > 2) st.klo = kl - 2;
+            st.lin = 2, st.lin_bin = (int)bin;
+        } else {
+            const Key hi = st.khi - ((Key)bin << d.shift), span = ((Key)1 << d.shift) - 1;
+            st.klo = hi - st.klo > span ? hi - span : st.klo;
+            st.khi = hi;
+        }
+        st.count_above += (long long)before_c;
+        if (st.phase == PHASE_TOPK) {
+            st.rank = rank - (long long)before_c;
+        } else {
+            st.goal = goal;
+            st.above = above + (low ? run_m - m1 : run_m - m1 - m0);
+        }
+        if (st.klo == st.khi) {                // one key: all of them ties
+            st.cut = st.klo;
+            if (st.phase == PHASE_TOPK) {
+                st.cut_ties = (uint32_t)st.rank;
+                draw_begin(st, p, PHASE_TOPP);
+            } else {
+                const double w = exp(draw_t<T>(st.cut, st.top, p.temperature));
+                const double r = ceil((st.goal - st.above) / w);
+                st.cut_ties = (uint32_t)fmin(r >= 1.0 ? r : 1.0, (double)cnt);
+                st.phase = PHASE_PICK;
+            }
+        } else if (st.count_above + (long long)cnt <= LIST) {
+            st.gather = st.gather_all = 1;
+        } else if (cnt <= LIST) {
+            st.gather = 1;
+        }
+        st.n_list = 0;
+    }
+    __syncthreads();
+}
+
+// LIST keys or fewer in l.key, l.idx: sort them by rank into l.key2, l.idx2.
+template <typename T>
+__device__ void draw_rank(DrawLds<T>& s, int n) {
     using Key = typename Score<T>::Key;
     const int tid = threadIdx.x;
     __syncthreads();
-    const Key k = tid < n ? s.l.key[tid] : 0;
-    const uint32_t ix = tid < n ? s.l.idx[tid] : 0;
     if (tid < n) {
+        const Key k = s.l.key[tid];
+        const uint32_t ix = s.l.idx[tid];
         int rank = 0;
         for (int j = 0; j < n; ++j) {
             const Key kj = s.l.key[j];
@@ -169,15 +442,54 @@ __device__ void draw_from_list(DrawLds<T>& s, const DrawArgs& a, const DrawRow& 
         s.l.idx2[rank] = ix;
     }
     __syncthreads();
+}
+
+// The list holds the keys klo .. khi of a step: the cut is one of them.
+template <typename T>
+__device__ void draw_cut_from_list(DrawLds<T>& s, const DrawRow& p, int n) {
+    using Key = typename Score<T>::Key;
+    const int tid = threadIdx.x;
+    DrawState<T>& st = s.st;
+    draw_rank(s, n);
+    const Key k = tid < n ? s.l.key2[tid] : 0;
+    bool in;
+    if (st.phase == PHASE_TOPK) {
+        in = tid < st.rank;
+    } else {
+        const double w = k ? exp(draw_t<T>(k, st.top, p.temperature)) : 0.0;
+        double all;
+        const double incl = block_scan(w, s.red, all);
+        in = k != 0 && (tid == 0 || st.above + (incl - w) < st.goal);
+    }
+    unsigned long long taken, same;
+    block_scan<unsigned long long>(in ? 1ull : 0ull, s.red_u, taken);
+    const Key cut = s.l.key2[taken ? (int)taken - 1 : 0];
+    block_scan<unsigned long long>(in && k == cut ? 1ull : 0ull, s.red_u, same);
+    __syncthreads();
+    if (tid == 0) {
+        st.cut = cut, st.cut_ties = (uint32_t)same;
+        if (st.phase == PHASE_TOPK) draw_begin(st, p, PHASE_TOPP);
+        else st.phase = PHASE_PICK;
+    }
+    __syncthreads();
+}
+
+// Everything behind the list: n <= LIST pairs that hold every score that can be kept.  goal < 0: top_p of the mass that top-k and
+// min-p leave; else the mass to reach.
+template <typename T>
+__device__ void draw_from_list(DrawLds<T>& s, const DrawArgs& a, const DrawRow& p, int64_t row, int n, typename Score<T>::Key top, double goal) {
+    using Key = typename Score<T>::Key;
+    const int tid = threadIdx.x;
+    draw_rank(s, n);
     // by rank from here on: thread = position
     const Key kr = tid < n ? s.l.key2[tid] : 0;
     const double w = kr ? exp(draw_t<T>(kr, top, p.temperature)) : 0.0;
     bool keep = kr != 0 && (p.top_k == 0 || tid < p.top_k) && w >= p.min_p;
     double total;
-    double run = block_scan(keep ? w : 0.0, s.red, total);
+    const double run = block_scan(keep ? w : 0.0, s.red, total);
     if (p.top_p < 1.0) {
-        keep = keep && (tid == 0 || run - w < p.top_p * total);
-        __syncthreads();
+        if (goal < 0.0) goal = p.top_p * total;
+        keep = keep && (tid == 0 || run - w < goal);
     }
     // the kept ones are the first `kept` positions; now in index order
     unsigned long long kept;
@@ -186,8 +498,7 @@ __device__ void draw_from_list(DrawLds<T>& s, const DrawArgs& a, const DrawRow& 
     int place = 0;
     if (keep)
         for (int j = 0; j < (int)kept; ++j) place += s.l.idx2[j] < my;
-    __syncthreads();
-    if (keep) {
+    if (keep) {                                // l.key was last read by draw_rank, l.c and l.pick not at all
         s.l.c[place] = w;
         s.l.pick[place] = my;
         s.l.key[place] = kr;
@@ -195,15 +506,14 @@ __device__ void draw_from_list(DrawLds<T>& s, const DrawArgs& a, const DrawRow& 
     __syncthreads();
     const double wi = tid < (int)kept ? s.l.c[tid] : 0.0;
     const double ci = block_scan(wi, s.red, total);
-    __syncthreads();
     if (tid < (int)kept) s.l.c[tid] = ci;
     __syncthreads();
     for (int64_t q = tid; q < a.draws; q += DRAW_THREADS) {
-        const double goal = fmax(a.u[row * a.draws + q], 0.0) * total;
-        int lo = 0, hi = (int)kept - 1;        // the first c > goal; the last kept one if rounding leaves none
+        const double at = fmax(a.u[row * a.draws + q], 0.0) * total;
+        int lo = 0, hi = (int)kept - 1;        // the first c > at; the last kept one if rounding leaves none
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (s.l.c[mid] > goal) hi = mid;
+            if (s.l.c[mid] > at) hi = mid;
             else lo = mid + 1;
         }
         // a weight of zero is never drawn: step back over those at the end
@@ -213,7 +523,102 @@ __device__ void draw_from_list(DrawLds<T>& s, const DrawArgs& a, const DrawRow& 
     }
 }
 
-// One workgroup a row.
+// The weights of a row once the cut is known.
+template <typename T>
+struct DrawKept {
+    using S = Score<T>;
+    using Key = typename S::Key;
+    Key top, cut;
+    double temperature, min_p, tie_w;
+    __device__ __forceinline__ DrawKept(const DrawState<T>& st, const DrawRow& p) : top(st.top), cut(st.cut), temperature(p.temperature), min_p(p.min_p) {
+        const double w = cut ? exp(draw_t<T>(cut, top, temperature)) : 0.0;
+        tie_w = w >= min_p ? w : 0.0;
+    }
+    __device__ __forceinline__ double strict(Key k) const {      // weight of a key above the cut
+        if (k <= cut) return 0.0;              // (an invalid score's key is 0)
+        const double w = exp(draw_t<T>(k, top, temperature));
+        return w >= min_p ? w : 0.0;
+    }
+};
+
+// One wave: mass above the cut, and ties with the cut, of elements [begin, end).
+template <typename T>
+__device__ void draw_tile_mass(const DrawKept<T>& kw, const T* x, uint32_t begin, uint32_t end, double& mass, uint32_t& ties) {
+    using Key = typename Score<T>::Key;
+    constexpr uint32_t V = Pack<T>::N;
+    const uint32_t lane = threadIdx.x & 63;
+    double m = 0.0;
+    uint32_t c = 0;
+    auto one = [&](T v) {
+        const Key k = Score<T>::key(v);
+        m += kw.strict(k);
+        c += k == kw.cut && k != 0;
+    };
+    for (uint32_t i = begin + lane * V; i < end; i += 64 * V) {
+        if (i + V <= end) {
+            const Pack<T> p = load_pack(x + i);
+#pragma unroll
+            for (uint32_t j = 0; j < V; ++j) one(p.v[j]);
+        } else {
+            for (uint32_t j = i; j < end; ++j) one(x[j]);
+        }
+    }
+    mass = wave_sum(m);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o);
+    ties = c;
+}
+
+// One wave: the pick inside [begin, end), of at most 64 * 64 elements, for mass `goal` with `run` in front of it and `ties` of the
+// cut's ties already met (of which cut_ties are kept).  A lane sums a run of neighbours, the lane that holds the goal is found
+// by a scan over the lanes, and then its run is spread over the lanes.
+template <typename T>
+__device__ int64_t draw_in_tile(const DrawKept<T>& kw, const T* x, uint32_t begin, uint32_t end, double run, uint32_t ties, uint32_t cut_ties, double goal) {
+    using Key = typename Score<T>::Key;
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t each = (end - begin + 63) / 64;
+    int64_t pick = -1;
+    for (int stage = 0; stage < 2; ++stage) {
+        const uint32_t b = min(end, begin + lane * each), e = min(end, b + each);
+        double m = 0.0;
+        uint32_t c = 0;
+        for (uint32_t i = b; i < e; ++i) {
+            const Key k = Score<T>::key(x[i]);
+            m += kw.strict(k);
+            c += k == kw.cut && k != 0;
+        }
+        uint32_t before = c;                   // ties in front of this lane
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t v = __shfl_up(before, o);
+            if (lane >= (uint32_t)o) before += v;
+        }
+        before += ties - c;
+        const uint32_t kept = before >= cut_ties ? 0 : min(c, cut_ties - before);
+        m += kept * kw.tie_w;
+        double incl = m;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const double v = __shfl_up(incl, o);
+            if (lane >= (uint32_t)o) incl += v;
+        }
+        const unsigned long long any = __ballot(m > 0.0), hit = __ballot(m > 0.0 && run + incl > goal);
+        if (!any) return pick;                 // cannot be: the tile was chosen for its mass
+        const int at = hit ? __ffsll(hit) - 1 : 63 - __clzll((long long)any);      // the last one with weight if rounding leaves none
+        run += __shfl(incl - m, at);
+        ties = __shfl(before, at);
+        begin = min(end, begin + at * each);
+        end = min(end, begin + each);
+        pick = begin;
+        if (each == 1) break;
+        each = 1;
+    }
+    return pick;
+}
+
+constexpr uint32_t TILE = 4096;
+
+// One workgroup a row (up to TILES tiles long).
 template <typename T>
 __global__ __launch_bounds__(DRAW_THREADS) void k_draw_row(DrawArgs a) {
     using S = Score<T>;
@@ -224,277 +629,74 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_row(DrawArgs a) {
     const T* x = (const T*)a.scores + row * a.stride;
     const uint32_t n = (uint32_t)a.cols;
     const DrawRow p(a, row);
-
-    // the best score and the lowest index that has it
-    Key bk = 0;
-    uint32_t bi = 0;
-    for (uint32_t i = tid; i < n; i += DRAW_THREADS) {
-        const Key k = S::key(x[i]);
-        if (k > bk) bk = k, bi = i;
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const Key k = __shfl_xor(bk, o);
-        const uint32_t i = __shfl_xor(bi, o);
-        if (k > bk || (k == bk && i < bi)) bk = k, bi = i;
-    }
-    if (lane == 0) s.best_key[wave] = bk, s.best_idx[wave] = bi;
-    __syncthreads();
-    bk = 0, bi = 0;
-    for (int i = 0; i < DRAW_THREADS / 64; ++i) {
-        const Key k = s.best_key[i];
-        if (k > bk || (k == bk && s.best_idx[i] < bi)) bk = k, bi = s.best_idx[i];
-    }
-    const Key top = bk;
-    if (top == 0 || p.greedy) {                // nothing can be drawn: index -1; or there is no choice
-        for (int64_t q = tid; q < a.draws; q += DRAW_THREADS) {
-            a.index[row * a.draws + q] = top ? (int64_t)bi : -1;
-            if (a.logp) a.logp[row * a.draws + q] = top ? 0.0 : -INFINITY;
-        }
+    Key top, bot;
+    uint32_t idx;
+    draw_extremes(s, x, 0, n, top, bot, idx);
+    if (top == 0 || p.greedy) {
+        draw_same<T>(a, row, top ? (int64_t)idx : -1, top ? 0.0 : -INFINITY);
         return;
     }
     if (n <= LIST) {
         if (tid < (int)n) s.l.key[tid] = S::key(x[tid]), s.l.idx[tid] = tid;
-        draw_from_list<T>(s, a, p, row, (int)n, top);
+        draw_from_list<T>(s, a, p, row, (int)n, top, -1.0);
         return;
     }
-
-    // kept = { key > cut } + the first cut_ties of those equal to it (by index), with w >= min_p
-    Key cut = 0;
-    uint32_t cut_ties = 0;
-    // mode 0: the cut of top-k, by counts; mode 1: of top-p, by masses, among what mode 0 left
-    for (int mode = 0; mode < 2; ++mode) {
-        if (mode == 0 ? p.top_k == 0 : !(p.top_p < 1.0)) continue;
-        const Key floor_key = cut;             // mode 1: keys at the cut of top-k are one group below all others
-        const uint32_t floor_ties = cut_ties;
-        double floor_mass = 0.0;
-        if (mode == 1 && floor_ties) {
-            const double w = exp(draw_t<T>(floor_key, top, p.temperature));
-            if (w >= p.min_p) floor_mass = w * floor_ties;
-        }
-        Key prefix = 0;
-        int left = S::BITS;                    // bits below the prefix
-        double above = 0.0, goal = 0.0;
-        long long rank = p.top_k;
-        bool done = false, spare = false;
-        while (!done) {
-            const int digit = min(DIGIT, left), shift = left - digit;
-            for (int b = tid; b < BINS; b += DRAW_THREADS) s.h.count[b] = 0, s.h.hi[b] = 0, s.h.lo[b] = 0;
-            __syncthreads();
-            for (uint32_t i = tid; i < n; i += DRAW_THREADS) {
-                const Key k = S::key(x[i]);
-                if (k == 0 || (left < S::BITS && (k >> (left & (S::BITS - 1))) != prefix)) continue;
-                const int b = (int)((k >> shift) & ((1u << digit) - 1));
-                if (mode == 0) {
-                    atomicAdd(&s.h.count[b], 1u);
-                } else {
-                    if (k <= floor_key) continue;
-                    const double w = exp(draw_t<T>(k, top, p.temperature));
-                    if (!(w >= p.min_p)) continue;
-                    unsigned long long hi, lo;
-                    to_fixed(w, hi, lo);
-                    atomicAdd(&s.h.count[b], 1u);
-                    atomicAdd(&s.h.hi[b], hi);
-                    if (lo) atomicAdd(&s.h.lo[b], lo);
-                }
-            }
-            __syncthreads();
-            // thread t owns bins from the top: BINS - 1 - 2t and the next lower one
-            const int b1 = BINS - 1 - 2 * tid, b0 = b1 - 1;
-            if (mode == 0) {
-                const unsigned long long c1 = s.h.count[b1], c0 = s.h.count[b0];
-                unsigned long long all;
-                const unsigned long long run = block_scan(c1 + c0, s.red_u, all) - c1 - c0;
-                if (left == S::BITS && all <= (unsigned long long)rank) {      // fewer valid scores than top_k: no cut
-                    spare = true;
-                } else {
-                    const long long r1 = (long long)run, r0 = (long long)(run + c1);
-                    if (c1 && r1 < rank && r1 + (long long)c1 >= rank) s.pick_bin = b1, s.rank_left = rank - r1, s.bin_count = (unsigned)c1;
-                    if (c0 && r0 < rank && r0 + (long long)c0 >= rank) s.pick_bin = b0, s.rank_left = rank - r0, s.bin_count = (unsigned)c0;
-                }
-            } else {
-                const double m1 = from_fixed(s.h.hi[b1], s.h.lo[b1]), m0 = from_fixed(s.h.hi[b0], s.h.lo[b0]);
-                double all;
-                const double incl = block_scan(m1 + m0, s.red, all);
-                if (left == S::BITS) goal = p.top_p * (all + floor_mass);
-                // the digit in which the running mass first reaches the goal; the lowest one in use if rounding leaves none
-                if (tid == 0) s.pick_bin = 0xffffffffu, s.cut_ties = 0xffffffffu;
-                __syncthreads();
-                spare = left == S::BITS && !(above + all >= goal);            // everything above the group is kept
-                if (s.h.count[b1] && above + (incl - m1 - m0) + m1 >= goal) atomicMin(&s.pick_bin, (unsigned)(BINS - 1 - b1));
-                if (s.h.count[b0] && above + incl >= goal) atomicMin(&s.pick_bin, (unsigned)(BINS - 1 - b0));
-                __syncthreads();
-                unsigned bin = s.pick_bin != 0xffffffffu ? BINS - 1 - s.pick_bin : 0xffffffffu;
-                if (bin == 0xffffffffu && !spare) {
-                    if (s.h.count[b0]) atomicMin(&s.cut_ties, (unsigned)b0);
-                    else if (s.h.count[b1]) atomicMin(&s.cut_ties, (unsigned)b1);
-                    __syncthreads();
-                    bin = s.cut_ties;
-                }
-                if (bin == (unsigned)b1) s.above = above + (incl - m1 - m0), s.bin_count = s.h.count[b1], s.rank_left = b1;
-                if (bin == (unsigned)b0) s.above = above + (incl - m0), s.bin_count = s.h.count[b0], s.rank_left = b0;
-            }
-            __syncthreads();
-            if (spare) break;
-            unsigned bin;
-            if (mode == 0) {
-                bin = s.pick_bin;
-                rank = s.rank_left;
-            } else {
-                bin = (unsigned)s.rank_left;
-                above = s.above;
-            }
-            const unsigned in_bin = s.bin_count;
-            prefix = (prefix << digit) | (Key)bin;
-            left = shift;
-            __syncthreads();
-            if (left == 0) {                   // one key: all of them ties
-                cut = prefix;
-                if (mode == 0) {
-                    cut_ties = (uint32_t)rank;
-                } else {
-                    const double w = exp(draw_t<T>(cut, top, p.temperature));
-                    double r = ceil((goal - above) / w);
-                    if (!(r >= 1.0)) r = 1.0;
-                    cut_ties = (uint32_t)fmin(r, (double)in_bin);
-                }
-                done = true;
-            } else if (in_bin <= LIST) {       // few enough to rank them against each other
-                if (tid == 0) s.n_list = 0;
-                __syncthreads();
-                for (uint32_t i = tid; i < n; i += DRAW_THREADS) {
-                    const Key k = S::key(x[i]);
-                    if (k == 0 || (k >> left) != prefix) continue;
-                    if (mode == 1 && (k <= floor_key || !(exp(draw_t<T>(k, top, p.temperature)) >= p.min_p))) continue;
-                    const uint32_t at = atomicAdd(&s.n_list, 1u);
-                    s.l.key[at] = k, s.l.idx[at] = i;
-                }
-                __syncthreads();
-                const int m = (int)s.n_list;
-                const Key k = tid < m ? s.l.key[tid] : 0;
-                const uint32_t ix = tid < m ? s.l.idx[tid] : 0;
-                if (tid < m) {
-                    int r = 0;
-                    for (int j = 0; j < m; ++j) {
-                        const Key kj = s.l.key[j];
-                        r += (kj > k) || (kj == k && s.l.idx[j] < ix);
-                    }
-                    s.l.key2[r] = k;
-                }
-                __syncthreads();
-                const Key kr = tid < m ? s.l.key2[tid] : 0;
-                bool in = false;
-                if (mode == 0) {
-                    in = tid < rank;
-                } else {
-                    const double w = kr ? exp(draw_t<T>(kr, top, p.temperature)) : 0.0;
-                    double all;
-                    const double incl = block_scan(w, s.red, all);
-                    in = kr != 0 && (tid == 0 || above + (incl - w) < goal);
-                }
-                unsigned long long taken;
-                block_scan<unsigned long long>(in ? 1ull : 0ull, s.red_u, taken);
-                cut = s.l.key2[(int)taken - 1];
-                unsigned long long same;
-                block_scan<unsigned long long>(in && kr == cut ? 1ull : 0ull, s.red_u, same);
-                cut_ties = (uint32_t)same;
-                done = true;
-                __syncthreads();
-            }
-        }
-        if (spare && mode == 1) {              // all above the group, and of the group as many as the mass still asks for
-            cut = floor_key;
-            cut_ties = floor_ties;
-            if (floor_ties) {
-                const double w = exp(draw_t<T>(floor_key, top, p.temperature));
-                double strict;
-                // mass above the group, again from the histogram: the total of its first level
-                const int b1 = BINS - 1 - 2 * tid, b0 = b1 - 1;
-                block_scan(from_fixed(s.h.hi[b1], s.h.lo[b1]) + from_fixed(s.h.hi[b0], s.h.lo[b0]), s.red, strict);
-                double r = w > 0.0 ? ceil((goal - strict) / w) : 0.0;
-                if (!(r >= 0.0)) r = 0.0;
-                cut_ties = (uint32_t)fmin(r, (double)floor_ties);
-            }
-            __syncthreads();
-        }
-    }
-
-    // kept mass of TILES pieces of the row, in index order: ties with the cut are counted first (they are kept by index)
-    const uint32_t piece = (uint32_t)round_up(ceil_div(n, TILES), 64);
-    __syncthreads();
-    for (uint32_t t = wave; t < TILES; t += DRAW_THREADS / 64) {
-        uint32_t c = 0;
-        if (cut_ties)
-            for (uint32_t i = 0; i < piece; i += 64) {
-                const uint64_t e = (uint64_t)t * piece + i + lane;
-                c += __popcll(__ballot(e < n && S::key(x[e < n ? e : 0]) == cut));
-            }
-        if (lane == 0) s.t.ties[t] = c;
+    if (tid == 0) {
+        s.st.top = top, s.st.bot = bot, s.st.best_idx = idx, s.st.cut = 0, s.st.cut_ties = 0;
+        draw_begin(s.st, p, PHASE_TOPK);
     }
     __syncthreads();
-    {
-        const unsigned long long v = s.t.ties[tid];
-        unsigned long long all;
-        const unsigned long long incl = block_scan(v, s.red_u, all);
+    while (s.st.phase < PHASE_PICK) {
+        const DrawStep<T> d(s.st, p);
+        if (!s.st.gather) {
+            draw_histogram(s, d, x, 0, n);
+            draw_decide(s, p);
+            continue;
+        }
+        each_score(x, 0, n, [&](Key k, uint32_t i) {
+            double w;
+            if (!d.counts(k, w)) return;
+            const uint32_t at = atomicAdd(&s.st.n_list, 1u);
+            if (at < LIST) s.l.key[at] = k, s.l.idx[at] = i;
+        });
         __syncthreads();
-        s.t.ties[tid] = (uint32_t)(incl - v);
-        __syncthreads();
+        const int m = min((int)s.st.n_list, LIST);
+        if (s.st.gather_all) {
+            draw_from_list<T>(s, a, p, row, m, top, s.st.phase == PHASE_TOPP ? s.st.goal : -1.0);
+            return;
+        }
+        draw_cut_from_list(s, p, m);
     }
-    auto weight = [&](uint64_t e, uint32_t& ties) -> double {     // of element e of this wave's 64; ties: of the cut so far
-        const Key k = e < n ? S::key(x[e]) : 0;
-        const bool tie = k == cut && cut_ties;
-        const unsigned long long votes = __ballot(tie);
-        const uint32_t mine = ties + __popcll(votes & ((1ull << lane) - 1));
-        ties += __popcll(votes);
-        if (k == 0 || (k <= cut && !(tie && mine < cut_ties))) return 0.0;
-        const double w = exp(draw_t<T>(k, top, p.temperature));
-        return w >= p.min_p ? w : 0.0;
-    };
+
+    // kept mass of the row's tiles, in index order
+    const DrawKept<T> kw(s.st, p);
+    const uint32_t tiles = (n + TILE - 1) / TILE;
     for (uint32_t t = wave; t < TILES; t += DRAW_THREADS / 64) {
-        uint32_t ties = s.t.ties[t];
         double m = 0.0;
-        for (uint32_t i = 0; i < piece; i += 64) m += weight((uint64_t)t * piece + i + lane, ties);
-        m = wave_sum(m);
-        if (lane == 0) s.t.c[t] = m;
+        uint32_t c = 0;
+        if (t < tiles) draw_tile_mass(kw, x, t * TILE, min(n, (t + 1) * TILE), m, c);
+        if (lane == 0) s.t.c[t] = m, s.t.ties[t] = c;
     }
     __syncthreads();
+    const uint32_t mine = s.t.ties[tid];
+    unsigned long long all_ties;
+    const uint32_t before = (uint32_t)(block_scan<unsigned long long>(mine, s.red_u, all_ties) - mine);
+    const uint32_t cut_ties = s.st.cut_ties;
+    const uint32_t kept = before >= cut_ties ? 0 : min(mine, cut_ties - before);
     double total;
-    {
-        const double incl = block_scan(s.t.c[tid], s.red, total);
-        __syncthreads();
-        s.t.c[tid] = incl;
-        __syncthreads();
-    }
+    const double incl = block_scan(s.t.c[tid] + kept * kw.tie_w, s.red, total);
+    s.t.c[tid] = incl, s.t.ties[tid] = before;
+    __syncthreads();
     for (int64_t q = wave; q < a.draws; q += DRAW_THREADS / 64) {
         const double goal = fmax(a.u[row * a.draws + q], 0.0) * total;
-        int lo = 0, hi = TILES - 1;            // the first tile whose sum passes the goal, the last with any mass if none does
+        int lo = 0, hi = (int)tiles - 1;       // the first tile whose sum passes the goal, the last with any mass if none does
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
             if (s.t.c[mid] > goal) hi = mid;
             else lo = mid + 1;
         }
         while (lo > 0 && s.t.c[lo] == s.t.c[lo - 1]) --lo;
-        uint32_t ties = s.t.ties[lo];
-        double run = lo ? s.t.c[lo - 1] : 0.0;
-        int64_t pick = -1;
-        for (uint32_t i = 0; i < piece; i += 64) {
-            const uint64_t e = (uint64_t)lo * piece + i + lane;
-            const double w = weight(e, ties);
-            double c = w;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const double v = __shfl_up(c, o);
-                if (lane >= o) c += v;
-            }
-            const unsigned long long any = __ballot(w > 0.0), hit = __ballot(w > 0.0 && run + c > goal);
-            const uint64_t at = (uint64_t)lo * piece + i;
-            if (hit) {
-                pick = (int64_t)(at + __ffsll((unsigned long long)hit) - 1);
-                break;
-            }
-            if (any) pick = (int64_t)(at + 63 - __clzll((long long)any));
-            run += __shfl(c, 63);
-        }
+        const int64_t pick = draw_in_tile(kw, x, lo * TILE, min(n, (lo + 1) * TILE), lo ? s.t.c[lo - 1] : 0.0, s.t.ties[lo], cut_ties, goal);
         if (lane == 0) {
             a.index[row * a.draws + q] = pick;
             if (a.logp) a.logp[row * a.draws + q] = draw_t<T>(S::key(x[pick]), top, p.temperature) - log(total);
@@ -502,9 +704,293 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_row(DrawArgs a) {
     }
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// Long rows: BLOCKS workgroups a row and step.  Workspace of a row: its state, one histogram, the list, the extremes of every
+// workgroup's share, and mass and ties of every tile.
 template <typename T>
-hipError_t draw_rows(hipStream_t st, const DrawArgs& a) {
-    hipLaunchKernelGGL(k_draw_row<T>, dim3((unsigned)a.rows), dim3(DRAW_THREADS), 0, st, a);
+struct DrawWork {
+    using Key = typename Score<T>::Key;
+    DrawState<T> st;
+    unsigned int count[BINS];
+    unsigned long long hi[BINS], lo[BINS];
+    Key key[LIST];
+    uint32_t idx[LIST];
+    Key top[1024], bot[1024];
+    uint32_t top_idx[1024];
+    double total;
+};
+template <typename T>
+__host__ __device__ constexpr int64_t draw_row_bytes(int64_t cols) {
+    return round_up((int64_t)sizeof(DrawWork<T>), 256) + round_up(ceil_div(cols, TILE) * 8, 256) + round_up(ceil_div(cols, TILE) * 4, 256);
+}
+template <typename T>
+struct DrawRowWork {
+    DrawWork<T>* w;
+    double* c;
+    uint32_t* ties;
+    __device__ __forceinline__ DrawRowWork(char* work, int64_t row, int64_t cols) {
+        char* at = work + row * draw_row_bytes<T>(cols);
+        w = (DrawWork<T>*)at;
+        c = (double*)(at + round_up((int64_t)sizeof(DrawWork<T>), 256));
+        ties = (uint32_t*)((char*)c + round_up(ceil_div(cols, TILE) * 8, 256));
+    }
+};
+
+// The share of workgroup b of `blocks` of a row of n elements: whole packs.
+__device__ __forceinline__ void draw_share(uint32_t n, uint32_t b, uint32_t blocks, uint32_t& begin, uint32_t& end) {
+    const uint32_t each = (uint32_t)round_up(ceil_div(n, blocks), 16);
+    begin = min(n, b * each);
+    end = min(n, begin + each);
+}
+
+// True in the workgroup that arrives last of the `blocks` of its row; what the others wrote before is then visible to it.  The
+// counter is back at zero for the next step.
+template <typename T>
+__device__ bool draw_last(DrawLds<T>& s, unsigned int* ticket, uint32_t blocks) {
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const unsigned int t = atomicAdd(ticket, 1u);
+        s.last = t == blocks - 1;
+        if (s.last) *ticket = 0;
+    }
+    __syncthreads();
+    if (s.last) __threadfence();
+    return s.last;
+}
+
+// Extremes of every share, a clean histogram and counters.
+template <typename T>
+__global__ __launch_bounds__(DRAW_THREADS) void k_draw_start(DrawArgs a, char* work) {
+    using Key = typename Score<T>::Key;
+    __shared__ DrawLds<T> s;
+    const int64_t row = blockIdx.y;
+    const DrawRowWork<T> rw(work, row, a.cols);
+    const T* x = (const T*)a.scores + row * a.stride;
+    uint32_t begin, end;
+    draw_share((uint32_t)a.cols, blockIdx.x, gridDim.x, begin, end);
+    Key top, bot;
+    uint32_t idx;
+    draw_extremes(s, x, begin, end, top, bot, idx);
+    if (threadIdx.x == 0) rw.w->top[blockIdx.x] = top, rw.w->bot[blockIdx.x] = bot, rw.w->top_idx[blockIdx.x] = idx;
+    if (blockIdx.x == 0) {
+        for (int b = threadIdx.x; b < BINS; b += DRAW_THREADS) rw.w->count[b] = 0, rw.w->hi[b] = 0, rw.w->lo[b] = 0;
+        if (threadIdx.x == 0) rw.w->st.ticket = 0;
+    }
+}
+
+// Joins the extremes; the first step, or the result where there is nothing to choose.  One workgroup a row.
+template <typename T>
+__global__ __launch_bounds__(DRAW_THREADS) void k_draw_begin(DrawArgs a, char* work, int shares) {
+    using Key = typename Score<T>::Key;
+    __shared__ Key rk[2][16];
+    __shared__ uint32_t ri[16];
+    const int64_t row = blockIdx.x;
+    const DrawRowWork<T> rw(work, row, a.cols);
+    const DrawRow p(a, row);
+    const int tid = threadIdx.x;
+    Key bk = tid < shares ? rw.w->top[tid] : 0, lk = tid < shares ? rw.w->bot[tid] : ~(Key)0;
+    uint32_t bi = tid < shares ? rw.w->top_idx[tid] : 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const Key k = __shfl_xor(bk, o), l = __shfl_xor(lk, o);
+        const uint32_t i = __shfl_xor(bi, o);
+        if (k > bk || (k == bk && i < bi)) bk = k, bi = i;
+        if (l < lk) lk = l;
+    }
+    if ((tid & 63) == 0) rk[0][tid >> 6] = bk, rk[1][tid >> 6] = lk, ri[tid >> 6] = bi;
+    __syncthreads();
+    for (int i = 0; i < DRAW_THREADS / 64; ++i) {
+        if (rk[0][i] > bk || (rk[0][i] == bk && ri[i] < bi)) bk = rk[0][i], bi = ri[i];
+        if (rk[1][i] < lk) lk = rk[1][i];
+    }
+    if (bk == 0 || p.greedy) draw_same<T>(a, row, bk ? (int64_t)bi : -1, bk ? 0.0 : -INFINITY);
+    if (tid == 0) {
+        DrawState<T>& st = rw.w->st;
+        st.top = bk, st.bot = lk, st.best_idx = bi, st.cut = 0, st.cut_ties = 0, st.n_list = 0;
+        if (bk == 0 || p.greedy) st.phase = PHASE_DONE;
+        else draw_begin(st, p, PHASE_TOPK);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(DRAW_THREADS) void k_draw_step(DrawArgs a, char* work) {
+    using Key = typename Score<T>::Key;
+    __shared__ DrawLds<T> s;
+    const int64_t row = blockIdx.y;
+    const DrawRowWork<T> rw(work, row, a.cols);
+    if (rw.w->st.phase >= PHASE_PICK) return;
+    const int tid = threadIdx.x;
+    const T* x = (const T*)a.scores + row * a.stride;
+    const DrawRow p(a, row);
+    const DrawStep<T> d(rw.w->st, p);
+    const bool gather = rw.w->st.gather;
+    uint32_t begin, end;
+    draw_share((uint32_t)a.cols, blockIdx.x, gridDim.x, begin, end);
+    if (gather) {
+        each_score(x, begin, end, [&](Key k, uint32_t i) {
+            double w;
+            if (!d.counts(k, w)) return;
+            const uint32_t at = atomicAdd(&rw.w->st.n_list, 1u);
+            if (at < LIST) rw.w->key[at] = k, rw.w->idx[at] = i;
+        });
+    } else {
+        draw_histogram(s, d, x, begin, end);
+        for (int b = tid; b < BINS; b += DRAW_THREADS)
+            if (s.h.count[b]) {
+                atomicAdd(&rw.w->count[b], s.h.count[b]);
+                if (s.h.hi[b]) atomicAdd(&rw.w->hi[b], s.h.hi[b]);
+                if (s.h.lo[b]) atomicAdd(&rw.w->lo[b], s.h.lo[b]);
+            }
+    }
+    if (!draw_last(s, &rw.w->st.ticket, gridDim.x)) return;
+    // what other workgroups left is read past this one's caches
+    auto fresh32 = [](unsigned int* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    if (tid == 0) {
+        s.st = rw.w->st;
+        s.st.n_list = fresh32(&rw.w->st.n_list);
+        s.st.ticket = 0;
+    }
+    __syncthreads();
+    if (!gather) {
+        for (int b = tid; b < BINS; b += DRAW_THREADS) {
+            s.h.count[b] = fresh32(&rw.w->count[b]);
+            s.h.hi[b] = __hip_atomic_load(&rw.w->hi[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            s.h.lo[b] = __hip_atomic_load(&rw.w->lo[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            rw.w->count[b] = 0, rw.w->hi[b] = 0, rw.w->lo[b] = 0;
+        }
+        __syncthreads();
+        draw_decide(s, p);
+    } else {
+        const int m = min((int)s.st.n_list, LIST);
+        if (tid < m) {
+            s.l.key[tid] = __hip_atomic_load(&rw.w->key[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            s.l.idx[tid] = fresh32(&rw.w->idx[tid]);
+        }
+        if (s.st.gather_all) {
+            draw_from_list<T>(s, a, p, row, m, s.st.top, s.st.phase == PHASE_TOPP ? s.st.goal : -1.0);
+            __syncthreads();
+            if (tid == 0) s.st.phase = PHASE_DONE;
+        } else {
+            draw_cut_from_list(s, p, m);
+        }
+        if (tid == 0) s.st.n_list = 0;
+    }
+    __syncthreads();
+    if (tid == 0) rw.w->st = s.st;
+}
+
+// Mass above the cut and ties of every tile, a wave each.
+template <typename T>
+__global__ __launch_bounds__(256) void k_draw_mass(DrawArgs a, char* work) {
+    const int64_t row = blockIdx.y;
+    const DrawRowWork<T> rw(work, row, a.cols);
+    if (rw.w->st.phase != PHASE_PICK) return;
+    const DrawRow p(a, row);
+    const DrawKept<T> kw(rw.w->st, p);
+    const T* x = (const T*)a.scores + row * a.stride;
+    const uint32_t n = (uint32_t)a.cols, tiles = (n + TILE - 1) / TILE;
+    for (uint32_t t = blockIdx.x * 4 + (threadIdx.x >> 6); t < tiles; t += gridDim.x * 4) {
+        double m;
+        uint32_t c;
+        draw_tile_mass(kw, x, t * TILE, min(n, (t + 1) * TILE), m, c);
+        if ((threadIdx.x & 63) == 0) rw.c[t] = m, rw.ties[t] = c;
+    }
+}
+
+// Running sums over the tiles.  One workgroup a row; the tiles in runs of 1024.
+template <typename T>
+__global__ __launch_bounds__(DRAW_THREADS) void k_draw_sums(DrawArgs a, char* work) {
+    __shared__ double red[32];
+    __shared__ unsigned long long red_u[32];
+    const int64_t row = blockIdx.x;
+    const DrawRowWork<T> rw(work, row, a.cols);
+    if (rw.w->st.phase != PHASE_PICK) return;
+    const DrawRow p(a, row);
+    const DrawKept<T> kw(rw.w->st, p);
+    const uint32_t tiles = (uint32_t)ceil_div(a.cols, TILE), cut_ties = rw.w->st.cut_ties;
+    double carry = 0.0;
+    unsigned long long carry_t = 0;
+    for (uint32_t t0 = 0; t0 < tiles; t0 += DRAW_THREADS) {
+        const uint32_t t = t0 + threadIdx.x;
+        const uint32_t mine = t < tiles ? rw.ties[t] : 0;
+        unsigned long long all_t;
+        const unsigned long long before = carry_t + block_scan<unsigned long long>(mine, red_u, all_t) - mine;
+        const uint32_t kept = before >= cut_ties ? 0 : (uint32_t)min((unsigned long long)mine, cut_ties - before);
+        double all;
+        const double incl = block_scan((t < tiles ? rw.c[t] : 0.0) + kept * kw.tie_w, red, all);
+        if (t < tiles) rw.c[t] = carry + incl, rw.ties[t] = (uint32_t)before;
+        carry += all;
+        carry_t += all_t;
+    }
+    if (threadIdx.x == 0) rw.w->total = carry;
+}
+
+// A wave a draw.
+template <typename T>
+__global__ __launch_bounds__(256) void k_draw_pick(DrawArgs a, char* work) {
+    const int64_t row = blockIdx.y;
+    const DrawRowWork<T> rw(work, row, a.cols);
+    if (rw.w->st.phase != PHASE_PICK) return;
+    const DrawRow p(a, row);
+    const DrawKept<T> kw(rw.w->st, p);
+    const T* x = (const T*)a.scores + row * a.stride;
+    const uint32_t n = (uint32_t)a.cols, tiles = (n + TILE - 1) / TILE;
+    const double total = rw.w->total;
+    for (int64_t q = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); q < a.draws; q += (int64_t)gridDim.x * 4) {
+        const double goal = fmax(a.u[row * a.draws + q], 0.0) * total;
+        int lo = 0, hi = (int)tiles - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (rw.c[mid] > goal) hi = mid;
+            else lo = mid + 1;
+        }
+        while (lo > 0 && rw.c[lo] == rw.c[lo - 1]) --lo;
+        const int64_t pick = draw_in_tile(kw, x, (uint32_t)lo * TILE, min(n, (uint32_t)(lo + 1) * TILE), lo ? rw.c[lo - 1] : 0.0, rw.ties[lo],
+                                          rw.w->st.cut_ties, goal);
+        if ((threadIdx.x & 63) == 0) {
+            a.index[row * a.draws + q] = pick;
+            if (a.logp) a.logp[row * a.draws + q] = draw_t<T>(Score<T>::key(x[pick]), kw.top, p.temperature) - log(total);
+        }
+    }
+}
+
+// One workgroup a row while the rows fill the card or a row is short; else many workgroups a row.
+inline bool draw_long(int64_t rows, int64_t cols) { return cols > (int64_t)TILE * TILES || (cols > 32768 && rows * 4 < 256 * 2); }
+
+template <typename T>
+int64_t draw_work_bytes(int64_t rows, int64_t cols) {
+    return draw_long(rows, cols) ? rows * draw_row_bytes<T>(cols) : 0;
+}
+
+template <typename T>
+hipError_t draw_rows(hipStream_t st, const DrawArgs& a, char* work) {
+    if (!draw_long(a.rows, a.cols)) {
+        hipLaunchKernelGGL(k_draw_row<T>, dim3((unsigned)a.rows), dim3(DRAW_THREADS), 0, st, a);
+        return hipGetLastError();
+    }
+    // two workgroups of 1024 threads a CU over all rows, at least one 16 K share each
+    const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>({ceil_div(512, a.rows), ceil_div(a.cols, 16384), 1024}));
+    for (int64_t r0 = 0; r0 < a.rows; r0 += 65535) {      // the grid's second dimension ends there
+        DrawArgs b = a;
+        b.rows = std::min<int64_t>(65535, a.rows - r0);
+        b.scores = (const T*)a.scores + r0 * a.stride, b.u = a.u + r0 * a.draws, b.index = a.index + r0 * a.draws;
+        b.logp = a.logp ? a.logp + r0 * a.draws : nullptr, b.params = a.params ? a.params + r0 * 4 : nullptr;
+        char* w = work + r0 * draw_row_bytes<T>(a.cols);
+        const dim3 wide((unsigned)blocks, (unsigned)b.rows), one((unsigned)b.rows);
+        hipLaunchKernelGGL(k_draw_start<T>, wide, dim3(DRAW_THREADS), 0, st, b, w);
+        hipLaunchKernelGGL(k_draw_begin<T>, one, dim3(DRAW_THREADS), 0, st, b, w, (int)blocks);
+        // a phase takes the linear step, at most ceil(bits / 11) steps on the keys and one for the list; what is decided earlier
+        // leaves the rest of the launches with nothing to do
+        const bool by_row = a.params != nullptr;
+        const int phases = (by_row || (a.top_k > 0 && a.top_k < a.cols)) + (by_row || a.top_p < 1.0);
+        const int steps = phases * (2 + (Score<T>::BITS + DIGIT - 1) / DIGIT);
+        for (int i = 0; i < steps; ++i) hipLaunchKernelGGL(k_draw_step<T>, wide, dim3(DRAW_THREADS), 0, st, b, w);
+        const int64_t tiles = ceil_div(a.cols, TILE);
+        hipLaunchKernelGGL(k_draw_mass<T>, dim3((unsigned)std::min<int64_t>(ceil_div(tiles, 4), 4096), (unsigned)b.rows), dim3(256), 0, st, b, w);
+        hipLaunchKernelGGL(k_draw_sums<T>, one, dim3(DRAW_THREADS), 0, st, b, w);
+        hipLaunchKernelGGL(k_draw_pick<T>, dim3((unsigned)std::min<int64_t>(ceil_div(a.draws, 4), 4096), (unsigned)b.rows), dim3(256), 0, st, b, w);
+    }
     return hipGetLastError();
 }
 
