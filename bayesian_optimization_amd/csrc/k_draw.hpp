@@ -4,12 +4,14 @@
 //   the mass in front of it is < top_p times their mass (the first always).
 //   pick(u): the lowest kept i, in index order, with C_i > u Z;  C the running sum of kept w, Z their mass;  logp = t_i - log Z.
 // No sort of the row: the kept set is { score > cut } plus the first few, by index, of those equal to the cut.  The cut is found by
-// histograms of 2048 bins, counts for top-k, masses for top-p: the first one linear in the score, which spreads what lies near
-// the best over many bins, the next ones of the integer range of keys that is left (a score's bits, mapped to an unsigned key of
-// the same order), until at most LIST keys remain to be ranked against each other; where that list holds all that can be kept,
-// the rest of the work is done on it alone.  Counts are integers, and so are the masses of a histogram (two words of 35 bits
-// each), so that the order in which atomics arrive changes nothing; all other sums are in 64 bits in a fixed order.
-// Bound by memory: a pass over the row per step, two to five of them, and by the exponential of every score of a top-p step.
+// histograms of 2048 bins over the range of scores that can hold it, counts for top-k, masses for top-p: the first two linear in
+// the score, which spreads what lies near the best over many bins, further ones of the range of keys that is left (a score's
+// bits, mapped to an unsigned key of the same order), until at most LIST keys remain to be sorted.  Where a list holds all that
+// can be kept, the rest of the work is done on it alone; that is tried first where a bound is at hand: the k-th best of the
+// maxima of disjoint parts of the row is a lower bound of the k-th best score, and min_p is one of all that is kept.
+// Counts are integers, and so are the masses of a histogram (two words of 35 bits each), so that the order in which atomics
+// arrive changes nothing; all other sums are in 64 bits in a fixed order.
+// Bound by memory: a pass over the row per step, two to five of them, and by the exponential of the scores of a top-p step.
 // Short rows: one workgroup a row does everything (k_draw_row).  Long rows: the same steps with many workgroups a row, one
 // launch a step, the state of a row in the workspace; the last workgroup to arrive at a step takes its decision.
 #pragma once
@@ -137,16 +139,16 @@ template <typename T>
 struct DrawState {
     using Key = typename Score<T>::Key;
     Key top, bot;                 // best and lowest valid key
-    Key klo, khi;                 // the cut lies among keys klo .. khi (and in linear bin lin_bin, if lin == 2)
+    Key klo, khi;                 // the cut lies among keys klo .. khi
     Key cut, floor_key;           // PHASE_TOPP: the cut of top-k, whose ties are one group below all other keys
-    double scale;                 // linear bins per score
     double above, goal;           // PHASE_TOPP: mass above khi; mass to reach
     double floor_mass;
     long long rank;               // PHASE_TOPK: how many of klo .. khi are kept
     long long count_above;        // keys above khi that may be kept
-    int phase, lin, lin_bin;      // lin: 0 no linear step, 1 this step is linear, 2 it has been
-    int gather, gather_all;       // this step collects the list; all keys from klo up, or klo .. khi only
-    uint32_t cut_ties, floor_ties, best_idx;
+    int phase, first;             // first: no histogram of this phase has been taken yet
+    int linear_left;              // linear steps still to try
+    int gather;                   // this step collects a list: 1 of klo .. khi, 2 of all that can be kept, 3 the same, on trial
+    uint32_t cut_ties, floor_ties;
     unsigned int n_list, ticket;
 };
 
@@ -156,25 +158,23 @@ struct DrawStep {
     using S = Score<T>;
     using Key = typename S::Key;
     Key top, klo, khi, floor_key;
-    double smax, scale, min_p, temperature;
-    int phase, lin, lin_bin, gather_all, shift;
+    double base, scale, min_p, temperature;
+    int phase, gather, shift;
+    bool linear;
     __device__ __forceinline__ DrawStep(const DrawState<T>& st, const DrawRow& p)
-        : top(st.top), klo(st.klo), khi(st.khi), floor_key(st.floor_key), smax(S::value(st.top)), scale(st.scale), min_p(p.min_p),
-          temperature(p.temperature), phase(st.phase), lin(st.lin), lin_bin(st.lin_bin), gather_all(st.gather_all) {
+        : top(st.top), klo(st.klo), khi(st.khi), floor_key(st.floor_key), base(S::value(st.khi)), min_p(p.min_p), temperature(p.temperature),
+          phase(st.phase), gather(st.gather) {
         const Key width = khi - klo;
         const int bits = width == 0 ? 0 : S::BITS == 64 ? 64 - __clzll((long long)width) : 32 - __clz((int)width);
         shift = bits > DIGIT ? bits - DIGIT : 0;
-    }
-    __device__ __forceinline__ int linear(Key k) const {
-        const double v = (smax - S::value(k)) * scale;
-        return v >= (double)(BINS - 1) ? BINS - 1 : (int)v;
+        const double span = base - S::value(klo);
+        scale = (double)(BINS - 1) / span;
+        linear = st.linear_left > 0 && shift > 0 && span < INFINITY && scale > 0.0 && scale < INFINITY;
     }
     __device__ __forceinline__ bool counts(Key k, double& w) const {
-        if (k < klo || k == 0 || (k > khi && !gather_all)) return false;
-        if (lin == 2) {
-            const int b = linear(k);
-            if (gather_all ? b > lin_bin : b != lin_bin) return false;
-        }
+        if (k < klo || k == 0) return false;
+        if (gather == 3) return true;
+        if (k > khi && gather != 2) return false;
         if (phase == PHASE_TOPP) {
             if (k <= floor_key) return false;
             w = exp(draw_t<T>(k, top, temperature));
@@ -182,7 +182,44 @@ struct DrawStep {
         }
         return true;
     }
-    __device__ __forceinline__ int bin(Key k) const { return lin == 1 ? linear(k) : (int)((khi - k) >> shift); }
+    // bins from the top down; never falling as the key falls
+    __device__ __forceinline__ int bin(Key k) const {
+        if (!linear) return (int)((khi - k) >> shift);
+        const double v = (base - S::value(k)) * scale;
+        return v >= (double)(BINS - 1) ? BINS - 1 : (int)v;
+    }
+    // the keys of a bin: for the linear step the first and last key that `bin` puts there, by bisection
+    __device__ void ends(int b, Key& lo, Key& hi) const {
+        if (!linear) {
+            const Key span = ((Key)1 << shift) - 1;
+            hi = khi - ((Key)b << shift);
+            lo = hi - klo > span ? hi - span : klo;
+            return;
+        }
+        auto last_at_most = [&](int q) -> Key {       // lowest key with bin(key) <= q
+            Key l = klo, h = khi;                     // bin(khi) = 0
+            const Key guess = S::key_of(base - (q + 1) / scale);
+            if (guess > klo && guess < khi) {         // the bisection starts around it, in growing steps
+                for (Key step = 4;; step <<= 4) {
+                    const Key a = guess - klo > step ? guess - step : klo, z = khi - guess > step ? guess + step : khi;
+                    if ((a == klo || bin(a) > q) && bin(z) <= q) {
+                        l = a, h = z;
+                        break;
+                    }
+                    if (a == klo && z == khi) break;
+                    if (step >> (S::BITS - 5)) break;
+                }
+            }
+            while (l < h) {
+                const Key mid = l + ((h - l) >> 1);
+                if (bin(mid) <= q) h = mid;
+                else l = mid + 1;
+            }
+            return h;
+        };
+        lo = last_at_most(b);
+        hi = b == 0 ? khi : last_at_most(b - 1) - 1;
+    }
 };
 
 template <typename T>
@@ -212,12 +249,24 @@ struct DrawLds {
     unsigned int bin, any_bin, last;
 };
 
-// Every score of elements [begin, end) of a row, 16 bytes a load, the workgroup's threads side by side: f(key, index).
-template <typename T, typename F>
+// Every score of elements [begin, end) of a row, 16 bytes a load, the workgroup's threads side by side: f(key, index).  SCORES
+// of them are under way before the first is looked at: with fewer, what f does with it stands between a load and the next.
+template <typename T, int SCORES = 8, typename F>
 __device__ __forceinline__ void each_score(const T* x, uint32_t begin, uint32_t end, F&& f) {
     constexpr uint32_t V = Pack<T>::N;
     const uint32_t packs = (end - begin) / V;
-    for (uint32_t c = threadIdx.x; c < packs; c += DRAW_THREADS) {
+    constexpr uint32_t U = V >= SCORES ? 1 : SCORES / V;
+    uint32_t c = threadIdx.x;
+    for (; c + (U - 1) * DRAW_THREADS < packs; c += U * DRAW_THREADS) {
+        Pack<T> p[U];
+#pragma unroll
+        for (uint32_t j = 0; j < U; ++j) p[j] = load_pack(x + begin + (c + j * DRAW_THREADS) * V);
+#pragma unroll
+        for (uint32_t j = 0; j < U; ++j)
+#pragma unroll
+            for (uint32_t i = 0; i < V; ++i) f(Score<T>::key(p[j].v[i]), begin + (c + j * DRAW_THREADS) * V + i);
+    }
+    for (; U > 1 && c < packs; c += DRAW_THREADS) {
         const Pack<T> p = load_pack(x + begin + c * V);
 #pragma unroll
         for (uint32_t i = 0; i < V; ++i) f(Score<T>::key(p.v[i]), begin + c * V + i);
@@ -225,16 +274,18 @@ __device__ __forceinline__ void each_score(const T* x, uint32_t begin, uint32_t 
     for (uint32_t i = begin + packs * V + threadIdx.x; i < end; i += DRAW_THREADS) f(Score<T>::key(x[i]), i);
 }
 
-// Best key with its lowest index, and lowest valid key, of [begin, end).
+// Best key with its lowest index, and lowest valid key, of [begin, end); own: the best key this thread saw.
 template <typename T>
-__device__ void draw_extremes(DrawLds<T>& s, const T* x, uint32_t begin, uint32_t end, typename Score<T>::Key& top, typename Score<T>::Key& bot, uint32_t& idx) {
+__device__ void draw_extremes(DrawLds<T>& s, const T* x, uint32_t begin, uint32_t end, typename Score<T>::Key& top, typename Score<T>::Key& bot, uint32_t& idx,
+                              typename Score<T>::Key& own) {
     using Key = typename Score<T>::Key;
     Key bk = 0, lk = ~(Key)0;
     uint32_t bi = 0;
-    each_score(x, begin, end, [&](Key k, uint32_t i) {
-        if (k > bk) bk = k, bi = i;            // a thread meets its indices in rising order, up to the tail's
+    each_score<T, 32>(x, begin, end, [&](Key k, uint32_t i) {
+        if (k > bk) bk = k, bi = i;            // a thread meets its indices in rising order
         if (k != 0 && k < lk) lk = k;
     });
+    own = bk;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
         const Key k = __shfl_xor(bk, o), l = __shfl_xor(lk, o);
@@ -263,31 +314,42 @@ __device__ void draw_same(const DrawArgs& a, int64_t row, int64_t index, double 
     }
 }
 
-// Thread 0: the first step of a phase, or the next phase that has any.
+// Thread 0: the first step of a phase, or the next phase that has any.  bound: a key that at least top_k valid keys reach, or 0.
 template <typename T>
-__device__ void draw_begin(DrawState<T>& st, const DrawRow& p, int phase) {
+__device__ void draw_begin(DrawState<T>& st, const DrawRow& p, int phase, typename Score<T>::Key bound = 0) {
     using S = Score<T>;
+    using Key = typename S::Key;
     if (phase == PHASE_TOPK && p.top_k == 0) phase = PHASE_TOPP;
-    if (phase == PHASE_TOPP && !(p.top_p < 1.0)) phase = PHASE_PICK;
+    if (phase == PHASE_TOPP && !(p.top_p < 1.0) && p.min_p == 0.0) phase = PHASE_PICK;
     st.phase = phase;
     if (phase >= PHASE_PICK) return;
     st.klo = st.bot, st.khi = st.top;
     st.above = st.goal = st.floor_mass = 0.0;
     st.count_above = 0;
     st.rank = p.top_k;
-    st.gather = st.gather_all = 0;
+    st.first = 1, st.linear_left = 2, st.gather = 0, st.n_list = 0;
     st.floor_key = 0, st.floor_ties = 0;
-    double span = S::value(st.top) - S::value(st.bot);
-    if (phase == PHASE_TOPP) {
-        st.floor_key = st.cut, st.floor_ties = st.cut_ties;
-        if (st.floor_ties) {
-            const double w = exp(draw_t<T>(st.floor_key, st.top, p.temperature));
-            if (w >= p.min_p) st.floor_mass = w * st.floor_ties;
+    if (phase == PHASE_TOPK) {
+        if (bound) {
+            st.klo = bound;
+            if (p.top_k <= LIST / 2) st.gather = 3;
         }
-        span = fmin(span, 48.0 * p.temperature);      // e^-48: below what a histogram's fixed point resolves
+        return;
     }
-    st.scale = (double)(BINS - 1) / span;
-    st.lin = span > 0.0 && span < INFINITY && st.scale < INFINITY && st.scale > 0.0;
+    st.floor_key = st.cut, st.floor_ties = st.cut_ties;
+    if (st.floor_ties) {
+        const double w = exp(draw_t<T>(st.floor_key, st.top, p.temperature));
+        if (w >= p.min_p) st.floor_mass = w * st.floor_ties;
+    }
+    // below e^-48.6 a weight is nothing in a histogram's fixed point, below min_p it is not kept: with room for all roundings
+    double reach = 48.6;
+    if (p.min_p > 0.0) {
+        reach = fmin(reach, -log(p.min_p) + 1e-9);
+        st.gather = 3;
+    }
+    const double smax = S::value(st.top);
+    const Key low = S::key_of(smax - reach * p.temperature * (1.0 + 1e-12) - fabs(smax) * 1e-14);
+    if (smax < INFINITY && low > st.klo) st.klo = low > 4 ? low - 4 : low;
 }
 
 // A step's histogram over [begin, end) into LDS.  The last bin of the linear step, where all that lies far from the best falls, is
@@ -305,7 +367,7 @@ __device__ void draw_histogram(DrawLds<T>& s, const DrawStep<T>& d, const T* x, 
         const int b = d.bin(k);
         unsigned long long hi = 0, lo = 0;
         if (d.phase == PHASE_TOPP) to_fixed(w, hi, lo);
-        if (d.lin == 1 && b == BINS - 1) {
+        if (d.linear && b == BINS - 1) {
             rest += 1, rest_hi += hi, rest_lo += lo;
         } else {
             atomicAdd(&s.h.count[b], 1u);
@@ -313,7 +375,7 @@ __device__ void draw_histogram(DrawLds<T>& s, const DrawStep<T>& d, const T* x, 
             if (lo) atomicAdd(&s.h.lo[b], lo);
         }
     });
-    if (d.lin == 1) {
+    if (d.linear) {
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) {
             rest += __shfl_xor(rest, o);
@@ -337,7 +399,7 @@ __device__ void draw_decide(DrawLds<T>& s, const DrawRow& p) {
     const int tid = threadIdx.x, b0 = 2 * tid, b1 = b0 + 1;      // bins from the top down
     DrawState<T>& st = s.st;
     const DrawStep<T> d(st, p);
-    const bool first = st.lin == 1 || (st.lin == 0 && st.klo == st.bot && st.khi == st.top);
+    const bool first = st.first;
     if (tid == 0) s.bin = 0xffffffffu, s.any_bin = 0;
     const unsigned long long c0 = s.h.count[b0], c1 = s.h.count[b1];
     unsigned long long all_c;
@@ -347,7 +409,7 @@ __device__ void draw_decide(DrawLds<T>& s, const DrawRow& p) {
     const double above = st.above;
     const long long rank = st.rank;
     if (st.phase == PHASE_TOPK) {
-        spare = first && all_c <= (unsigned long long)rank;                    // fewer valid scores than top_k: no cut
+        spare = first && all_c < (unsigned long long)rank;                     // fewer valid scores than top_k: no cut
         const long long before = (long long)(run_c - c0 - c1);
         if (c0 && before < rank && before + (long long)c0 >= rank) s.bin = b0;
         if (c1 && before + (long long)c0 < rank && before + (long long)(c0 + c1) >= rank) s.bin = b1;
@@ -383,19 +445,10 @@ __device__ void draw_decide(DrawLds<T>& s, const DrawRow& p) {
     } else if (bin == (unsigned)b0 || bin == (unsigned)b1) {
         const bool low = bin == (unsigned)b1;
         const unsigned long long cnt = low ? c1 : c0, before_c = run_c - (low ? c1 : c0 + c1);
-        if (st.lin == 1) {
-            // keys that can fall into the bin: its ends, moved out by more than the rounding of either side
-            const double smax = S::value(st.top);
-            const double hi_s = smax - bin / st.scale * (1.0 - 1e-14), lo_s = smax - (bin + 1) / st.scale * (1.0 + 1e-14);
-            const Key kh = S::key_of(hi_s), kl = S::key_of(lo_s);
-            if (bin > 0 && kh != 0 && st.top - kh > 2) st.khi = kh + 2;
-            if (bin < BINS - 1 && kl != 0 && kl > st.bot && kl - st.bot > 2) st.klo = kl - 2;
-            st.lin = 2, st.lin_bin = (int)bin;
-        } else {
-            const Key hi = st.khi - ((Key)bin << d.shift), span = ((Key)1 << d.shift) - 1;
-            st.klo = hi - st.klo > span ? hi - span : st.klo;
-            st.khi = hi;
-        }
+        Key lo, hi;
+        d.ends((int)bin, lo, hi);
+        st.klo = lo, st.khi = hi;
+        st.first = 0, st.linear_left -= 1;
         st.count_above += (long long)before_c;
         if (st.phase == PHASE_TOPK) {
             st.rank = rank - (long long)before_c;
@@ -415,7 +468,7 @@ __device__ void draw_decide(DrawLds<T>& s, const DrawRow& p) {
                 st.phase = PHASE_PICK;
             }
         } else if (st.count_above + (long long)cnt <= LIST) {
-            st.gather = st.gather_all = 1;
+            st.gather = 2;
         } else if (cnt <= LIST) {
             st.gather = 1;
         }
@@ -424,24 +477,45 @@ __device__ void draw_decide(DrawLds<T>& s, const DrawRow& p) {
     __syncthreads();
 }
 
-// LIST keys or fewer in l.key, l.idx: sort them by rank into l.key2, l.idx2.
+// Bitonic sort of one pair a thread over the first `size` threads (a power of two, at least 64): by rank, or by index.  Partners
+// in one wave exchange through registers, others through LDS (buf_k, buf_i); 1024 pairs take 55 exchanges, 10 of them with
+// barriers, 3 us; every pair counting the ones in front of it took 27.
+template <typename Key, bool BY_INDEX>
+__device__ __forceinline__ void block_sort(Key& k, uint32_t& i, int size, Key* buf_k, uint32_t* buf_i) {
+    const int tid = threadIdx.x;
+    for (int run = 2; run <= size; run <<= 1)
+        for (int step = run >> 1; step > 0; step >>= 1) {
+            Key ok;
+            uint32_t oi;
+            if (step >= 64) {
+                __syncthreads();
+                if (tid < size) buf_k[tid] = k, buf_i[tid] = i;
+                __syncthreads();
+                ok = buf_k[(tid ^ step) & (LIST - 1)], oi = buf_i[(tid ^ step) & (LIST - 1)];
+            } else {
+                ok = __shfl_xor(k, step), oi = __shfl_xor(i, step);
+            }
+            const bool mine_first = BY_INDEX ? i < oi : (k > ok || (k == ok && i < oi));
+            const bool want_first = ((tid & step) == 0) == ((tid & run) == 0 || run == size);
+            if (mine_first != want_first) k = ok, i = oi;      // equal pairs are the fillers: either way the same
+        }
+}
+
+// LIST keys or fewer in l.key, l.idx: sort them by rank into l.key2, l.idx2 (behind them keys of 0).
 template <typename T>
-__device__ void draw_rank(DrawLds<T>& s, int n) {
+__device__ int draw_rank(DrawLds<T>& s, int n) {
     using Key = typename Score<T>::Key;
     const int tid = threadIdx.x;
+    int size = 64;
+    while (size < n) size <<= 1;
     __syncthreads();
-    if (tid < n) {
-        const Key k = s.l.key[tid];
-        const uint32_t ix = s.l.idx[tid];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) {
-            const Key kj = s.l.key[j];
-            rank += (kj > k) || (kj == k && s.l.idx[j] < ix);
-        }
-        s.l.key2[rank] = k;
-        s.l.idx2[rank] = ix;
-    }
+    Key k = tid < n ? s.l.key[tid] : 0;
+    uint32_t ix = tid < n ? s.l.idx[tid] : 0xffffffffu;
+    block_sort<Key, false>(k, ix, size, s.l.key2, s.l.idx2);
     __syncthreads();
+    if (tid < size) s.l.key2[tid] = k, s.l.idx2[tid] = ix;
+    __syncthreads();
+    return size;
 }
 
 // The list holds the keys klo .. khi of a step: the cut is one of them.
@@ -480,7 +554,7 @@ template <typename T>
 __device__ void draw_from_list(DrawLds<T>& s, const DrawArgs& a, const DrawRow& p, int64_t row, int n, typename Score<T>::Key top, double goal) {
     using Key = typename Score<T>::Key;
     const int tid = threadIdx.x;
-    draw_rank(s, n);
+    const int size = draw_rank(s, n);
     // by rank from here on: thread = position
     const Key kr = tid < n ? s.l.key2[tid] : 0;
     const double w = kr ? exp(draw_t<T>(kr, top, p.temperature)) : 0.0;
@@ -494,18 +568,12 @@ __device__ void draw_from_list(DrawLds<T>& s, const DrawArgs& a, const DrawRow& 
     // the kept ones are the first `kept` positions; now in index order
     unsigned long long kept;
     block_scan<unsigned long long>(keep ? 1ull : 0ull, s.red_u, kept);
-    const uint32_t my = s.l.idx2[tid < n ? tid : 0];
-    int place = 0;
-    if (keep)
-        for (int j = 0; j < (int)kept; ++j) place += s.l.idx2[j] < my;
-    if (keep) {                                // l.key was last read by draw_rank, l.c and l.pick not at all
-        s.l.c[place] = w;
-        s.l.pick[place] = my;
-        s.l.key[place] = kr;
-    }
-    __syncthreads();
-    const double wi = tid < (int)kept ? s.l.c[tid] : 0.0;
-    const double ci = block_scan(wi, s.red, total);
+    Key ki = keep ? kr : 0;
+    uint32_t ii = keep ? s.l.idx2[tid] : 0xffffffffu;
+    block_sort<Key, true>(ki, ii, size, s.l.key, s.l.idx);
+    const double wi = tid < (int)kept ? exp(draw_t<T>(ki, top, p.temperature)) : 0.0;
+    const double ci = block_scan(wi, s.red, total);      // its barriers stand between the sort's last reads of l.key and this
+    if (tid < (int)kept) s.l.key[tid] = ki, s.l.pick[tid] = ii;
     if (tid < (int)kept) s.l.c[tid] = ci;
     __syncthreads();
     for (int64_t q = tid; q < a.draws; q += DRAW_THREADS) {
@@ -521,6 +589,59 @@ __device__ void draw_from_list(DrawLds<T>& s, const DrawArgs& a, const DrawRow& 
         a.index[row * a.draws + q] = s.l.pick[lo];
         if (a.logp) a.logp[row * a.draws + q] = draw_t<T>(s.l.key[lo], top, p.temperature) - log(total);
     }
+}
+
+// One workgroup: the scores of [begin, end) that count go to the list; behind LIST of them nothing is written and the counter
+// stops growing soon.
+template <typename T>
+__device__ void draw_gather(DrawLds<T>& s, const DrawStep<T>& d, const T* x, uint32_t begin, uint32_t end) {
+    using Key = typename Score<T>::Key;
+    each_score(x, begin, end, [&](Key k, uint32_t i) {
+        double w;
+        if (!d.counts(k, w)) return;
+        if (__hip_atomic_load(&s.st.n_list, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) > LIST) return;
+        const uint32_t at = atomicAdd(&s.st.n_list, 1u);
+        if (at < LIST) s.l.key[at] = k, s.l.idx[at] = i;
+    });
+    __syncthreads();
+}
+
+// A list of a step is in l: the picks (true), or the next step.
+template <typename T>
+__device__ bool draw_use_list(DrawLds<T>& s, const DrawArgs& a, const DrawRow& p, int64_t row) {
+    const int gather = s.st.gather, m = min((int)s.st.n_list, LIST);
+    const bool over = s.st.n_list > LIST;
+    if (gather == 1) {
+        draw_cut_from_list(s, p, m);
+    } else if (gather == 3 && over) {          // the trial failed: on with histograms
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            s.st.gather = 0;
+            s.st.n_list = 0;
+            if (s.st.phase == PHASE_TOPP && !(p.top_p < 1.0)) s.st.phase = PHASE_PICK;
+        }
+        __syncthreads();
+    } else {
+        draw_from_list<T>(s, a, p, row, m, s.st.top, gather == 2 && s.st.phase == PHASE_TOPP ? s.st.goal : -1.0);
+        return true;
+    }
+    return false;
+}
+
+// One workgroup takes all steps that are left; true if that included the picks.
+template <typename T>
+__device__ bool draw_search(DrawLds<T>& s, const DrawArgs& a, const DrawRow& p, const T* x, int64_t row) {
+    while (s.st.phase < PHASE_PICK) {
+        const DrawStep<T> d(s.st, p);
+        if (s.st.gather) {
+            draw_gather(s, d, x, 0, (uint32_t)a.cols);
+            if (draw_use_list(s, a, p, row)) return true;
+        } else {
+            draw_histogram(s, d, x, 0, (uint32_t)a.cols);
+            draw_decide(s, p);
+        }
+    }
+    return false;
 }
 
 // The weights of a row once the cut is known.
@@ -629,9 +750,9 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_row(DrawArgs a) {
     const T* x = (const T*)a.scores + row * a.stride;
     const uint32_t n = (uint32_t)a.cols;
     const DrawRow p(a, row);
-    Key top, bot;
+    Key top, bot, own;
     uint32_t idx;
-    draw_extremes(s, x, 0, n, top, bot, idx);
+    draw_extremes(s, x, 0, n, top, bot, idx, own);
     if (top == 0 || p.greedy) {
         draw_same<T>(a, row, top ? (int64_t)idx : -1, top ? 0.0 : -INFINITY);
         return;
@@ -641,32 +762,20 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_row(DrawArgs a) {
         draw_from_list<T>(s, a, p, row, (int)n, top, -1.0);
         return;
     }
+    Key bound = 0;
+    if (p.top_k > 0 && p.top_k <= DRAW_THREADS) {      // the threads' own maxima, sorted: top_k of them reach the top_k-th
+        uint32_t none = tid;
+        block_sort<Key, false>(own, none, DRAW_THREADS, s.l.key2, s.l.idx2);
+        if (tid == (int)p.top_k - 1) s.red_k[0][0] = own;
+        __syncthreads();
+        bound = s.red_k[0][0];
+    }
     if (tid == 0) {
-        s.st.top = top, s.st.bot = bot, s.st.best_idx = idx, s.st.cut = 0, s.st.cut_ties = 0;
-        draw_begin(s.st, p, PHASE_TOPK);
+        s.st.top = top, s.st.bot = bot, s.st.cut = 0, s.st.cut_ties = 0;
+        draw_begin(s.st, p, PHASE_TOPK, bound);
     }
     __syncthreads();
-    while (s.st.phase < PHASE_PICK) {
-        const DrawStep<T> d(s.st, p);
-        if (!s.st.gather) {
-            draw_histogram(s, d, x, 0, n);
-            draw_decide(s, p);
-            continue;
-        }
-        each_score(x, 0, n, [&](Key k, uint32_t i) {
-            double w;
-            if (!d.counts(k, w)) return;
-            const uint32_t at = atomicAdd(&s.st.n_list, 1u);
-            if (at < LIST) s.l.key[at] = k, s.l.idx[at] = i;
-        });
-        __syncthreads();
-        const int m = min((int)s.st.n_list, LIST);
-        if (s.st.gather_all) {
-            draw_from_list<T>(s, a, p, row, m, top, s.st.phase == PHASE_TOPP ? s.st.goal : -1.0);
-            return;
-        }
-        draw_cut_from_list(s, p, m);
-    }
+    if (draw_search(s, a, p, x, row)) return;
 
     // kept mass of the row's tiles, in index order
     const DrawKept<T> kw(s.st, p);
@@ -743,19 +852,22 @@ __device__ __forceinline__ void draw_share(uint32_t n, uint32_t b, uint32_t bloc
     end = min(n, begin + each);
 }
 
-// True in the workgroup that arrives last of the `blocks` of its row; what the others wrote before is then visible to it.  The
-// counter is back at zero for the next step.
+// True in the workgroup that arrives last of the `blocks` of its row; what the others wrote before is then visible to it.  One
+// thread fences for its workgroup, behind the barrier that orders the other threads' writes before it: a fence writes the L2
+// back, and one of every wave cost 8 times the step itself.  The counter is back at zero for the next step.
 template <typename T>
 __device__ bool draw_last(DrawLds<T>& s, unsigned int* ticket, uint32_t blocks) {
-    __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
+        __threadfence();
         const unsigned int t = atomicAdd(ticket, 1u);
         s.last = t == blocks - 1;
-        if (s.last) *ticket = 0;
+        if (s.last) {
+            __threadfence();
+            *ticket = 0;
+        }
     }
     __syncthreads();
-    if (s.last) __threadfence();
     return s.last;
 }
 
@@ -769,9 +881,9 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_start(DrawArgs a, char* w
     const T* x = (const T*)a.scores + row * a.stride;
     uint32_t begin, end;
     draw_share((uint32_t)a.cols, blockIdx.x, gridDim.x, begin, end);
-    Key top, bot;
+    Key top, bot, own;
     uint32_t idx;
-    draw_extremes(s, x, begin, end, top, bot, idx);
+    draw_extremes(s, x, begin, end, top, bot, idx, own);
     if (threadIdx.x == 0) rw.w->top[blockIdx.x] = top, rw.w->bot[blockIdx.x] = bot, rw.w->top_idx[blockIdx.x] = idx;
     if (blockIdx.x == 0) {
         for (int b = threadIdx.x; b < BINS; b += DRAW_THREADS) rw.w->count[b] = 0, rw.w->hi[b] = 0, rw.w->lo[b] = 0;
@@ -783,14 +895,23 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_start(DrawArgs a, char* w
 template <typename T>
 __global__ __launch_bounds__(DRAW_THREADS) void k_draw_begin(DrawArgs a, char* work, int shares) {
     using Key = typename Score<T>::Key;
-    __shared__ Key rk[2][16];
-    __shared__ uint32_t ri[16];
+    __shared__ Key rk[2][16], sort_k[LIST], bound_s;
+    __shared__ uint32_t ri[16], sort_i[LIST];
     const int64_t row = blockIdx.x;
     const DrawRowWork<T> rw(work, row, a.cols);
     const DrawRow p(a, row);
     const int tid = threadIdx.x;
     Key bk = tid < shares ? rw.w->top[tid] : 0, lk = tid < shares ? rw.w->bot[tid] : ~(Key)0;
     uint32_t bi = tid < shares ? rw.w->top_idx[tid] : 0;
+    Key bound = 0;
+    if (p.top_k > 0 && p.top_k <= shares) {    // the shares' maxima, sorted: top_k of them reach the top_k-th
+        Key own = bk;
+        uint32_t none = tid;
+        block_sort<Key, false>(own, none, DRAW_THREADS, sort_k, sort_i);
+        if (tid == (int)p.top_k - 1) bound_s = own;
+        __syncthreads();
+        bound = bound_s;
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
         const Key k = __shfl_xor(bk, o), l = __shfl_xor(lk, o);
@@ -807,9 +928,9 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_begin(DrawArgs a, char* w
     if (bk == 0 || p.greedy) draw_same<T>(a, row, bk ? (int64_t)bi : -1, bk ? 0.0 : -INFINITY);
     if (tid == 0) {
         DrawState<T>& st = rw.w->st;
-        st.top = bk, st.bot = lk, st.best_idx = bi, st.cut = 0, st.cut_ties = 0, st.n_list = 0;
+        st.top = bk, st.bot = lk, st.cut = 0, st.cut_ties = 0, st.n_list = 0;
         if (bk == 0 || p.greedy) st.phase = PHASE_DONE;
-        else draw_begin(st, p, PHASE_TOPK);
+        else draw_begin(st, p, PHASE_TOPK, bound);
     }
 }
 
@@ -827,13 +948,14 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_step(DrawArgs a, char* wo
     const bool gather = rw.w->st.gather;
     uint32_t begin, end;
     draw_share((uint32_t)a.cols, blockIdx.x, gridDim.x, begin, end);
-    if (gather) {
-        each_score(x, begin, end, [&](Key k, uint32_t i) {
-            double w;
-            if (!d.counts(k, w)) return;
-            const uint32_t at = atomicAdd(&rw.w->st.n_list, 1u);
-            if (at < LIST) rw.w->key[at] = k, rw.w->idx[at] = i;
-        });
+    if (gather) {                              // a list of the share's own, then one place in the row's
+        if (tid == 0) s.st.n_list = 0;
+        __syncthreads();
+        draw_gather(s, d, x, begin, end);
+        if (tid == 0 && s.st.n_list) s.bin = atomicAdd(&rw.w->st.n_list, s.st.n_list);
+        __syncthreads();
+        const uint32_t mine = s.st.n_list, at = mine ? s.bin + tid : LIST;
+        if (mine <= LIST && tid < (int)mine && at < LIST) rw.w->key[at] = s.l.key[tid], rw.w->idx[at] = s.l.idx[tid];
     } else {
         draw_histogram(s, d, x, begin, end);
         for (int b = tid; b < BINS; b += DRAW_THREADS)
@@ -862,22 +984,37 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_step(DrawArgs a, char* wo
         __syncthreads();
         draw_decide(s, p);
     } else {
-        const int m = min((int)s.st.n_list, LIST);
-        if (tid < m) {
+        if (tid < min((int)s.st.n_list, LIST)) {
             s.l.key[tid] = __hip_atomic_load(&rw.w->key[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             s.l.idx[tid] = fresh32(&rw.w->idx[tid]);
         }
-        if (s.st.gather_all) {
-            draw_from_list<T>(s, a, p, row, m, s.st.top, s.st.phase == PHASE_TOPP ? s.st.goal : -1.0);
-            __syncthreads();
-            if (tid == 0) s.st.phase = PHASE_DONE;
-        } else {
-            draw_cut_from_list(s, p, m);
+        const bool done = draw_use_list(s, a, p, row);
+        __syncthreads();
+        if (tid == 0) {
+            if (done) s.st.phase = PHASE_DONE;
+            s.st.n_list = 0;
         }
-        if (tid == 0) s.st.n_list = 0;
     }
     __syncthreads();
     if (tid == 0) rw.w->st = s.st;
+}
+
+// What the launched steps left over, if scores are spread so badly that they did: one workgroup a row.
+template <typename T>
+__global__ __launch_bounds__(DRAW_THREADS) void k_draw_rest(DrawArgs a, char* work) {
+    __shared__ DrawLds<T> s;
+    const int64_t row = blockIdx.x;
+    const DrawRowWork<T> rw(work, row, a.cols);
+    if (rw.w->st.phase >= PHASE_PICK) return;
+    const DrawRow p(a, row);
+    if (threadIdx.x == 0) s.st = rw.w->st;
+    __syncthreads();
+    const bool done = draw_search(s, a, p, (const T*)a.scores + row * a.stride, row);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        if (done) s.st.phase = PHASE_DONE;
+        rw.w->st = s.st;
+    }
 }
 
 // Mass above the cut and ties of every tile, a wave each.
@@ -980,12 +1117,13 @@ hipError_t draw_rows(hipStream_t st, const DrawArgs& a, char* work) {
         const dim3 wide((unsigned)blocks, (unsigned)b.rows), one((unsigned)b.rows);
         hipLaunchKernelGGL(k_draw_start<T>, wide, dim3(DRAW_THREADS), 0, st, b, w);
         hipLaunchKernelGGL(k_draw_begin<T>, one, dim3(DRAW_THREADS), 0, st, b, w, (int)blocks);
-        // a phase takes the linear step, at most ceil(bits / 11) steps on the keys and one for the list; what is decided earlier
-        // leaves the rest of the launches with nothing to do
+        // a phase rarely takes more than a list on trial, two linear steps, one on the keys and one more list; what is decided
+        // earlier leaves the rest of the launches with nothing to do, what is not is left to one workgroup a row
         const bool by_row = a.params != nullptr;
-        const int phases = (by_row || (a.top_k > 0 && a.top_k < a.cols)) + (by_row || a.top_p < 1.0);
-        const int steps = phases * (2 + (Score<T>::BITS + DIGIT - 1) / DIGIT);
+        const int phases = (by_row || (a.top_k > 0 && a.top_k < a.cols)) + (by_row || a.top_p < 1.0 || a.min_p > 0.0);
+        const int steps = phases == 0 ? 0 : a.top_p < 1.0 || phases == 2 || by_row ? 1 + 4 * phases : 4;
         for (int i = 0; i < steps; ++i) hipLaunchKernelGGL(k_draw_step<T>, wide, dim3(DRAW_THREADS), 0, st, b, w);
+        if (phases) hipLaunchKernelGGL(k_draw_rest<T>, one, dim3(DRAW_THREADS), 0, st, b, w);
         const int64_t tiles = ceil_div(a.cols, TILE);
         hipLaunchKernelGGL(k_draw_mass<T>, dim3((unsigned)std::min<int64_t>(ceil_div(tiles, 4), 4096), (unsigned)b.rows), dim3(256), 0, st, b, w);
         hipLaunchKernelGGL(k_draw_sums<T>, one, dim3(DRAW_THREADS), 0, st, b, w);
