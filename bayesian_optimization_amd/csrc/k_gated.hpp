@@ -39,21 +39,40 @@ __device__ __forceinline__ f32x4 mma<float>(const uint4& a, const uint4& b, f32x
 }
 
 // act(g) and act'(g).  silu through the logistic function, whose exponential saturates to 0 or infinity with the right limit;
-// gelu through erfc, which keeps the far negative tail that 1 + erf loses.
+// gelu through erfc, which keeps the far negative tail that 1 + erf loses.  For results of 16 bits the hardware's exponential and
+// reciprocal (one unit in the last place each) and, for erfc, the five-term rational form of Abramowitz and Stegun 7.1.26 (1.5e-7):
+// the activation of every output is as much vector work as a short contraction is matrix work (1 M x 256 -> 512: 1.27 -> 0.83 ms).
+template <typename T>
 __device__ __forceinline__ void activation(float g, int act, float& a, float& da) {
-    if (act == GPBO_ACT_SILU) {
-        const float s = 1.0f / (1.0f + expf(-g));
-        a = g * s;
-        da = s + a * (1.0f - s);
+    if constexpr (sizeof(T) == 4) {
+        if (act == GPBO_ACT_SILU) {
+            const float s = 1.0f / (1.0f + expf(-g));
+            a = g * s;
+            da = s + a * (1.0f - s);
+        } else {
+            const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
+            a = g * cdf;
+            da = cdf + g * (0.39894228040143268f * expf(-0.5f * g * g));
+        }
     } else {
-        const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
-        a = g * cdf;
-        da = cdf + g * (0.39894228040143268f * expf(-0.5f * g * g));
+        if (act == GPBO_ACT_SILU) {
+            const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * g));
+            a = g * s;
+            da = s + a * (1.0f - s);
+        } else {
+            const float e = __builtin_amdgcn_exp2f(-0.72134752044448170f * g * g);      // exp(-g^2 / 2)
+            const float t = __builtin_amdgcn_rcpf(1.0f + (0.3275911f * 0.70710678118654752f) * fabsf(g));
+            const float q = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+            const float cdf = g < 0.0f ? q : 1.0f - q;
+            a = g * cdf;
+            da = cdf + 0.39894228040143268f * g * e;
+        }
     }
 }
+template <typename T>
 __device__ __forceinline__ float activate(float g, int act) {
     float a, da;
-    activation(g, act, a, da);
+    activation<T>(g, act, a, da);
     return a;
 }
 
@@ -192,7 +211,7 @@ __global__ __launch_bounds__(256) void k_gated_tile(GatedArgs g) {
                 if (col + r >= g.n) continue;
                 if constexpr (MODE == GATED_FWD) {
                     const float gv = acc[0][i][j][r], uv = acc[NB - 1][i][j][r];
-                    ((T*)g.out[0])[row * g.os + col + r] = from_float<T>(activate(gv, g.act) * uv);
+                    ((T*)g.out[0])[row * g.os + col + r] = from_float<T>(activate<T>(gv, g.act) * uv);
                     if (g.keep_g) {
                         g.keep_g[row * g.n + col + r] = gv;
                         g.keep_u[row * g.n + col + r] = uv;
@@ -204,6 +223,102 @@ __global__ __launch_bounds__(256) void k_gated_tile(GatedArgs g) {
                 }
             }
         }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Small products: what counts is how soon the last load is back, so 32 x 32 outputs a workgroup, its 8 waves take turns along the
+// contraction with fragments loaded straight into registers, and their sums are joined in LDS in a fixed order.  No staging, no
+// barrier until then (95 x 621 -> 128 in 32 bits: 40 -> 6 us against the 64 x 64 tile, which has 4 workgroups of 20 steps there).
+constexpr int SB = 32, SMALL_WAVES = 8;
+
+template <typename T, bool KC>
+__device__ __forceinline__ uint4 small_fragment(const Operand& o, int64_t row, int64_t k, int64_t k1) {
+    constexpr int V = 16 / sizeof(T);
+    const T* p = (const T*)o.p;
+    Pack<T> r;
+    if constexpr (KC) {
+        if (k + V <= k1) r = load_pack(p + row * o.sr + k);
+        else
+#pragma unroll
+            for (int j = 0; j < V; ++j) r.v[j] = k + j < k1 ? p[row * o.sr + k + j] : from_float<T>(0.0f);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) r.v[j] = k + j < k1 ? p[(k + j) * o.sk + row] : from_float<T>(0.0f);
+    }
+    return __builtin_bit_cast(uint4, r);
+}
+
+template <typename T, int MODE, bool AKC, bool BKC>
+__global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small(GatedArgs g) {
+    constexpr int SLAB = 64 / sizeof(T), V = 16 / sizeof(T), NB = MODE == GATED_FWD ? 2 : 1;
+    __shared__ f32x4 sums[SMALL_WAVES][NB * 4][64];
+    const int64_t nt = (g.n + SB - 1) / SB;
+    const int64_t row0 = (int64_t)(blockIdx.x / nt) * SB, col0 = (int64_t)(blockIdx.x % nt) * SB;
+    const int z = MODE == GATED_PAIR ? blockIdx.z : 0, split = blockIdx.y;
+    const int64_t per = ((g.k + g.splits - 1) / g.splits + SLAB - 1) / SLAB * SLAB;
+    const int64_t kb = min(split * per, g.k), ke = min(kb + per, g.k);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    f32x4 acc[NB][2][2];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) acc[b][i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    int64_t ra[2], rb[2];                      // rows behind the last repeat it: their outputs are not stored
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ra[i] = min(row0 + i * 16 + (lane & 15), g.m - 1), rb[i] = min(col0 + i * 16 + (lane & 15), g.n - 1);
+#pragma unroll
+    for (int part = 0; part < (MODE == GATED_SUM ? 2 : 1); ++part) {
+        const Operand oa = MODE == GATED_PAIR && z ? g.a[1] : g.a[part], ob = g.b[part];
+#pragma unroll 4
+        for (int64_t k0 = kb + wave * SLAB; k0 < ke; k0 += SMALL_WAVES * SLAB) {
+            const int64_t k = k0 + (lane >> 4) * V;
+            uint4 fa[2], fb[NB][2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                fa[i] = small_fragment<T, AKC>(oa, ra[i], k, ke);
+                fb[0][i] = small_fragment<T, BKC>(ob, rb[i], k, ke);
+                if constexpr (NB == 2) fb[NB - 1][i] = small_fragment<T, BKC>(g.b[1], rb[i], k, ke);
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) acc[b][i][j] = mma<T>(fb[b][j], fa[i], acc[b][i][j]);
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) sums[wave][b * 4 + i * 2 + j][lane] = acc[b][i][j];
+    __syncthreads();
+    // wave f of the first four takes fragment f
+    if (wave >= 4) return;
+    f32x4 v[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        v[b] = sums[0][b * 4 + wave][lane];
+#pragma unroll
+        for (int w = 1; w < SMALL_WAVES; ++w) v[b] += sums[w][b * 4 + wave][lane];
+    }
+    const int64_t row = row0 + (wave >> 1) * 16 + (lane & 15), col = col0 + (wave & 1) * 16 + (lane >> 4) * 4;
+    if (row >= g.m) return;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        if (col + r >= g.n) continue;
+        if constexpr (MODE == GATED_FWD) {
+            ((T*)g.out[0])[row * g.os + col + r] = from_float<T>(activate<T>(v[0][r], g.act) * v[NB - 1][r]);
+            if (g.keep_g) g.keep_g[row * g.n + col + r] = v[0][r], g.keep_u[row * g.n + col + r] = v[NB - 1][r];
+        } else if (g.splits > 1) {
+            g.part[(((int64_t)z * g.splits + split) * g.m + row) * g.n + col + r] = v[0][r];
+        } else {
+            ((T*)(z ? g.out[1] : g.out[0]))[row * g.os + col + r] = from_float<T>(v[0][r]);
+        }
+    }
 }
 
 // The split sums of one output, added in split order.
@@ -246,7 +361,7 @@ __global__ __launch_bounds__(256) void k_gated_slopes(const T* __restrict__ dh, 
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             float a, da;
-            activation(gv[i], act, a, da);
+            activation<T>(gv[i], act, a, da);
             og.v[i] = from_float<T>(to_float(pd.v[i]) * uv[i] * da);
             ou.v[i] = from_float<T>(to_float(pd.v[i]) * a);
         }
@@ -261,10 +376,27 @@ __global__ __launch_bounds__(256) void k_gated_slopes(const T* __restrict__ dh, 
     }
 }
 
-// Pieces of the contraction for a product of few tiles: up to two workgroups a CU, at least 4 steps each.
-inline int gated_splits(int64_t tiles, int64_t k, int64_t step) {
-    if (tiles < 1 || tiles >= 256) return 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(512, tiles), k / (4 * step)));
+// A product that the whole-step kernels do not take: the small form up to two workgroups of 512 threads a CU (twice over), the 64 x 64
+// tiles above; either with the contraction in pieces where the outputs alone leave CUs empty, of at least 4 steps.
+struct AnyPlan {
+    bool small = true;
+    int splits = 1;
+};
+template <typename T>
+AnyPlan any_plan(int64_t m, int64_t n, int64_t k, int zs, bool can_split) {
+    AnyPlan p;
+    const int64_t t32 = zs * ceil_div(m, SB) * ceil_div(n, SB), t64 = zs * ceil_div(m, TB) * ceil_div(n, TB);
+    p.small = t32 <= 1024;
+    const int64_t tiles = p.small ? t32 : t64, step = p.small ? SMALL_WAVES * 64 / (int64_t)sizeof(T) : STEP_BYTES / (int64_t)sizeof(T);
+    if (can_split && tiles > 0 && tiles < 256) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(512, tiles), k / (4 * step)));
+    return p;
+}
+template <typename T, int MODE, bool AKC, bool BKC>
+void launch_any(hipStream_t st, const GatedArgs& g, const AnyPlan& p) {
+    const int64_t b = p.small ? SB : TB;
+    const dim3 grid((unsigned)(ceil_div(g.m, b) * ceil_div(g.n, b)), (unsigned)g.splits, MODE == GATED_PAIR ? 2 : 1);
+    if (p.small) hipLaunchKernelGGL((k_gated_small<T, MODE, AKC, BKC>), grid, dim3(64 * SMALL_WAVES), 0, st, g);
+    else hipLaunchKernelGGL((k_gated_tile<T, MODE, AKC, BKC>), grid, dim3(256), 0, st, g);
 }
 
 }  // namespace gpbo_static

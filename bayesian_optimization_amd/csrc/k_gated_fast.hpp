@@ -138,7 +138,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 256 ? 1 : 2) void k_gated_fast(
             float v[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                if constexpr (MODE == GATED_FWD) v[r] = activate(acc[i][j][r], g.act) * acc[i][j + FN / 2][r];
+                if constexpr (MODE == GATED_FWD) v[r] = activate<T>(acc[i][j][r], g.act) * acc[i][j + FN / 2][r];
                 else v[r] = acc[i][j][r];
             }
             if (MODE != GATED_FWD && g.splits > 1) {
@@ -248,7 +248,7 @@ __global__ __launch_bounds__(256) void k_gated_slopes_both(const T* __restrict__
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             float a, da;
-            activation(gv[k], act, a, da);
+            activation<T>(gv[k], act, a, da);
             og[k] = from_float<T>(k < len ? to_float(dv[k]) * uv[k] * da : 0.0f);
             ou[k] = from_float<T>(k < len ? to_float(dv[k]) * a : 0.0f);
             tg[ty + i * 16][tx * 4 + k] = og[k];
@@ -269,6 +269,53 @@ __global__ __launch_bounds__(256) void k_gated_slopes_both(const T* __restrict__
         for (int k = 0; k < 4; ++k) og[k] = tg[tx * 4 + k][ty + i * 16], ou[k] = tu[tx * 4 + k][ty + i * 16];
         __builtin_memcpy(dgt + c * mp + r, og, sizeof(og));
         __builtin_memcpy(dut + c * mp + r, ou, sizeof(ou));
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// A few rows (one candidate at a time): bound by reading the weights once.  A wave takes one hidden unit: both its weight rows in
+// 16-byte packs, R rows of x against them, sums over the lanes at the end.
+template <typename T, int R>
+__global__ __launch_bounds__(256) void k_gated_few(GatedArgs g) {
+    constexpr int V = Pack<T>::N;
+    const int lane = threadIdx.x & 63;
+    const int64_t h = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), row0 = (int64_t)blockIdx.y * R;
+    if (h >= g.n) return;
+    const T *wg = (const T*)g.b[0].p + h * g.b[0].sr, *wu = (const T*)g.b[1].p + h * g.b[1].sr;
+    const T* x[R];
+    float sg[R], su[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) x[r] = (const T*)g.a[0].p + min(row0 + r, g.m - 1) * g.a[0].sr, sg[r] = su[r] = 0.0f;
+    const int64_t whole = g.k / V * V;
+#pragma unroll 4
+    for (int64_t k = lane * V; k < whole; k += 64 * V) {
+        const Pack<T> pg = load_pack(wg + k), pu = load_pack(wu + k);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const Pack<T> px = load_pack(x[r] + k);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                sg[r] = fmaf(to_float(px.v[i]), to_float(pg.v[i]), sg[r]);
+                su[r] = fmaf(to_float(px.v[i]), to_float(pu.v[i]), su[r]);
+            }
+        }
+    }
+    if (whole + lane < g.k) {
+        const float vg = to_float(wg[whole + lane]), vu = to_float(wu[whole + lane]);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float v = to_float(x[r][whole + lane]);
+            sg[r] = fmaf(v, vg, sg[r]);
+            su[r] = fmaf(v, vu, su[r]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const float a = wave_sum(sg[r]), b = wave_sum(su[r]);
+        if (lane == 0 && row0 + r < g.m) {
+            ((T*)g.out[0])[(row0 + r) * g.os + h] = from_float<T>(activate<T>(a, g.act) * b);
+            if (g.keep_g) g.keep_g[(row0 + r) * g.n + h] = a, g.keep_u[(row0 + r) * g.n + h] = b;
+        }
     }
 }
 
@@ -294,7 +341,7 @@ ForwardPlan forward_plan(int64_t m, int64_t k, int64_t h) {
     p.kp = round_up(k, KS);
     p.fast = m * h >= 128 * 64 * 64 && 4 * m * h * k >= (int64_t)1 << 31 && k * (int64_t)sizeof(T) < (1 << 23);
     p.pack = p.fast && k % KS != 0;
-    if (ceil_div(m, 256) * ceil_div(h, 128) >= 256 && k >= 8 * KS) p.tile = 256;
+    if (ceil_div(m, 256) * ceil_div(h, 128) >= 256) p.tile = 256;
     p.x_bytes = round_up(m * p.kp * (int64_t)sizeof(T), 256);
     p.w_bytes = round_up(h * p.kp * (int64_t)sizeof(T), 256);
     return p;
@@ -329,9 +376,14 @@ hipError_t gated_forward(hipStream_t st, GatedArgs g, char* work) {
         }
         static_assert(KS >= 32, "a step");
         launch_fast<T, GATED_FWD>(st, g, p.tile);
+    } else if (g.m <= 16) {
+        const unsigned hidden = (unsigned)ceil_div(g.n, 4);
+        if (g.m == 1) hipLaunchKernelGGL((k_gated_few<T, 1>), dim3(hidden, 1), dim3(256), 0, st, g);
+        else if (g.m == 2) hipLaunchKernelGGL((k_gated_few<T, 2>), dim3(hidden, 1), dim3(256), 0, st, g);
+        else if (g.m <= 4) hipLaunchKernelGGL((k_gated_few<T, 4>), dim3(hidden, 1), dim3(256), 0, st, g);
+        else hipLaunchKernelGGL((k_gated_few<T, 8>), dim3(hidden, (unsigned)ceil_div(g.m, 8)), dim3(256), 0, st, g);
     } else {
-        const int64_t tiles = ceil_div(g.m, TB) * ceil_div(g.n, TB);
-        hipLaunchKernelGGL((k_gated_tile<T, GATED_FWD, true, true>), dim3((unsigned)tiles), dim3(256), 0, st, g);
+        launch_any<T, GATED_FWD, true, true>(st, g, any_plan<T>(g.m, g.n, g.k, 1, false));
     }
     return hipGetLastError();
 }
@@ -341,6 +393,7 @@ hipError_t gated_forward(hipStream_t st, GatedArgs g, char* work) {
 struct BackwardPlan {
     bool fast = false;
     int tile_x = 128, tile_w = 128, splits_x = 1, splits_w = 1;
+    AnyPlan any_x, any_w;
     int64_t hp = 0, mp = 0;
     int64_t d_bytes = 0, dt_bytes = 0, xt_bytes = 0, wt_bytes = 0, part_bytes = 0;
     int64_t bytes() const { return 2 * d_bytes + 2 * dt_bytes + xt_bytes + 2 * wt_bytes + part_bytes; }
@@ -364,8 +417,8 @@ BackwardPlan backward_plan(int64_t m, int64_t k, int64_t h) {
         p.xt_bytes = round_up(k * p.mp * B, 256), p.wt_bytes = round_up(k * p.hp * B, 256);
     } else {
         p.d_bytes = round_up(m * h * B, 256);
-        p.splits_x = gated_splits(ceil_div(m, TB) * ceil_div(k, TB), h, KS);
-        p.splits_w = gated_splits(2 * ceil_div(h, TB) * ceil_div(k, TB), m, KS);
+        p.any_x = any_plan<T>(m, k, h, 1, true), p.any_w = any_plan<T>(h, k, m, 2, true);
+        p.splits_x = p.any_x.splits, p.splits_w = p.any_w.splits;
     }
     p.part_bytes = std::max<int64_t>(p.splits_x > 1 ? p.splits_x * m * k * 4 : 0, p.splits_w > 1 ? 2 * p.splits_w * h * k * 4 : 0);
     return p;
@@ -406,8 +459,7 @@ hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const voi
             launch_fast<T, GATED_SUM>(st, g, p.tile_x);
         } else {
             g.a[0] = {dg, h, 1}, g.a[1] = {du, h, 1}, g.b[0] = {wg, 1, ws}, g.b[1] = {wu, 1, ws}, g.k = h;
-            hipLaunchKernelGGL((k_gated_tile<T, GATED_SUM, true, false>), dim3((unsigned)(ceil_div(m, TB) * ceil_div(k, TB)), (unsigned)g.splits),
-                               dim3(256), 0, st, g);
+            launch_any<T, GATED_SUM, true, false>(st, g, p.any_x);
         }
         if (g.splits > 1) hipLaunchKernelGGL(k_gated_join<T>, dim3((unsigned)ceil_div(m * k, 256), 1), dim3(256), 0, st, g);
     }
@@ -419,8 +471,7 @@ hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const voi
             launch_fast<T, GATED_PAIR>(st, g, p.tile_w);
         } else {
             g.a[0] = {dg, 1, h}, g.a[1] = {du, 1, h}, g.b[0] = g.b[1] = {x, 1, xs}, g.k = m;
-            hipLaunchKernelGGL((k_gated_tile<T, GATED_PAIR, false, false>), dim3((unsigned)(ceil_div(h, TB) * ceil_div(k, TB)), (unsigned)g.splits, 2),
-                               dim3(256), 0, st, g);
+            launch_any<T, GATED_PAIR, false, false>(st, g, p.any_w);
         }
         if (g.splits > 1) hipLaunchKernelGGL(k_gated_join<T>, dim3((unsigned)ceil_div(h * k, 256), 2), dim3(256), 0, st, g);
     }
