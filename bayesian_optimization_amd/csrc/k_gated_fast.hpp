@@ -341,7 +341,7 @@ ForwardPlan forward_plan(int64_t m, int64_t k, int64_t h) {
     p.kp = round_up(k, KS);
     p.fast = m * h >= 128 * 64 * 64 && 4 * m * h * k >= (int64_t)1 << 31 && k * (int64_t)sizeof(T) < (1 << 23);
     p.pack = p.fast && k % KS != 0;
-    if (ceil_div(m, 256) * ceil_div(h, 128) >= 256) p.tile = 256;
+    if (ceil_div(m, 256) * ceil_div(h, 128) >= 256 && k >= 8 * KS) p.tile = 256;
     p.x_bytes = round_up(m * p.kp * (int64_t)sizeof(T), 256);
     p.w_bytes = round_up(h * p.kp * (int64_t)sizeof(T), 256);
     return p;

@@ -7,19 +7,25 @@ import math
 import torch
 
 from . import _lib as L
-from ._device import TYPES, check_status, on_device, pointer, rows_of, stream_of, workspace
+from ._device import TYPES, Tensor, check_status, pointer, rows_of, scratch, stream_of, tensor, workspace
 
 _TYPES = dict(TYPES)
 _TYPES[torch.float64] = L.TYPE_F64
+_f64 = torch.float64
 
 
-def _setting(name, v, rows, device):
-    """A Python number, or a tensor of one number per row."""
-    if isinstance(v, torch.Tensor) and v.dim() > 0:
-        if v.shape != (rows,) or v.device != device:
-            raise ValueError('%s must be a number or a (%d,) tensor on %s; got %s on %s' % (name, rows, device, tuple(v.shape), v.device))
-        return v.detach().to(torch.float64)
-    return float(v)
+def _per_row(settings, rows, device, at):
+    """(rows, 4) float64 on the GPU from four settings, each a number or a tensor of one number per row."""
+    columns = []
+    for name, v in zip(('temperature', 'top_k', 'top_p', 'min_p'), settings):
+        if isinstance(v, Tensor) and v.dim() > 0:
+            tensor(name, v, at)
+            if tuple(v.shape) != (rows,):
+                raise ValueError('%s must be a number or a (%d,) tensor; got %s' % (name, rows, tuple(v.shape)))
+            columns.append(v.detach().to(_f64))
+        else:
+            columns.append(torch.full((rows,), float(v), dtype=_f64, device=device))
+    return torch.stack(columns, dim=1)
 
 
 def sample(scores, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -32,31 +38,29 @@ def sample(scores, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     whole.  temperature = 0 takes the best score.  Each setting is a number, or a (rows,) tensor on the same GPU.
     Returns (index (rows, draws) int64, logp (rows, draws) float64); index -1 and logp -inf in a row with nothing to draw.
     Runs on the current stream and does not wait for it."""
-    rows, cols, stride = rows_of('scores', scores, _TYPES)
-    on_device('u', u, scores.device)
-    if u.dim() != 2 or u.shape[0] != rows or u.dtype != torch.float64:
+    rows, cols, stride, at = rows_of('scores', scores, _TYPES)
+    tensor('u', u, at)
+    if u.dim() != 2 or u.shape[0] != rows or u.dtype != _f64:
         raise ValueError('u must be (%d, draws) float64; got %s %s' % (rows, tuple(u.shape), u.dtype))
-    settings = [_setting(n, v, rows, scores.device) for n, v in
-                (('temperature', temperature), ('top_k', top_k), ('top_p', top_p), ('min_p', min_p))]
-    params = None
-    if any(isinstance(v, torch.Tensor) for v in settings):
-        params = torch.stack([v if isinstance(v, torch.Tensor) else torch.full((rows,), v, dtype=torch.float64, device=scores.device)
-                              for v in settings], dim=1).contiguous()
-        settings = [1.0, 0, 1.0, 0.0]
-    t, k, tp, mp = settings
-    if not (t >= 0.0 and math.isfinite(t)):
-        raise ValueError('temperature must be finite and >= 0; got %r' % (t,))
-    if not (k >= 0 and k == int(k)):
-        raise ValueError('top_k must be a whole number >= 0; got %r' % (k,))
-    if not (0.0 <= tp <= 1.0 and 0.0 <= mp <= 1.0):
-        raise ValueError('top_p and min_p must lie in [0, 1]; got %r and %r' % (tp, mp))
-    u = u.contiguous()
-    draws = u.shape[1]
-    lib = L.load()
-    index = torch.empty((rows, draws), dtype=torch.int64, device=scores.device)
-    logp = torch.empty((rows, draws), dtype=torch.float64, device=scores.device)
-    work, nbytes = workspace(lib.gpbo_draw_static_workspace(_TYPES[scores.dtype], rows, cols, draws), scores.device)
-    check_status('gpbo_draw_static', lib.gpbo_draw_static(
-        scores.device.index, stream_of(scores), _TYPES[scores.dtype], scores.data_ptr(), stride, rows, cols, u.data_ptr(), draws, t,
-        min(int(k), 1 << 62), tp, mp, pointer(params), index.data_ptr(), logp.data_ptr(), pointer(work), nbytes))
+    device, params = scores.device, None
+    if isinstance(temperature, Tensor) or isinstance(top_k, Tensor) or isinstance(top_p, Tensor) or isinstance(min_p, Tensor):
+        params = _per_row((temperature, top_k, top_p, min_p), rows, device, at)
+        temperature, top_k, top_p, min_p = 1.0, 0, 1.0, 0.0
+    if not (temperature >= 0.0 and math.isfinite(temperature)):
+        raise ValueError('temperature must be finite and >= 0; got %r' % (temperature,))
+    if not (top_k >= 0 and top_k == int(top_k)):
+        raise ValueError('top_k must be a whole number >= 0; got %r' % (top_k,))
+    if not (0.0 <= top_p <= 1.0 and 0.0 <= min_p <= 1.0):
+        raise ValueError('top_p and min_p must lie in [0, 1]; got %r and %r' % (top_p, min_p))
+    if not u.is_contiguous():
+        u = u.contiguous()
+    draws, code = u.shape[1], _TYPES[scores.dtype]
+    index = torch.empty((rows, draws), dtype=torch.int64, device=device)
+    logp = torch.empty((rows, draws), dtype=_f64, device=device)
+    nbytes = workspace('gpbo_draw_static_workspace', code, rows, cols, draws)
+    work = scratch(nbytes, device)
+    st = L.load().gpbo_draw_static(at, stream_of(at), code, scores.data_ptr(), stride, rows, cols, u.data_ptr(), draws, temperature,
+                                   min(int(top_k), 1 << 62), top_p, min_p, pointer(params), index.data_ptr(), logp.data_ptr(), pointer(work), nbytes)
+    if st:
+        check_status('gpbo_draw_static', st)
     return index, logp

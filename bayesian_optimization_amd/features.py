@@ -10,61 +10,69 @@ import numpy as np
 import torch
 
 from . import _lib as L
-from ._device import TYPES, check_status, on_device, pointer, rows_of, stream_of, vector_of, workspace
+from ._device import TYPES, check_status, pointer, rows_of, scratch, stream_of, tensor, vector_of, workspace
 
 ACTIVATIONS = {'silu': L.ACT_SILU, 'gelu': L.ACT_GELU}
+_empty, _f32 = torch.empty, torch.float32
 
 
 def _act(act):
-    if act not in ACTIVATIONS:
+    a = ACTIVATIONS.get(act)
+    if a is None:
         raise ValueError('act must be one of %s; got %r' % (sorted(ACTIVATIONS), act))
-    return ACTIVATIONS[act]
+    return a
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the rows of x (rows, cols) float32 / bfloat16 / float16; weight and bias
     (cols,) of x's type or None.  Returns y, mean (rows,) and rstd (rows,), the last two float32, for layer_norm_backward."""
-    rows, cols, stride = rows_of('x', x)
-    weight, bias = vector_of('weight', weight, cols, x.dtype, x.device), vector_of('bias', bias, cols, x.dtype, x.device)
-    if not 0.0 <= float(eps) < float('inf'):
+    rows, cols, stride, at = rows_of('x', x)
+    dtype, device = x.dtype, x.device
+    if weight is not None:
+        weight = vector_of('weight', weight, cols, dtype, at)
+    if bias is not None:
+        bias = vector_of('bias', bias, cols, dtype, at)
+    if not 0.0 <= eps < float('inf'):
         raise ValueError('eps must be finite and >= 0; got %r' % (eps,))
-    y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-    check_status('gpbo_layernorm', L.load().gpbo_layernorm(
-        x.device.index, stream_of(x), TYPES[x.dtype], x.data_ptr(), stride, rows, cols, pointer(weight), pointer(bias), float(eps),
-        y.data_ptr(), cols, stats[0].data_ptr(), stats[1].data_ptr()))
-    return y, stats[0], stats[1]
+    y = _empty((rows, cols), dtype=dtype, device=device)
+    mean, rstd = _empty(rows, dtype=_f32, device=device), _empty(rows, dtype=_f32, device=device)
+    st = L.load().gpbo_layernorm(at, stream_of(at), TYPES[dtype], x.data_ptr(), stride, rows, cols, pointer(weight), pointer(bias), eps,
+                                 y.data_ptr(), cols, mean.data_ptr(), rstd.data_ptr())
+    if st:
+        check_status('gpbo_layernorm', st)
+    return y, mean, rstd
 
 
 def layer_norm_backward(dy, x, weight, mean, rstd):
     """Gradients (dx, dweight, dbias) of layer_norm from dy, with the mean and rstd it returned.  dweight and dbias have x's
     type; they are the column sums whether or not the forward pass had a weight and a bias."""
-    rows, cols, stride = rows_of('x', x)
-    _, _, dstride = rows_of('dy', dy, dtype=x.dtype, shape=(rows, cols), device=x.device)
-    weight = vector_of('weight', weight, cols, x.dtype, x.device)
-    mean, rstd = vector_of('mean', mean, rows, torch.float32, x.device), vector_of('rstd', rstd, rows, torch.float32, x.device)
-    if mean is None or rstd is None:
-        raise ValueError('mean and rstd of the forward pass are needed')
-    lib = L.load()
-    dx = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-    dwb = torch.empty((2, cols), dtype=x.dtype, device=x.device)
-    work, nbytes = workspace(lib.gpbo_layernorm_backward_workspace(TYPES[x.dtype], rows, cols), x.device)
-    check_status('gpbo_layernorm_backward', lib.gpbo_layernorm_backward(
-        x.device.index, stream_of(x), TYPES[x.dtype], dy.data_ptr(), dstride, x.data_ptr(), stride, rows, cols, pointer(weight),
-        mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), cols, dwb[0].data_ptr(), dwb[1].data_ptr(), pointer(work), nbytes))
-    return dx, dwb[0], dwb[1]
+    rows, cols, stride, at = rows_of('x', x)
+    dtype, device = x.dtype, x.device
+    dstride = rows_of('dy', dy, dtype=dtype, shape=(rows, cols), device=at)[2]
+    if weight is not None:
+        weight = vector_of('weight', weight, cols, dtype, at)
+    mean, rstd = vector_of('mean', mean, rows, _f32, at), vector_of('rstd', rstd, rows, _f32, at)
+    code = TYPES[dtype]
+    dx = _empty((rows, cols), dtype=dtype, device=device)
+    dw, db = _empty(cols, dtype=dtype, device=device), _empty(cols, dtype=dtype, device=device)
+    nbytes = workspace('gpbo_layernorm_backward_workspace', code, rows, cols)
+    work = scratch(nbytes, device)
+    st = L.load().gpbo_layernorm_backward(at, stream_of(at), code, dy.data_ptr(), dstride, x.data_ptr(), stride, rows, cols, pointer(weight),
+                                          mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), cols, dw.data_ptr(), db.data_ptr(), pointer(work), nbytes)
+    if st:
+        check_status('gpbo_layernorm_backward', st)
+    return dx, dw, db
 
 
 def _weights(x, w_gate, w_up):
-    rows, cols, stride = rows_of('x', x)
-    on_device('w_gate', w_gate, x.device)
-    if w_gate.dim() != 2 or w_gate.shape[0] < 1 or w_gate.shape[1] != cols:
+    rows, cols, stride, at = rows_of('x', x)
+    hidden, wcols, wg_stride, _ = rows_of('w_gate', w_gate, dtype=x.dtype, device=at)
+    if wcols != cols or hidden < 1:
         raise ValueError('w_gate must be (hidden, %d) with hidden >= 1; got %s' % (cols, tuple(w_gate.shape)))
-    hidden, _, wg_stride = rows_of('w_gate', w_gate, dtype=x.dtype, device=x.device)
-    _, _, wu_stride = rows_of('w_up', w_up, dtype=x.dtype, shape=(hidden, cols), device=x.device)
+    wu_stride = rows_of('w_up', w_up, dtype=x.dtype, shape=(hidden, cols), device=at)[2]
     if wg_stride != wu_stride:      # one row stride for both: weights laid out apart are brought together
         w_gate, w_up, wg_stride = w_gate.contiguous(), w_up.contiguous(), cols
-    return rows, cols, stride, hidden, w_gate, w_up, wg_stride
+    return rows, cols, stride, at, hidden, w_gate, w_up, wg_stride
 
 
 def gated_unit(x, w_gate, w_up, act='silu', keep=False):
@@ -72,35 +80,48 @@ def gated_unit(x, w_gate, w_up, act='silu', keep=False):
     act 'silu' or 'gelu'.  keep: also return x w_gate^T and x w_up^T as one (2, rows, hidden) float32 tensor, which
     gated_unit_backward needs."""
     a = _act(act)
-    rows, cols, stride, hidden, w_gate, w_up, ws = _weights(x, w_gate, w_up)
-    lib = L.load()
-    h = torch.empty((rows, hidden), dtype=x.dtype, device=x.device)
-    kept = torch.empty((2, rows, hidden), dtype=torch.float32, device=x.device) if keep else None
-    work, nbytes = workspace(lib.gpbo_gated_workspace(TYPES[x.dtype], rows, cols, hidden), x.device)
-    check_status('gpbo_gated', lib.gpbo_gated(
-        x.device.index, stream_of(x), TYPES[x.dtype], a, x.data_ptr(), stride, rows, cols, w_gate.data_ptr(), w_up.data_ptr(), ws, hidden,
-        h.data_ptr(), hidden, kept[0].data_ptr() if keep else None, kept[1].data_ptr() if keep else None, pointer(work), nbytes))
+    rows, cols, stride, at, hidden, w_gate, w_up, ws = _weights(x, w_gate, w_up)
+    dtype, device = x.dtype, x.device
+    code = TYPES[dtype]
+    h = _empty((rows, hidden), dtype=dtype, device=device)
+    kept = kg = ku = None
+    if keep:
+        kept = _empty((2, rows, hidden), dtype=_f32, device=device)
+        kg = kept.data_ptr()
+        ku = kg + 4 * rows * hidden
+    nbytes = workspace('gpbo_gated_workspace', code, rows, cols, hidden)
+    work = scratch(nbytes, device)
+    st = L.load().gpbo_gated(at, stream_of(at), code, a, x.data_ptr(), stride, rows, cols, w_gate.data_ptr(), w_up.data_ptr(), ws, hidden,
+                             h.data_ptr(), hidden, kg, ku, pointer(work), nbytes)
+    if st:
+        check_status('gpbo_gated', st)
     return (h, kept) if keep else h
 
 
 def gated_unit_backward(dh, x, w_gate, w_up, kept, act='silu', need_dx=True, need_dw=True):
     """Gradients (dx, dw_gate, dw_up) of gated_unit from dh (rows, hidden), with what it kept; None for those not needed."""
     a = _act(act)
-    rows, cols, stride, hidden, w_gate, w_up, ws = _weights(x, w_gate, w_up)
-    _, _, dstride = rows_of('dh', dh, dtype=x.dtype, shape=(rows, hidden), device=x.device)
-    on_device('kept', kept, x.device)
-    if kept.shape != (2, rows, hidden) or kept.dtype != torch.float32:
+    rows, cols, stride, at, hidden, w_gate, w_up, ws = _weights(x, w_gate, w_up)
+    dtype, device = x.dtype, x.device
+    code = TYPES[dtype]
+    dstride = rows_of('dh', dh, dtype=dtype, shape=(rows, hidden), device=at)[2]
+    tensor('kept', kept, at)
+    if tuple(kept.shape) != (2, rows, hidden) or kept.dtype != _f32:
         raise ValueError('kept must be (2, %d, %d) float32; got %s %s' % (rows, hidden, tuple(kept.shape), kept.dtype))
-    kept = kept.contiguous()
-    lib = L.load()
-    dx = torch.empty((rows, cols), dtype=x.dtype, device=x.device) if need_dx else None
-    dw = torch.empty((2, hidden, cols), dtype=x.dtype, device=x.device) if need_dw else None
-    work, nbytes = workspace(lib.gpbo_gated_backward_workspace(TYPES[x.dtype], rows, cols, hidden), x.device)
-    check_status('gpbo_gated_backward', lib.gpbo_gated_backward(
-        x.device.index, stream_of(x), TYPES[x.dtype], a, dh.data_ptr(), dstride, x.data_ptr(), stride, rows, cols, w_gate.data_ptr(),
-        w_up.data_ptr(), ws, hidden, kept[0].data_ptr(), kept[1].data_ptr(), pointer(dx), cols, dw[0].data_ptr() if need_dw else None,
-        dw[1].data_ptr() if need_dw else None, cols, pointer(work), nbytes))
-    return dx, (dw[0] if need_dw else None), (dw[1] if need_dw else None)
+    if not kept.is_contiguous():
+        kept = kept.contiguous()
+    kg = kept.data_ptr()
+    dx = _empty((rows, cols), dtype=dtype, device=device) if need_dx else None
+    dwg = _empty((hidden, cols), dtype=dtype, device=device) if need_dw else None
+    dwu = _empty((hidden, cols), dtype=dtype, device=device) if need_dw else None
+    nbytes = workspace('gpbo_gated_backward_workspace', code, rows, cols, hidden)
+    work = scratch(nbytes, device)
+    st = L.load().gpbo_gated_backward(at, stream_of(at), code, a, dh.data_ptr(), dstride, x.data_ptr(), stride, rows, cols, w_gate.data_ptr(),
+                                      w_up.data_ptr(), ws, hidden, kg, kg + 4 * rows * hidden, pointer(dx), cols, pointer(dwg), pointer(dwu),
+                                      cols, pointer(work), nbytes)
+    if st:
+        check_status('gpbo_gated_backward', st)
+    return dx, dwg, dwu
 
 
 class FeatureMap:
