@@ -644,6 +644,58 @@ __device__ bool draw_search(DrawLds<T>& s, const DrawArgs& a, const DrawRow& p, 
     return false;
 }
 
+// A row of up to LIST scores, thread = index: one sort by rank gives the best and the last kept pair; whether a thread's own score
+// is kept is then a comparison, and the running sum in index order needs no second sort.
+template <typename T>
+__device__ void draw_short(DrawLds<T>& s, const DrawArgs& a, const DrawRow& p, const T* x, int64_t row, int n) {
+    using Key = typename Score<T>::Key;
+    const int tid = threadIdx.x;
+    const Key mine = tid < n ? Score<T>::key(x[tid]) : 0;
+    int size = 64;
+    while (size < n) size <<= 1;
+    Key k = mine;
+    uint32_t i = tid;
+    block_sort<Key, false>(k, i, size, s.l.key, s.l.idx);
+    if (tid == 0) s.red_k[0][0] = k, s.red_i[0] = i;
+    __syncthreads();
+    const Key top = s.red_k[0][0];
+    if (top == 0 || p.greedy) {
+        draw_same<T>(a, row, top ? (int64_t)s.red_i[0] : -1, top ? 0.0 : -INFINITY);
+        return;
+    }
+    const bool ranked = tid < size && k != 0;
+    const double w = ranked ? exp(draw_t<T>(k, top, p.temperature)) : 0.0;
+    bool in = ranked && (p.top_k == 0 || tid < p.top_k) && w >= p.min_p;
+    double total;
+    if (p.top_p < 1.0) {
+        const double run = block_scan(in ? w : 0.0, s.red, total);
+        in = in && (tid == 0 || run - w < p.top_p * total);
+    }
+    // the kept ones are the first in rank: the last of them is the one behind which the next position is not kept
+    s.l.pick[tid] = in;
+    __syncthreads();
+    if (in && (tid == DRAW_THREADS - 1 || !s.l.pick[tid + 1])) s.red_k[1][0] = k, s.red_i[1] = i;
+    __syncthreads();
+    const Key cut = s.red_k[1][0];
+    const bool keep = mine != 0 && (mine > cut || (mine == cut && (uint32_t)tid <= s.red_i[1]));
+    const double c = block_scan(keep ? exp(draw_t<T>(mine, top, p.temperature)) : 0.0, s.red, total);
+    s.l.c[tid] = c;
+    s.l.key[tid] = mine;
+    __syncthreads();
+    for (int64_t q = tid; q < a.draws; q += DRAW_THREADS) {
+        const double at = fmax(a.u[row * a.draws + q], 0.0) * total;
+        int lo = 0, hi = n - 1;                // the first c > at; the last kept one if rounding leaves none
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (s.l.c[mid] > at) hi = mid;
+            else lo = mid + 1;
+        }
+        while (lo > 0 && s.l.c[lo] == s.l.c[lo - 1]) --lo;
+        a.index[row * a.draws + q] = lo;
+        if (a.logp) a.logp[row * a.draws + q] = draw_t<T>(s.l.key[lo], top, p.temperature) - log(total);
+    }
+}
+
 // The weights of a row once the cut is known.
 template <typename T>
 struct DrawKept {
@@ -750,16 +802,15 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_row(DrawArgs a) {
     const T* x = (const T*)a.scores + row * a.stride;
     const uint32_t n = (uint32_t)a.cols;
     const DrawRow p(a, row);
+    if (n <= LIST) {
+        draw_short(s, a, p, x, row, (int)n);
+        return;
+    }
     Key top, bot, own;
     uint32_t idx;
     draw_extremes(s, x, 0, n, top, bot, idx, own);
     if (top == 0 || p.greedy) {
         draw_same<T>(a, row, top ? (int64_t)idx : -1, top ? 0.0 : -INFINITY);
-        return;
-    }
-    if (n <= LIST) {
-        if (tid < (int)n) s.l.key[tid] = S::key(x[tid]), s.l.idx[tid] = tid;
-        draw_from_list<T>(s, a, p, row, (int)n, top, -1.0);
         return;
     }
     Key bound = 0;
