@@ -32,6 +32,22 @@ __device__ __forceinline__ float row_sum(float v, float* lds) {
     }
 }
 
+// Two of them with one barrier.
+template <int TPR>
+__device__ __forceinline__ void row_sum2(float& v, float& u, float* lds_v, float* lds_u) {
+    if constexpr (TPR <= 64) {
+        v = row_sum<TPR>(v, nullptr), u = row_sum<TPR>(u, nullptr);
+    } else {
+        v = wave_sum(v), u = wave_sum(u);
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) lds_v[wave] = v, lds_u[wave] = u;
+        __syncthreads();
+        v = u = 0.0f;
+#pragma unroll
+        for (int i = 0; i < TPR / 64; ++i) v += lds_v[i], u += lds_u[i];
+    }
+}
+
 // Pack c of a row of `cols` elements.  The last pack of a row whose length is no multiple of N is moved back so that it ends
 // with the row: it is loaded and stored whole, its first `dup` elements are the pack before's (left out of sums, stored twice
 // with the same value).  Rows shorter than one pack go element by element.
@@ -76,7 +92,9 @@ struct NormArgs {
     float* part;                               // [groups][2][cols] column sums of dy xh and dy
 };
 
-// Rows of up to TPR * NCH packs.
+// Rows of more than TPR * (NCH - 1) and up to TPR * NCH packs: only a thread's last pack can be broken or missing, so only there
+// does an element need to be asked whether it counts.  Held as 32-bit numbers from the load on: per element one conversion, two
+// additions and two products, then the output -- on a row of a few hundred elements the vector instructions bind as much as memory.
 template <typename T, int TPR, int NCH>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_fwd(NormArgs a) {
     constexpr int V = Pack<T>::N, BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR;
@@ -84,12 +102,13 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_fwd(NormArgs a) 
     const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
     const T *w = (const T*)a.w, *b = (const T*)a.b;
     const int cols = (int)a.cols;
+    const Span<T> tail(lane + (NCH - 1) * TPR, cols);
+    auto at = [&](int k) { return (int64_t)(lane + k * TPR) * V; };
     Pack<T> pw[NCH], pb[NCH];
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-        const Span<T> sp(lane + k * TPR, cols);
-        if (w) pw[k] = sp.load(w);
-        if (b) pb[k] = sp.load(b);
+        if (w) pw[k] = k < NCH - 1 ? load_pack(w + at(k)) : tail.load(w);
+        if (b) pb[k] = k < NCH - 1 ? load_pack(b + at(k)) : tail.load(b);
     }
     const float n = (float)cols;
     // the trip count is the same for all threads of a workgroup: row sums of wide rows hold barriers
@@ -97,27 +116,28 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_fwd(NormArgs a) 
         const int64_t r = r0 + group;
         const bool on = r < a.rows;
         const T* x = (const T*)a.x + (on ? r : 0) * a.xs;
+        float v[NCH][V];
+        float s = 0.0f;
         Pack<T> px[NCH];
 #pragma unroll
-        for (int k = 0; k < NCH; ++k) px[k] = Span<T>(lane + k * TPR, cols).load(x);
-        float s = 0.0f;
+        for (int k = 0; k < NCH; ++k) px[k] = k < NCH - 1 ? load_pack(x + at(k)) : tail.load(x);
 #pragma unroll
-        for (int k = 0; k < NCH; ++k) {
-            const Span<T> sp(lane + k * TPR, cols);
+        for (int k = 0; k < NCH; ++k)
 #pragma unroll
-            for (int i = 0; i < V; ++i) s += sp.own(i) ? to_float(px[k].v[i]) : 0.0f;
-        }
+            for (int i = 0; i < V; ++i) {
+                v[k][i] = to_float(px[k].v[i]);
+                s += k < NCH - 1 || tail.own(i) ? v[k][i] : 0.0f;
+            }
         const float mu = row_sum<TPR>(s, lds[0]) / n;
         float q = 0.0f;
 #pragma unroll
-        for (int k = 0; k < NCH; ++k) {
-            const Span<T> sp(lane + k * TPR, cols);
+        for (int k = 0; k < NCH; ++k)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float d = to_float(px[k].v[i]) - mu;
-                q += sp.own(i) ? d * d : 0.0f;
+                v[k][i] -= mu;
+                const float d = k < NCH - 1 || tail.own(i) ? v[k][i] : 0.0f;
+                q = fmaf(d, d, q);
             }
-        }
         const float rstd = 1.0f / sqrtf(row_sum<TPR>(q, lds[1]) / n + a.eps);
         if (!on) continue;                     // only where TPR <= 64: no barrier is skipped
         T* y = (T*)a.y + r * a.ys;
@@ -126,10 +146,11 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_fwd(NormArgs a) 
             Pack<T> py;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float xh = (to_float(px[k].v[i]) - mu) * rstd;
-                py.v[i] = from_float<T>((w ? xh * to_float(pw[k].v[i]) : xh) + (b ? to_float(pb[k].v[i]) : 0.0f));
+                const float xh = v[k][i] * rstd;
+                py.v[i] = from_float<T>(fmaf(xh, w ? to_float(pw[k].v[i]) : 1.0f, b ? to_float(pb[k].v[i]) : 0.0f));
             }
-            Span<T>(lane + k * TPR, cols).store(y, py);
+            if (k < NCH - 1) store_pack(y + at(k), py);
+            else tail.store(y, py);
         }
         if (lane == 0) {
             if (a.mean) a.mean[r] = mu;
@@ -198,11 +219,13 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_bwd(NormArgs a) 
     const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
     const T* w = (const T*)a.w;
     const int cols = (int)a.cols;
+    const Span<T> tail(lane + (NCH - 1) * TPR, cols);
+    auto at = [&](int k) { return (int64_t)(lane + k * TPR) * V; };
     Pack<T> pw[NCH];
     float aw[NCH][V], ab[NCH][V];
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-        if (w) pw[k] = Span<T>(lane + k * TPR, cols).load(w);
+        if (w) pw[k] = k < NCH - 1 ? load_pack(w + at(k)) : tail.load(w);
 #pragma unroll
         for (int i = 0; i < V; ++i) aw[k][i] = ab[k][i] = 0.0f;
     }
@@ -212,32 +235,32 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_bwd(NormArgs a) 
         const int64_t r = r0 + group;
         const bool on = r < a.rows;
         const int64_t rr = on ? r : 0;
-        const T* x = (const T*)a.x + rr * a.xs;
-        const T* dy = (const T*)a.dy + rr * a.dys;
+        const T *x = (const T*)a.x + rr * a.xs, *dy = (const T*)a.dy + rr * a.dys;
         Pack<T> px[NCH], pd[NCH];
 #pragma unroll
         for (int k = 0; k < NCH; ++k) {
-            const Span<T> sp(lane + k * TPR, cols);
-            px[k] = sp.load(x);
-            pd[k] = sp.load(dy);
+            px[k] = k < NCH - 1 ? load_pack(x + at(k)) : tail.load(x);
+            pd[k] = k < NCH - 1 ? load_pack(dy + at(k)) : tail.load(dy);
         }
         const float mu = a.mean[rr], rstd = a.rstd[rr];
         float s1 = 0.0f, s2 = 0.0f;
+        float xh[NCH][V];
 #pragma unroll
-        for (int k = 0; k < NCH; ++k) {
-            const Span<T> sp(lane + k * TPR, cols);
+        for (int k = 0; k < NCH; ++k)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float xh = (to_float(px[k].v[i]) - mu) * rstd, d = to_float(pd[k].v[i]);
+                xh[k][i] = (to_float(px[k].v[i]) - mu) * rstd;
+                const float d = RPB == 1 || on ? to_float(pd[k].v[i]) : 0.0f;      // rows behind the last add nothing
                 const float g = w ? d * to_float(pw[k].v[i]) : d;
-                s1 += sp.own(i) ? g : 0.0f;
-                s2 += sp.own(i) ? g * xh : 0.0f;
-                aw[k][i] += on ? d * xh : 0.0f;
-                ab[k][i] += on ? d : 0.0f;
+                const bool own = k < NCH - 1 || tail.own(i);
+                s1 += own ? g : 0.0f;
+                s2 = fmaf(own ? g : 0.0f, xh[k][i], s2);
+                aw[k][i] = fmaf(d, xh[k][i], aw[k][i]);
+                ab[k][i] += d;
             }
-        }
-        const float m1 = row_sum<TPR>(s1, lds[par]) / n, m2 = row_sum<TPR>(s2, lds[par + 1]) / n;
+        row_sum2<TPR>(s1, s2, lds[par], lds[par + 1]);
         par ^= 2;
+        const float m1 = s1 / n, m2 = s2 / n;
         if (!on) continue;
         T* dx = (T*)a.dx + r * a.dxs;
 #pragma unroll
@@ -245,15 +268,45 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_bwd(NormArgs a) 
             Pack<T> po;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float xh = (to_float(px[k].v[i]) - mu) * rstd, d = to_float(pd[k].v[i]);
-                const float g = w ? d * to_float(pw[k].v[i]) : d;
-                po.v[i] = from_float<T>(rstd * (g - m1 - xh * m2));
+                const float d = to_float(pd[k].v[i]), g = w ? d * to_float(pw[k].v[i]) : d;
+                po.v[i] = from_float<T>(rstd * (g - m1 - xh[k][i] * m2));
             }
-            Span<T>(lane + k * TPR, cols).store(dx, po);
+            if (k < NCH - 1) store_pack(dx + at(k), po);
+            else tail.store(dx, po);
         }
     }
     if (!a.part) return;
-    float* part = a.part + ((int64_t)blockIdx.x * RPB + group) * 2 * a.cols;
+    // one pair of column sums a workgroup: row groups of a wave by exchange, waves through LDS, in a fixed order
+    if constexpr (TPR < 64) {
+#pragma unroll
+        for (int k = 0; k < NCH; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+#pragma unroll
+                for (int o = 32; o >= TPR; o >>= 1) {
+                    aw[k][i] += __shfl_xor(aw[k][i], o);
+                    ab[k][i] += __shfl_xor(ab[k][i], o);
+                }
+    }
+    if constexpr (TPR <= 64) {
+        __shared__ float sums[4][2 * NCH * V][64];
+        const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) sums[wave][k * V + i][wl] = aw[k][i], sums[wave][(NCH + k) * V + i][wl] = ab[k][i];
+        __syncthreads();
+        if (wave > 0 || wl >= TPR) return;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                aw[k][i] = (sums[0][k * V + i][wl] + sums[1][k * V + i][wl]) + (sums[2][k * V + i][wl] + sums[3][k * V + i][wl]);
+                ab[k][i] = (sums[0][(NCH + k) * V + i][wl] + sums[1][(NCH + k) * V + i][wl]) +
+                           (sums[2][(NCH + k) * V + i][wl] + sums[3][(NCH + k) * V + i][wl]);
+            }
+    }
+    float* part = a.part + (int64_t)blockIdx.x * 2 * a.cols;
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
         const Span<T> sp(lane + k * TPR, cols);
@@ -295,8 +348,9 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(NormArgs a) {
             s1 += t1;
             s2 += t2;
         }
-        const float m1 = row_sum<1024>(s1, lds[par]) / n, m2 = row_sum<1024>(s2, lds[par + 1]) / n;
+        row_sum2<1024>(s1, s2, lds[par], lds[par + 1]);
         par ^= 2;
+        const float m1 = s1 / n, m2 = s2 / n;
         T* dx = (T*)a.dx + r * a.dxs;
         for (int64_t c = threadIdx.x; c < chunks; c += 1024) {
             const Span<T> sp(c, a.cols);
@@ -373,62 +427,70 @@ struct NormPlan {
     int64_t grid, groups;
 };
 
-// Threads a row, by the packs it has.  8 threads up to 8 packs: eight short rows share a wave; a wave up to 128 packs: sums
-// without a barrier; a workgroup of 256 and of 1024 above, so that no thread holds more than 2 packs of x (and, going back,
-// 2 of dy and 16 column sums a pack; 4 packs spill): beyond 2048 packs the row does not fit and is read again.
+// Threads a row, by the packs it has: as few as leave a thread at most 5 packs (forward) or 3 (backward, which holds two column
+// sums an element as well), so that several short rows share a wave and few of its lanes idle (621 elements of 16 bits, 78 packs:
+// 16 threads of 5 packs waste 2 of 80, a wave of 2 packs 50 of 128: 942 -> 525 us on a million rows, 5.0 TB/s); from there a workgroup of
+// 256 or 1024, sums through LDS; beyond 2048 packs the row does not fit into registers and is read again.
 inline NormPlan norm_plan(int64_t rows, int64_t cols, int vec, bool backward) {
     const int64_t packs = ceil_div(cols, vec);
     NormPlan p{};
-    if (packs <= 8) p.tpr = 8, p.nch = 1;
-    else if (packs <= 128) p.tpr = 64, p.nch = packs <= 64 ? 1 : 2;
-    else if (packs <= 512) p.tpr = 256, p.nch = packs <= 256 ? 1 : 2;
-    else if (packs <= 2048) p.tpr = 1024, p.nch = packs <= 1024 ? 1 : 2;
-    else p.tpr = 1024, p.nch = 0;
+    const int most_packs = backward ? 3 : 5;
+    if (packs <= 8) p.tpr = 8;
+    else if (packs <= 16 * most_packs) p.tpr = 16;
+    else if (packs <= 128) p.tpr = backward ? 64 : 32;
+    else if (packs <= 512) p.tpr = 256;
+    else p.tpr = 1024;
+    p.nch = packs > 2048 ? 0 : (int)ceil_div(packs, p.tpr);
     const int64_t block = p.tpr > 256 ? p.tpr : 256, rpb = block / p.tpr;
     // forward: as many workgroups as the card holds; backward: fewer, since each leaves column sums behind
-    const int64_t most = backward ? (p.tpr == 1024 ? 256 : p.tpr == 256 ? 1024 : 1024) : (p.tpr == 1024 ? 512 : 2048);
+    const int64_t most = backward ? (p.tpr == 1024 ? 256 : 1024) : (p.tpr == 1024 ? 512 : 2048);
     p.grid = std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, rpb), most));
-    if (backward && p.nch == 0) p.groups = std::max<int64_t>(1, std::min<int64_t>(rows, 64));
-    else p.groups = p.grid * rpb;
+    p.groups = backward && p.nch == 0 ? std::max<int64_t>(1, std::min<int64_t>(rows, 64)) : p.grid;
     return p;
+}
+
+// The kernels that norm_plan names.
+template <typename T>
+void launch_norm(hipStream_t st, const NormArgs& a, const NormPlan& p, bool backward) {
+    const dim3 grid((unsigned)p.grid), block(p.tpr > 256 ? p.tpr : 256);
+    auto fwd = [&](auto k) { hipLaunchKernelGGL(k, grid, block, 0, st, a); };
+    switch (p.tpr * 8 + p.nch) {
+        case 8 * 8 + 1: return backward ? fwd(k_norm_bwd<T, 8, 1>) : fwd(k_norm_fwd<T, 8, 1>);
+        case 16 * 8 + 1: return backward ? fwd(k_norm_bwd<T, 16, 1>) : fwd(k_norm_fwd<T, 16, 1>);
+        case 16 * 8 + 2: return backward ? fwd(k_norm_bwd<T, 16, 2>) : fwd(k_norm_fwd<T, 16, 2>);
+        case 16 * 8 + 3: return backward ? fwd(k_norm_bwd<T, 16, 3>) : fwd(k_norm_fwd<T, 16, 3>);
+        case 16 * 8 + 4: return fwd(k_norm_fwd<T, 16, 4>);
+        case 16 * 8 + 5: return fwd(k_norm_fwd<T, 16, 5>);
+        case 32 * 8 + 3: return fwd(k_norm_fwd<T, 32, 3>);
+        case 32 * 8 + 4: return fwd(k_norm_fwd<T, 32, 4>);
+        case 64 * 8 + 1: return fwd(k_norm_bwd<T, 64, 1>);
+        case 64 * 8 + 2: return fwd(k_norm_bwd<T, 64, 2>);
+        case 256 * 8 + 1: return backward ? fwd(k_norm_bwd<T, 256, 1>) : fwd(k_norm_fwd<T, 256, 1>);
+        case 256 * 8 + 2: return backward ? fwd(k_norm_bwd<T, 256, 2>) : fwd(k_norm_fwd<T, 256, 2>);
+        case 1024 * 8 + 1: return backward ? fwd(k_norm_bwd<T, 1024, 1>) : fwd(k_norm_fwd<T, 1024, 1>);
+        case 1024 * 8 + 2: return backward ? fwd(k_norm_bwd<T, 1024, 2>) : fwd(k_norm_fwd<T, 1024, 2>);
+        default: return backward ? fwd(k_norm_bwd_long<T>) : fwd(k_norm_fwd_long<T>);      // p.nch == 0
+    }
 }
 
 template <typename T>
 hipError_t norm_forward(hipStream_t st, const NormArgs& a) {
     if (a.rows == 0) return hipSuccess;
-    const NormPlan p = norm_plan(a.rows, a.cols, Pack<T>::N, false);
-    const dim3 g((unsigned)p.grid), b256(256), b1024(1024);
-    if (p.nch == 0) hipLaunchKernelGGL(k_norm_fwd_long<T>, g, b1024, 0, st, a);
-    else if (p.tpr == 8) hipLaunchKernelGGL((k_norm_fwd<T, 8, 1>), g, b256, 0, st, a);
-    else if (p.tpr == 64 && p.nch == 1) hipLaunchKernelGGL((k_norm_fwd<T, 64, 1>), g, b256, 0, st, a);
-    else if (p.tpr == 64 && p.nch == 2) hipLaunchKernelGGL((k_norm_fwd<T, 64, 2>), g, b256, 0, st, a);
-    else if (p.tpr == 256 && p.nch == 1) hipLaunchKernelGGL((k_norm_fwd<T, 256, 1>), g, b256, 0, st, a);
-    else if (p.tpr == 256) hipLaunchKernelGGL((k_norm_fwd<T, 256, 2>), g, b256, 0, st, a);
-    else if (p.nch == 1) hipLaunchKernelGGL((k_norm_fwd<T, 1024, 1>), g, b1024, 0, st, a);
-    else hipLaunchKernelGGL((k_norm_fwd<T, 1024, 2>), g, b1024, 0, st, a);
+    launch_norm<T>(st, a, norm_plan(a.rows, a.cols, Pack<T>::N, false), false);
     return hipGetLastError();
 }
 
 template <typename T>
 hipError_t norm_backward(hipStream_t st, const NormArgs& a, void* dw, void* db) {
     const NormPlan p = norm_plan(a.rows, a.cols, Pack<T>::N, true);
-    const dim3 g((unsigned)p.grid), b256(256), b1024(1024);
     if (a.rows > 0) {
-        if (p.nch == 0) {
-            hipLaunchKernelGGL(k_norm_bwd_long<T>, g, b1024, 0, st, a);
-            if (a.part)
-                hipLaunchKernelGGL(k_norm_bwd_long_cols<T>, dim3((unsigned)ceil_div(ceil_div(a.cols, Pack<T>::N), 256), (unsigned)p.groups),
-                                   b256, 0, st, a);
-        } else if (p.tpr == 8) hipLaunchKernelGGL((k_norm_bwd<T, 8, 1>), g, b256, 0, st, a);
-        else if (p.tpr == 64 && p.nch == 1) hipLaunchKernelGGL((k_norm_bwd<T, 64, 1>), g, b256, 0, st, a);
-        else if (p.tpr == 64 && p.nch == 2) hipLaunchKernelGGL((k_norm_bwd<T, 64, 2>), g, b256, 0, st, a);
-        else if (p.tpr == 256 && p.nch == 1) hipLaunchKernelGGL((k_norm_bwd<T, 256, 1>), g, b256, 0, st, a);
-        else if (p.tpr == 256) hipLaunchKernelGGL((k_norm_bwd<T, 256, 2>), g, b256, 0, st, a);
-        else if (p.nch == 1) hipLaunchKernelGGL((k_norm_bwd<T, 1024, 1>), g, b1024, 0, st, a);
-        else hipLaunchKernelGGL((k_norm_bwd<T, 1024, 2>), g, b1024, 0, st, a);
+        launch_norm<T>(st, a, p, true);
+        if (p.nch == 0 && a.part)
+            hipLaunchKernelGGL(k_norm_bwd_long_cols<T>, dim3((unsigned)ceil_div(ceil_div(a.cols, Pack<T>::N), 256), (unsigned)p.groups), dim3(256), 0,
+                               st, a);
     }
     if (dw || db)
-        hipLaunchKernelGGL(k_norm_cols<T>, dim3((unsigned)ceil_div(a.cols, 64), 2), b1024, 0, st, (const float*)a.part,
+        hipLaunchKernelGGL(k_norm_cols<T>, dim3((unsigned)ceil_div(a.cols, 64), 2), dim3(1024), 0, st, (const float*)a.part,
                            a.rows > 0 ? (int)p.groups : 0, a.cols, (T*)dw, (T*)db);
     return hipGetLastError();
 }
