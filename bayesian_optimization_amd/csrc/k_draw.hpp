@@ -742,12 +742,41 @@ __device__ void draw_tile_mass(const DrawKept<T>& kw, const T* x, uint32_t begin
     ties = c;
 }
 
+// One wave: the same for the neighbouring tiles of `tile` < 64 V elements (a power of two, at least 64) that 64 packs cover, from
+// `begin` on: the lanes of a tile add up among themselves, and each of them has its tile's sums.
+template <typename T>
+__device__ void draw_tiles_mass(const DrawKept<T>& kw, const T* x, uint32_t begin, uint32_t end, uint32_t tile, double& mass, uint32_t& ties) {
+    using Key = typename Score<T>::Key;
+    constexpr uint32_t V = Pack<T>::N;
+    double m = 0.0;
+    uint32_t c = 0;
+    auto one = [&](T v) {
+        const Key k = Score<T>::key(v);
+        m += kw.strict(k);
+        c += k == kw.cut && k != 0;
+    };
+    const uint32_t i = begin + (threadIdx.x & 63) * V;
+    if (i + V <= end) {
+        const Pack<T> p = load_pack(x + i);
+#pragma unroll
+        for (uint32_t j = 0; j < V; ++j) one(p.v[j]);
+    } else {
+        for (uint32_t j = i; j < end; ++j) one(x[j]);
+    }
+    for (uint32_t o = tile / V / 2; o > 0; o >>= 1) {
+        m += __shfl_xor(m, o);
+        c += __shfl_xor(c, o);
+    }
+    mass = m, ties = c;
+}
+
 // One wave: the pick inside [begin, end), of at most 64 * 64 elements, for mass `goal` with `run` in front of it and `ties` of the
 // cut's ties already met (of which cut_ties are kept).  A lane sums a run of neighbours, the lane that holds the goal is found
 // by a scan over the lanes, and then its run is spread over the lanes.
 template <typename T>
 __device__ int64_t draw_in_tile(const DrawKept<T>& kw, const T* x, uint32_t begin, uint32_t end, double run, uint32_t ties, uint32_t cut_ties, double goal) {
     using Key = typename Score<T>::Key;
+    constexpr uint32_t V = Pack<T>::N;
     const uint32_t lane = threadIdx.x & 63;
     uint32_t each = (end - begin + 63) / 64;
     int64_t pick = -1;
@@ -755,11 +784,18 @@ __device__ int64_t draw_in_tile(const DrawKept<T>& kw, const T* x, uint32_t begi
         const uint32_t b = min(end, begin + lane * each), e = min(end, b + each);
         double m = 0.0;
         uint32_t c = 0;
-        for (uint32_t i = b; i < e; ++i) {
-            const Key k = Score<T>::key(x[i]);
+        auto one = [&](T v) {
+            const Key k = Score<T>::key(v);
             m += kw.strict(k);
             c += k == kw.cut && k != 0;
+        };
+        uint32_t i = b;
+        for (; i + V <= e; i += V) {
+            const Pack<T> p = load_pack(x + i);
+#pragma unroll
+            for (uint32_t j = 0; j < V; ++j) one(p.v[j]);
         }
+        for (; i < e; ++i) one(x[i]);
         uint32_t before = c;                   // ties in front of this lane
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -830,12 +866,27 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_row(DrawArgs a) {
 
     // kept mass of the row's tiles, in index order
     const DrawKept<T> kw(s.st, p);
-    const uint32_t tiles = (n + TILE - 1) / TILE;
-    for (uint32_t t = wave; t < TILES; t += DRAW_THREADS / 64) {
-        double m = 0.0;
-        uint32_t c = 0;
-        if (t < tiles) draw_tile_mass(kw, x, t * TILE, min(n, (t + 1) * TILE), m, c);
-        if (lane == 0) s.t.c[t] = m, s.t.ties[t] = c;
+    constexpr uint32_t V = Pack<T>::N;
+    uint32_t tile = 64;                        // as short as TILES of them allow: a pick looks through one
+    while ((uint64_t)tile * TILES < n) tile <<= 1;
+    const uint32_t tiles = (n + tile - 1) / tile;
+    s.t.c[tid] = 0.0, s.t.ties[tid] = 0;
+    __syncthreads();
+    if (tile < 64 * V) {
+        const uint32_t lanes = tile / V, at_once = 64 / lanes;
+        for (uint32_t t = wave * at_once; t < tiles; t += DRAW_THREADS / 64 * at_once) {
+            double m;
+            uint32_t c;
+            draw_tiles_mass(kw, x, t * tile, n, tile, m, c);
+            if (lane % lanes == 0 && t + lane / lanes < tiles) s.t.c[t + lane / lanes] = m, s.t.ties[t + lane / lanes] = c;
+        }
+    } else {
+        for (uint32_t t = wave; t < tiles; t += DRAW_THREADS / 64) {
+            double m;
+            uint32_t c;
+            draw_tile_mass(kw, x, t * tile, min(n, (t + 1) * tile), m, c);
+            if (lane == 0) s.t.c[t] = m, s.t.ties[t] = c;
+        }
     }
     __syncthreads();
     const uint32_t mine = s.t.ties[tid];
@@ -856,7 +907,7 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_row(DrawArgs a) {
             else lo = mid + 1;
         }
         while (lo > 0 && s.t.c[lo] == s.t.c[lo - 1]) --lo;
-        const int64_t pick = draw_in_tile(kw, x, lo * TILE, min(n, (lo + 1) * TILE), lo ? s.t.c[lo - 1] : 0.0, s.t.ties[lo], cut_ties, goal);
+        const int64_t pick = draw_in_tile(kw, x, lo * tile, min(n, (lo + 1) * tile), lo ? s.t.c[lo - 1] : 0.0, s.t.ties[lo], cut_ties, goal);
         if (lane == 0) {
             a.index[row * a.draws + q] = pick;
             if (a.logp) a.logp[row * a.draws + q] = draw_t<T>(S::key(x[pick]), top, p.temperature) - log(total);

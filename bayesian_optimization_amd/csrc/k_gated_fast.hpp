@@ -189,33 +189,46 @@ struct PackArgs {
     int count;
 };
 
-// dst[r][c] = src[r][c] (TRANSPOSE: dst[c][r] = src[r][c]), zero up to the pitch.
+// dst[r][c] = src[r][c] (TRANSPOSE: dst[c][r] = src[r][c]), zero up to the pitch.  16 bytes a load and store (the pitch is a whole
+// number of them); a transposed tile goes through LDS.
 template <typename T, bool TRANSPOSE>
 __global__ __launch_bounds__(256) void k_gated_pack(PackArgs a) {
+    constexpr int V = Pack<T>::N, ACROSS = 64 / V, DOWN = 256 / ACROSS;
     int64_t id = blockIdx.x;
     int which = 0;
     while (which + 1 < a.count && id >= a.job[which].blocks) id -= a.job[which++].blocks;
     const PackJob& jb = a.job[which];
-    __shared__ T tile[64][65];
+    __shared__ T tile[64][64 + 4 / sizeof(T)];
     const T* src = (const T*)jb.src;
     T* dst = (T*)jb.dst;
-    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    const int tx = threadIdx.x % ACROSS, ty = threadIdx.x / ACROSS;
     // the grid covers the padded destination: destination columns are source columns, or (transposed) source rows
     const int64_t tiles_c = ((TRANSPOSE ? jb.cols : jb.pitch) + 63) / 64;
     const int64_t r0 = id / tiles_c * 64, c0 = id % tiles_c * 64;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int64_t r = r0 + ty + i * 4, c = c0 + tx;
-        const T v = r < jb.rows && c < jb.cols ? src[r * jb.stride + c] : from_float<T>(0.0f);
-        if constexpr (TRANSPOSE) tile[ty + i * 4][tx] = v;
-        else if (r < jb.rows && c < jb.pitch) dst[r * jb.pitch + c] = v;
+    for (int i = 0; i < 64 / DOWN; ++i) {
+        const int64_t r = r0 + ty + i * DOWN, c = c0 + tx * V;
+        Pack<T> p;
+        if (r < jb.rows && c + V <= jb.cols) p = load_pack(src + r * jb.stride + c);
+        else
+#pragma unroll
+            for (int j = 0; j < V; ++j) p.v[j] = r < jb.rows && c + j < jb.cols ? src[r * jb.stride + c + j] : from_float<T>(0.0f);
+        if constexpr (TRANSPOSE) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) tile[ty + i * DOWN][tx * V + j] = p.v[j];
+        } else if (r < jb.rows && c < jb.pitch) {
+            store_pack(dst + r * jb.pitch + c, p);
+        }
     }
     if constexpr (TRANSPOSE) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int64_t c = c0 + ty + i * 4, r = r0 + tx;      // pitch is a multiple of 64: r < pitch
-            if (c < jb.cols) dst[c * jb.pitch + r] = tile[tx][ty + i * 4];
+        for (int i = 0; i < 64 / DOWN; ++i) {
+            const int64_t c = c0 + ty + i * DOWN, r = r0 + tx * V;      // the pitch is a multiple of 64: r < pitch
+            Pack<T> p;
+#pragma unroll
+            for (int j = 0; j < V; ++j) p.v[j] = tile[tx * V + j][ty + i * DOWN];
+            if (c < jb.cols) store_pack(dst + c * jb.pitch + r, p);
         }
     }
 }
@@ -403,7 +416,8 @@ BackwardPlan backward_plan(int64_t m, int64_t k, int64_t h) {
     constexpr int KS = STEP_BYTES / sizeof(T);
     constexpr int64_t B = sizeof(T);
     BackwardPlan p;
-    p.fast = m >= 128 && h >= 128 && k >= 64 && 8 * m * h * k >= (int64_t)1 << 32 && m * B < (1 << 23) && h * B < (1 << 23);
+    // 4 GFLOP, or two million elements over many rows: below, the copies cost more than they save
+    p.fast = m >= 128 && (8 * m * h * k >= (int64_t)1 << 32 || (m >= 4096 && std::max(h, k) >= 128 && m * std::max(h, k) >= (int64_t)1 << 21)) && m * B < (1 << 23) && h * B < (1 << 23);
     if (p.fast) {
         p.hp = round_up(h, 64), p.mp = round_up(m, 64);
         auto choose = [&](int64_t rows, int64_t cols, int64_t zs, int64_t steps, int& tile, int& splits) {
