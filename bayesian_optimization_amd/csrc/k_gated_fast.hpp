@@ -286,6 +286,100 @@ __global__ __launch_bounds__(256) void k_gated_slopes_both(const T* __restrict__
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
+// Many rows, a short contraction (up to 256 elements of 16 bits): the tiles above would spend their time starting and ending.  Here
+// a wave keeps its 32 hidden units' weights for the whole contraction in registers (128 of them at 256 elements) and the
+// workgroup walks over tiles of 128 rows of x, the next one on its way into LDS while this one is multiplied; a row fragment is
+// read once for four matrix instructions.  wn of the 8 waves stand side by side over hidden units, the others share the rows.
+// Bound by its two halves about alike, matrix instructions and the activation's vector instructions (48 cycles an output and
+// wave), which two waves a SIMD overlap.  The weight rows are dealt to the fragments so that a lane ends up with 8 neighbouring
+// outputs: 16-byte stores.
+constexpr int STREAM_ROWS = 128, STREAM_MOST = 256;
+template <typename T, int SL>
+__global__ __launch_bounds__(512) void k_gated_stream(GatedArgs g, int wn, int groups) {
+    constexpr int CHUNKS = SL * 4, LOADS = STREAM_ROWS * CHUNKS / 512;
+    __shared__ uint4 buf0[STREAM_ROWS * CHUNKS], buf1[STREAM_ROWS * CHUNKS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // workgroups on the same rows land on the same XCD (ids go round the eight of them) and share x in its L2
+    const int stride = gridDim.x / groups, spread = stride % 8 == 0 ? 8 : 1;
+    const int group = blockIdx.x / spread % groups, first = blockIdx.x / (spread * groups) * spread + blockIdx.x % spread;
+    const int64_t base = (int64_t)group * wn * 32 + (wave % wn) * 32;
+    const int64_t tiles = (g.m + STREAM_ROWS - 1) / STREAM_ROWS;
+    uint4 fb[2][2][SL];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int64_t h = min(base + ((lane & 15) >> 2) * 8 + j * 4 + (lane & 3), g.n - 1);
+#pragma unroll
+        for (int s = 0; s < SL; ++s) {
+            const int64_t at = s * 64 + (lane >> 4) * 16;
+            fb[j][0][s] = *(const uint4*)((const char*)g.b[0].p + h * g.b[0].sr * (int64_t)sizeof(T) + at);
+            fb[j][1][s] = *(const uint4*)((const char*)g.b[1].p + h * g.b[1].sr * (int64_t)sizeof(T) + at);
+        }
+    }
+    const int64_t sa = g.a[0].sr * (int64_t)sizeof(T);
+    auto fetch = [&](uint4* buf, int64_t t) {
+        const int64_t row0 = t * STREAM_ROWS, last = g.m - 1 - row0;
+        const auto ra = buffer_of((const char*)g.a[0].p + row0 * sa);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int id = i * 512 + tid, r = id / CHUNKS, c = (id % CHUNKS) ^ (r & 7);
+            load_lds(ra, buf + i * 512 + wave * 64, (uint32_t)(min((int64_t)r, last) * sa + c * 16), 0);
+        }
+    };
+    auto work = [&](const uint4* buf, int64_t t) {
+        for (int f = wave / wn; f < STREAM_ROWS / 16; f += 8 / wn) {
+            f32x4 acc[2][2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) acc[j][0] = acc[j][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            const uint4* pa = buf + (f * 16 + (lane & 15)) * CHUNKS;
+#pragma unroll
+            for (int s = 0; s < SL; ++s) {
+                const uint4 fa = pa[(s * 4 + (lane >> 4)) ^ (lane & 7)];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    acc[j][0] = mma<T>(fb[j][0][s], fa, acc[j][0]);
+                    acc[j][1] = mma<T>(fb[j][1][s], fa, acc[j][1]);
+                }
+            }
+            const int64_t row = t * STREAM_ROWS + f * 16 + (lane & 15), col = base + (lane >> 4) * 8;
+            if (row >= g.m || col >= g.n) continue;
+            const int len = (int)min((int64_t)8, g.n - col);
+            T o[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) o[r] = from_float<T>(activate<T>(acc[r >> 2][0][r & 3], g.act) * acc[r >> 2][1][r & 3]);
+            T* p = (T*)g.out[0] + row * g.os + col;
+            if (len == 8) __builtin_memcpy(p, o, sizeof(o));
+            else
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < len) p[r] = o[r];
+            if (g.keep_g) {
+                float *kg = g.keep_g + row * g.n + col, *ku = g.keep_u + row * g.n + col;
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < len) kg[r] = acc[r >> 2][0][r & 3], ku[r] = acc[r >> 2][1][r & 3];
+            }
+        }
+    };
+    if (first >= tiles) return;
+    fetch(buf0, first);
+    __syncthreads();
+    for (int64_t t = first;; t += 2 * stride) {
+        const bool more = t + stride < tiles;
+        if (more) fetch(buf1, t + stride);
+        __builtin_amdgcn_sched_barrier(0);
+        work(buf0, t);
+        __syncthreads();
+        if (!more) break;
+        const bool again = t + 2 * stride < tiles;
+        if (again) fetch(buf0, t + 2 * stride);
+        __builtin_amdgcn_sched_barrier(0);
+        work(buf1, t + stride);
+        __syncthreads();
+        if (!again) break;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
 // A few rows (one candidate at a time): bound by reading the weights once.  A wave takes one hidden unit: both its weight rows in
 // 16-byte packs, R rows of x against them, sums over the lanes at the end.
 template <typename T, int R>
@@ -340,7 +434,7 @@ inline bool aligned16(const void* p, int64_t stride, int64_t bytes) {
 }
 
 struct ForwardPlan {
-    bool fast = false, pack = false;
+    bool fast = false, pack = false, stream = false;
     int tile = 128;
     int64_t kp = 0, x_bytes = 0, w_bytes = 0;
     int64_t bytes() const { return pack ? x_bytes + 2 * w_bytes : 0; }
@@ -353,6 +447,9 @@ ForwardPlan forward_plan(int64_t m, int64_t k, int64_t h) {
     ForwardPlan p;
     p.kp = round_up(k, KS);
     p.fast = m * h >= 128 * 64 * 64 && 4 * m * h * k >= (int64_t)1 << 31 && k * (int64_t)sizeof(T) < (1 << 23);
+    // at least two tiles of rows for every workgroup of the streaming form
+    p.stream = sizeof(T) == 2 && p.kp <= STREAM_MOST && m * h >= (int64_t)1 << 21 && ceil_div(m, STREAM_ROWS) * ceil_div(h, 256) >= 512;
+    p.fast = p.fast || p.stream;
     p.pack = p.fast && k % KS != 0;
     if (ceil_div(m, 256) * ceil_div(h, 128) >= 256 && k >= 8 * KS) p.tile = 256;
     p.x_bytes = round_up(m * p.kp * (int64_t)sizeof(T), 256);
@@ -372,6 +469,22 @@ void launch_fast(hipStream_t st, const GatedArgs& g, int tile) {
 }
 
 template <typename T>
+void launch_stream(hipStream_t st, const GatedArgs& g) {
+    if constexpr (sizeof(T) == 2) {
+        int wn = 1;
+        while (wn < 8 && wn * 32 < g.n) wn *= 2;
+        const int groups = (int)ceil_div(g.n, wn * 32);
+        int64_t walkers = std::max<int64_t>(1, std::min<int64_t>(256 / std::min(groups, 256), ceil_div(g.m, STREAM_ROWS)));
+        if (walkers > 8) walkers -= walkers % 8;
+        const dim3 grid((unsigned)(groups * walkers));
+        if (g.k <= 64) hipLaunchKernelGGL((k_gated_stream<T, 2>), grid, dim3(512), 0, st, g, wn, groups);
+        else if (g.k <= 128) hipLaunchKernelGGL((k_gated_stream<T, 4>), grid, dim3(512), 0, st, g, wn, groups);
+        else if (g.k <= 192) hipLaunchKernelGGL((k_gated_stream<T, 6>), grid, dim3(512), 0, st, g, wn, groups);
+        else hipLaunchKernelGGL((k_gated_stream<T, 8>), grid, dim3(512), 0, st, g, wn, groups);
+    }
+}
+
+template <typename T>
 hipError_t gated_forward(hipStream_t st, GatedArgs g, char* work) {
     constexpr int KS = STEP_BYTES / sizeof(T);
     const ForwardPlan p = forward_plan<T>(g.m, g.k, g.n);
@@ -388,7 +501,8 @@ hipError_t gated_forward(hipStream_t st, GatedArgs g, char* work) {
             g.k = p.kp;
         }
         static_assert(KS >= 32, "a step");
-        launch_fast<T, GATED_FWD>(st, g, p.tile);
+        if (p.stream) launch_stream<T>(st, g);
+        else launch_fast<T, GATED_FWD>(st, g, p.tile);
     } else if (g.m <= 16) {
         const unsigned hidden = (unsigned)ceil_div(g.n, 4);
         if (g.m == 1) hipLaunchKernelGGL((k_gated_few<T, 1>), dim3(hidden, 1), dim3(256), 0, st, g);

@@ -181,7 +181,8 @@ def test_gated_unit_forward_and_backward(dtype, act, rows, cols, hidden):
 # large enough for the kernels that load straight into LDS, both tile sizes, whole and broken steps, split contractions, edges
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('rows,cols,hidden', [(1100, 1024, 1000), (2050, 621, 777), (300, 4096, 1030), (128, 2048, 2111), (4100, 520, 2049), (2305, 1024, 4224), (20000, 64, 128),
-                                              (129, 8192, 640), (8200, 640, 1024)])
+                                              (129, 8192, 640), (8200, 640, 1024),
+                                              (70001, 40, 90), (66000, 128, 33), (40000, 190, 300), (33000, 256, 515)])
 def test_gated_unit_large(dtype, rows, cols, hidden):
     check_gated(dtype, 'gelu' if rows % 2 else 'silu', rows, cols, hidden)
 
