@@ -325,7 +325,14 @@ __global__ __launch_bounds__(512) void k_gated_stream(GatedArgs g, int wn, int g
             load_lds(ra, buf + i * 512 + wave * 64, (uint32_t)(min((int64_t)r, last) * sa + c * 16), 0);
         }
     };
+    const int64_t col = base + (lane >> 4) * 8;
+    const int len = (int)max((int64_t)0, min((int64_t)8, g.n - col));
+    T* const out = (T*)g.out[0] + (lane & 15) * g.os + col;
+    float *const kg = g.keep_g ? g.keep_g + (lane & 15) * g.n + col : nullptr, *const ku = g.keep_g ? g.keep_u + (lane & 15) * g.n + col : nullptr;
+    const bool whole_cols = base + 32 <= g.n;
     auto work = [&](const uint4* buf, int64_t t) {
+        const bool whole = whole_cols && (t + 1) * STREAM_ROWS <= g.m;         // uniform: no lane has anything to leave out
+#pragma unroll 2
         for (int f = wave / wn; f < STREAM_ROWS / 16; f += 8 / wn) {
             f32x4 acc[2][2];
 #pragma unroll
@@ -340,23 +347,26 @@ __global__ __launch_bounds__(512) void k_gated_stream(GatedArgs g, int wn, int g
                     acc[j][1] = mma<T>(fb[j][1][s], fa, acc[j][1]);
                 }
             }
-            const int64_t row = t * STREAM_ROWS + f * 16 + (lane & 15), col = base + (lane >> 4) * 8;
-            if (row >= g.m || col >= g.n) continue;
-            const int len = (int)min((int64_t)8, g.n - col);
+            const int64_t row = t * STREAM_ROWS + f * 16;                      // the fragment's first
             T o[8];
 #pragma unroll
             for (int r = 0; r < 8; ++r) o[r] = from_float<T>(activate<T>(acc[r >> 2][0][r & 3], g.act) * acc[r >> 2][1][r & 3]);
-            T* p = (T*)g.out[0] + row * g.os + col;
-            if (len == 8) __builtin_memcpy(p, o, sizeof(o));
-            else
+            T* p = out + row * g.os;
+            if (whole) {
+                __builtin_memcpy(p, o, sizeof(o));
+                if (kg) {
+                    __builtin_memcpy(kg + row * g.n, &acc[0][0], 16);
+                    __builtin_memcpy(kg + row * g.n + 4, &acc[1][0], 16);
+                    __builtin_memcpy(ku + row * g.n, &acc[0][1], 16);
+                    __builtin_memcpy(ku + row * g.n + 4, &acc[1][1], 16);
+                }
+            } else if (row + (lane & 15) < g.m) {
 #pragma unroll
                 for (int r = 0; r < 8; ++r)
-                    if (r < len) p[r] = o[r];
-            if (g.keep_g) {
-                float *kg = g.keep_g + row * g.n + col, *ku = g.keep_u + row * g.n + col;
-#pragma unroll
-                for (int r = 0; r < 8; ++r)
-                    if (r < len) kg[r] = acc[r >> 2][0][r & 3], ku[r] = acc[r >> 2][1][r & 3];
+                    if (r < len) {
+                        p[r] = o[r];
+                        if (kg) kg[row * g.n + r] = acc[r >> 2][0][r & 3], ku[row * g.n + r] = acc[r >> 2][1][r & 3];
+                    }
             }
         }
     };
