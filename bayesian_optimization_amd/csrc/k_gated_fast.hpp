@@ -8,9 +8,11 @@ namespace gpbo_static {
 
 // Tile of BM x BN outputs by WM x WN waves; a step is 128 bytes of contraction of BM + BN rows.  The step after the current one
 // is on its way into the other LDS buffer (16 bytes a lane, no registers) while the current one is multiplied: one barrier a
-// step.  Row r of a step lies at 128 r, its 16-byte chunk c at slot c ^ (r & 7): a fragment read touches 16 rows, and without the
+// step.  Row r of a step lies at 128 r, its 16-byte chunk c at slot c ^ swap(r): a fragment read touches 16 rows, and without the
 // exchange all of them would start in the same bank; the loads do the exchange by the address each lane fetches from, since
-// their destination is fixed (wave base + 16 lane).
+// their destination is fixed (wave base + 16 lane).  Fragments of the second operand come in pairs over 32 output columns, dealt
+// out by fours, so that a lane ends up with 8 neighbouring outputs of a row (16384 x 2048 -> 8192 in 16 bits: the forward pass
+// 1.40 -> 1.29 ms, each backward product 0.91 -> 0.88 ms, 1.24 PFLOP/s).
 template <typename T, int MODE, int BM, int BN, int WM, int WN>
 struct FastTile {
     static constexpr int THREADS = 64 * WM * WN, KS = STEP_BYTES / sizeof(T);
@@ -18,6 +20,10 @@ struct FastTile {
     static constexpr int LA = BM * 8 / THREADS, LB = BN * 8 / THREADS;      // 16-byte loads of a thread and step
     static constexpr int COLS = MODE == GATED_FWD ? BN / 2 : BN;            // output columns of a tile
 };
+
+// The slots of 8 rows that one access touches are all different for rows 8 n .. 8 n + 7 as well as for rows 16 n + {0..3, 8..11} and
+// 16 n + {4..7, 12..15}.
+__device__ __forceinline__ constexpr int swap_of(int r) { return (r ^ ((r >> 1) & 4)) & 7; }
 
 typedef __attribute__((address_space(3))) void* LdsPtr;
 
@@ -61,12 +67,12 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 256 ? 1 : 2) void k_gated_fast(
     const int64_t sa = g.a[0].sr * (int64_t)sizeof(T), sb = g.b[0].sr * (int64_t)sizeof(T);
 #pragma unroll
     for (int i = 0; i < F::LA; ++i) {
-        const int r = (i * F::THREADS + tid) >> 3, c = (tid & 7) ^ (r & 7);
+        const int r = (i * F::THREADS + tid) >> 3, c = (tid & 7) ^ swap_of(r);
         oa[i] = (uint32_t)(min((int64_t)r, g.m - 1 - row0) * sa + c * 16);
     }
 #pragma unroll
     for (int i = 0; i < F::LB; ++i) {
-        const int r = (i * F::THREADS + tid) >> 3, c = (tid & 7) ^ (r & 7);
+        const int r = (i * F::THREADS + tid) >> 3, c = (tid & 7) ^ swap_of(r);
         const int q = MODE == GATED_FWD ? r % F::COLS : r;
         ob[i] = (uint32_t)(min((int64_t)q, g.n - 1 - col0) * sb + c * 16);
     }
@@ -95,11 +101,15 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 256 ? 1 : 2) void k_gated_fast(
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
             uint4 fa[FM], fb[FN];
-            const int c = (kk * 4 + (lane >> 4)) ^ (lane & 7);              // every fragment starts at a multiple of 8 rows
-            const uint4* pa = buf + (wm * FM * 16 + (lane & 15)) * 8 + c;
-            const uint4* pb = buf + (BM + (MODE == GATED_FWD ? wn * (FN / 2 * 16) : wn * FN * 16) + (lane & 15)) * 8 + c;
+            const int m = lane & 15, c = kk * 4 + (lane >> 4), deal = (m >> 2) * 8 + (m & 3);
+            const uint4* pa = buf + (wm * FM * 16 + m) * 8 + (c ^ swap_of(m));
+            const uint4* pb = buf + (BM + (MODE == GATED_FWD ? wn * (FN / 2 * 16) : wn * FN * 16) + deal) * 8;
 #pragma unroll
-            for (int j = 0; j < FN; ++j) fb[j] = pb[MODE == GATED_FWD ? ((j >= FN / 2) * F::COLS + (j % (FN / 2)) * 16) * 8 : j * 16 * 8];
+            for (int j = 0; j < FN; ++j) {
+                // pairs of fragments: 32 columns each; going forward the second half of them is the other weight matrix
+                const int at = MODE == GATED_FWD ? (j >= FN / 2) * F::COLS + (j % (FN / 2)) / 2 * 32 : j / 2 * 32;
+                fb[j] = pb[(at + (j & 1) * 4) * 8 + (c ^ swap_of(deal + (j & 1) * 4))];
+            }
 #pragma unroll
             for (int i = 0; i < FM; ++i) fa[i] = pa[i * 16 * 8];
 #pragma unroll
@@ -125,50 +135,55 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 256 ? 1 : 2) void k_gated_fast(
         if (s < steps) multiply(buf0);
     }
 
-    // lane: row lane % 16 of a fragment, four neighbouring columns from (lane / 16) * 4 on
+    // lane: row lane % 16 of a fragment, eight neighbouring columns of a pair of them
+    static_assert(FN % 4 == 0, "fragments come in pairs, of both weight matrices");
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
         const int64_t row = row0 + wm * FM * 16 + i * 16 + (lane & 15);
         if (row >= g.m) continue;
 #pragma unroll
-        for (int j = 0; j < (MODE == GATED_FWD ? FN / 2 : FN); ++j) {
-            const int64_t col = col0 + (MODE == GATED_FWD ? wn * (FN / 2 * 16) : wn * FN * 16) + j * 16 + (lane >> 4) * 4;
+        for (int j = 0; j < (MODE == GATED_FWD ? FN / 2 : FN); j += 2) {
+            const int64_t col = col0 + (MODE == GATED_FWD ? wn * (FN / 2 * 16) : wn * FN * 16) + j * 16 + (lane >> 4) * 8;
             if (col >= g.n) continue;
-            const int len = (int)min((int64_t)4, g.n - col);
-            float v[4];
+            const int len = (int)min((int64_t)8, g.n - col);
+            constexpr int UP = MODE == GATED_FWD ? FN / 2 : 0;
+            float v[8];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                if constexpr (MODE == GATED_FWD) v[r] = activate<T>(acc[i][j][r], g.act) * acc[i][j + FN / 2][r];
-                else v[r] = acc[i][j][r];
+            for (int r = 0; r < 8; ++r) {
+                if constexpr (MODE == GATED_FWD) v[r] = activate<T>(acc[i][j + (r >> 2)][r & 3], g.act) * acc[i][j + (r >> 2) + UP][r & 3];
+                else v[r] = acc[i][j + (r >> 2)][r & 3];
             }
             if (MODE != GATED_FWD && g.splits > 1) {
                 float* p = g.part + (((int64_t)z * g.splits + split) * g.m + row) * g.n + col;
-                if (len == 4) __builtin_memcpy(p, v, 16);
+                if (len == 8) __builtin_memcpy(p, v, 32);
                 else
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
+                    for (int r = 0; r < 8; ++r)
                         if (r < len) p[r] = v[r];
                 continue;
             }
-            T o[4];
+            T o[8];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = from_float<T>(v[r]);
+            for (int r = 0; r < 8; ++r) o[r] = from_float<T>(v[r]);
             T* p = (T*)(z ? g.out[1] : g.out[0]) + row * g.os + col;
-            if (len == 4) __builtin_memcpy(p, o, sizeof(o));
+            if (len == 8) __builtin_memcpy(p, o, sizeof(o));
             else
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
+                for (int r = 0; r < 8; ++r)
                     if (r < len) p[r] = o[r];
             if (MODE == GATED_FWD && g.keep_g) {
+                // (stores past the caches were no faster: an instruction leaves out every other 16 bytes, which only the L2 joins)
                 float *kg = g.keep_g + row * g.n + col, *ku = g.keep_u + row * g.n + col;
-                const f32x4 vg = acc[i][j], vu = acc[i][MODE == GATED_FWD ? j + FN / 2 : j];
-                if (len == 4) {
-                    __builtin_memcpy(kg, &vg, 16);
-                    __builtin_memcpy(ku, &vu, 16);
+                if (len == 8) {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        __builtin_memcpy(kg + q * 4, &acc[i][j + q], 16);
+                        __builtin_memcpy(ku + q * 4, &acc[i][j + q + UP], 16);
+                    }
                 } else {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (r < len) kg[r] = vg[r], ku[r] = vu[r];
+                    for (int r = 0; r < 8; ++r)
+                        if (r < len) kg[r] = acc[i][j + (r >> 2)][r & 3], ku[r] = acc[i][j + (r >> 2) + UP][r & 3];
                 }
             }
         }
