@@ -8,6 +8,8 @@
 // du once each, to the type of x: they are operands of the matrix instructions.
 #pragma once
 
+#include <type_traits>
+
 #include "static_ops.hpp"
 
 namespace gpbo_static {
@@ -228,67 +230,80 @@ __global__ __launch_bounds__(256) void k_gated_tile(GatedArgs g) {
 // ---------------------------------------------------------------------------------------------------------------------
 // Small products: what counts is how soon the last load is back, so 32 x 32 outputs a workgroup, its 8 waves take turns along the
 // contraction with fragments loaded straight into registers, and their sums are joined in LDS in a fixed order.  No staging, no
-// barrier until then (95 x 621 -> 128 in 32 bits: 40 -> 6 us against the 64 x 64 tile, which has 4 workgroups of 20 steps there).
+// barrier until then (95 x 621 -> 128 in 32 bits: 40 -> 8 us against the 64 x 64 tile, which has 4 workgroups of 20 steps there).
 constexpr int SB = 32, SMALL_WAVES = 8;
 
-template <typename T, bool KC>
+template <typename T, bool KC, bool WHOLE>
 __device__ __forceinline__ uint4 small_fragment(const Operand& o, int64_t row, int64_t k, int64_t k1) {
     constexpr int V = 16 / sizeof(T);
     const T* p = (const T*)o.p;
     Pack<T> r;
-    if constexpr (KC) {
-        if (k + V <= k1) r = load_pack(p + row * o.sr + k);
-        else
-#pragma unroll
-            for (int j = 0; j < V; ++j) r.v[j] = k + j < k1 ? p[row * o.sr + k + j] : from_float<T>(0.0f);
+    if constexpr (KC && WHOLE) {
+        r = load_pack(p + row * o.sr + k);
     } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) r.v[j] = k + j < k1 ? p[(k + j) * o.sk + row] : from_float<T>(0.0f);
+        for (int j = 0; j < V; ++j) r.v[j] = WHOLE || k + j < k1 ? p[KC ? row * o.sr + k + j : (k + j) * o.sk + row] : from_float<T>(0.0f);
     }
     return __builtin_bit_cast(uint4, r);
 }
 
-template <typename T, int MODE, bool AKC, bool BKC>
-__global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small(GatedArgs g) {
-    constexpr int SLAB = 64 / sizeof(T), V = 16 / sizeof(T), NB = MODE == GATED_FWD ? 2 : 1;
-    __shared__ f32x4 sums[SMALL_WAVES][NB * 4][64];
-    const int64_t nt = (g.n + SB - 1) / SB;
-    const int64_t row0 = (int64_t)(blockIdx.x / nt) * SB, col0 = (int64_t)(blockIdx.x % nt) * SB;
-    const int z = MODE == GATED_PAIR ? blockIdx.z : 0, split = blockIdx.y;
-    const int64_t per = ((g.k + g.splits - 1) / g.splits + SLAB - 1) / SLAB * SLAB;
-    const int64_t kb = min(split * per, g.k), ke = min(kb + per, g.k);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    f32x4 acc[NB][2][2];
+// What the backward products of a small problem need of dg (which = 0) and du (1), computed where it is used and rounded as
+// k_gated_slopes would: element (row, k) of the operand is element (row, k) of dh, g, u if KC, else (k, row).
+struct SlopeOperand {
+    const void* dh;
+    const float *kg, *ku;
+    int64_t dhs, n;               // row strides of dh; of kg and ku
+    int act;
+};
+template <typename T, bool KC, bool WHOLE>
+__device__ __forceinline__ uint4 slope_fragment(const SlopeOperand& o, int which, int64_t row, int64_t k, int64_t k1) {
+    constexpr int V = 16 / sizeof(T);
+    Pack<T> r;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) acc[b][i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    int64_t ra[2], rb[2];                      // rows behind the last repeat it: their outputs are not stored
-#pragma unroll
-    for (int i = 0; i < 2; ++i) ra[i] = min(row0 + i * 16 + (lane & 15), g.m - 1), rb[i] = min(col0 + i * 16 + (lane & 15), g.n - 1);
-#pragma unroll
-    for (int part = 0; part < (MODE == GATED_SUM ? 2 : 1); ++part) {
-        const Operand oa = MODE == GATED_PAIR && z ? g.a[1] : g.a[part], ob = g.b[part];
-#pragma unroll 4
-        for (int64_t k0 = kb + wave * SLAB; k0 < ke; k0 += SMALL_WAVES * SLAB) {
-            const int64_t k = k0 + (lane >> 4) * V;
-            uint4 fa[2], fb[NB][2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                fa[i] = small_fragment<T, AKC>(oa, ra[i], k, ke);
-                fb[0][i] = small_fragment<T, BKC>(ob, rb[i], k, ke);
-                if constexpr (NB == 2) fb[NB - 1][i] = small_fragment<T, BKC>(g.b[1], rb[i], k, ke);
-            }
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) acc[b][i][j] = mma<T>(fb[b][j], fa[i], acc[b][i][j]);
+    for (int j = 0; j < V; ++j) {
+        const int64_t i = KC ? row : k + j, c = KC ? k + j : row;
+        if (WHOLE || k + j < k1) {
+            float a, da;
+            activation<T>(o.kg[i * o.n + c], o.act, a, da);
+            const float d = to_float(((const T*)o.dh)[i * o.dhs + c]);
+            r.v[j] = from_float<T>(which ? d * a : d * o.ku[i * o.n + c] * da);
+        } else {
+            r.v[j] = from_float<T>(0.0f);
         }
     }
+    return __builtin_bit_cast(uint4, r);
+}
+
+// The body: NB products side by side (one first operand, NB second ones), slabs of contraction [kb, ke) dealt to the waves; fa(i, k, whole)
+// and fb(b, i, k, whole) give fragments i = 0, 1.  Leaves fragment `wave` of the 32 x 32 outputs in v of waves 0 .. 3.
+template <typename T, int NB, typename FA, typename FB>
+__device__ __forceinline__ void small_sums(f32x4 (&acc)[NB][2][2], int64_t kb, int64_t ke, FA&& fa, FB&& fb) {
+    constexpr int SLAB = 64 / sizeof(T), V = 16 / sizeof(T);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t slabs = (ke - kb) / SLAB;
+    auto slab = [&](int64_t k0, auto whole) {
+        const int64_t k = k0 + (lane >> 4) * V;
+        uint4 a[2], b[NB][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            a[i] = fa(i, k, whole);
+#pragma unroll
+            for (int q = 0; q < NB; ++q) b[q][i] = fb(q, i, k, whole);
+        }
+#pragma unroll
+        for (int q = 0; q < NB; ++q)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) acc[q][i][j] = mma<T>(b[q][j], a[i], acc[q][i][j]);
+    };
+#pragma unroll 4
+    for (int64_t s = wave; s < slabs; s += SMALL_WAVES) slab(kb + s * SLAB, std::true_type{});
+    if (kb + slabs * SLAB < ke && slabs % SMALL_WAVES == wave) slab(kb + slabs * SLAB, std::false_type{});      // the broken last one
+}
+template <int NB>
+__device__ __forceinline__ void small_join(const f32x4 (&acc)[NB][2][2], f32x4 (&v)[NB], f32x4 (*sums)[NB * 4][64]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -296,15 +311,37 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small(GatedArgs g) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) sums[wave][b * 4 + i * 2 + j][lane] = acc[b][i][j];
     __syncthreads();
-    // wave f of the first four takes fragment f
-    if (wave >= 4) return;
-    f32x4 v[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        v[b] = sums[0][b * 4 + wave][lane];
+        v[b] = sums[0][b * 4 + (wave & 3)][lane];
 #pragma unroll
-        for (int w = 1; w < SMALL_WAVES; ++w) v[b] += sums[w][b * 4 + wave][lane];
+        for (int w = 1; w < SMALL_WAVES; ++w) v[b] += sums[w][b * 4 + (wave & 3)][lane];
     }
+}
+
+template <typename T, int MODE, bool AKC, bool BKC>
+__global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small(GatedArgs g) {
+    constexpr int SLAB = 64 / sizeof(T), NB = MODE == GATED_FWD ? 2 : 1;
+    __shared__ f32x4 sums[SMALL_WAVES][NB * 4][64];
+    const int64_t nt = (g.n + SB - 1) / SB;
+    const int64_t row0 = (int64_t)(blockIdx.x / nt) * SB, col0 = (int64_t)(blockIdx.x % nt) * SB;
+    const int z = MODE == GATED_PAIR ? blockIdx.z : 0, split = blockIdx.y;
+    const int64_t per = ((g.k + g.splits - 1) / g.splits + SLAB - 1) / SLAB * SLAB;
+    const int64_t kb = min(split * per, g.k), ke = min(kb + per, g.k);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    f32x4 acc[NB][2][2] = {};
+    int64_t ra[2], rb[2];                      // rows behind the last repeat it: their outputs are not stored
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ra[i] = min(row0 + i * 16 + (lane & 15), g.m - 1), rb[i] = min(col0 + i * 16 + (lane & 15), g.n - 1);
+#pragma unroll
+    for (int part = 0; part < (MODE == GATED_SUM ? 2 : 1); ++part) {
+        const Operand oa = MODE == GATED_PAIR && z ? g.a[1] : g.a[part], ob = g.b[part], ob2 = g.b[1];
+        small_sums<T, NB>(acc, kb, ke, [&](int i, int64_t k, auto whole) { return small_fragment<T, AKC, whole.value>(oa, ra[i], k, ke); },
+                          [&](int b, int i, int64_t k, auto whole) { return small_fragment<T, BKC, whole.value>(b ? ob2 : ob, rb[i], k, ke); });
+    }
+    f32x4 v[NB];
+    small_join<NB>(acc, v, sums);
+    if (wave >= 4) return;
     const int64_t row = row0 + (wave >> 1) * 16 + (lane & 15), col = col0 + (wave & 1) * 16 + (lane >> 4) * 4;
     if (row >= g.m) return;
 #pragma unroll
@@ -319,6 +356,52 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small(GatedArgs g) {
             ((T*)(z ? g.out[1] : g.out[0]))[row * g.os + col + r] = from_float<T>(v[0][r]);
         }
     }
+}
+
+// The whole backward pass of a small problem in one launch: the tiles of dx, then those of dwg and of dwu, each with its part of dg
+// and du computed on the way into the matrix instructions (every tile column again, which is why it has to be small).
+template <typename T>
+__global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small_back(SlopeOperand s, Operand x, Operand wg, Operand wu, int64_t m, int64_t k, int64_t h,
+                                                                       void* dx, int64_t dxs, void* dwg, void* dwu, int64_t dws) {
+    __shared__ f32x4 sums[SMALL_WAVES][4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t nt = (k + SB - 1) / SB, tiles_x = dx ? (m + SB - 1) / SB * nt : 0, tiles_w = (h + SB - 1) / SB * nt;
+    int64_t id = blockIdx.x;
+    f32x4 acc[1][2][2] = {};
+    f32x4 v[1];
+    const int64_t col0 = id < tiles_x ? id % nt * SB : (id - tiles_x) % nt * SB;
+    int64_t rb[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) rb[i] = min(col0 + i * 16 + (lane & 15), k - 1);
+    void* out;
+    int64_t row0, rows, os;
+    if (id < tiles_x) {                        // dx = dg wg + du wu, contraction over the hidden units
+        row0 = id / nt * SB, rows = m, os = dxs, out = dx;
+        int64_t ra[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) ra[i] = min(row0 + i * 16 + (lane & 15), m - 1);
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+            small_sums<T, 1>(acc, 0, h, [&](int i, int64_t q, auto whole) { return slope_fragment<T, true, whole.value>(s, which, ra[i], q, h); },
+                             [&](int, int i, int64_t q, auto whole) { return small_fragment<T, false, whole.value>(which ? wu : wg, rb[i], q, h); });
+    } else {                                   // dw = d^T x, contraction over the rows
+        id -= tiles_x;
+        const int which = id >= tiles_w;
+        if (which) id -= tiles_w;
+        row0 = id / nt * SB, rows = h, os = dws, out = which ? dwu : dwg;
+        int64_t ra[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) ra[i] = min(row0 + i * 16 + (lane & 15), h - 1);
+        small_sums<T, 1>(acc, 0, m, [&](int i, int64_t q, auto whole) { return slope_fragment<T, false, whole.value>(s, which, ra[i], q, m); },
+                         [&](int, int i, int64_t q, auto whole) { return small_fragment<T, false, whole.value>(x, rb[i], q, m); });
+    }
+    small_join<1>(acc, v, sums);
+    if (wave >= 4) return;
+    const int64_t row = row0 + (wave >> 1) * 16 + (lane & 15), col = col0 + (wave & 1) * 16 + (lane >> 4) * 4;
+    if (row >= rows) return;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (col + r < k) ((T*)out)[row * os + col + r] = from_float<T>(v[0][r]);
 }
 
 // The split sums of one output, added in split order.

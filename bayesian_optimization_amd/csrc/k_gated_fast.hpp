@@ -543,7 +543,7 @@ hipError_t gated_forward(hipStream_t st, GatedArgs g, char* work) {
 // Backward.  Large: dg and du are written both ways round, x and the weights transposed, so that every product contracts along
 // rows; these copies are a few per cent of the products' time.
 struct BackwardPlan {
-    bool fast = false;
+    bool fast = false, one = false;      // one: k_gated_small_back
     int tile_x = 128, tile_w = 128, splits_x = 1, splits_w = 1;
     AnyPlan any_x, any_w;
     int64_t hp = 0, mp = 0;
@@ -569,6 +569,9 @@ BackwardPlan backward_plan(int64_t m, int64_t k, int64_t h) {
         p.d_bytes = round_up(m * p.hp * B, 256), p.dt_bytes = round_up(h * p.mp * B, 256);
         p.xt_bytes = round_up(k * p.mp * B, 256), p.wt_bytes = round_up(k * p.hp * B, 256);
     } else {
+        // one launch while all tiles together work out dg and du no more than a million times, and a tile's waves have few slabs
+        p.one = m > 0 && 4 * m * h * ceil_div(k, SB) <= (int64_t)1 << 20 && std::max(m, 2 * h) <= 64 * KS;
+        if (p.one) return p;
         p.d_bytes = round_up(m * h * B, 256);
         p.any_x = any_plan<T>(m, k, h, 1, true), p.any_w = any_plan<T>(h, k, m, 2, true);
         p.splits_x = p.any_x.splits, p.splits_w = p.any_w.splits;
@@ -582,6 +585,13 @@ hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const voi
                           const float* kg, const float* ku, int64_t m, int64_t k, int64_t h, int act, void* dx, int64_t dxs, void* dwg,
                           void* dwu, int64_t dws, char* work) {
     const BackwardPlan p = backward_plan<T>(m, k, h);
+    if (p.one) {
+        const int64_t nt = ceil_div(k, SB), tiles = (dx ? ceil_div(m, SB) * nt : 0) + (dwg ? 2 * ceil_div(h, SB) * nt : 0);
+        if (tiles > 0)
+            hipLaunchKernelGGL(k_gated_small_back<T>, dim3((unsigned)tiles), dim3(64 * SMALL_WAVES), 0, st, SlopeOperand{dh, kg, ku, dhs, h, act},
+                               Operand{x, 1, xs}, Operand{wg, 1, ws}, Operand{wu, 1, ws}, m, k, h, dx, dxs, dwg, dwu, dws);
+        return hipGetLastError();
+    }
     char* at = work;
     auto take = [&](int64_t bytes) { char* r = at; at += bytes; return r; };
     T *dg = (T*)take(p.d_bytes), *du = (T*)take(p.d_bytes), *dgt = (T*)take(p.dt_bytes), *dut = (T*)take(p.dt_bytes), *xt = (T*)take(p.xt_bytes),
