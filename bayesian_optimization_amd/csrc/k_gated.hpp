@@ -228,9 +228,10 @@ __global__ __launch_bounds__(256) void k_gated_tile(GatedArgs g) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Small products: what counts is how soon the last load is back, so 32 x 32 outputs a workgroup, its 8 waves take turns along the
-// contraction with fragments loaded straight into registers, and their sums are joined in LDS in a fixed order.  No staging, no
-// barrier until then (95 x 621 -> 128 in 32 bits: 40 -> 8 us against the 64 x 64 tile, which has 4 workgroups of 20 steps there).
+// Small products: what counts is how soon the last load is back, so FR x FR fragments of outputs a workgroup, its 8 waves take turns
+// along the contraction with fragments loaded straight into registers, and their sums are joined in LDS in a fixed order.  No
+// staging, no barrier until then (95 x 621 -> 128 in 32 bits: 40 us with the 64 x 64 tile, which has 4 workgroups of 20 steps there;
+// 12 with 2 x 2 fragments, where 12 CUs are short of matrix instructions; 7 with one).
 constexpr int SB = 32, SMALL_WAVES = 8;
 
 template <typename T, bool KC, bool WHOLE>
@@ -275,17 +276,17 @@ __device__ __forceinline__ uint4 slope_fragment(const SlopeOperand& o, int which
 }
 
 // The body: NB products side by side (one first operand, NB second ones), slabs of contraction [kb, ke) dealt to the waves; fa(i, k, whole)
-// and fb(b, i, k, whole) give fragments i = 0, 1.  Leaves fragment `wave` of the 32 x 32 outputs in v of waves 0 .. 3.
-template <typename T, int NB, typename FA, typename FB>
-__device__ __forceinline__ void small_sums(f32x4 (&acc)[NB][2][2], int64_t kb, int64_t ke, FA&& fa, FB&& fb) {
+// and fb(b, i, k, whole) give fragments i < FR.
+template <typename T, int NB, int FR, typename FA, typename FB>
+__device__ __forceinline__ void small_sums(f32x4 (&acc)[NB][FR][FR], int64_t kb, int64_t ke, FA&& fa, FB&& fb) {
     constexpr int SLAB = 64 / sizeof(T), V = 16 / sizeof(T);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t slabs = (ke - kb) / SLAB;
     auto slab = [&](int64_t k0, auto whole) {
         const int64_t k = k0 + (lane >> 4) * V;
-        uint4 a[2], b[NB][2];
+        uint4 a[FR], b[NB][FR];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < FR; ++i) {
             a[i] = fa(i, k, whole);
 #pragma unroll
             for (int q = 0; q < NB; ++q) b[q][i] = fb(q, i, k, whole);
@@ -293,56 +294,58 @@ __device__ __forceinline__ void small_sums(f32x4 (&acc)[NB][2][2], int64_t kb, i
 #pragma unroll
         for (int q = 0; q < NB; ++q)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < FR; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) acc[q][i][j] = mma<T>(b[q][j], a[i], acc[q][i][j]);
+                for (int j = 0; j < FR; ++j) acc[q][i][j] = mma<T>(b[q][j], a[i], acc[q][i][j]);
     };
 #pragma unroll 4
     for (int64_t s = wave; s < slabs; s += SMALL_WAVES) slab(kb + s * SLAB, std::true_type{});
     if (kb + slabs * SLAB < ke && slabs % SMALL_WAVES == wave) slab(kb + slabs * SLAB, std::false_type{});      // the broken last one
 }
-template <int NB>
-__device__ __forceinline__ void small_join(const f32x4 (&acc)[NB][2][2], f32x4 (&v)[NB], f32x4 (*sums)[NB * 4][64]) {
+// The waves' sums, in wave order: fragment `wave` of the FR * FR in v of the first waves.
+template <int NB, int FR>
+__device__ __forceinline__ void small_join(const f32x4 (&acc)[NB][FR][FR], f32x4 (&v)[NB], f32x4 (*sums)[NB * FR * FR][64]) {
+    constexpr int F = FR * FR;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < FR; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) sums[wave][b * 4 + i * 2 + j][lane] = acc[b][i][j];
+            for (int j = 0; j < FR; ++j) sums[wave][b * F + i * FR + j][lane] = acc[b][i][j];
     __syncthreads();
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        v[b] = sums[0][b * 4 + (wave & 3)][lane];
+        v[b] = sums[0][b * F + wave % F][lane];
 #pragma unroll
-        for (int w = 1; w < SMALL_WAVES; ++w) v[b] += sums[w][b * 4 + (wave & 3)][lane];
+        for (int w = 1; w < SMALL_WAVES; ++w) v[b] += sums[w][b * F + wave % F][lane];
     }
 }
 
-template <typename T, int MODE, bool AKC, bool BKC>
+template <typename T, int MODE, bool AKC, bool BKC, int FR>
 __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small(GatedArgs g) {
-    constexpr int SLAB = 64 / sizeof(T), NB = MODE == GATED_FWD ? 2 : 1;
-    __shared__ f32x4 sums[SMALL_WAVES][NB * 4][64];
+    constexpr int SLAB = 64 / sizeof(T), NB = MODE == GATED_FWD ? 2 : 1, SB = 16 * FR;
+    __shared__ f32x4 sums[SMALL_WAVES][NB * FR * FR][64];
     const int64_t nt = (g.n + SB - 1) / SB;
     const int64_t row0 = (int64_t)(blockIdx.x / nt) * SB, col0 = (int64_t)(blockIdx.x % nt) * SB;
     const int z = MODE == GATED_PAIR ? blockIdx.z : 0, split = blockIdx.y;
     const int64_t per = ((g.k + g.splits - 1) / g.splits + SLAB - 1) / SLAB * SLAB;
     const int64_t kb = min(split * per, g.k), ke = min(kb + per, g.k);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    f32x4 acc[NB][2][2] = {};
-    int64_t ra[2], rb[2];                      // rows behind the last repeat it: their outputs are not stored
+    f32x4 acc[NB][FR][FR] = {};
+    int64_t ra[FR], rb[FR];                      // rows behind the last repeat it: their outputs are not stored
 #pragma unroll
-    for (int i = 0; i < 2; ++i) ra[i] = min(row0 + i * 16 + (lane & 15), g.m - 1), rb[i] = min(col0 + i * 16 + (lane & 15), g.n - 1);
+    for (int i = 0; i < FR; ++i) ra[i] = min(row0 + i * 16 + (lane & 15), g.m - 1), rb[i] = min(col0 + i * 16 + (lane & 15), g.n - 1);
 #pragma unroll
     for (int part = 0; part < (MODE == GATED_SUM ? 2 : 1); ++part) {
         const Operand oa = MODE == GATED_PAIR && z ? g.a[1] : g.a[part], ob = g.b[part], ob2 = g.b[1];
-        small_sums<T, NB>(acc, kb, ke, [&](int i, int64_t k, auto whole) { return small_fragment<T, AKC, whole.value>(oa, ra[i], k, ke); },
+        small_sums<T, NB, FR>(acc, kb, ke, [&](int i, int64_t k, auto whole) { return small_fragment<T, AKC, whole.value>(oa, ra[i], k, ke); },
                           [&](int b, int i, int64_t k, auto whole) { return small_fragment<T, BKC, whole.value>(b ? ob2 : ob, rb[i], k, ke); });
     }
     f32x4 v[NB];
-    small_join<NB>(acc, v, sums);
-    if (wave >= 4) return;
-    const int64_t row = row0 + (wave >> 1) * 16 + (lane & 15), col = col0 + (wave & 1) * 16 + (lane >> 4) * 4;
+    small_join<NB, FR>(acc, v, sums);
+    if (wave >= FR * FR) return;
+    const int64_t row = row0 + wave / FR * 16 + (lane & 15), col = col0 + wave % FR * 16 + (lane >> 4) * 4;
     if (row >= g.m) return;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -382,7 +385,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small_back(SlopeOper
         for (int i = 0; i < 2; ++i) ra[i] = min(row0 + i * 16 + (lane & 15), m - 1);
 #pragma unroll
         for (int which = 0; which < 2; ++which)
-            small_sums<T, 1>(acc, 0, h, [&](int i, int64_t q, auto whole) { return slope_fragment<T, true, whole.value>(s, which, ra[i], q, h); },
+            small_sums<T, 1, 2>(acc, 0, h, [&](int i, int64_t q, auto whole) { return slope_fragment<T, true, whole.value>(s, which, ra[i], q, h); },
                              [&](int, int i, int64_t q, auto whole) { return small_fragment<T, false, whole.value>(which ? wu : wg, rb[i], q, h); });
     } else {                                   // dw = d^T x, contraction over the rows
         id -= tiles_x;
@@ -392,10 +395,10 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small_back(SlopeOper
         int64_t ra[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) ra[i] = min(row0 + i * 16 + (lane & 15), h - 1);
-        small_sums<T, 1>(acc, 0, m, [&](int i, int64_t q, auto whole) { return slope_fragment<T, false, whole.value>(s, which, ra[i], q, m); },
+        small_sums<T, 1, 2>(acc, 0, m, [&](int i, int64_t q, auto whole) { return slope_fragment<T, false, whole.value>(s, which, ra[i], q, m); },
                          [&](int, int i, int64_t q, auto whole) { return small_fragment<T, false, whole.value>(x, rb[i], q, m); });
     }
-    small_join<1>(acc, v, sums);
+    small_join<1, 2>(acc, v, sums);
     if (wave >= 4) return;
     const int64_t row = row0 + (wave >> 1) * 16 + (lane & 15), col = col0 + (wave & 1) * 16 + (lane >> 4) * 4;
     if (row >= rows) return;
@@ -463,22 +466,25 @@ __global__ __launch_bounds__(256) void k_gated_slopes(const T* __restrict__ dh, 
 // tiles above; either with the contraction in pieces where the outputs alone leave CUs empty, of at least 4 steps.
 struct AnyPlan {
     bool small = true;
-    int splits = 1;
+    int fragments = 2, splits = 1;      // of the small form, in each direction
 };
 template <typename T>
 AnyPlan any_plan(int64_t m, int64_t n, int64_t k, int zs, bool can_split) {
     AnyPlan p;
     const int64_t t32 = zs * ceil_div(m, SB) * ceil_div(n, SB), t64 = zs * ceil_div(m, TB) * ceil_div(n, TB);
     p.small = t32 <= 1024;
+    if (t32 < 128 && !can_split) p.fragments = 1;      // (a product that can be split fills the card that way)
     const int64_t tiles = p.small ? t32 : t64, step = p.small ? SMALL_WAVES * 64 / (int64_t)sizeof(T) : STEP_BYTES / (int64_t)sizeof(T);
     if (can_split && tiles > 0 && tiles < 256) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(512, tiles), k / (4 * step)));
     return p;
 }
 template <typename T, int MODE, bool AKC, bool BKC>
 void launch_any(hipStream_t st, const GatedArgs& g, const AnyPlan& p) {
-    const int64_t b = p.small ? SB : TB;
+    const int64_t b = p.small ? 16 * p.fragments : TB;
     const dim3 grid((unsigned)(ceil_div(g.m, b) * ceil_div(g.n, b)), (unsigned)g.splits, MODE == GATED_PAIR ? 2 : 1);
-    if (p.small) hipLaunchKernelGGL((k_gated_small<T, MODE, AKC, BKC>), grid, dim3(64 * SMALL_WAVES), 0, st, g);
+    if (p.small && MODE == GATED_FWD && p.fragments == 1)
+        hipLaunchKernelGGL((k_gated_small<T, GATED_FWD, true, true, 1>), grid, dim3(64 * SMALL_WAVES), 0, st, g);
+    else if (p.small) hipLaunchKernelGGL((k_gated_small<T, MODE, AKC, BKC, 2>), grid, dim3(64 * SMALL_WAVES), 0, st, g);
     else hipLaunchKernelGGL((k_gated_tile<T, MODE, AKC, BKC>), grid, dim3(256), 0, st, g);
 }
 
