@@ -90,6 +90,8 @@ struct NormArgs {
     float eps;
     float *mean, *rstd;
     float* part;                               // [groups][2][cols] column sums of dy xh and dy
+    int row_blocks;                            // backward: > 0 if further workgroups take the column sums (few rows)
+    void *dw, *db;                             // then
 };
 
 // Rows of more than TPR * (NCH - 1) and up to TPR * NCH packs: only a thread's last pack can be broken or missing, so only there
@@ -212,9 +214,40 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_long(NormArgs a) {
     }
 }
 
+// dw and db of 64 columns over all rows, with mean and rstd from the forward pass: what a few rows' column sums need is in the
+// caches, and reading it twice is sooner done than a second launch for the sums of sums.
+template <typename T, int BLOCK>
+__device__ __forceinline__ void norm_columns(const NormArgs& a, int64_t which) {
+    __shared__ float sums[2][BLOCK / 64][64];
+    const int cl = threadIdx.x & 63, group = threadIdx.x >> 6;
+    const int64_t c = which * 64 + cl;
+    float w = 0.0f, b = 0.0f;
+    if (c < a.cols) {
+#pragma unroll 8
+        for (int64_t r = group; r < a.rows; r += BLOCK / 64) {
+            const float d = to_float(((const T*)a.dy)[r * a.dys + c]);
+            w = fmaf(d, (to_float(((const T*)a.x)[r * a.xs + c]) - a.mean[r]) * a.rstd[r], w);
+            b += d;
+        }
+    }
+    sums[0][group][cl] = w, sums[1][group][cl] = b;
+    __syncthreads();
+    if (group > 0 || c >= a.cols) return;
+    w = b = 0.0f;
+#pragma unroll
+    for (int i = 0; i < BLOCK / 64; ++i) w += sums[0][i][cl], b += sums[1][i][cl];
+    if (a.dw) ((T*)a.dw)[c] = from_float<T>(w);
+    if (a.db) ((T*)a.db)[c] = from_float<T>(b);
+}
+
 template <typename T, int TPR, int NCH>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_bwd(NormArgs a) {
     constexpr int V = Pack<T>::N, BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR;
+    const int blocks = a.row_blocks ? a.row_blocks : gridDim.x;
+    if ((int)blockIdx.x >= blocks) {
+        norm_columns<T, BLOCK>(a, blockIdx.x - blocks);
+        return;
+    }
     __shared__ float lds[4][16];
     const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
     const T* w = (const T*)a.w;
@@ -231,7 +264,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_bwd(NormArgs a) 
     }
     const float n = (float)cols;
     int par = 0;
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)blocks * RPB) {
         const int64_t r = r0 + group;
         const bool on = r < a.rows;
         const int64_t rr = on ? r : 0;
@@ -425,6 +458,7 @@ __global__ __launch_bounds__(1024) void k_norm_cols(const float* __restrict__ pa
 struct NormPlan {
     int tpr, nch;
     int64_t grid, groups;
+    bool few;
 };
 
 // Threads a row, by the packs it has: as few as leave a thread at most 5 packs (forward) or 3 (backward, which holds two column
@@ -445,14 +479,16 @@ inline NormPlan norm_plan(int64_t rows, int64_t cols, int vec, bool backward) {
     // forward: as many workgroups as the card holds; backward: fewer, since each leaves column sums behind
     const int64_t most = backward ? (p.tpr == 1024 ? 256 : 1024) : (p.tpr == 1024 ? 512 : 2048);
     p.grid = std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, rpb), most));
-    p.groups = backward && p.nch == 0 ? std::max<int64_t>(1, std::min<int64_t>(rows, 64)) : p.grid;
+    // few rows: the columns' workgroups read all of them again, 64 columns each (up to 512 rows of at most 1 MB together)
+    p.few = backward && p.nch > 0 && rows <= 512 && rows * cols * 16 / vec <= (int64_t)1 << 20;
+    p.groups = p.few ? 0 : backward && p.nch == 0 ? std::max<int64_t>(1, std::min<int64_t>(rows, 64)) : p.grid;
     return p;
 }
 
 // The kernels that norm_plan names.
 template <typename T>
 void launch_norm(hipStream_t st, const NormArgs& a, const NormPlan& p, bool backward) {
-    const dim3 grid((unsigned)p.grid), block(p.tpr > 256 ? p.tpr : 256);
+    const dim3 grid((unsigned)(p.grid + (a.row_blocks ? ceil_div(a.cols, 64) : 0))), block(p.tpr > 256 ? p.tpr : 256);
     auto fwd = [&](auto k) { hipLaunchKernelGGL(k, grid, block, 0, st, a); };
     switch (p.tpr * 8 + p.nch) {
         case 8 * 8 + 1: return backward ? fwd(k_norm_bwd<T, 8, 1>) : fwd(k_norm_fwd<T, 8, 1>);
@@ -481,9 +517,15 @@ hipError_t norm_forward(hipStream_t st, const NormArgs& a) {
 }
 
 template <typename T>
-hipError_t norm_backward(hipStream_t st, const NormArgs& a, void* dw, void* db) {
+hipError_t norm_backward(hipStream_t st, NormArgs a, void* dw, void* db) {
     const NormPlan p = norm_plan(a.rows, a.cols, Pack<T>::N, true);
     if (a.rows > 0) {
+        if (p.few) {
+            a.part = nullptr;
+            if (dw || db) a.row_blocks = (int)p.grid, a.dw = dw, a.db = db;
+            launch_norm<T>(st, a, p, true);
+            return hipGetLastError();
+        }
         launch_norm<T>(st, a, p, true);
         if (p.nch == 0 && a.part)
             hipLaunchKernelGGL(k_norm_bwd_long_cols<T>, dim3((unsigned)ceil_div(ceil_div(a.cols, Pack<T>::N), 256), (unsigned)p.groups), dim3(256), 0,

@@ -55,8 +55,8 @@ def sample(scores, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if not u.is_contiguous():
         u = u.contiguous()
     draws, code = u.shape[1], _TYPES[scores.dtype]
-    index = torch.empty((rows, draws), dtype=torch.int64, device=device)
-    logp = torch.empty((rows, draws), dtype=_f64, device=device)
+    index = u.new_empty((rows, draws), dtype=torch.int64)
+    logp = u.new_empty((rows, draws))
     nbytes = workspace('gpbo_draw_static_workspace', code, rows, cols, draws)
     work = scratch(nbytes, device)
     st = L.load().gpbo_draw_static(at, stream_of(at), code, scores.data_ptr(), stride, rows, cols, u.data_ptr(), draws, temperature,

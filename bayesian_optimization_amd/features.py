@@ -13,7 +13,7 @@ from . import _lib as L
 from ._device import TYPES, check_status, pointer, rows_of, scratch, stream_of, tensor, vector_of, workspace
 
 ACTIVATIONS = {'silu': L.ACT_SILU, 'gelu': L.ACT_GELU}
-_empty, _f32 = torch.empty, torch.float32
+_like, _f32 = torch.empty_like, torch.float32
 
 
 def _act(act):
@@ -27,15 +27,15 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the rows of x (rows, cols) float32 / bfloat16 / float16; weight and bias
     (cols,) of x's type or None.  Returns y, mean (rows,) and rstd (rows,), the last two float32, for layer_norm_backward."""
     rows, cols, stride, at = rows_of('x', x)
-    dtype, device = x.dtype, x.device
+    dtype = x.dtype
     if weight is not None:
         weight = vector_of('weight', weight, cols, dtype, at)
     if bias is not None:
         bias = vector_of('bias', bias, cols, dtype, at)
     if not 0.0 <= eps < float('inf'):
         raise ValueError('eps must be finite and >= 0; got %r' % (eps,))
-    y = _empty((rows, cols), dtype=dtype, device=device)
-    mean, rstd = _empty(rows, dtype=_f32, device=device), _empty(rows, dtype=_f32, device=device)
+    y = _like(x) if stride == cols else x.new_empty((rows, cols))
+    mean, rstd = x.new_empty(rows, dtype=_f32), x.new_empty(rows, dtype=_f32)
     st = L.load().gpbo_layernorm(at, stream_of(at), TYPES[dtype], x.data_ptr(), stride, rows, cols, pointer(weight), pointer(bias), eps,
                                  y.data_ptr(), cols, mean.data_ptr(), rstd.data_ptr())
     if st:
@@ -47,16 +47,16 @@ def layer_norm_backward(dy, x, weight, mean, rstd):
     """Gradients (dx, dweight, dbias) of layer_norm from dy, with the mean and rstd it returned.  dweight and dbias have x's
     type; they are the column sums whether or not the forward pass had a weight and a bias."""
     rows, cols, stride, at = rows_of('x', x)
-    dtype, device = x.dtype, x.device
+    dtype = x.dtype
     dstride = rows_of('dy', dy, dtype=dtype, shape=(rows, cols), device=at)[2]
     if weight is not None:
         weight = vector_of('weight', weight, cols, dtype, at)
     mean, rstd = vector_of('mean', mean, rows, _f32, at), vector_of('rstd', rstd, rows, _f32, at)
     code = TYPES[dtype]
-    dx = _empty((rows, cols), dtype=dtype, device=device)
-    dw, db = _empty(cols, dtype=dtype, device=device), _empty(cols, dtype=dtype, device=device)
+    dx = _like(x) if stride == cols else x.new_empty((rows, cols))
+    dw, db = x.new_empty(cols), x.new_empty(cols)
     nbytes = workspace('gpbo_layernorm_backward_workspace', code, rows, cols)
-    work = scratch(nbytes, device)
+    work = scratch(nbytes, x.device)
     st = L.load().gpbo_layernorm_backward(at, stream_of(at), code, dy.data_ptr(), dstride, x.data_ptr(), stride, rows, cols, pointer(weight),
                                           mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), cols, dw.data_ptr(), db.data_ptr(), pointer(work), nbytes)
     if st:
@@ -81,16 +81,16 @@ def gated_unit(x, w_gate, w_up, act='silu', keep=False):
     gated_unit_backward needs."""
     a = _act(act)
     rows, cols, stride, at, hidden, w_gate, w_up, ws = _weights(x, w_gate, w_up)
-    dtype, device = x.dtype, x.device
+    dtype = x.dtype
     code = TYPES[dtype]
-    h = _empty((rows, hidden), dtype=dtype, device=device)
+    h = x.new_empty((rows, hidden))
     kept = kg = ku = None
     if keep:
-        kept = _empty((2, rows, hidden), dtype=_f32, device=device)
+        kept = x.new_empty((2, rows, hidden), dtype=_f32)
         kg = kept.data_ptr()
         ku = kg + 4 * rows * hidden
     nbytes = workspace('gpbo_gated_workspace', code, rows, cols, hidden)
-    work = scratch(nbytes, device)
+    work = scratch(nbytes, x.device)
     st = L.load().gpbo_gated(at, stream_of(at), code, a, x.data_ptr(), stride, rows, cols, w_gate.data_ptr(), w_up.data_ptr(), ws, hidden,
                              h.data_ptr(), hidden, kg, ku, pointer(work), nbytes)
     if st:
@@ -102,7 +102,7 @@ def gated_unit_backward(dh, x, w_gate, w_up, kept, act='silu', need_dx=True, nee
     """Gradients (dx, dw_gate, dw_up) of gated_unit from dh (rows, hidden), with what it kept; None for those not needed."""
     a = _act(act)
     rows, cols, stride, at, hidden, w_gate, w_up, ws = _weights(x, w_gate, w_up)
-    dtype, device = x.dtype, x.device
+    dtype = x.dtype
     code = TYPES[dtype]
     dstride = rows_of('dh', dh, dtype=dtype, shape=(rows, hidden), device=at)[2]
     tensor('kept', kept, at)
@@ -111,11 +111,11 @@ def gated_unit_backward(dh, x, w_gate, w_up, kept, act='silu', need_dx=True, nee
     if not kept.is_contiguous():
         kept = kept.contiguous()
     kg = kept.data_ptr()
-    dx = _empty((rows, cols), dtype=dtype, device=device) if need_dx else None
-    dwg = _empty((hidden, cols), dtype=dtype, device=device) if need_dw else None
-    dwu = _empty((hidden, cols), dtype=dtype, device=device) if need_dw else None
+    dx = (_like(x) if stride == cols else x.new_empty((rows, cols))) if need_dx else None
+    dwg = x.new_empty((hidden, cols)) if need_dw else None
+    dwu = x.new_empty((hidden, cols)) if need_dw else None
     nbytes = workspace('gpbo_gated_backward_workspace', code, rows, cols, hidden)
-    work = scratch(nbytes, device)
+    work = scratch(nbytes, x.device)
     st = L.load().gpbo_gated_backward(at, stream_of(at), code, a, dh.data_ptr(), dstride, x.data_ptr(), stride, rows, cols, w_gate.data_ptr(),
                                       w_up.data_ptr(), ws, hidden, kg, kg + 4 * rows * hidden, pointer(dx), cols, pointer(dwg), pointer(dwu),
                                       cols, pointer(work), nbytes)

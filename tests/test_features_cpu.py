@@ -59,17 +59,19 @@ BIG = MOST + 1
                         dict(ys=7), dict(eps=-1.0), dict(eps=float('nan')), dict(eps=float('inf')), dict(device=-1), dict(device=64), dict(x=None), dict(y=None))
 ] + [
     (norm_back, k) for k in (dict(dtype=L.TYPE_F64), dict(rows=-1), dict(cols=0), dict(dys=7), dict(xs=7), dict(dxs=7), dict(dy=None), dict(x=None), dict(mean=None),
-                             dict(rstd=None), dict(dx=None), dict(work=None), dict(nbytes=8), dict(work=C.c_void_p(4097)), dict(device=64))
+                             dict(rstd=None), dict(dx=None), dict(rows=4096, work=None), dict(rows=4096, nbytes=8), dict(rows=4096, nbytes=1 << 30, work=C.c_void_p(4097)), dict(device=64))
 ] + [
     (gated, k) for k in (dict(dtype=L.TYPE_F64), dict(act=2), dict(rows=-1), dict(cols=0), dict(hidden=0), dict(xs=7), dict(ws=7), dict(hs=15), dict(x=None), dict(wg=None),
                          dict(wu=None), dict(h=None), dict(kg=None), dict(ku=None), dict(rows=MOST, hidden=MOST, hs=MOST), dict(device=-1))
 ] + [
+    (gated, dict(rows=8192, cols=100, xs=100, ws=100, hidden=4096, hs=4096, **k)) for k in (dict(work=None), dict(nbytes=8), dict(work=C.c_void_p(4097)))
+] + [
     (gated_back, k) for k in (dict(dtype=L.TYPE_F64), dict(act=-1), dict(dhs=15), dict(xs=7), dict(ws=7), dict(dxs=7), dict(dws=7), dict(dh=None), dict(x=None), dict(wg=None),
-                              dict(kg=None), dict(ku=None), dict(dwg=None), dict(dwu=None), dict(work=None), dict(nbytes=8), dict(work=C.c_void_p(4097)), dict(device=64))
+                              dict(kg=None), dict(ku=None), dict(dwg=None), dict(dwu=None), dict(rows=65536, work=None), dict(rows=65536, nbytes=8), dict(rows=65536, work=C.c_void_p(4097)), dict(device=64))
 ] + [
     (draw, k) for k in (dict(dtype=4), dict(dtype=-1), dict(rows=-1), dict(cols=0), dict(cols=(1 << 28) + 1, stride=(1 << 28) + 1), dict(draws=-1), dict(stride=9),
                         dict(temperature=-1.0), dict(temperature=float('nan')), dict(temperature=float('inf')), dict(top_k=-1), dict(top_p=1.1), dict(top_p=-0.1),
-                        dict(min_p=1.1), dict(min_p=float('nan')), dict(s=None), dict(u=None), dict(index=None), dict(device=-1), dict(device=64))
+                        dict(min_p=1.1), dict(min_p=float('nan')), dict(cols=1 << 20, stride=1 << 20, work=None), dict(cols=1 << 20, stride=1 << 20, nbytes=8), dict(s=None), dict(u=None), dict(index=None), dict(device=-1), dict(device=64))
 ])
 def test_bad_arguments_are_refused(lib, call, kw):
     assert call(lib, **kw) == L.ERR_BAD_ARG
