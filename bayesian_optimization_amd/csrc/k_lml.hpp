@@ -350,11 +350,15 @@ __device__ __forceinline__ void lml_small_finish(const SmallLds& m, int n, int d
         }
         __syncthreads();
         for (int e = tid; e < n * d; e += TG * TG) {
-            const int i = e / d, t = e - i * d;
+            const int t = e / n, i = e - t * n;          // neighbouring lanes: neighbouring points of one column, no bank twice
             const double xi = m.xs[t * PB + i];
-            double s = 0.0;
-            for (int k = 0; k < n; ++k) s = fma(Wl[k * SMALL_WP + i], xi - m.xs[t * PB + k], s);
-            out_gx[e] = bad ? NAN : s * (1.0 / th[t]);
+            double s[4] = {0.0, 0.0, 0.0, 0.0};
+            int k = 0;
+            for (; k + 4 <= n; k += 4)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) s[q] = fma(Wl[(k + q) * SMALL_WP + i], xi - m.xs[t * PB + k + q], s[q]);
+            for (; k < n; ++k) s[0] = fma(Wl[k * SMALL_WP + i], xi - m.xs[t * PB + k], s[0]);
+            out_gx[(long)i * d + t] = bad ? NAN : ((s[0] + s[1]) + (s[2] + s[3])) * (1.0 / th[t]);
         }
     }
 }
