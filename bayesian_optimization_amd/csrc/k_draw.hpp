@@ -503,7 +503,7 @@ __device__ __forceinline__ void block_sort(Key& k, uint32_t& i, int size, Key* b
 
 // LIST keys or fewer in l.key, l.idx: sort them by rank into l.key2, l.idx2 (behind them keys of 0).
 template <typename T>
-__device__ int draw_rank(DrawLds<T>& s, int n) {
+__device__ void draw_rank(DrawLds<T>& s, int n) {
     using Key = typename Score<T>::Key;
     const int tid = threadIdx.x;
     int size = 64;
@@ -515,7 +515,6 @@ __device__ int draw_rank(DrawLds<T>& s, int n) {
     __syncthreads();
     if (tid < size) s.l.key2[tid] = k, s.l.idx2[tid] = ix;
     __syncthreads();
-    return size;
 }
 
 // The list holds the keys klo .. khi of a step: the cut is one of them.
@@ -554,7 +553,7 @@ template <typename T>
 __device__ void draw_from_list(DrawLds<T>& s, const DrawArgs& a, const DrawRow& p, int64_t row, int n, typename Score<T>::Key top, double goal) {
     using Key = typename Score<T>::Key;
     const int tid = threadIdx.x;
-    const int size = draw_rank(s, n);
+    draw_rank(s, n);
     // by rank from here on: thread = position
     const Key kr = tid < n ? s.l.key2[tid] : 0;
     const double w = kr ? exp(draw_t<T>(kr, top, p.temperature)) : 0.0;
@@ -570,7 +569,9 @@ __device__ void draw_from_list(DrawLds<T>& s, const DrawArgs& a, const DrawRow& 
     block_scan<unsigned long long>(keep ? 1ull : 0ull, s.red_u, kept);
     Key ki = keep ? kr : 0;
     uint32_t ii = keep ? s.l.idx2[tid] : 0xffffffffu;
-    block_sort<Key, true>(ki, ii, size, s.l.key, s.l.idx);
+    int few = 64;                              // they stand in front: no more than they need to be sorted
+    while (few < (int)kept) few <<= 1;
+    block_sort<Key, true>(ki, ii, few, s.l.key, s.l.idx);
     const double wi = tid < (int)kept ? exp(draw_t<T>(ki, top, p.temperature)) : 0.0;
     const double ci = block_scan(wi, s.red, total);      // its barriers stand between the sort's last reads of l.key and this
     if (tid < (int)kept) s.l.key[tid] = ki, s.l.pick[tid] = ii;
@@ -596,13 +597,22 @@ __device__ void draw_from_list(DrawLds<T>& s, const DrawArgs& a, const DrawRow& 
 template <typename T>
 __device__ void draw_gather(DrawLds<T>& s, const DrawStep<T>& d, const T* x, uint32_t begin, uint32_t end) {
     using Key = typename Score<T>::Key;
-    each_score(x, begin, end, [&](Key k, uint32_t i) {
-        double w;
-        if (!d.counts(k, w)) return;
+    auto take = [&](Key k, uint32_t i) {
         if (__hip_atomic_load(&s.st.n_list, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) > LIST) return;
         const uint32_t at = atomicAdd(&s.st.n_list, 1u);
         if (at < LIST) s.l.key[at] = k, s.l.idx[at] = i;
-    });
+    };
+    if (d.gather == 3) {                       // all from klo up: nothing to work out, more loads at a time
+        const Key bound = d.klo ? d.klo : 1;
+        each_score<T, 32>(x, begin, end, [&](Key k, uint32_t i) {
+            if (k >= bound) take(k, i);
+        });
+    } else {
+        each_score(x, begin, end, [&](Key k, uint32_t i) {
+            double w;
+            if (d.counts(k, w)) take(k, i);
+        });
+    }
     __syncthreads();
 }
 
@@ -849,10 +859,21 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_row(DrawArgs a) {
         draw_same<T>(a, row, top ? (int64_t)idx : -1, top ? 0.0 : -INFINITY);
         return;
     }
+    // A lower bound of the top_k-th score: the top_k-th of the maxima of groups of threads, sorted.  A quarter more groups than
+    // top_k keep the list behind the bound short (some n log n of them, at most); few of them sort soonest (64 in one wave: 1.5 us;
+    // 1024: 10 us).
     Key bound = 0;
-    if (p.top_k > 0 && p.top_k <= DRAW_THREADS) {      // the threads' own maxima, sorted: top_k of them reach the top_k-th
+    if (p.top_k > 0 && p.top_k <= DRAW_THREADS) {
+        const int groups = p.top_k * 5 <= 64 * 4 ? 64 : p.top_k * 5 <= 256 * 4 ? 256 : DRAW_THREADS, each = DRAW_THREADS / groups;
+        for (int o = each / 2; o > 0; o >>= 1) {
+            const Key k = __shfl_xor(own, o);
+            if (k > own) own = k;
+        }
+        if (tid % each == 0) s.l.key[tid / each] = own;
+        __syncthreads();
+        own = tid < groups ? s.l.key[tid] : 0;
         uint32_t none = tid;
-        block_sort<Key, false>(own, none, DRAW_THREADS, s.l.key2, s.l.idx2);
+        block_sort<Key, false>(own, none, groups, s.l.key2, s.l.idx2);
         if (tid == (int)p.top_k - 1) s.red_k[0][0] = own;
         __syncthreads();
         bound = s.red_k[0][0];
