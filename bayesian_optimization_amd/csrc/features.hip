@@ -2,7 +2,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "k_gated_fast.hpp"
+#include "k_gated_plan.hpp"
 #include "k_norm.hpp"
 
 using namespace gpbo_static;

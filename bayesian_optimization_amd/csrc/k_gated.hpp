@@ -414,6 +414,7 @@ __global__ __launch_bounds__(256) void k_gated_join(GatedArgs g) {
     if (e >= g.m * g.n) return;
     const float* p = g.part + z * g.splits * g.m * g.n + e;
     float v = 0.0f;
+#pragma unroll 8
     for (int s = 0; s < g.splits; ++s) v += p[(int64_t)s * g.m * g.n];
     ((T*)g.out[z])[e / g.n * g.os + e % g.n] = from_float<T>(v);
 }

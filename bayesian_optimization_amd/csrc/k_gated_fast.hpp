@@ -451,194 +451,4 @@ __global__ __launch_bounds__(256) void k_gated_few(GatedArgs g) {
     }
 }
 
-// ---------------------------------------------------------------------------------------------------------------------
-// Which kernels a call takes, and its workspace.
-
-inline bool aligned16(const void* p, int64_t stride, int64_t bytes) {
-    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * bytes % 16 == 0 && stride * bytes < (1 << 23);
-}
-
-struct ForwardPlan {
-    bool fast = false, pack = false, stream = false;
-    int tile = 128;
-    int64_t kp = 0, x_bytes = 0, w_bytes = 0;
-    int64_t bytes() const { return pack ? x_bytes + 2 * w_bytes : 0; }
-};
-// The loads straight into LDS need whole steps and 16-byte rows.  A contraction that is no whole number of steps is packed into the
-// workspace first, which pays from some 2 GFLOP on; below, and for few tiles, the any-shape kernel starts sooner.
-template <typename T>
-ForwardPlan forward_plan(int64_t m, int64_t k, int64_t h) {
-    constexpr int KS = STEP_BYTES / sizeof(T);
-    ForwardPlan p;
-    p.kp = round_up(k, KS);
-    p.fast = m * h >= 128 * 64 * 64 && 4 * m * h * k >= (int64_t)1 << 31 && k * (int64_t)sizeof(T) < (1 << 23);
-    // at least two tiles of rows for every workgroup of the streaming form
-    p.stream = sizeof(T) == 2 && p.kp <= STREAM_MOST && m * h >= (int64_t)1 << 21 && ceil_div(m, STREAM_ROWS) * ceil_div(h, 256) >= 512;
-    p.fast = p.fast || p.stream;
-    p.pack = p.fast && k % KS != 0;
-    if (ceil_div(m, 256) * ceil_div(h, 128) >= 256 && k >= 8 * KS) p.tile = 256;
-    p.x_bytes = round_up(m * p.kp * (int64_t)sizeof(T), 256);
-    p.w_bytes = round_up(h * p.kp * (int64_t)sizeof(T), 256);
-    return p;
-}
-
-template <typename T, int MODE>
-void launch_fast(hipStream_t st, const GatedArgs& g, int tile) {
-    const int zs = MODE == GATED_PAIR ? 2 : 1;
-    if (tile == 256)
-        hipLaunchKernelGGL((k_gated_fast<T, MODE, 256, 256, 2, 4>),
-                           dim3((unsigned)(ceil_div(g.m, 256) * ceil_div(g.n, MODE == GATED_FWD ? 128 : 256)), (unsigned)g.splits, zs), dim3(512), 0, st, g);
-    else
-        hipLaunchKernelGGL((k_gated_fast<T, MODE, 128, 128, 2, 2>),
-                           dim3((unsigned)(ceil_div(g.m, 128) * ceil_div(g.n, MODE == GATED_FWD ? 64 : 128)), (unsigned)g.splits, zs), dim3(256), 0, st, g);
-}
-
-template <typename T>
-void launch_stream(hipStream_t st, const GatedArgs& g) {
-    if constexpr (sizeof(T) == 2) {
-        int wn = 1;
-        while (wn < 8 && wn * 32 < g.n) wn *= 2;
-        const int groups = (int)ceil_div(g.n, wn * 32);
-        int64_t walkers = std::max<int64_t>(1, std::min<int64_t>(256 / std::min(groups, 256), ceil_div(g.m, STREAM_ROWS)));
-        if (walkers > 8) walkers -= walkers % 8;
-        const dim3 grid((unsigned)(groups * walkers));
-        if (g.k <= 64) hipLaunchKernelGGL((k_gated_stream<T, 2>), grid, dim3(512), 0, st, g, wn, groups);
-        else if (g.k <= 128) hipLaunchKernelGGL((k_gated_stream<T, 4>), grid, dim3(512), 0, st, g, wn, groups);
-        else if (g.k <= 192) hipLaunchKernelGGL((k_gated_stream<T, 6>), grid, dim3(512), 0, st, g, wn, groups);
-        else hipLaunchKernelGGL((k_gated_stream<T, 8>), grid, dim3(512), 0, st, g, wn, groups);
-    }
-}
-
-template <typename T>
-hipError_t gated_forward(hipStream_t st, GatedArgs g, char* work) {
-    constexpr int KS = STEP_BYTES / sizeof(T);
-    const ForwardPlan p = forward_plan<T>(g.m, g.k, g.n);
-    const bool direct = aligned16(g.a[0].p, g.a[0].sr, sizeof(T)) && aligned16(g.b[0].p, g.b[0].sr, sizeof(T)) && aligned16(g.b[1].p, g.b[1].sr, sizeof(T));
-    if (p.fast && (p.pack || direct)) {
-        if (p.pack) {
-            PackArgs a{};
-            a.count = 3;
-            a.job[0] = {g.a[0].p, g.a[0].sr, g.m, g.k, work, p.kp, ceil_div(g.m, 64) * ceil_div(p.kp, 64)};
-            a.job[1] = {g.b[0].p, g.b[0].sr, g.n, g.k, work + p.x_bytes, p.kp, ceil_div(g.n, 64) * ceil_div(p.kp, 64)};
-            a.job[2] = {g.b[1].p, g.b[1].sr, g.n, g.k, work + p.x_bytes + p.w_bytes, p.kp, ceil_div(g.n, 64) * ceil_div(p.kp, 64)};
-            hipLaunchKernelGGL((k_gated_pack<T, false>), dim3((unsigned)(a.job[0].blocks + a.job[1].blocks + a.job[2].blocks)), dim3(256), 0, st, a);
-            g.a[0] = {a.job[0].dst, p.kp, 1}, g.b[0] = {a.job[1].dst, p.kp, 1}, g.b[1] = {a.job[2].dst, p.kp, 1};
-            g.k = p.kp;
-        }
-        static_assert(KS >= 32, "a step");
-        if (p.stream) launch_stream<T>(st, g);
-        else launch_fast<T, GATED_FWD>(st, g, p.tile);
-    } else if (g.m <= 16) {
-        const unsigned hidden = (unsigned)ceil_div(g.n, 4);
-        if (g.m == 1) hipLaunchKernelGGL((k_gated_few<T, 1>), dim3(hidden, 1), dim3(256), 0, st, g);
-        else if (g.m == 2) hipLaunchKernelGGL((k_gated_few<T, 2>), dim3(hidden, 1), dim3(256), 0, st, g);
-        else if (g.m <= 4) hipLaunchKernelGGL((k_gated_few<T, 4>), dim3(hidden, 1), dim3(256), 0, st, g);
-        else hipLaunchKernelGGL((k_gated_few<T, 8>), dim3(hidden, (unsigned)ceil_div(g.m, 8)), dim3(256), 0, st, g);
-    } else {
-        launch_any<T, GATED_FWD, true, true>(st, g, any_plan<T>(g.m, g.n, g.k, 1, false));
-    }
-    return hipGetLastError();
-}
-
-// Backward.  Large: dg and du are written both ways round, x and the weights transposed, so that every product contracts along
-// rows; these copies are a few per cent of the products' time.
-struct BackwardPlan {
-    bool fast = false, one = false;      // one: k_gated_small_back
-    int tile_x = 128, tile_w = 128, splits_x = 1, splits_w = 1;
-    AnyPlan any_x, any_w;
-    int64_t hp = 0, mp = 0;
-    int64_t d_bytes = 0, dt_bytes = 0, xt_bytes = 0, wt_bytes = 0, part_bytes = 0;
-    int64_t bytes() const { return 2 * d_bytes + 2 * dt_bytes + xt_bytes + 2 * wt_bytes + part_bytes; }
-};
-template <typename T>
-BackwardPlan backward_plan(int64_t m, int64_t k, int64_t h) {
-    constexpr int KS = STEP_BYTES / sizeof(T);
-    constexpr int64_t B = sizeof(T);
-    BackwardPlan p;
-    // 4 GFLOP, or two million elements over many rows: below, the copies cost more than they save
-    p.fast = m >= 128 && (8 * m * h * k >= (int64_t)1 << 32 || (m >= 4096 && std::max(h, k) >= 128 && m * std::max(h, k) >= (int64_t)1 << 21)) && m * B < (1 << 23) && h * B < (1 << 23);
-    if (p.fast) {
-        p.hp = round_up(h, 64), p.mp = round_up(m, 64);
-        auto choose = [&](int64_t rows, int64_t cols, int64_t zs, int64_t steps, int& tile, int& splits) {
-            const int64_t t256 = zs * ceil_div(rows, 256) * ceil_div(cols, 256), t128 = zs * ceil_div(rows, 128) * ceil_div(cols, 128);
-            tile = t256 >= 256 ? 256 : 128;
-            splits = tile == 256 || t128 >= 256 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(512, t128), steps / 8));
-        };
-        choose(m, k, 1, p.hp / KS, p.tile_x, p.splits_x);
-        choose(h, k, 2, p.mp / KS, p.tile_w, p.splits_w);
-        p.d_bytes = round_up(m * p.hp * B, 256), p.dt_bytes = round_up(h * p.mp * B, 256);
-        p.xt_bytes = round_up(k * p.mp * B, 256), p.wt_bytes = round_up(k * p.hp * B, 256);
-    } else {
-        // one launch while all tiles together work out dg and du no more than a million times, and a tile's waves have few slabs
-        p.one = m > 0 && 4 * m * h * ceil_div(k, SB) <= (int64_t)1 << 20 && std::max(m, 2 * h) <= 64 * KS;
-        if (p.one) return p;
-        p.d_bytes = round_up(m * h * B, 256);
-        p.any_x = any_plan<T>(m, k, h, 1, true), p.any_w = any_plan<T>(h, k, m, 2, true);
-        p.splits_x = p.any_x.splits, p.splits_w = p.any_w.splits;
-    }
-    p.part_bytes = std::max<int64_t>(p.splits_x > 1 ? p.splits_x * m * k * 4 : 0, p.splits_w > 1 ? 2 * p.splits_w * h * k * 4 : 0);
-    return p;
-}
-
-template <typename T>
-hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const void* x, int64_t xs, const void* wg, const void* wu, int64_t ws,
-                          const float* kg, const float* ku, int64_t m, int64_t k, int64_t h, int act, void* dx, int64_t dxs, void* dwg,
-                          void* dwu, int64_t dws, char* work) {
-    const BackwardPlan p = backward_plan<T>(m, k, h);
-    if (p.one) {
-        const int64_t nt = ceil_div(k, SB), tiles = (dx ? ceil_div(m, SB) * nt : 0) + (dwg ? 2 * ceil_div(h, SB) * nt : 0);
-        if (tiles > 0)
-            hipLaunchKernelGGL(k_gated_small_back<T>, dim3((unsigned)tiles), dim3(64 * SMALL_WAVES), 0, st, SlopeOperand{dh, kg, ku, dhs, h, act},
-                               Operand{x, 1, xs}, Operand{wg, 1, ws}, Operand{wu, 1, ws}, m, k, h, dx, dxs, dwg, dwu, dws);
-        return hipGetLastError();
-    }
-    char* at = work;
-    auto take = [&](int64_t bytes) { char* r = at; at += bytes; return r; };
-    T *dg = (T*)take(p.d_bytes), *du = (T*)take(p.d_bytes), *dgt = (T*)take(p.dt_bytes), *dut = (T*)take(p.dt_bytes), *xt = (T*)take(p.xt_bytes),
-      *wgt = (T*)take(p.wt_bytes), *wut = (T*)take(p.wt_bytes);
-    float* part = (float*)take(p.part_bytes);
-    if (p.fast) {
-        hipLaunchKernelGGL(k_gated_slopes_both<T>, dim3((unsigned)(p.mp / 64 * (p.hp / 64))), dim3(256), 0, st, (const T*)dh, dhs, kg, ku, m, h, act,
-                           dg, du, p.hp, dgt, dut, p.mp);
-        PackArgs a{};
-        if (dwg) a.job[a.count++] = {x, xs, m, k, xt, p.mp, p.mp / 64 * ceil_div(k, 64)};
-        if (dx) {
-            a.job[a.count++] = {wg, ws, h, k, wgt, p.hp, p.hp / 64 * ceil_div(k, 64)};
-            a.job[a.count++] = {wu, ws, h, k, wut, p.hp, p.hp / 64 * ceil_div(k, 64)};
-        }
-        int64_t blocks = 0;
-        for (int i = 0; i < a.count; ++i) blocks += a.job[i].blocks;
-        if (blocks) hipLaunchKernelGGL((k_gated_pack<T, true>), dim3((unsigned)blocks), dim3(256), 0, st, a);
-    } else if (m > 0) {
-        const int64_t packs = m * ceil_div(h, Pack<T>::N);
-        hipLaunchKernelGGL(k_gated_slopes<T>, dim3((unsigned)std::min<int64_t>(ceil_div(packs, 256), 8192)), dim3(256), 0, st, (const T*)dh, dhs,
-                           kg, ku, m, h, act, dg, du);
-    }
-    if (dx && m > 0) {
-        GatedArgs g{};
-        g.m = m, g.n = k, g.out[0] = dx, g.os = dxs, g.splits = p.splits_x, g.part = part;
-        if (p.fast) {
-            g.a[0] = {dg, p.hp, 1}, g.a[1] = {du, p.hp, 1}, g.b[0] = {wgt, p.hp, 1}, g.b[1] = {wut, p.hp, 1}, g.k = p.hp;
-            launch_fast<T, GATED_SUM>(st, g, p.tile_x);
-        } else {
-            g.a[0] = {dg, h, 1}, g.a[1] = {du, h, 1}, g.b[0] = {wg, 1, ws}, g.b[1] = {wu, 1, ws}, g.k = h;
-            launch_any<T, GATED_SUM, true, false>(st, g, p.any_x);
-        }
-        if (g.splits > 1) hipLaunchKernelGGL(k_gated_join<T>, dim3((unsigned)ceil_div(m * k, 256), 1), dim3(256), 0, st, g);
-    }
-    if (dwg) {
-        GatedArgs g{};
-        g.m = h, g.n = k, g.out[0] = dwg, g.out[1] = dwu, g.os = dws, g.splits = p.splits_w, g.part = part;
-        if (p.fast) {
-            g.a[0] = {dgt, p.mp, 1}, g.a[1] = {dut, p.mp, 1}, g.b[0] = g.b[1] = {xt, p.mp, 1}, g.k = p.mp;
-            launch_fast<T, GATED_PAIR>(st, g, p.tile_w);
-        } else {
-            g.a[0] = {dg, 1, h}, g.a[1] = {du, 1, h}, g.b[0] = g.b[1] = {x, 1, xs}, g.k = m;
-            launch_any<T, GATED_PAIR, false, false>(st, g, p.any_w);
-        }
-        if (g.splits > 1) hipLaunchKernelGGL(k_gated_join<T>, dim3((unsigned)ceil_div(h * k, 256), 2), dim3(256), 0, st, g);
-    }
-    return hipGetLastError();
-}
-
 }  // namespace gpbo_static

@@ -115,7 +115,7 @@ def test_layer_norm_gradient_against_differences():
             e[at] = 1e-5
             hi, lo = ((t.double() + s * e.view_as(t)) for s in (1, -1))
             args = [v.double() for v in (x, w, b)]
-            k = [x, w, b].index(t) if False else next(i for i, v in enumerate((x, w, b)) if v is t)
+            k = next(i for i, v in enumerate((x, w, b)) if v is t)
             up, down = list(args), list(args)
             up[k], down[k] = hi, lo
             assert abs((loss(*up) - loss(*down)) / 2e-5 - float(grad.flatten()[at])) < 1e-4
@@ -185,6 +185,47 @@ def test_gated_unit_forward_and_backward(dtype, act, rows, cols, hidden):
                                               (70001, 40, 90), (66000, 128, 33), (40000, 190, 300), (33000, 256, 515)])
 def test_gated_unit_large(dtype, rows, cols, hidden):
     check_gated(dtype, 'gelu' if rows % 2 else 'silu', rows, cols, hidden)
+
+
+# many rows and few hidden units: every number of fragments, whole and padded, less than 64 columns, pieces of the contraction of
+# which the last is empty (20017 rows over 39 pieces of 33 slabs)
+@pytest.mark.parametrize('rows,cols,hidden', [(16384, 64, 1), (16385, 65, 8), (17003, 483, 4), (20017, 61, 16), (20017, 621, 21), (16391, 100, 24), (30011, 40, 31),
+                                              (16411, 129, 32), (16500, 67, 33), (20021, 621, 48), (33000, 32, 57), (24001, 130, 64), (66000, 17, 3), (16384, 2050, 12)])
+@pytest.mark.parametrize('act', ['silu', 'gelu'])
+def test_gated_unit_many_rows_few_hidden_units(act, rows, cols, hidden):
+    check_gated(torch.float32, act, rows, cols, hidden)
+
+
+def test_gated_unit_many_rows_strides_infinities_and_parts():
+    from bayesian_optimization_amd import features
+    rows, cols, hidden = 16390, 70, 5
+    x = rand((rows, cols + 9), torch.float32, 81)[:, 3:3 + cols]
+    far = torch.zeros((hidden, 1 << 22), device='cuda')      # rows of weights far apart
+    wg, wu = far[:, 1:1 + cols], far[:, 200:200 + cols]
+    wg.copy_(rand((hidden, cols), torch.float32, 82, 0.1))
+    wu.copy_(rand((hidden, cols), torch.float32, 83, 0.1))
+    dh = rand((rows, hidden + 2), torch.float32, 84)[:, 1:1 + hidden]
+    h, kept = features.gated_unit(x, wg, wu, keep=True)
+    near = [v.contiguous() for v in (x, wg, wu)]
+    h2, kept2 = features.gated_unit(*near, keep=True)
+    full = features.gated_unit_backward(dh.contiguous(), *near, kept2)
+    for a, b in [(h, h2), (kept, kept2)] + list(zip(features.gated_unit_backward(dh, x, wg, wu, kept), full)):
+        assert float((a.double() - b.double()).abs().max()) <= 2e-6 * float(b.double().abs().max()) + 1e-6
+    part = features.gated_unit_backward(dh, *near, kept2, need_dw=False)
+    assert torch.equal(part[0], full[0]) and part[1] is None and part[2] is None
+    part = features.gated_unit_backward(dh, *near, kept2, need_dx=False)
+    assert part[0] is None and torch.equal(part[1], full[1]) and torch.equal(part[2], full[2])
+    # an infinite weight of the last hidden unit, a NaN row of x: what they enter and nothing else
+    x, wg, wu = near
+    wu[4, 69] = float('inf')
+    dx, _, _ = features.gated_unit_backward(torch.ones_like(h), x, wg, wu, kept2)
+    g, _, a, _ = gated_ref(x, near[1], near[2].nan_to_num(posinf=0.0), 'silu')
+    assert bool((dx[:, 69] == torch.where(a[:, 4] > 0, float('inf'), -float('inf'))).all()) and bool(torch.isfinite(dx[:, :69]).all())
+    wu[4, 69] = 0.5
+    h, kept = features.gated_unit(x, wg, wu, keep=True)
+    x[77] = float('nan')
+    h2, kept2 = features.gated_unit(x, wg, wu, keep=True)
+    assert bool(torch.isnan(h2[77]).all()) and torch.equal(torch.cat([h[:77], h[78:]]), torch.cat([h2[:77], h2[78:]]))
 
 
 def check_gated(dtype, act, rows, cols, hidden):
