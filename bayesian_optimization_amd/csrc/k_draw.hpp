@@ -22,7 +22,7 @@
 
 namespace gpbo_static {
 
-constexpr int DRAW_THREADS = 1024, LIST = 1024, TILES = 1024;
+constexpr int DRAW_THREADS = 1024, LIST = 1024, LONG_LIST = 16384, TILES = 1024;
 constexpr int DIGIT = 11, BINS = 1 << DIGIT;
 
 template <typename T>
@@ -111,8 +111,8 @@ __device__ __forceinline__ double from_fixed(unsigned long long hi, unsigned lon
     return (double)hi * (1.0 / 34359738368.0) + (double)lo * (1.0 / 34359738368.0 / 34359738368.0);
 }
 
-// Inclusive sums over the workgroup's threads, in thread order; the total comes back too.  Two barriers; red: 32 doubles.
-template <typename V>
+// Inclusive sums over the workgroup's threads, in thread order; the total comes back too.  Two barriers; red: a place a wave.
+template <int THREADS = DRAW_THREADS, typename V>
 __device__ __forceinline__ V block_scan(V v, V* red, V& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -125,7 +125,7 @@ __device__ __forceinline__ V block_scan(V v, V* red, V& total) {
     __syncthreads();
     V before = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < DRAW_THREADS / 64; ++i) {
+    for (int i = 0; i < THREADS / 64; ++i) {
         if (i == wave) before = all;
         all += red[i];
     }
@@ -150,6 +150,7 @@ struct DrawState {
     int gather;                   // this step collects a list: 1 of klo .. khi, 2 of all that can be kept, 3 the same, on trial
     uint32_t cut_ties, floor_ties;
     unsigned int n_list, ticket;
+    unsigned int listed;          // long rows: > 0 if the row's list in memory holds that many scores, all that can be kept
 };
 
 // What of a score counts in the present step; w is its weight (PHASE_TOPP).
@@ -274,6 +275,28 @@ __device__ __forceinline__ void each_score(const T* x, uint32_t begin, uint32_t 
     for (uint32_t i = begin + packs * V + threadIdx.x; i < end; i += DRAW_THREADS) f(Score<T>::key(x[i]), i);
 }
 
+// What a step looks at: a share of a row, or (listed > 0) a long list that other workgroups left in memory, read past this one's
+// caches, that holds all scores that can be kept.
+template <typename T>
+struct DrawFrom {
+    using Key = typename Score<T>::Key;
+    const T* x;
+    uint32_t begin, end;
+    const Key* key = nullptr;
+    const uint32_t* idx = nullptr;
+    uint32_t listed = 0;
+    template <int SCORES = 8, typename F>
+    __device__ __forceinline__ void each(F&& f) const {
+        if (listed) {
+            for (uint32_t i = threadIdx.x; i < listed; i += DRAW_THREADS)
+                f((Key)__hip_atomic_load(key + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
+                  (uint32_t)__hip_atomic_load(idx + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+        } else {
+            each_score<T, SCORES>(x, begin, end, f);
+        }
+    }
+};
+
 // Best key with its lowest index, and lowest valid key, of [begin, end); own: the best key this thread saw.
 template <typename T>
 __device__ void draw_extremes(DrawLds<T>& s, const T* x, uint32_t begin, uint32_t end, typename Score<T>::Key& top, typename Score<T>::Key& bot, uint32_t& idx,
@@ -308,15 +331,16 @@ __device__ void draw_extremes(DrawLds<T>& s, const T* x, uint32_t begin, uint32_
 // Nothing to choose: no valid score (index -1), or the best one.
 template <typename T>
 __device__ void draw_same(const DrawArgs& a, int64_t row, int64_t index, double logp) {
-    for (int64_t q = threadIdx.x; q < a.draws; q += DRAW_THREADS) {
+    for (int64_t q = threadIdx.x; q < a.draws; q += blockDim.x) {
         a.index[row * a.draws + q] = index;
         if (a.logp) a.logp[row * a.draws + q] = logp;
     }
 }
 
-// Thread 0: the first step of a phase, or the next phase that has any.  bound: a key that at least top_k valid keys reach, or 0.
+// Thread 0: the first step of a phase, or the next phase that has any.  bound: a key that at least top_k valid keys reach, or 0; a list
+// from there on is tried for a top_k of up to `most`.
 template <typename T>
-__device__ void draw_begin(DrawState<T>& st, const DrawRow& p, int phase, typename Score<T>::Key bound = 0) {
+__device__ void draw_begin(DrawState<T>& st, const DrawRow& p, int phase, typename Score<T>::Key bound = 0, int most = LIST / 2) {
     using S = Score<T>;
     using Key = typename S::Key;
     if (phase == PHASE_TOPK && p.top_k == 0) phase = PHASE_TOPP;
@@ -332,7 +356,7 @@ __device__ void draw_begin(DrawState<T>& st, const DrawRow& p, int phase, typena
     if (phase == PHASE_TOPK) {
         if (bound) {
             st.klo = bound;
-            if (p.top_k <= LIST / 2) st.gather = 3;
+            if (p.top_k <= most) st.gather = 3;
         }
         return;
     }
@@ -352,16 +376,16 @@ __device__ void draw_begin(DrawState<T>& st, const DrawRow& p, int phase, typena
     if (smax < INFINITY && low > st.klo) st.klo = low > 4 ? low - 4 : low;
 }
 
-// A step's histogram over [begin, end) into LDS.  The last bin of the linear step, where all that lies far from the best falls, is
+// A step's histogram over `from` into LDS.  The last bin of the linear step, where all that lies far from the best falls, is
 // summed in registers: thousands of atomics on one address would take their turns.
 template <typename T>
-__device__ void draw_histogram(DrawLds<T>& s, const DrawStep<T>& d, const T* x, uint32_t begin, uint32_t end) {
+__device__ void draw_histogram(DrawLds<T>& s, const DrawStep<T>& d, const DrawFrom<T>& from) {
     using Key = typename Score<T>::Key;
     for (int b = threadIdx.x; b < BINS; b += DRAW_THREADS) s.h.count[b] = 0, s.h.hi[b] = 0, s.h.lo[b] = 0;
     __syncthreads();
     unsigned int rest = 0;
     unsigned long long rest_hi = 0, rest_lo = 0;
-    each_score(x, begin, end, [&](Key k, uint32_t) {
+    from.each([&](Key k, uint32_t) {
         double w = 0.0;
         if (!d.counts(k, w)) return;
         const int b = d.bin(k);
@@ -477,28 +501,55 @@ __device__ void draw_decide(DrawLds<T>& s, const DrawRow& p) {
     __syncthreads();
 }
 
+// The value of lane `lane ^ X`, by vector instructions: an exchange through LDS hardware (__shfl_xor) takes several times as long.
+template <int X>
+__device__ __forceinline__ uint32_t xor_lane(uint32_t v) {
+    if constexpr (X == 1) return __builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, true);                     // quad_perm 1 0 3 2
+    if constexpr (X == 2) return __builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, true);                     // quad_perm 2 3 0 1
+    if constexpr (X == 4) {                                                                                   // i ^ 7, then i ^ 3
+        const uint32_t m = __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true);                          // row_half_mirror
+        return __builtin_amdgcn_update_dpp(0, m, 0x1b, 0xf, 0xf, true);                                       // quad_perm 3 2 1 0
+    }
+    if constexpr (X == 8) return __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, true);                    // row_ror 8
+    if constexpr (X == 16) {                   // both results from v: rows 0 0 2 2 and 1 1 3 3
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return threadIdx.x & 16 ? r[0] : r[1];
+    }
+    if constexpr (X == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return threadIdx.x & 32 ? r[0] : r[1];
+    }
+}
+template <int X>
+__device__ __forceinline__ uint64_t xor_lane(uint64_t v) {
+    return (uint64_t)xor_lane<X>((uint32_t)(v >> 32)) << 32 | xor_lane<X>((uint32_t)v);
+}
+
 // Bitonic sort of one pair a thread over the first `size` threads (a power of two, at least 64): by rank, or by index.  Partners
-// in one wave exchange through registers, others through LDS (buf_k, buf_i); 1024 pairs take 55 exchanges, 10 of them with
-// barriers, 3 us; every pair counting the ones in front of it took 27.
+// in one wave exchange by vector instructions, others through LDS (buf_k, buf_i): 1024 pairs take 55 exchanges, 10 of them with
+// barriers (a draw from 400 scores: 11.5 us, 14.3 with __shfl_xor; every pair counting the ones in front of it took 27 alone).
 template <typename Key, bool BY_INDEX>
 __device__ __forceinline__ void block_sort(Key& k, uint32_t& i, int size, Key* buf_k, uint32_t* buf_i) {
     const int tid = threadIdx.x;
-    for (int run = 2; run <= size; run <<= 1)
-        for (int step = run >> 1; step > 0; step >>= 1) {
-            Key ok;
-            uint32_t oi;
-            if (step >= 64) {
-                __syncthreads();
-                if (tid < size) buf_k[tid] = k, buf_i[tid] = i;
-                __syncthreads();
-                ok = buf_k[(tid ^ step) & (LIST - 1)], oi = buf_i[(tid ^ step) & (LIST - 1)];
-            } else {
-                ok = __shfl_xor(k, step), oi = __shfl_xor(i, step);
-            }
+    for (int run = 2; run <= size; run <<= 1) {
+        const bool up = (tid & run) == 0 || run == size;
+        auto exchange = [&](int step, Key ok, uint32_t oi) {
             const bool mine_first = BY_INDEX ? i < oi : (k > ok || (k == ok && i < oi));
-            const bool want_first = ((tid & step) == 0) == ((tid & run) == 0 || run == size);
-            if (mine_first != want_first) k = ok, i = oi;      // equal pairs are the fillers: either way the same
+            if (mine_first != (((tid & step) == 0) == up)) k = ok, i = oi;      // equal pairs are the fillers: either way the same
+        };
+        for (int step = run >> 1; step >= 64; step >>= 1) {
+            __syncthreads();
+            if (tid < size) buf_k[tid] = k, buf_i[tid] = i;
+            __syncthreads();
+            exchange(step, buf_k[tid ^ step], buf_i[tid ^ step]);
         }
+        if (run >= 64) exchange(32, xor_lane<32>(k), xor_lane<32>(i));
+        if (run >= 32) exchange(16, xor_lane<16>(k), xor_lane<16>(i));
+        if (run >= 16) exchange(8, xor_lane<8>(k), xor_lane<8>(i));
+        if (run >= 8) exchange(4, xor_lane<4>(k), xor_lane<4>(i));
+        if (run >= 4) exchange(2, xor_lane<2>(k), xor_lane<2>(i));
+        exchange(1, xor_lane<1>(k), xor_lane<1>(i));
+    }
 }
 
 // LIST keys or fewer in l.key, l.idx: sort them by rank into l.key2, l.idx2 (behind them keys of 0).
@@ -535,9 +586,9 @@ __device__ void draw_cut_from_list(DrawLds<T>& s, const DrawRow& p, int n) {
         in = k != 0 && (tid == 0 || st.above + (incl - w) < st.goal);
     }
     unsigned long long taken, same;
-    block_scan<unsigned long long>(in ? 1ull : 0ull, s.red_u, taken);
+    block_scan(in ? 1ull : 0ull, s.red_u, taken);
     const Key cut = s.l.key2[taken ? (int)taken - 1 : 0];
-    block_scan<unsigned long long>(in && k == cut ? 1ull : 0ull, s.red_u, same);
+    block_scan(in && k == cut ? 1ull : 0ull, s.red_u, same);
     __syncthreads();
     if (tid == 0) {
         st.cut = cut, st.cut_ties = (uint32_t)same;
@@ -566,7 +617,7 @@ __device__ void draw_from_list(DrawLds<T>& s, const DrawArgs& a, const DrawRow& 
     }
     // the kept ones are the first `kept` positions; now in index order
     unsigned long long kept;
-    block_scan<unsigned long long>(keep ? 1ull : 0ull, s.red_u, kept);
+    block_scan(keep ? 1ull : 0ull, s.red_u, kept);
     Key ki = keep ? kr : 0;
     uint32_t ii = keep ? s.l.idx2[tid] : 0xffffffffu;
     int few = 64;                              // they stand in front: no more than they need to be sorted
@@ -592,10 +643,10 @@ __device__ void draw_from_list(DrawLds<T>& s, const DrawArgs& a, const DrawRow& 
     }
 }
 
-// One workgroup: the scores of [begin, end) that count go to the list; behind LIST of them nothing is written and the counter
+// One workgroup: the scores of `from` that count go to the list; behind LIST of them nothing is written and the counter
 // stops growing soon.
 template <typename T>
-__device__ void draw_gather(DrawLds<T>& s, const DrawStep<T>& d, const T* x, uint32_t begin, uint32_t end) {
+__device__ void draw_gather(DrawLds<T>& s, const DrawStep<T>& d, const DrawFrom<T>& from) {
     using Key = typename Score<T>::Key;
     auto take = [&](Key k, uint32_t i) {
         if (__hip_atomic_load(&s.st.n_list, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) > LIST) return;
@@ -604,11 +655,11 @@ __device__ void draw_gather(DrawLds<T>& s, const DrawStep<T>& d, const T* x, uin
     };
     if (d.gather == 3) {                       // all from klo up: nothing to work out, more loads at a time
         const Key bound = d.klo ? d.klo : 1;
-        each_score<T, 32>(x, begin, end, [&](Key k, uint32_t i) {
+        from.template each<32>([&](Key k, uint32_t i) {
             if (k >= bound) take(k, i);
         });
     } else {
-        each_score(x, begin, end, [&](Key k, uint32_t i) {
+        from.each([&](Key k, uint32_t i) {
             double w;
             if (d.counts(k, w)) take(k, i);
         });
@@ -640,69 +691,73 @@ __device__ bool draw_use_list(DrawLds<T>& s, const DrawArgs& a, const DrawRow& p
 
 // One workgroup takes all steps that are left; true if that included the picks.
 template <typename T>
-__device__ bool draw_search(DrawLds<T>& s, const DrawArgs& a, const DrawRow& p, const T* x, int64_t row) {
+__device__ bool draw_search(DrawLds<T>& s, const DrawArgs& a, const DrawRow& p, const DrawFrom<T>& from, int64_t row) {
     while (s.st.phase < PHASE_PICK) {
         const DrawStep<T> d(s.st, p);
         if (s.st.gather) {
-            draw_gather(s, d, x, 0, (uint32_t)a.cols);
+            draw_gather(s, d, from);
             if (draw_use_list(s, a, p, row)) return true;
         } else {
-            draw_histogram(s, d, x, 0, (uint32_t)a.cols);
+            draw_histogram(s, d, from);
             draw_decide(s, p);
         }
     }
     return false;
 }
 
-// A row of up to LIST scores, thread = index: one sort by rank gives the best and the last kept pair; whether a thread's own score
-// is kept is then a comparison, and the running sum in index order needs no second sort.
-template <typename T>
-__device__ void draw_short(DrawLds<T>& s, const DrawArgs& a, const DrawRow& p, const T* x, int64_t row, int n) {
+// Rows of up to LIST scores, a workgroup each, as many threads as scores or the next power of two, thread = index: one sort by rank
+// gives the best and the last kept pair; whether a thread's own score is kept is then a comparison, and the running sum in index
+// order needs no second sort (400 scores with 512 threads 8.9 us, with 1024 11.5; 10000 rows of 60 15 us, 164).
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_draw_short(DrawArgs a) {
     using Key = typename Score<T>::Key;
-    const int tid = threadIdx.x;
+    __shared__ Key key_s[THREADS], top_s, cut_s;
+    __shared__ uint32_t idx_s[THREADS], top_i, cut_i;
+    __shared__ double c_s[THREADS], red[16];
+    const int tid = threadIdx.x, n = (int)a.cols;
+    const int64_t row = blockIdx.x;
+    const T* x = (const T*)a.scores + row * a.stride;
+    const DrawRow p(a, row);
     const Key mine = tid < n ? Score<T>::key(x[tid]) : 0;
-    int size = 64;
-    while (size < n) size <<= 1;
     Key k = mine;
     uint32_t i = tid;
-    block_sort<Key, false>(k, i, size, s.l.key, s.l.idx);
-    if (tid == 0) s.red_k[0][0] = k, s.red_i[0] = i;
+    block_sort<Key, false>(k, i, THREADS, key_s, idx_s);
+    if (tid == 0) top_s = k, top_i = i;
     __syncthreads();
-    const Key top = s.red_k[0][0];
+    const Key top = top_s;
     if (top == 0 || p.greedy) {
-        draw_same<T>(a, row, top ? (int64_t)s.red_i[0] : -1, top ? 0.0 : -INFINITY);
+        draw_same<T>(a, row, top ? (int64_t)top_i : -1, top ? 0.0 : -INFINITY);
         return;
     }
-    const bool ranked = tid < size && k != 0;
-    const double w = ranked ? exp(draw_t<T>(k, top, p.temperature)) : 0.0;
-    bool in = ranked && (p.top_k == 0 || tid < p.top_k) && w >= p.min_p;
+    const double w = k ? exp(draw_t<T>(k, top, p.temperature)) : 0.0;
+    bool in = k != 0 && (p.top_k == 0 || tid < p.top_k) && w >= p.min_p;
     double total;
     if (p.top_p < 1.0) {
-        const double run = block_scan(in ? w : 0.0, s.red, total);
+        const double run = block_scan<THREADS>(in ? w : 0.0, red, total);
         in = in && (tid == 0 || run - w < p.top_p * total);
     }
     // the kept ones are the first in rank: the last of them is the one behind which the next position is not kept
-    s.l.pick[tid] = in;
+    idx_s[tid] = in;
     __syncthreads();
-    if (in && (tid == DRAW_THREADS - 1 || !s.l.pick[tid + 1])) s.red_k[1][0] = k, s.red_i[1] = i;
+    if (in && (tid == THREADS - 1 || !idx_s[tid + 1])) cut_s = k, cut_i = i;
     __syncthreads();
-    const Key cut = s.red_k[1][0];
-    const bool keep = mine != 0 && (mine > cut || (mine == cut && (uint32_t)tid <= s.red_i[1]));
-    const double c = block_scan(keep ? exp(draw_t<T>(mine, top, p.temperature)) : 0.0, s.red, total);
-    s.l.c[tid] = c;
-    s.l.key[tid] = mine;
+    const Key cut = cut_s;
+    const bool keep = mine != 0 && (mine > cut || (mine == cut && (uint32_t)tid <= cut_i));
+    const double c = block_scan<THREADS>(keep ? exp(draw_t<T>(mine, top, p.temperature)) : 0.0, red, total);
+    c_s[tid] = c;
+    key_s[tid] = mine;
     __syncthreads();
-    for (int64_t q = tid; q < a.draws; q += DRAW_THREADS) {
+    for (int64_t q = tid; q < a.draws; q += THREADS) {
         const double at = fmax(a.u[row * a.draws + q], 0.0) * total;
         int lo = 0, hi = n - 1;                // the first c > at; the last kept one if rounding leaves none
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (s.l.c[mid] > at) hi = mid;
+            if (c_s[mid] > at) hi = mid;
             else lo = mid + 1;
         }
-        while (lo > 0 && s.l.c[lo] == s.l.c[lo - 1]) --lo;
+        while (lo > 0 && c_s[lo] == c_s[lo - 1]) --lo;
         a.index[row * a.draws + q] = lo;
-        if (a.logp) a.logp[row * a.draws + q] = draw_t<T>(s.l.key[lo], top, p.temperature) - log(total);
+        if (a.logp) a.logp[row * a.draws + q] = draw_t<T>(key_s[lo], top, p.temperature) - log(total);
     }
 }
 
@@ -848,10 +903,6 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_row(DrawArgs a) {
     const T* x = (const T*)a.scores + row * a.stride;
     const uint32_t n = (uint32_t)a.cols;
     const DrawRow p(a, row);
-    if (n <= LIST) {
-        draw_short(s, a, p, x, row, (int)n);
-        return;
-    }
     Key top, bot, own;
     uint32_t idx;
     draw_extremes(s, x, 0, n, top, bot, idx, own);
@@ -883,7 +934,7 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_row(DrawArgs a) {
         draw_begin(s.st, p, PHASE_TOPK, bound);
     }
     __syncthreads();
-    if (draw_search(s, a, p, x, row)) return;
+    if (draw_search(s, a, p, DrawFrom<T>{x, 0, n}, row)) return;
 
     // kept mass of the row's tiles, in index order
     const DrawKept<T> kw(s.st, p);
@@ -912,7 +963,7 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_row(DrawArgs a) {
     __syncthreads();
     const uint32_t mine = s.t.ties[tid];
     unsigned long long all_ties;
-    const uint32_t before = (uint32_t)(block_scan<unsigned long long>(mine, s.red_u, all_ties) - mine);
+    const uint32_t before = (uint32_t)(block_scan((unsigned long long)mine, s.red_u, all_ties) - mine);
     const uint32_t cut_ties = s.st.cut_ties;
     const uint32_t kept = before >= cut_ties ? 0 : min(mine, cut_ties - before);
     double total;
@@ -937,18 +988,20 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_row(DrawArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Long rows: BLOCKS workgroups a row and step.  Workspace of a row: its state, one histogram, the list, the extremes of every
-// workgroup's share, and mass and ties of every tile.
+// Long rows: up to SHARES workgroups a row and step (one a CU: a step with nothing to do costs less, 16.8 M scores take 116 us and 124
+// with two).  Workspace of a row: its state, one histogram, the list, the extremes of every workgroup's share, and mass and ties
+// of every tile.
+constexpr int SHARES = 256;
 template <typename T>
 struct DrawWork {
     using Key = typename Score<T>::Key;
     DrawState<T> st;
     unsigned int count[BINS];
     unsigned long long hi[BINS], lo[BINS];
-    Key key[LIST];
-    uint32_t idx[LIST];
-    Key top[1024], bot[1024];
-    uint32_t top_idx[1024];
+    Key key[LONG_LIST];
+    uint32_t idx[LONG_LIST];
+    Key top[SHARES], bot[SHARES], quarter[4 * SHARES];
+    uint32_t top_idx[SHARES];
     double total;
 };
 template <typename T>
@@ -978,20 +1031,19 @@ __device__ __forceinline__ void draw_share(uint32_t n, uint32_t b, uint32_t bloc
 // True in the workgroup that arrives last of the `blocks` of its row; what the others wrote before is then visible to it.  One
 // thread fences for its workgroup, behind the barrier that orders the other threads' writes before it: a fence writes the L2
 // back, and one of every wave cost 8 times the step itself.  The counter is back at zero for the next step.
-template <typename T>
-__device__ bool draw_last(DrawLds<T>& s, unsigned int* ticket, uint32_t blocks) {
+__device__ __forceinline__ bool draw_last(unsigned int& last, unsigned int* ticket, uint32_t blocks) {
     __syncthreads();
     if (threadIdx.x == 0) {
         __threadfence();
         const unsigned int t = atomicAdd(ticket, 1u);
-        s.last = t == blocks - 1;
-        if (s.last) {
+        last = t == blocks - 1;
+        if (last) {
             __threadfence();
             *ticket = 0;
         }
     }
     __syncthreads();
-    return s.last;
+    return last;
 }
 
 // Extremes of every share, a clean histogram and counters.
@@ -1008,6 +1060,11 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_start(DrawArgs a, char* w
     uint32_t idx;
     draw_extremes(s, x, begin, end, top, bot, idx, own);
     if (threadIdx.x == 0) rw.w->top[blockIdx.x] = top, rw.w->bot[blockIdx.x] = bot, rw.w->top_idx[blockIdx.x] = idx;
+    if (threadIdx.x < 4) {                     // (the waves' best keys are still there)
+        Key k = 0;
+        for (int i = 0; i < DRAW_THREADS / 256; ++i) k = max(k, s.red_k[0][threadIdx.x * (DRAW_THREADS / 256) + i]);
+        rw.w->quarter[blockIdx.x * 4 + threadIdx.x] = k;
+    }
     if (blockIdx.x == 0) {
         for (int b = threadIdx.x; b < BINS; b += DRAW_THREADS) rw.w->count[b] = 0, rw.w->hi[b] = 0, rw.w->lo[b] = 0;
         if (threadIdx.x == 0) rw.w->st.ticket = 0;
@@ -1027,10 +1084,11 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_begin(DrawArgs a, char* w
     Key bk = tid < shares ? rw.w->top[tid] : 0, lk = tid < shares ? rw.w->bot[tid] : ~(Key)0;
     uint32_t bi = tid < shares ? rw.w->top_idx[tid] : 0;
     Key bound = 0;
-    if (p.top_k > 0 && p.top_k <= shares) {    // the shares' maxima, sorted: top_k of them reach the top_k-th
-        Key own = bk;
+    if (p.top_k > 0 && p.top_k <= 4 * shares) {      // the maxima of shares, or quarters of them, sorted: top_k of them reach the top_k-th
+        const bool fine = p.top_k > shares;
+        Key own = fine ? (tid < 4 * shares ? rw.w->quarter[tid] : 0) : bk;
         uint32_t none = tid;
-        block_sort<Key, false>(own, none, DRAW_THREADS, sort_k, sort_i);
+        block_sort<Key, false>(own, none, fine ? DRAW_THREADS : SHARES, sort_k, sort_i);
         if (tid == (int)p.top_k - 1) bound_s = own;
         __syncthreads();
         bound = bound_s;
@@ -1051,19 +1109,21 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_begin(DrawArgs a, char* w
     if (bk == 0 || p.greedy) draw_same<T>(a, row, bk ? (int64_t)bi : -1, bk ? 0.0 : -INFINITY);
     if (tid == 0) {
         DrawState<T>& st = rw.w->st;
-        st.top = bk, st.bot = lk, st.cut = 0, st.cut_ties = 0, st.n_list = 0;
+        st.top = bk, st.bot = lk, st.cut = 0, st.cut_ties = 0, st.n_list = 0, st.listed = 0;
         if (bk == 0 || p.greedy) st.phase = PHASE_DONE;
-        else draw_begin(st, p, PHASE_TOPK, bound);
+        else draw_begin(st, p, PHASE_TOPK, bound, DRAW_THREADS);
     }
 }
 
+// A step over all shares; the last workgroup to arrive decides.  A list on trial may hold up to LONG_LIST scores: the steps that then
+// remain need no others, and are left to k_draw_rest.
 template <typename T>
 __global__ __launch_bounds__(DRAW_THREADS) void k_draw_step(DrawArgs a, char* work) {
     using Key = typename Score<T>::Key;
     __shared__ DrawLds<T> s;
     const int64_t row = blockIdx.y;
     const DrawRowWork<T> rw(work, row, a.cols);
-    if (rw.w->st.phase >= PHASE_PICK) return;
+    if (rw.w->st.phase >= PHASE_PICK || rw.w->st.listed) return;
     const int tid = threadIdx.x;
     const T* x = (const T*)a.scores + row * a.stride;
     const DrawRow p(a, row);
@@ -1074,13 +1134,13 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_step(DrawArgs a, char* wo
     if (gather) {                              // a list of the share's own, then one place in the row's
         if (tid == 0) s.st.n_list = 0;
         __syncthreads();
-        draw_gather(s, d, x, begin, end);
-        if (tid == 0 && s.st.n_list) s.bin = atomicAdd(&rw.w->st.n_list, s.st.n_list);
+        draw_gather(s, d, DrawFrom<T>{x, begin, end});
+        if (tid == 0 && s.st.n_list) s.bin = atomicAdd(&rw.w->st.n_list, s.st.n_list > LIST ? LONG_LIST + 1 : s.st.n_list);
         __syncthreads();
-        const uint32_t mine = s.st.n_list, at = mine ? s.bin + tid : LIST;
-        if (mine <= LIST && tid < (int)mine && at < LIST) rw.w->key[at] = s.l.key[tid], rw.w->idx[at] = s.l.idx[tid];
+        const uint32_t mine = s.st.n_list, at = mine ? s.bin + tid : LONG_LIST;
+        if (mine <= LIST && tid < (int)mine && at < LONG_LIST) rw.w->key[at] = s.l.key[tid], rw.w->idx[at] = s.l.idx[tid];
     } else {
-        draw_histogram(s, d, x, begin, end);
+        draw_histogram(s, d, DrawFrom<T>{x, begin, end});
         for (int b = tid; b < BINS; b += DRAW_THREADS)
             if (s.h.count[b]) {
                 atomicAdd(&rw.w->count[b], s.h.count[b]);
@@ -1088,7 +1148,7 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_step(DrawArgs a, char* wo
                 if (s.h.lo[b]) atomicAdd(&rw.w->lo[b], s.h.lo[b]);
             }
     }
-    if (!draw_last(s, &rw.w->st.ticket, gridDim.x)) return;
+    if (!draw_last(s.last, &rw.w->st.ticket, gridDim.x)) return;
     // what other workgroups left is read past this one's caches
     auto fresh32 = [](unsigned int* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
     if (tid == 0) {
@@ -1107,14 +1167,18 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_step(DrawArgs a, char* wo
         __syncthreads();
         draw_decide(s, p);
     } else {
-        if (tid < min((int)s.st.n_list, LIST)) {
+        if (s.st.n_list <= LIST && tid < (int)s.st.n_list) {
             s.l.key[tid] = __hip_atomic_load(&rw.w->key[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             s.l.idx[tid] = fresh32(&rw.w->idx[tid]);
         }
+        const unsigned int n = s.st.n_list;
+        const bool trial = s.st.gather == 3;
+        __syncthreads();
         const bool done = draw_use_list(s, a, p, row);
         __syncthreads();
         if (tid == 0) {
             if (done) s.st.phase = PHASE_DONE;
+            else if (trial && n <= LONG_LIST) s.st.listed = n;
             s.st.n_list = 0;
         }
     }
@@ -1122,7 +1186,8 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_step(DrawArgs a, char* wo
     if (tid == 0) rw.w->st = s.st;
 }
 
-// What the launched steps left over, if scores are spread so badly that they did: one workgroup a row.
+// What the launched steps left over, one workgroup a row: the steps over a long list (16.8 M scores of which 1800 pass min_p: two passes
+// over the row less, 138 -> 124 us), or, if scores are spread so badly that there are any, further ones over the row.
 template <typename T>
 __global__ __launch_bounds__(DRAW_THREADS) void k_draw_rest(DrawArgs a, char* work) {
     __shared__ DrawLds<T> s;
@@ -1132,7 +1197,7 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_rest(DrawArgs a, char* wo
     const DrawRow p(a, row);
     if (threadIdx.x == 0) s.st = rw.w->st;
     __syncthreads();
-    const bool done = draw_search(s, a, p, (const T*)a.scores + row * a.stride, row);
+    const bool done = draw_search(s, a, p, DrawFrom<T>{(const T*)a.scores + row * a.stride, 0, (uint32_t)a.cols, rw.w->key, rw.w->idx, s.st.listed}, row);
     __syncthreads();
     if (threadIdx.x == 0) {
         if (done) s.st.phase = PHASE_DONE;
@@ -1140,9 +1205,13 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_rest(DrawArgs a, char* wo
     }
 }
 
-// Mass above the cut and ties of every tile, a wave each.
+// Mass above the cut and ties of every tile, a wave each; the last workgroup to arrive turns them into running sums, 1024 tiles at a
+// time.
 template <typename T>
-__global__ __launch_bounds__(256) void k_draw_mass(DrawArgs a, char* work) {
+__global__ __launch_bounds__(DRAW_THREADS) void k_draw_mass(DrawArgs a, char* work) {
+    __shared__ double red[32];
+    __shared__ unsigned long long red_u[32];
+    __shared__ unsigned int last;
     const int64_t row = blockIdx.y;
     const DrawRowWork<T> rw(work, row, a.cols);
     if (rw.w->st.phase != PHASE_PICK) return;
@@ -1150,35 +1219,25 @@ __global__ __launch_bounds__(256) void k_draw_mass(DrawArgs a, char* work) {
     const DrawKept<T> kw(rw.w->st, p);
     const T* x = (const T*)a.scores + row * a.stride;
     const uint32_t n = (uint32_t)a.cols, tiles = (n + TILE - 1) / TILE;
-    for (uint32_t t = blockIdx.x * 4 + (threadIdx.x >> 6); t < tiles; t += gridDim.x * 4) {
+    for (uint32_t t = blockIdx.x * (DRAW_THREADS / 64) + (threadIdx.x >> 6); t < tiles; t += gridDim.x * (DRAW_THREADS / 64)) {
         double m;
         uint32_t c;
         draw_tile_mass(kw, x, t * TILE, min(n, (t + 1) * TILE), m, c);
         if ((threadIdx.x & 63) == 0) rw.c[t] = m, rw.ties[t] = c;
     }
-}
-
-// Running sums over the tiles.  One workgroup a row; the tiles in runs of 1024.
-template <typename T>
-__global__ __launch_bounds__(DRAW_THREADS) void k_draw_sums(DrawArgs a, char* work) {
-    __shared__ double red[32];
-    __shared__ unsigned long long red_u[32];
-    const int64_t row = blockIdx.x;
-    const DrawRowWork<T> rw(work, row, a.cols);
-    if (rw.w->st.phase != PHASE_PICK) return;
-    const DrawRow p(a, row);
-    const DrawKept<T> kw(rw.w->st, p);
-    const uint32_t tiles = (uint32_t)ceil_div(a.cols, TILE), cut_ties = rw.w->st.cut_ties;
+    if (!draw_last(last, &rw.w->st.ticket, gridDim.x)) return;
+    const uint32_t cut_ties = rw.w->st.cut_ties;
     double carry = 0.0;
     unsigned long long carry_t = 0;
     for (uint32_t t0 = 0; t0 < tiles; t0 += DRAW_THREADS) {
         const uint32_t t = t0 + threadIdx.x;
-        const uint32_t mine = t < tiles ? rw.ties[t] : 0;
+        const uint32_t mine = t < tiles ? __hip_atomic_load(rw.ties + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+        const double mass = t < tiles ? __hip_atomic_load(rw.c + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
         unsigned long long all_t;
-        const unsigned long long before = carry_t + block_scan<unsigned long long>(mine, red_u, all_t) - mine;
+        const unsigned long long before = carry_t + block_scan((unsigned long long)mine, red_u, all_t) - mine;
         const uint32_t kept = before >= cut_ties ? 0 : (uint32_t)min((unsigned long long)mine, cut_ties - before);
         double all;
-        const double incl = block_scan((t < tiles ? rw.c[t] : 0.0) + kept * kw.tie_w, red, all);
+        const double incl = block_scan(mass + kept * kw.tie_w, red, all);
         if (t < tiles) rw.c[t] = carry + incl, rw.ties[t] = (uint32_t)before;
         carry += all;
         carry_t += all_t;
@@ -1225,12 +1284,21 @@ int64_t draw_work_bytes(int64_t rows, int64_t cols) {
 
 template <typename T>
 hipError_t draw_rows(hipStream_t st, const DrawArgs& a, char* work) {
+    if (a.cols <= LIST) {
+        auto launch = [&](auto k, int threads) { hipLaunchKernelGGL(k, dim3((unsigned)a.rows), dim3(threads), 0, st, a); };
+        if (a.cols <= 64) launch(k_draw_short<T, 64>, 64);
+        else if (a.cols <= 128) launch(k_draw_short<T, 128>, 128);
+        else if (a.cols <= 256) launch(k_draw_short<T, 256>, 256);
+        else if (a.cols <= 512) launch(k_draw_short<T, 512>, 512);
+        else launch(k_draw_short<T, 1024>, 1024);
+        return hipGetLastError();
+    }
     if (!draw_long(a.rows, a.cols)) {
         hipLaunchKernelGGL(k_draw_row<T>, dim3((unsigned)a.rows), dim3(DRAW_THREADS), 0, st, a);
         return hipGetLastError();
     }
-    // two workgroups of 1024 threads a CU over all rows, at least one 16 K share each
-    const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>({ceil_div(512, a.rows), ceil_div(a.cols, 16384), 1024}));
+    // a workgroup of 1024 threads a CU over all rows, shares of at least 16 K
+    const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>(ceil_div(SHARES, a.rows), ceil_div(a.cols, 16384)));
     for (int64_t r0 = 0; r0 < a.rows; r0 += 65535) {      // the grid's second dimension ends there
         DrawArgs b = a;
         b.rows = std::min<int64_t>(65535, a.rows - r0);
@@ -1248,8 +1316,8 @@ hipError_t draw_rows(hipStream_t st, const DrawArgs& a, char* work) {
         for (int i = 0; i < steps; ++i) hipLaunchKernelGGL(k_draw_step<T>, wide, dim3(DRAW_THREADS), 0, st, b, w);
         if (phases) hipLaunchKernelGGL(k_draw_rest<T>, one, dim3(DRAW_THREADS), 0, st, b, w);
         const int64_t tiles = ceil_div(a.cols, TILE);
-        hipLaunchKernelGGL(k_draw_mass<T>, dim3((unsigned)std::min<int64_t>(ceil_div(tiles, 4), 4096), (unsigned)b.rows), dim3(256), 0, st, b, w);
-        hipLaunchKernelGGL(k_draw_sums<T>, one, dim3(DRAW_THREADS), 0, st, b, w);
+        hipLaunchKernelGGL(k_draw_mass<T>, dim3((unsigned)std::min<int64_t>(ceil_div(tiles, DRAW_THREADS / 64), blocks), (unsigned)b.rows), dim3(DRAW_THREADS),
+                           0, st, b, w);
         hipLaunchKernelGGL(k_draw_pick<T>, dim3((unsigned)std::min<int64_t>(ceil_div(a.draws, 4), 4096), (unsigned)b.rows), dim3(256), 0, st, b, w);
     }
     return hipGetLastError();

@@ -48,7 +48,7 @@ def sample(scores, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         temperature, top_k, top_p, min_p = 1.0, 0, 1.0, 0.0
     if not (temperature >= 0.0 and math.isfinite(temperature)):
         raise ValueError('temperature must be finite and >= 0; got %r' % (temperature,))
-    if not (top_k >= 0 and top_k == int(top_k)):
+    if not (0 <= top_k < math.inf and top_k == int(top_k)):
         raise ValueError('top_k must be a whole number >= 0; got %r' % (top_k,))
     if not (0.0 <= top_p <= 1.0 and 0.0 <= min_p <= 1.0):
         raise ValueError('top_p and min_p must lie in [0, 1]; got %r and %r' % (top_p, min_p))

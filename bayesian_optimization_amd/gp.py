@@ -381,8 +381,8 @@ class GP:
 
 def _draw(gp, fn, u, temperature, top_k, top_p, min_p):
     u = _f64(np.asarray(u).reshape(-1), 1)
-    if top_k != int(top_k):
-        raise ValueError('top_k must be a whole number; got %r' % (top_k,))
+    if not (0 <= top_k < float('inf') and top_k == int(top_k)):
+        raise ValueError('top_k must be a whole number >= 0; got %r' % (top_k,))
     index, logp = np.empty(u.shape[0], dtype=np.int64), np.empty(u.shape[0])
     gp._check(fn(gp._h, L.dptr(u), u.shape[0], float(temperature), min(int(top_k), 1 << 62), float(top_p), float(min_p),
                  index.ctypes.data_as(C.POINTER(C.c_int64)), L.dptr(logp)))

@@ -131,6 +131,47 @@ def test_most_scores_zero_as_expected_improvement_has_them():
         check(s, u, *draws.sample(s, u, **st), **st)
 
 
+@pytest.mark.parametrize('dtype', [torch.float64, torch.float32, torch.float16])
+@pytest.mark.parametrize('many', [900, 1024, 1025, 1500, 5000, 16383, 16384, 16385, 30000])
+@pytest.mark.parametrize('spread', [True, False])
+def test_lists_on_trial_of_every_length(dtype, many, spread):
+    """`many` scores pass min_p, over the whole row or next to each other: lists that one workgroup sorts, that it has to work through
+    in steps, that are too long as a whole, and that one share alone is too long for."""
+    from bayesian_optimization_amd import draws
+    cols = 400003
+    g = torch.Generator(device='cuda').manual_seed(many)
+    s = rand_scores(2, cols, torch.float64, many) - 60.0
+    for r in range(2):
+        at = torch.randperm(cols, generator=g, device='cuda')[:many] if spread else torch.arange(many, device='cuda') + 123456
+        s[r, at] = torch.rand(many, generator=g, device='cuda', dtype=torch.float64) * 4.0
+    s, u = s.to(dtype), rand_u(2, 64, many)
+    for st in (dict(min_p=0.01), dict(min_p=0.01, top_p=0.9), dict(min_p=0.01, top_p=0.3), dict(min_p=0.3, top_p=0.8), dict(min_p=0.01, top_k=97), dict(top_k=97),
+               dict(top_k=99, top_p=0.9), dict(top_k=300, min_p=0.5, top_p=0.99)):
+        check(s, u, *draws.sample(s, u, **st), **st)
+
+
+@pytest.mark.parametrize('dtype', [torch.float64, torch.bfloat16])
+@pytest.mark.parametrize('top_k', [25, 26, 60, 100, 101, 256, 257, 512, 820, 1000, 1024])
+def test_top_k_bounds_from_shares_and_their_quarters(dtype, top_k):
+    from bayesian_optimization_amd import draws
+    for rows, cols in ((1, 400003), (3, 100001)):
+        s, u = rand_scores(rows, cols, dtype, top_k), rand_u(rows, 40, top_k)
+        for st in (dict(top_k=top_k, temperature=2.0), dict(top_k=top_k, top_p=0.95, temperature=1.5), dict(top_k=top_k, top_p=0.9, min_p=0.3, temperature=1.5)):
+            check(s, u, *draws.sample(s, u, **st), **st)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('cols', [1, 2, 17, 31, 32, 33, 64, 65, 127, 128, 129, 255, 256, 257, 511, 512, 513, 1023, 1024])
+def test_short_rows_of_every_workgroup_size(dtype, cols):
+    from bayesian_optimization_amd import draws
+    s, u = rand_scores(5, cols, dtype, cols), rand_u(5, 70, cols)
+    s[1] = s[1].round()                # ties
+    s[2, ::3] = -float('inf')
+    s[2, 0] = 1.0
+    for st in (dict(), dict(top_k=max(1, cols // 2), temperature=2.0), dict(top_p=0.7), dict(min_p=0.2), dict(top_k=9, top_p=0.9, min_p=0.01)):
+        check(s, u, *draws.sample(s, u, **st), **st)
+
+
 def test_settings_per_row():
     from bayesian_optimization_amd import draws
     rows = 6
@@ -216,7 +257,7 @@ def test_the_longest_row():
 def test_refusals():
     from bayesian_optimization_amd import draws
     s, u = rand_scores(2, 10, torch.float32, 13), rand_u(2, 3, 13)
-    for bad in (dict(temperature=-1.0), dict(temperature=float('nan')), dict(temperature=float('inf')), dict(top_k=-1), dict(top_k=2.5), dict(top_p=1.5), dict(top_p=-0.1),
+    for bad in (dict(temperature=-1.0), dict(temperature=float('nan')), dict(temperature=float('inf')), dict(top_k=-1), dict(top_k=2.5), dict(top_k=float('inf')), dict(top_k=float('nan')), dict(top_p=1.5), dict(top_p=-0.1),
                 dict(min_p=2.0), dict(top_p=float('nan')), dict(top_k=torch.ones(3, device='cuda')), dict(top_p=torch.ones(2))):
         with pytest.raises(ValueError):
             draws.sample(s, u, **bad)
@@ -244,7 +285,7 @@ def test_gp_draw_after_acquire(gp0):
     T = lambda a: torch.from_numpy(np.asarray(a)[None]).cuda()
     check(T(ei), T(u), T(index), T(logp), **st)
     assert gp0.draw([0.5], temperature=0)[0][0] == best
-    for bad in (dict(temperature=-1), dict(top_k=-3), dict(top_k=1.5), dict(top_p=2), dict(min_p=-1), dict(temperature=float('nan'))):
+    for bad in (dict(temperature=-1), dict(top_k=-3), dict(top_k=1.5), dict(top_k=float('inf')), dict(top_p=2), dict(min_p=-1), dict(temperature=float('nan'))):
         with pytest.raises(ValueError):
             gp0.draw(u, **bad)
     with pytest.raises(ValueError):
