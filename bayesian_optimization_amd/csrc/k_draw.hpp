@@ -14,6 +14,9 @@
 // Bound by memory: a pass over the row per step, two to five of them, and by the exponential of the scores of a top-p step.
 // Short rows: one workgroup a row does everything (k_draw_row).  Long rows: the same steps with many workgroups a row, one
 // launch a step, the state of a row in the workspace; the last workgroup to arrive at a step takes its decision.
+// Measured: 256 rows of 65537 scores of 16 bits with top_k and top_p 37 us (a pass over them 7 at the rate of a copy; what is left is
+// one workgroup's chain of small steps), 16.8 M float64 scores with min_p and top_p 116 us (two passes of 30, launches with nothing
+// to do 2 to 4 each, the cut and the picks 40 in one workgroup).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -911,8 +914,8 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_row(DrawArgs a) {
         return;
     }
     // A lower bound of the top_k-th score: the top_k-th of the maxima of groups of threads, sorted.  A quarter more groups than
-    // top_k keep the list behind the bound short (some n log n of them, at most); few of them sort soonest (64 in one wave: 1.5 us;
-    // 1024: 10 us).
+    // top_k keep the list behind the bound short (some n log n of them, at most), and few of them are sooner sorted: 64 without leaving
+    // a wave (256 x 65537 scores of 16 bits, top_k 50: 40 us with all 1024, 38.5 with 64).
     Key bound = 0;
     if (p.top_k > 0 && p.top_k <= DRAW_THREADS) {
         const int groups = p.top_k * 5 <= 64 * 4 ? 64 : p.top_k * 5 <= 256 * 4 ? 256 : DRAW_THREADS, each = DRAW_THREADS / groups;
