@@ -310,7 +310,7 @@ __global__ __launch_bounds__(256) void k_gated_slopes_both(const T* __restrict__
 // wave), which two waves a SIMD overlap (1 M x 256 -> 512 f16: 0.60 ms, 0.92 PFLOP/s; with the tiles 0.99).  The weight rows are dealt to the fragments so that a lane ends up with 8 neighbouring
 // outputs: 16-byte stores.
 constexpr int STREAM_ROWS = 128, STREAM_MOST = 256;
-template <typename T, int SL>
+template <typename T, int SL, int ACT>
 __global__ __launch_bounds__(512) void k_gated_stream(GatedArgs g, int wn, int groups) {
     constexpr int CHUNKS = SL * 4, LOADS = STREAM_ROWS * CHUNKS / 512;
     __shared__ uint4 buf0[STREAM_ROWS * CHUNKS], buf1[STREAM_ROWS * CHUNKS];
@@ -346,8 +346,7 @@ __global__ __launch_bounds__(512) void k_gated_stream(GatedArgs g, int wn, int g
     T* const out = (T*)g.out[0] + (lane & 15) * g.os + col;
     float *const kg = g.keep_g ? g.keep_g + (lane & 15) * g.n + col : nullptr, *const ku = g.keep_g ? g.keep_u + (lane & 15) * g.n + col : nullptr;
     const bool whole_cols = base + 32 <= g.n;
-    auto work = [&](const uint4* buf, int64_t t) {
-        const bool whole = whole_cols && (t + 1) * STREAM_ROWS <= g.m;         // uniform: no lane has anything to leave out
+    auto work_as = [&](const uint4* buf, int64_t t, auto whole) {
 #pragma unroll 2
         for (int f = wave / wn; f < STREAM_ROWS / 16; f += 8 / wn) {
             f32x4 acc[2][2];
@@ -366,9 +365,9 @@ __global__ __launch_bounds__(512) void k_gated_stream(GatedArgs g, int wn, int g
             const int64_t row = t * STREAM_ROWS + f * 16;                      // the fragment's first
             T o[8];
 #pragma unroll
-            for (int r = 0; r < 8; ++r) o[r] = from_float<T>(activate<T>(acc[r >> 2][0][r & 3], g.act) * acc[r >> 2][1][r & 3]);
+            for (int r = 0; r < 8; ++r) o[r] = from_float<T>(activate<T>(acc[r >> 2][0][r & 3], ACT) * acc[r >> 2][1][r & 3]);
             T* p = out + row * g.os;
-            if (whole) {
+            if constexpr (whole.value) {
                 __builtin_memcpy(p, o, sizeof(o));
                 if (kg) {
                     __builtin_memcpy(kg + row * g.n, &acc[0][0], 16);
@@ -385,6 +384,10 @@ __global__ __launch_bounds__(512) void k_gated_stream(GatedArgs g, int wn, int g
                     }
             }
         }
+    };
+    auto work = [&](const uint4* buf, int64_t t) {
+        if (whole_cols && (t + 1) * STREAM_ROWS <= g.m) work_as(buf, t, std::true_type{});      // no lane has anything to leave out
+        else work_as(buf, t, std::false_type{});
     };
     if (first >= tiles) return;
     fetch(buf0, first);

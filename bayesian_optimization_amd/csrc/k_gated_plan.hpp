@@ -76,11 +76,13 @@ void launch_stream(hipStream_t st, const GatedArgs& g) {
         const int groups = (int)ceil_div(g.n, wn * 32);
         int64_t walkers = std::max<int64_t>(1, std::min<int64_t>(256 / std::min(groups, 256), ceil_div(g.m, STREAM_ROWS)));
         if (walkers > 8) walkers -= walkers % 8;
-        const dim3 grid((unsigned)(groups * walkers));
-        if (g.k <= 64) hipLaunchKernelGGL((k_gated_stream<T, 2>), grid, dim3(512), 0, st, g, wn, groups);
-        else if (g.k <= 128) hipLaunchKernelGGL((k_gated_stream<T, 4>), grid, dim3(512), 0, st, g, wn, groups);
-        else if (g.k <= 192) hipLaunchKernelGGL((k_gated_stream<T, 6>), grid, dim3(512), 0, st, g, wn, groups);
-        else hipLaunchKernelGGL((k_gated_stream<T, 8>), grid, dim3(512), 0, st, g, wn, groups);
+        auto launch = [&](auto silu, auto gelu) {
+            hipLaunchKernelGGL(g.act == GPBO_ACT_SILU ? silu : gelu, dim3((unsigned)(groups * walkers)), dim3(512), 0, st, g, wn, groups);
+        };
+        if (g.k <= 64) launch(k_gated_stream<T, 2, GPBO_ACT_SILU>, k_gated_stream<T, 2, GPBO_ACT_GELU>);
+        else if (g.k <= 128) launch(k_gated_stream<T, 4, GPBO_ACT_SILU>, k_gated_stream<T, 4, GPBO_ACT_GELU>);
+        else if (g.k <= 192) launch(k_gated_stream<T, 6, GPBO_ACT_SILU>, k_gated_stream<T, 6, GPBO_ACT_GELU>);
+        else launch(k_gated_stream<T, 8, GPBO_ACT_SILU>, k_gated_stream<T, 8, GPBO_ACT_GELU>);
     }
 }
 
