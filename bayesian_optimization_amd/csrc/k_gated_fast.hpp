@@ -347,21 +347,23 @@ __global__ __launch_bounds__(512) void k_gated_stream(GatedArgs g, int wn, int g
     float *const kg = g.keep_g ? g.keep_g + (lane & 15) * g.n + col : nullptr, *const ku = g.keep_g ? g.keep_u + (lane & 15) * g.n + col : nullptr;
     const bool whole_cols = base + 32 <= g.n;
     auto work_as = [&](const uint4* buf, int64_t t, auto whole) {
-#pragma unroll 2
-        for (int f = wave / wn; f < STREAM_ROWS / 16; f += 8 / wn) {
+        auto load = [&](uint4 (&fa)[SL], int f) {
+            const uint4* pa = buf + (f * 16 + (lane & 15)) * CHUNKS;
+            const uint4 *even = pa + ((lane >> 4) ^ (lane & 7)), *odd = pa + ((4 + (lane >> 4)) ^ (lane & 7));
+#pragma unroll
+            for (int s = 0; s < SL; ++s) fa[s] = (s & 1 ? odd : even)[s / 2 * 8];
+        };
+        auto one = [&](const uint4 (&fa)[SL], int f) {
             f32x4 acc[2][2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) acc[j][0] = acc[j][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            const uint4* pa = buf + (f * 16 + (lane & 15)) * CHUNKS;
 #pragma unroll
-            for (int s = 0; s < SL; ++s) {
-                const uint4 fa = pa[(s * 4 + (lane >> 4)) ^ (lane & 7)];
+            for (int s = 0; s < SL; ++s)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    acc[j][0] = mma<T>(fb[j][0][s], fa, acc[j][0]);
-                    acc[j][1] = mma<T>(fb[j][1][s], fa, acc[j][1]);
+                    acc[j][0] = mma<T>(fb[j][0][s], fa[s], acc[j][0]);
+                    acc[j][1] = mma<T>(fb[j][1][s], fa[s], acc[j][1]);
                 }
-            }
             const int64_t row = t * STREAM_ROWS + f * 16;                      // the fragment's first
             T o[8];
 #pragma unroll
@@ -383,7 +385,21 @@ __global__ __launch_bounds__(512) void k_gated_stream(GatedArgs g, int wn, int g
                         if (kg) kg[row * g.n + r] = acc[r >> 2][0][r & 3], ku[row * g.n + r] = acc[r >> 2][1][r & 3];
                     }
             }
+        };
+        // the next fragment of rows is on its way from LDS while this one is multiplied
+        const int by = 8 / wn, last = STREAM_ROWS / 16 - by + wave / wn;
+        uint4 f0[SL], f1[SL];
+        int f = wave / wn;
+        load(f0, f);
+        for (; f < last; f += 2 * by) {
+            load(f1, f + by);
+            __builtin_amdgcn_sched_barrier(0);
+            one(f0, f);
+            load(f0, min(f + 2 * by, last));
+            __builtin_amdgcn_sched_barrier(0);
+            one(f1, f + by);
         }
+        if (f == last) one(f0, f);
     };
     auto work = [&](const uint4* buf, int64_t t) {
         if (whole_cols && (t + 1) * STREAM_ROWS <= g.m) work_as(buf, t, std::true_type{});      // no lane has anything to leave out
