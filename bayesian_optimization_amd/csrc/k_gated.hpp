@@ -43,7 +43,7 @@ __device__ __forceinline__ f32x4 mma<float>(const uint4& a, const uint4& b, f32x
 // act(g) and act'(g).  silu through the logistic function, whose exponential saturates to 0 or infinity with the right limit;
 // gelu through erfc, which keeps the far negative tail that 1 + erf loses.  For results of 16 bits the hardware's exponential and
 // reciprocal (one unit in the last place each) and, for erfc, the five-term rational form of Abramowitz and Stegun 7.1.26 (1.5e-7):
-// the activation of every output is as much vector work as a short contraction is matrix work (1 M x 256 -> 512: 1.27 -> 0.83 ms).
+// the activation of every output is as much vector work as a short contraction is matrix work (1 M x 256 -> 512, with tiles: 1.27 -> 0.83 ms).
 template <typename T>
 __device__ __forceinline__ void activation(float g, int act, float& a, float& da) {
     if constexpr (sizeof(T) == 4) {

@@ -306,9 +306,9 @@ __global__ __launch_bounds__(256) void k_gated_slopes_both(const T* __restrict__
 // a wave keeps its 32 hidden units' weights for the whole contraction in registers (128 of them at 256 elements) and the
 // workgroup walks over tiles of 128 rows of x, the next one on its way into LDS while this one is multiplied; a row fragment is
 // read once for four matrix instructions.  wn of the 8 waves stand side by side over hidden units, the others share the rows.
-// Bound by its two halves about alike, matrix instructions and the activation's vector instructions (48 cycles an output and
-// wave), which two waves a SIMD overlap (1 M x 256 -> 512 f16: 0.60 ms, 0.92 PFLOP/s; with the tiles 0.99).  The weight rows are dealt to the fragments so that a lane ends up with 8 neighbouring
-// outputs: 16-byte stores.
+// Bound by matrix instructions (busy 58 % of the time) and the activation's vector instructions (48 cycles an output and wave), which
+// two waves a SIMD overlap: 1 M x 256 -> 512 f16 in 0.525 ms, 1.05 PFLOP/s, of 1.45 of a large library product; with the tiles
+// above 0.99 ms.  The weight rows are dealt to the fragments so that a lane ends up with 8 neighbouring outputs: 16-byte stores.
 constexpr int STREAM_ROWS = 128, STREAM_MOST = 256;
 template <typename T, int SL, int ACT>
 __global__ __launch_bounds__(512) void k_gated_stream(GatedArgs g, int wn, int groups) {
