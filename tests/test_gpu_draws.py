@@ -203,7 +203,7 @@ def test_strided_rows_streams_and_graphs():
         base = rand_scores(6, cols + 11, dtype, 11)
         s = base[::2, 5:5 + cols]
         u = rand_u(3, 9, 11)
-        st = dict(temperature=0.7, top_k=2000, top_p=0.9)
+        st = dict(temperature=0.7, top_k=2000, top_p=0.9) if cols < 100000 else dict(temperature=0.7, top_p=0.9, min_p=1e-3)
         first = draws.sample(s, u, **st)
         check(s, u, *first, **st)
         assert all(torch.equal(a, b) for a, b in zip(first, draws.sample(s.contiguous(), u, **st)))
@@ -307,3 +307,38 @@ def test_gp_draw_after_acquire(gp0):
     assert (one.draw(u, **st)[0] == index).all()
     mg.close()
     one.close()
+
+
+@pytest.mark.parametrize('lattice', [False, True])
+def test_gp_draw_after_append_acquire(gp0, lattice):
+    """The acquisition an append leaves behind: draws come from what read() returns, or both are refused."""
+    import bayesian_optimization_amd as bo
+    from bayesian_optimization_amd import _lib as L
+    rng = np.random.default_rng(2)
+    axes = [np.linspace(0, 1, 24)] * 3
+    grid = np.stack(np.meshgrid(*axes, indexing='ij'), -1).reshape(-1, 3)
+    X = grid[rng.choice(len(grid), 12, replace=False)]
+    f = lambda p: float(np.sin(4 * p.sum()))
+    gp = bo.GP(0)
+    gp.reserve_appends(8)
+    gp.fit(X, np.array([f(p) for p in X]), [0.3, 0.4, 0.5], 0.05, variant=L.VARIANT_SINGLE)
+    gp.set_candidates_lattice(axes) if lattice else gp.set_candidates(grid)
+    gp.posterior()
+    j, _ = gp.acquire()
+    u, st, T = rng.random(40), dict(temperature=0.01, top_p=0.9, min_p=1e-3), lambda a: torch.from_numpy(np.asarray(a)[None]).cuda()
+    for _ in range(6):
+        _, j, _ = gp.append_acquire(grid[j], f(grid[j]))
+        try:
+            acq = gp.read(mu=False, var=False, acq=True)
+        except ValueError:
+            with pytest.raises(ValueError):
+                gp.draw(u, **st)
+            continue
+        index, logp = gp.draw(u, **st)
+        check(T(acq), T(u), T(index), T(logp), **st)
+        assert gp.draw([0.3], temperature=0)[0][0] == j
+    gp.acquire()
+    gp.append(grid[j], f(grid[j]))
+    with pytest.raises(ValueError):
+        gp.draw(u)                     # the posterior has moved on
+    gp.close()

@@ -345,7 +345,7 @@ def test_gated_unit_offsets_past_32_bits():
 def test_operators_repeat_bit_for_bit_and_replay_from_a_graph(dtype):
     """Captured once, replayed on new inputs in the same buffers with eager work in between; every replay equals the eager call."""
     from bayesian_optimization_amd import features
-    for rows, cols, hidden in ((95, 621, 128), (512, 512, 256), (1100, 1000, 1024)):
+    for rows, cols, hidden in ((95, 621, 128), (512, 512, 256), (1100, 1000, 1024), (17000, 70, 12), (66000, 128, 33)):
         x, dh = rand((rows, cols), dtype, 61), rand((rows, hidden), dtype, 62)
         w, wg, wu = rand((cols,), dtype, 63), rand((hidden, cols), dtype, 64, 0.05), rand((hidden, cols), dtype, 65, 0.05)
 
@@ -375,6 +375,41 @@ def test_operators_repeat_bit_for_bit_and_replay_from_a_graph(dtype):
             torch.cuda.synchronize()
             eager = step()
             assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(eager, out, out2)), (rows, i)
+
+
+def test_calls_at_the_same_time():
+    """Two threads, a stream each, in step: every call has its workspace to itself."""
+    import threading
+    from bayesian_optimization_amd import draws, features
+    jobs = [(torch.float32, 20017, 70, 12), (torch.bfloat16, 1100, 1000, 1024)]
+    data = []
+    for i, (dtype, rows, cols, hidden) in enumerate(jobs):
+        data.append((rand((rows, cols), dtype, 101 + i), rand((hidden, cols), dtype, 111 + i, 0.05), rand((hidden, cols), dtype, 121 + i, 0.05),
+                     rand((rows, hidden), dtype, 131 + i), rand((2, 200000), dtype, 141 + i), torch.rand(2, 30, device='cuda', dtype=torch.float64)))
+
+    def step(x, wg, wu, dh, s, u):
+        y, mean, rstd = features.layer_norm(x)
+        h, kept = features.gated_unit(y, wg, wu, keep=True)
+        dy, dwg, dwu = features.gated_unit_backward(dh, y, wg, wu, kept)
+        return (h, dwg, dwu) + features.layer_norm_backward(dy, x, None, mean, rstd) + draws.sample(s, u, top_p=0.9, min_p=0.01)
+    want = [step(*d) for d in data]
+    torch.cuda.synchronize()
+    wrong, gate = [], threading.Barrier(2)
+
+    def run(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(5):
+                gate.wait(60)
+                got = step(*data[i])
+                stream.synchronize()
+                wrong.extend(k for k, (a, b) in enumerate(zip(got, want[i])) if not torch.equal(a, b))
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 def test_refusals_on_the_gpu():
