@@ -14,6 +14,7 @@ extern "C" {
 
 int64_t gpbo_draw_static_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_t draws) {
     if (type_bytes(dtype) == 0 || rows < 0 || rows > MOST_ROWS || cols < 1 || cols > MOST_COLS || draws < 0 || draws > MOST_ROWS) return -1;
+    if (draw_long(rows, cols) && rows > MOST_LONG_ROWS) return -1;
     switch (dtype) {
         case GPBO_TYPE_F64: return draw_work_bytes<double>(rows, cols);
         case GPBO_TYPE_F32: return draw_work_bytes<float>(rows, cols);

@@ -1278,6 +1278,7 @@ __global__ __launch_bounds__(256) void k_draw_pick(DrawArgs a, char* work) {
 }
 
 // One workgroup a row while the rows fill the card or a row is short; else many workgroups a row.
+constexpr int64_t MOST_LONG_ROWS = 65535;      // a grid's second dimension (more of them would not fit into the card's memory)
 inline bool draw_long(int64_t rows, int64_t cols) { return cols > (int64_t)TILE * TILES || (cols > 32768 && rows * 4 < 256 * 2); }
 
 template <typename T>
@@ -1302,27 +1303,20 @@ hipError_t draw_rows(hipStream_t st, const DrawArgs& a, char* work) {
     }
     // a workgroup of 1024 threads a CU over all rows, shares of at least 16 K
     const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>(ceil_div(SHARES, a.rows), ceil_div(a.cols, 16384)));
-    for (int64_t r0 = 0; r0 < a.rows; r0 += 65535) {      // the grid's second dimension ends there
-        DrawArgs b = a;
-        b.rows = std::min<int64_t>(65535, a.rows - r0);
-        b.scores = (const T*)a.scores + r0 * a.stride, b.u = a.u + r0 * a.draws, b.index = a.index + r0 * a.draws;
-        b.logp = a.logp ? a.logp + r0 * a.draws : nullptr, b.params = a.params ? a.params + r0 * 4 : nullptr;
-        char* w = work + r0 * draw_row_bytes<T>(a.cols);
-        const dim3 wide((unsigned)blocks, (unsigned)b.rows), one((unsigned)b.rows);
-        hipLaunchKernelGGL(k_draw_start<T>, wide, dim3(DRAW_THREADS), 0, st, b, w);
-        hipLaunchKernelGGL(k_draw_begin<T>, one, dim3(DRAW_THREADS), 0, st, b, w, (int)blocks);
-        // a phase rarely takes more than a list on trial, two linear steps, one on the keys and one more list; what is decided
-        // earlier leaves the rest of the launches with nothing to do, what is not is left to one workgroup a row
-        const bool by_row = a.params != nullptr;
-        const int phases = (by_row || (a.top_k > 0 && a.top_k < a.cols)) + (by_row || a.top_p < 1.0 || a.min_p > 0.0);
-        const int steps = phases == 0 ? 0 : a.top_p < 1.0 || phases == 2 || by_row ? 1 + 4 * phases : 4;
-        for (int i = 0; i < steps; ++i) hipLaunchKernelGGL(k_draw_step<T>, wide, dim3(DRAW_THREADS), 0, st, b, w);
-        if (phases) hipLaunchKernelGGL(k_draw_rest<T>, one, dim3(DRAW_THREADS), 0, st, b, w);
-        const int64_t tiles = ceil_div(a.cols, TILE);
-        hipLaunchKernelGGL(k_draw_mass<T>, dim3((unsigned)std::min<int64_t>(ceil_div(tiles, DRAW_THREADS / 64), blocks), (unsigned)b.rows), dim3(DRAW_THREADS),
-                           0, st, b, w);
-        hipLaunchKernelGGL(k_draw_pick<T>, dim3((unsigned)std::min<int64_t>(ceil_div(a.draws, 4), 4096), (unsigned)b.rows), dim3(256), 0, st, b, w);
-    }
+    const dim3 wide((unsigned)blocks, (unsigned)a.rows), one((unsigned)a.rows);
+    hipLaunchKernelGGL(k_draw_start<T>, wide, dim3(DRAW_THREADS), 0, st, a, work);
+    hipLaunchKernelGGL(k_draw_begin<T>, one, dim3(DRAW_THREADS), 0, st, a, work, (int)blocks);
+    // a phase rarely takes more than a list on trial, two linear steps, one on the keys and one more list; what is decided
+    // earlier leaves the rest of the launches with nothing to do, what is not is left to one workgroup a row
+    const bool by_row = a.params != nullptr;
+    const int phases = (by_row || (a.top_k > 0 && a.top_k < a.cols)) + (by_row || a.top_p < 1.0 || a.min_p > 0.0);
+    const int steps = phases == 0 ? 0 : a.top_p < 1.0 || phases == 2 || by_row ? 1 + 4 * phases : 4;
+    for (int i = 0; i < steps; ++i) hipLaunchKernelGGL(k_draw_step<T>, wide, dim3(DRAW_THREADS), 0, st, a, work);
+    if (phases) hipLaunchKernelGGL(k_draw_rest<T>, one, dim3(DRAW_THREADS), 0, st, a, work);
+    const int64_t tiles = ceil_div(a.cols, TILE);
+    hipLaunchKernelGGL(k_draw_mass<T>, dim3((unsigned)std::min<int64_t>(ceil_div(tiles, DRAW_THREADS / 64), blocks), (unsigned)a.rows), dim3(DRAW_THREADS), 0,
+                       st, a, work);
+    hipLaunchKernelGGL(k_draw_pick<T>, dim3((unsigned)std::min<int64_t>(ceil_div(a.draws, 4), 4096), (unsigned)a.rows), dim3(256), 0, st, a, work);
     return hipGetLastError();
 }
 

@@ -32,13 +32,14 @@ void by_fragments(int f, L&& launch) {
 }
 
 struct ForwardPlan {
-    bool narrow = false, fast = false, pack = false, stream = false;
+    bool narrow = false, fast = false, stream = false;
     int tile = 128;
     int64_t kp = 0, x_bytes = 0, w_bytes = 0;
-    int64_t bytes() const { return pack ? x_bytes + 2 * w_bytes : 0; }
+    int64_t bytes() const { return fast ? x_bytes + 2 * w_bytes : 0; }
 };
-// The loads straight into LDS need whole steps and 16-byte rows.  A contraction that is no whole number of steps is packed into the
-// workspace first, which pays from some 2 GFLOP on; below, and for few tiles, the any-shape kernel starts sooner.
+// The loads straight into LDS need whole steps and 16-byte rows.  What has neither is packed into the workspace first, which pays from
+// some 2 GFLOP on (8192 x 2048 -> 4096 bf16 on rows that start anywhere: 653 us with the any-shape kernel, 295 packed, 265 where they do not need it);
+// below, and for few tiles, the any-shape kernel starts sooner.
 template <typename T>
 ForwardPlan forward_plan(int64_t m, int64_t k, int64_t h) {
     constexpr int KS = STEP_BYTES / sizeof(T);
@@ -50,7 +51,6 @@ ForwardPlan forward_plan(int64_t m, int64_t k, int64_t h) {
     // at least two tiles of rows for every workgroup of the streaming form
     p.stream = sizeof(T) == 2 && p.kp <= STREAM_MOST && m * h >= (int64_t)1 << 21 && ceil_div(m, STREAM_ROWS) * ceil_div(h, 256) >= 512;
     p.fast = p.fast || p.stream;
-    p.pack = p.fast && k % KS != 0;
     if (ceil_div(m, 256) * ceil_div(h, 128) >= 256 && k >= 8 * KS) p.tile = 256;
     p.x_bytes = round_up(m * p.kp * (int64_t)sizeof(T), 256);
     p.w_bytes = round_up(h * p.kp * (int64_t)sizeof(T), 256);
@@ -99,8 +99,8 @@ hipError_t gated_forward(hipStream_t st, GatedArgs g, char* work) {
     const bool direct = aligned16(g.a[0].p, g.a[0].sr, sizeof(T)) && aligned16(g.b[0].p, g.b[0].sr, sizeof(T)) && aligned16(g.b[1].p, g.b[1].sr, sizeof(T));
     if (p.narrow && std::max(g.a[0].sr, g.b[0].sr) < NARROW_STRIDE) {
         launch_narrow(st, g);
-    } else if (p.fast && (p.pack || direct)) {
-        if (p.pack) {
+    } else if (p.fast) {
+        if (!direct || g.k % KS != 0) {
             PackArgs a{};
             a.count = 3;
             a.job[0] = {g.a[0].p, g.a[0].sr, g.m, g.k, work, p.kp, ceil_div(g.m, 64) * ceil_div(p.kp, 64)};

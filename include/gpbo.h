@@ -406,7 +406,7 @@ int gpbo_gated_backward(int32_t device, void* stream, int32_t dtype, int32_t act
  * in a row without a valid score; logp_out (rows, draws) float64 = log(w_i / Z), may be NULL, -inf where the index is -1.
  * temperature = 0: the best score, lowest index, logp 0.  params (rows, 4) float64 {temperature, top_k, top_p, min_p} gives
  * every row settings of its own (the scalars are then not read; numbers out of range count as the nearest end), or is NULL.
- * cols may be up to 2^28 (268,435,456) as for gpbo_acquire_static. */
+ * cols may be up to 2^28 (268,435,456) as for gpbo_acquire_static, with at most 65,535 rows beyond 2^22. */
 int64_t gpbo_draw_static_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_t draws);
 int gpbo_draw_static(int32_t device, void* stream, int32_t dtype, const void* scores, int64_t score_stride, int64_t rows,
                      int64_t cols, const double* u, int64_t draws, double temperature, int64_t top_k, double top_p, double min_p,

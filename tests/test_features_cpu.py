@@ -84,6 +84,8 @@ def test_workspace_sizes_of_bad_arguments_are_negative(lib):
     assert lib.gpbo_gated_backward_workspace(L.TYPE_F32, 4, 8, 0) == -1
     assert lib.gpbo_draw_static_workspace(7, 1, 8, 1) == -1
     assert lib.gpbo_draw_static_workspace(L.TYPE_F64, 1, (1 << 28) + 1, 1) == -1
+    assert lib.gpbo_draw_static_workspace(L.TYPE_F16, 65536, (1 << 22) + 1, 1) == -1
+    assert lib.gpbo_draw_static_workspace(L.TYPE_F16, 65535, (1 << 22) + 1, 1) > 0
 
 
 def test_nothing_to_do_launches_nothing(lib):
