@@ -40,36 +40,36 @@ __device__ __forceinline__ f32x4 mma<float>(const uint4& a, const uint4& b, f32x
     return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.w), __uint_as_float(b.w), c, 0, 0, 0);
 }
 
-// act(g) and act'(g).  silu through the logistic function, whose exponential saturates to 0 or infinity with the right limit;
-// gelu through erfc, which keeps the far negative tail that 1 + erf loses.  For results of 16 bits the hardware's exponential and
-// reciprocal (one unit in the last place each) and, for erfc, the five-term rational form of Abramowitz and Stegun 7.1.26 (1.5e-7):
-// the activation of every output is as much vector work as a short contraction is matrix work (1 M x 256 -> 512, with tiles: 1.27 -> 0.83 ms).
+// act(g) and act'(g), with the hardware's exponential and reciprocal (one unit in the last place each).  silu through the logistic
+// function, whose exponential saturates to 0 or infinity with the right limit; gelu through q = Phi(-|g|) = 1/2 erfc(|g| / sqrt 2) = exp(-g^2 / 2)
+// t R(t), t = 1 / (1 + c |g|), which keeps the far negative tail that 1 + erf loses: for results of 16 bits the five terms of Abramowitz and Stegun
+// 7.1.26 (1.5e-7 in erf), for 32 bits ten (a least-squares fit, reweighted to even out its relative error, of erfcx(z) / t with c = 0.45 / sqrt 2:
+// 3.2e-8, half a rounding).  With all roundings a result is within 3 units of 2^-24 (1 + |g|) min(|g|, 1).  The activation of every output is as much
+// vector work as a short contraction is matrix work (1 M x 256 -> 512 in 16 bits, with tiles: 1.27 -> 0.83 ms against expf and erfcf).
 template <typename T>
 __device__ __forceinline__ void activation(float g, int act, float& a, float& da) {
-    if constexpr (sizeof(T) == 4) {
-        if (act == GPBO_ACT_SILU) {
-            const float s = 1.0f / (1.0f + expf(-g));
-            a = g * s;
-            da = s + a * (1.0f - s);
-        } else {
-            const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
-            a = g * cdf;
-            da = cdf + g * (0.39894228040143268f * expf(-0.5f * g * g));
-        }
-    } else {
-        if (act == GPBO_ACT_SILU) {
-            const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * g));
-            a = g * s;
-            da = s + a * (1.0f - s);
-        } else {
-            const float e = __builtin_amdgcn_exp2f(-0.72134752044448170f * g * g);      // exp(-g^2 / 2)
-            const float t = __builtin_amdgcn_rcpf(1.0f + (0.3275911f * 0.70710678118654752f) * fabsf(g));
-            const float q = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-            const float cdf = g < 0.0f ? q : 1.0f - q;
-            a = g * cdf;
-            da = cdf + 0.39894228040143268f * g * e;
-        }
+    if (act == GPBO_ACT_SILU) {
+        const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * g));
+        a = g * s;
+        da = s + a * (1.0f - s);
+        return;
     }
+    constexpr bool WIDE = sizeof(T) == 4;
+    const float e = __builtin_amdgcn_exp2f(-0.72134752044448170f * g * g);      // exp(-g^2 / 2)
+    const float t = __builtin_amdgcn_rcpf(1.0f + ((WIDE ? 0.45f : 0.3275911f) * 0.70710678118654752f) * fabsf(g));
+    float r;
+    if constexpr (WIDE) {
+        constexpr float R[10] = {0.253885329f, 0.253883153f, 0.228271648f, 0.175252140f, 0.119950369f, -0.0223577060f, 0.142400503f, -0.300581962f, 0.190687597f, -0.0413910411f};
+        r = R[9];
+#pragma unroll
+        for (int i = 8; i >= 0; --i) r = fmaf(r, t, R[i]);
+    } else {
+        r = 0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)));
+    }
+    const float q = 0.5f * e * t * r;
+    const float cdf = g < 0.0f ? q : 1.0f - q;
+    a = g * cdf;
+    da = cdf + 0.39894228040143268f * g * e;
 }
 template <typename T>
 __device__ __forceinline__ float activate(float g, int act) {
