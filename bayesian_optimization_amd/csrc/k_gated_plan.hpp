@@ -1,7 +1,7 @@
 // Which kernels a call of the gated unit takes, and its workspace.
 #pragma once
 
-#include "k_gated_narrow.hpp"
+#include "k_gated_short.hpp"
 #include "k_gated_fast.hpp"
 
 namespace gpbo_static {
@@ -128,7 +128,7 @@ hipError_t gated_forward(hipStream_t st, GatedArgs g, char* work) {
 // Backward.  Large: dg and du are written both ways round, x and the weights transposed, so that every product contracts along
 // rows; these copies are a few per cent of the products' time.
 struct BackwardPlan {
-    bool fast = false, one = false, narrow = false;      // one: k_gated_small_back
+    bool fast = false, one = false, narrow = false, few_cols = false;      // one: k_gated_small_back
     int tile_x = 128, tile_w = 128, splits_x = 1, splits_w = 1;
     AnyPlan any_x, any_w;
     int64_t hp = 0, mp = 0;
@@ -149,6 +149,13 @@ BackwardPlan backward_plan(int64_t m, int64_t k, int64_t h) {
         p.splits_narrow = (int)std::max<int64_t>(1, std::min<int64_t>((f == 1 ? 1024 : f <= 3 ? 768 : 512) / ceil_div(k, 64), m / 512));
         p.narrow_d_bytes = round_up(m * 16 * f * 4, 256);
         p.narrow_bytes = p.narrow_d_bytes + (p.splits_narrow > 1 ? 2 * p.splits_narrow * h * k * 4 : 0);
+    }
+    // few columns: worth it from four million hidden outputs on (50000 x 16 -> 256: 290 us with the forward pass, 163 here; 8000 x 16 -> 256: 50 and 55)
+    p.few_cols = sizeof(T) == 4 && k <= SHORT_COLS && h > NARROW_HIDDEN && m >= 4096 && m * h >= (int64_t)1 << 22;
+    if (p.few_cols) {
+        p.splits_w = (int)std::max<int64_t>(1, std::min<int64_t>(512 / ceil_div(h, 64), m / 512));
+        p.part_bytes = p.splits_w > 1 ? 2 * p.splits_w * h * k * 4 : 0;
+        return p;
     }
     // 4 GFLOP, or two million elements over many rows: below, the copies cost more than they save
     p.fast = !p.narrow && m >= 128 && (8 * m * h * k >= (int64_t)1 << 32 || (m >= 4096 && std::max(h, k) >= 128 && m * std::max(h, k) >= (int64_t)1 << 21)) && m * B < (1 << 23) && h * B < (1 << 23);
@@ -212,6 +219,31 @@ hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const voi
         if (tiles > 0)
             hipLaunchKernelGGL(k_gated_small_back<T>, dim3((unsigned)tiles), dim3(64 * SMALL_WAVES), 0, st, SlopeOperand{dh, kg, ku, dhs, h, act},
                                Operand{x, 1, xs}, Operand{wg, 1, ws}, Operand{wu, 1, ws}, m, k, h, dx, dxs, dwg, dwu, dws);
+        return hipGetLastError();
+    }
+    if (p.few_cols) {
+        ShortBack g{};
+        g.dh = (const float*)dh, g.kg = kg, g.ku = ku, g.x = (const float*)x, g.w[0] = (const float*)wg, g.w[1] = (const float*)wu;
+        g.dhs = dhs, g.xs = xs, g.ws = ws, g.m = m, g.k = k, g.h = h, g.act = act;
+        auto by_columns = [&](auto&& launch) {
+            if (k <= 16) launch(std::integral_constant<int, 1>{});
+            else if (k <= 32) launch(std::integral_constant<int, 2>{});
+            else if (k <= 48) launch(std::integral_constant<int, 3>{});
+            else launch(std::integral_constant<int, 4>{});
+        };
+        if (dx) {
+            g.out[0] = (float*)dx, g.os = dxs;
+            by_columns([&](auto c) { hipLaunchKernelGGL(k_gated_short_dx<c.value>, dim3((unsigned)ceil_div(m, c.value <= 3 ? 32 : 16)), dim3(256), 0, st, g); });
+        }
+        if (dwg) {
+            g.out[0] = (float*)dwg, g.out[1] = (float*)dwu, g.os = dws, g.splits = p.splits_w, g.part = (float*)work;
+            by_columns([&](auto c) {
+                hipLaunchKernelGGL(k_gated_short_dw<c.value>, dim3((unsigned)ceil_div(h, 64), (unsigned)g.splits), dim3(256), 0, st, g);
+            });
+            GatedArgs j{};
+            j.m = h, j.n = k, j.out[0] = dwg, j.out[1] = dwu, j.os = dws, j.splits = g.splits, j.part = g.part;
+            if (j.splits > 1) hipLaunchKernelGGL(k_gated_join<T>, dim3((unsigned)ceil_div(h * k, 256), 2), dim3(256), 0, st, j);
+        }
         return hipGetLastError();
     }
     char* at = work;

@@ -196,6 +196,40 @@ def test_gated_unit_many_rows_few_hidden_units(act, rows, cols, hidden):
     check_gated(torch.float32, act, rows, cols, hidden)
 
 
+# many rows, few columns, many hidden units: every number of column fragments, whole and broken slabs on both sides
+@pytest.mark.parametrize('rows,cols,hidden', [(4096, 1, 1025), (4099, 3, 1040), (5001, 16, 1000), (50007, 15, 129), (20011, 17, 300), (9999, 32, 640), (33001, 33, 200),
+                                              (33009, 48, 144), (16501, 49, 333), (40001, 64, 131), (65536, 4, 65)])
+@pytest.mark.parametrize('act', ['silu', 'gelu'])
+def test_gated_unit_few_columns(act, rows, cols, hidden):
+    check_gated(torch.float32, act, rows, cols, hidden)
+
+
+def test_gated_unit_few_columns_strides_infinities_and_parts():
+    from bayesian_optimization_amd import features
+    rows, cols, hidden = 20005, 19, 213
+    x = rand((rows, cols + 9), torch.float32, 85)[:, 3:3 + cols]
+    wg, wu = (rand((hidden, cols + 5), torch.float32, s, 0.2)[:, 1:1 + cols] for s in (86, 87))
+    dh = rand((rows, hidden + 2), torch.float32, 88)[:, 1:1 + hidden]
+    near = [v.contiguous() for v in (x, wg, wu)]
+    _, kept = features.gated_unit(*near, keep=True)
+    full = features.gated_unit_backward(dh.contiguous(), *near, kept)
+    assert all(torch.equal(a, b) for a, b in zip(features.gated_unit_backward(dh, x, wg, wu, kept), full))
+    part = features.gated_unit_backward(dh, *near, kept, need_dw=False)
+    assert torch.equal(part[0], full[0]) and part[1] is None and part[2] is None
+    part = features.gated_unit_backward(dh, *near, kept, need_dx=False)
+    assert part[0] is None and torch.equal(part[1], full[1]) and torch.equal(part[2], full[2])
+    x, wg, wu = near
+    a = gated_ref(x, wg, wu, 'silu')[2]
+    wu[hidden - 1, 18] = float('inf')      # the last weight of all: nothing but its own column
+    dx, _, _ = features.gated_unit_backward(torch.ones_like(kept[0]), x, wg, wu, kept)
+    assert bool((dx[:, 18] == torch.where(a[:, -1] > 0, float('inf'), -float('inf'))).all()) and bool(torch.isfinite(dx[:, :18]).all())
+    bad = dh.contiguous()
+    bad[77, 5] = float('nan')
+    dx, dwg, dwu = features.gated_unit_backward(bad, *[v.contiguous() for v in (x, wg, near[2].nan_to_num(posinf=0.5))], kept)
+    assert bool(torch.isnan(dx[77]).all()) and bool(torch.isfinite(dx[:77]).all()) and bool(torch.isfinite(dx[78:]).all())
+    assert bool(torch.isnan(dwg[5]).all()) and int(torch.isnan(dwg).sum()) == cols and int(torch.isnan(dwu).sum()) == cols
+
+
 def test_gated_unit_many_rows_strides_infinities_and_parts():
     from bayesian_optimization_amd import features
     rows, cols, hidden = 16390, 70, 5
