@@ -110,7 +110,7 @@ hipError_t gated_forward(hipStream_t st, GatedArgs g, char* work) {
             g.a[0] = {a.job[0].dst, p.kp, 1}, g.b[0] = {a.job[1].dst, p.kp, 1}, g.b[1] = {a.job[2].dst, p.kp, 1};
             g.k = p.kp;
         }
-        static_assert(KS >= 32, "a step");
+        
         if (p.stream) launch_stream<T>(st, g);
         else launch_fast<T, GATED_FWD>(st, g, p.tile);
     } else if (g.m <= 16) {
@@ -171,8 +171,10 @@ BackwardPlan backward_plan(int64_t m, int64_t k, int64_t h) {
         p.d_bytes = round_up(m * p.hp * B, 256), p.dt_bytes = round_up(h * p.mp * B, 256);
         p.xt_bytes = round_up(k * p.mp * B, 256), p.wt_bytes = round_up(k * p.hp * B, 256);
     } else {
-        // one launch while all tiles together work out dg and du no more than a million times, and a tile's waves have few slabs
-        p.one = m > 0 && 4 * m * h * ceil_div(k, SB) <= (int64_t)1 << 20 && std::max(m, 2 * h) <= 64 * KS;
+        // one launch while all tiles together work out dg and du no more than a million times, and a tile's waves have few slabs: with the
+        // forward pass 22 us against 30 with three launches (95 x 621 -> 128, 400 x 30 -> 24), even at 512 rows or 256 hidden units
+        // (27 to 29 and 30), worse from there on (1000 x 30 -> 24: 44, 20 x 30 -> 1000: 60)
+        p.one = m > 0 && 4 * m * h * ceil_div(k, SB) <= (int64_t)1 << 20 && std::max(m, 2 * h) <= 512;
         if (p.one) return p;
         p.d_bytes = round_up(m * h * B, 256);
         p.any_x = any_plan<T>(m, k, h, 1, true), p.any_w = any_plan<T>(h, k, m, 2, true);
