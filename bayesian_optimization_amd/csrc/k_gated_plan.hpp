@@ -31,6 +31,13 @@ void by_fragments(int f, L&& launch) {
     }
 }
 
+// Tiles of 256 x 256, one a CU at a time, or of 128 x 128, two a CU: by the rounds that the card takes over them.  A round of the large ones is
+// as much work as two of the small ones, which take an eighth longer over it (float32, 25000 x 640 -> 382, 294 tiles or 1176: 311 us with the
+// large ones, 201 with the small; 50000 x 640 -> 146: 311 and 200; 16384 x 2048 -> 8192, 16 full rounds: 1.27 and 1.44 ms in bf16).
+inline int better_tile(int64_t t256, int64_t t128) {
+    return t256 >= 256 && 32 * ceil_div(t256, 256) <= 18 * ceil_div(t128, 512) ? 256 : 128;
+}
+
 struct ForwardPlan {
     bool narrow = false, fast = false, stream = false;
     int tile = 128;
@@ -51,7 +58,7 @@ ForwardPlan forward_plan(int64_t m, int64_t k, int64_t h) {
     // at least two tiles of rows for every workgroup of the streaming form
     p.stream = sizeof(T) == 2 && p.kp <= STREAM_MOST && m * h >= (int64_t)1 << 21 && ceil_div(m, STREAM_ROWS) * ceil_div(h, 256) >= 512;
     p.fast = p.fast || p.stream;
-    if (ceil_div(m, 256) * ceil_div(h, 128) >= 256 && k >= 8 * KS) p.tile = 256;
+    if (k >= 8 * KS) p.tile = better_tile(ceil_div(m, 256) * ceil_div(h, 128), ceil_div(m, 128) * ceil_div(h, 64));
     p.x_bytes = round_up(m * p.kp * (int64_t)sizeof(T), 256);
     p.w_bytes = round_up(h * p.kp * (int64_t)sizeof(T), 256);
     return p;
@@ -110,7 +117,6 @@ hipError_t gated_forward(hipStream_t st, GatedArgs g, char* work) {
             g.a[0] = {a.job[0].dst, p.kp, 1}, g.b[0] = {a.job[1].dst, p.kp, 1}, g.b[1] = {a.job[2].dst, p.kp, 1};
             g.k = p.kp;
         }
-        
         if (p.stream) launch_stream<T>(st, g);
         else launch_fast<T, GATED_FWD>(st, g, p.tile);
     } else if (g.m <= 16) {
@@ -163,7 +169,7 @@ BackwardPlan backward_plan(int64_t m, int64_t k, int64_t h) {
         p.hp = round_up(h, 64), p.mp = round_up(m, 64);
         auto choose = [&](int64_t rows, int64_t cols, int64_t zs, int64_t steps, int& tile, int& splits) {
             const int64_t t256 = zs * ceil_div(rows, 256) * ceil_div(cols, 256), t128 = zs * ceil_div(rows, 128) * ceil_div(cols, 128);
-            tile = t256 >= 256 ? 256 : 128;
+            tile = better_tile(t256, t128);
             splits = tile == 256 || t128 >= 256 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(512, t128), steps / 8));
         };
         choose(m, k, 1, p.hp / KS, p.tile_x, p.splits_x);
