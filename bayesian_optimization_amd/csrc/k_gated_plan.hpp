@@ -163,14 +163,17 @@ BackwardPlan backward_plan(int64_t m, int64_t k, int64_t h) {
         p.part_bytes = p.splits_w > 1 ? 2 * p.splits_w * h * k * 4 : 0;
         return p;
     }
-    // 4 GFLOP, or two million elements over many rows: below, the copies cost more than they save
-    p.fast = !p.narrow && m >= 128 && (8 * m * h * k >= (int64_t)1 << 32 || (m >= 4096 && std::max(h, k) >= 128 && m * std::max(h, k) >= (int64_t)1 << 21)) && m * B < (1 << 23) && h * B < (1 << 23);
+    // Below these the copies cost more than they save: 4 GFLOP in 32 bits (2000 x 520 -> 200, 1.7: 83 us with the forward pass, 125 with them), in 16
+    // bits 1.9 (1000 x 520 -> 1000, 4.2: 98 without, 66 with; 1000 x 520 -> 400, 1.7: 44 and 57) or, over many rows, 1 (2000 x 520 -> 200: 59
+    // and 53); or two million elements over many rows.
+    const int64_t enough = B == 4 ? (int64_t)1 << 32 : m >= 2000 ? (int64_t)1 << 30 : (int64_t)7 << 28;
+    p.fast = !p.narrow && m >= 128 && (8 * m * h * k >= enough || (m >= 4096 && std::max(h, k) >= 128 && m * std::max(h, k) >= (int64_t)1 << 21)) && m * B < (1 << 23) && h * B < (1 << 23);
     if (p.fast) {
         p.hp = round_up(h, 64), p.mp = round_up(m, 64);
         auto choose = [&](int64_t rows, int64_t cols, int64_t zs, int64_t steps, int& tile, int& splits) {
             const int64_t t256 = zs * ceil_div(rows, 256) * ceil_div(cols, 256), t128 = zs * ceil_div(rows, 128) * ceil_div(cols, 128);
             tile = better_tile(t256, t128);
-            splits = tile == 256 || t128 >= 256 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(512, t128), steps / 8));
+            splits = tile == 256 || t128 >= 256 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(512 / t128, steps / 8));
         };
         choose(m, k, 1, p.hp / KS, p.tile_x, p.splits_x);
         choose(h, k, 2, p.mp / KS, p.tile_w, p.splits_w);
