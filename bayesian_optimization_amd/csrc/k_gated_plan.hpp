@@ -156,8 +156,10 @@ BackwardPlan backward_plan(int64_t m, int64_t k, int64_t h) {
         p.narrow_d_bytes = round_up(m * 16 * f * 4, 256);
         p.narrow_bytes = p.narrow_d_bytes + (p.splits_narrow > 1 ? 2 * p.splits_narrow * h * k * 4 : 0);
     }
-    // few columns: worth it from four million hidden outputs on (50000 x 16 -> 256: 290 us with the forward pass, 163 here; 8000 x 16 -> 256: 50 and 55)
-    p.few_cols = sizeof(T) == 4 && k <= SHORT_COLS && h > NARROW_HIDDEN && m >= 4096 && m * h >= (int64_t)1 << 22;
+    // few columns: worth it from four million hidden outputs on (50000 x 16 -> 256: 290 us with the forward pass, 163 here; 8000 x 16 -> 256: 50 and 55);
+    // in 16 bits, where the other way has faster products, up to 16 of them and from eight million on (1 M x 4 -> 128: 1055 and 898; 50000 x
+    // 64 -> 256: 120 and 167)
+    p.few_cols = k <= (B == 4 ? SHORT_COLS : 16) && h > NARROW_HIDDEN && m >= 4096 && m * h >= (B == 4 ? (int64_t)1 << 22 : (int64_t)1 << 23);
     if (p.few_cols) {
         p.splits_w = (int)std::max<int64_t>(1, std::min<int64_t>(512 / ceil_div(h, 64), m / 512));
         p.part_bytes = p.splits_w > 1 ? 2 * p.splits_w * h * k * 4 : 0;
@@ -197,6 +199,7 @@ template <typename T>
 hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const void* x, int64_t xs, const void* wg, const void* wu, int64_t ws,
                           const float* kg, const float* ku, int64_t m, int64_t k, int64_t h, int act, void* dx, int64_t dxs, void* dwg,
                           void* dwu, int64_t dws, char* work) {
+    constexpr int64_t B = sizeof(T);
     const BackwardPlan p = backward_plan<T>(m, k, h);
     if (p.narrow && std::max(xs, ws) < NARROW_STRIDE) {
         const int fragments = narrow_fragments(h);
@@ -233,23 +236,25 @@ hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const voi
         return hipGetLastError();
     }
     if (p.few_cols) {
-        ShortBack g{};
-        g.dh = (const float*)dh, g.kg = kg, g.ku = ku, g.x = (const float*)x, g.w[0] = (const float*)wg, g.w[1] = (const float*)wu;
+        ShortBack<T> g{};
+        g.dh = (const T*)dh, g.kg = kg, g.ku = ku, g.x = (const T*)x, g.w[0] = (const T*)wg, g.w[1] = (const T*)wu;
         g.dhs = dhs, g.xs = xs, g.ws = ws, g.m = m, g.k = k, g.h = h, g.act = act;
         auto by_columns = [&](auto&& launch) {
             if (k <= 16) launch(std::integral_constant<int, 1>{});
-            else if (k <= 32) launch(std::integral_constant<int, 2>{});
-            else if (k <= 48) launch(std::integral_constant<int, 3>{});
-            else launch(std::integral_constant<int, 4>{});
+            if constexpr (B == 4) {
+                if (k > 16 && k <= 32) launch(std::integral_constant<int, 2>{});
+                if (k > 32 && k <= 48) launch(std::integral_constant<int, 3>{});
+                if (k > 48) launch(std::integral_constant<int, 4>{});
+            }
         };
         if (dx) {
-            g.out[0] = (float*)dx, g.os = dxs;
-            by_columns([&](auto c) { hipLaunchKernelGGL(k_gated_short_dx<c.value>, dim3((unsigned)ceil_div(m, c.value <= 3 ? 32 : 16)), dim3(256), 0, st, g); });
+            g.out[0] = (T*)dx, g.os = dxs;
+            by_columns([&](auto c) { hipLaunchKernelGGL((k_gated_short_dx<T, c.value>), dim3((unsigned)ceil_div(m, c.value <= 3 ? 32 : 16)), dim3(256), 0, st, g); });
         }
         if (dwg) {
-            g.out[0] = (float*)dwg, g.out[1] = (float*)dwu, g.os = dws, g.splits = p.splits_w, g.part = (float*)work;
+            g.out[0] = (T*)dwg, g.out[1] = (T*)dwu, g.os = dws, g.splits = p.splits_w, g.part = (float*)work;
             by_columns([&](auto c) {
-                hipLaunchKernelGGL(k_gated_short_dw<c.value>, dim3((unsigned)ceil_div(h, 64), (unsigned)g.splits), dim3(256), 0, st, g);
+                hipLaunchKernelGGL((k_gated_short_dw<T, c.value>), dim3((unsigned)ceil_div(h, 64), (unsigned)g.splits), dim3(256), 0, st, g);
             });
             GatedArgs j{};
             j.m = h, j.n = k, j.out[0] = dwg, j.out[1] = dwu, j.os = dws, j.splits = g.splits, j.part = g.part;

@@ -1,7 +1,7 @@
-// Backward pass of the gated unit in 32 bits with many rows, up to 64 columns of x and more hidden units than that (a wide map of a few raw
-// inputs).  Nearly all of the traffic is dh and the kept g and u; the tiles for large operands write dg and du four times over and
+// Backward pass of the gated unit with many rows, up to 64 columns of x (16 bits: 16) and more hidden units than that (a wide map of a few
+// raw inputs).  Nearly all of the traffic is dh and the kept g and u; the tiles for large operands write dg and du four times over and
 // multiply mostly padding.  Here dg and du are worked out on the way into the matrix instructions and never stored: once for dx, once for
-// the weights' gradients, so the three arrays are read twice and nothing else moves (145829 x 30 -> 3235: backward 10.7 -> 3.7 ms, of 2.4 that two
+// the weights' gradients, so the three arrays are read twice and nothing else moves; the products are those of 32 bits for every type (145829 x 30 -> 3235: backward 10.7 -> 3.7 ms, of 2.4 that two
 // passes over them take; 1 M x 4 -> 128: 2.7 -> 1.1 ms).
 #pragma once
 
@@ -11,38 +11,67 @@ namespace gpbo_static {
 
 constexpr int64_t SHORT_COLS = 64;
 
+template <typename T>
 struct ShortBack {
-    const float *dh, *kg, *ku, *x, *w[2];
+    const T *dh, *x, *w[2];
+    const float *kg, *ku;
     int64_t dhs, xs, ws, m, k, h;
     int act;
-    float* out[2];                // dx, or dwg and dwu
+    T* out[2];                    // dx, or dwg and dwu
     int64_t os;
     int splits;
     float* part;                  // [z][split][h][k]
 };
 
+// Four neighbouring numbers as they lie in memory (those from `len` on zero): converted where they are used, so that nothing waits for
+// the load before.
+template <typename T>
+struct Four {
+    T v[4];
+    __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(v, p, sizeof(v)); }
+    __device__ __forceinline__ void load(const T* p, int64_t len) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = i < len ? p[i] : from_float<T>(0.0f);
+    }
+};
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const f32x4& v, int64_t len) {
+    T o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = from_float<T>(v[i]);
+    if (len >= 4) __builtin_memcpy(p, o, sizeof(o));
+    else
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (i < len) p[i] = o[i];
+}
+
 // dg and du of four neighbours.
-__device__ __forceinline__ void slopes4(const f32x4& dh, const f32x4& g, const f32x4& u, int act, f32x4& dg, f32x4& du) {
+template <typename T>
+__device__ __forceinline__ void slopes4(const Four<T>& dh, const f32x4& g, const f32x4& u, int act, f32x4& dg, f32x4& du) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         float a, da;
-        activation<float>(g[i], act, a, da);
-        dg[i] = dh[i] * u[i] * da, du[i] = dh[i] * a;
+        activation<T>(g[i], act, a, da);
+        const float d = to_float(dh.v[i]);
+        dg[i] = d * u[i] * da, du[i] = d * a;
     }
 }
 
 // dx = dg wg + du wu: a workgroup has 16 RF rows and all columns, in CF fragments of 16; its waves take slabs of 16 hidden units in turn and
 // join their sums through LDS in a fixed order.
-template <int CF>
-__global__ __launch_bounds__(256, 2) void k_gated_short_dx(ShortBack g) {
+template <typename T, int CF>
+__global__ __launch_bounds__(256, 2) void k_gated_short_dx(ShortBack<T> g) {
     constexpr int RF = CF <= 3 ? 2 : 1;          // (what two slabs leave of the registers)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, q = lane >> 4;
     const int64_t row0 = (int64_t)blockIdx.x * (16 * RF);
     struct Slab {
-        f32x4 dh[RF], g[RF], u[RF];
-        float w[2][4][CF];
+        Four<T> dh[RF];
+        f32x4 g[RF], u[RF];
+        T w[2][4][CF];
     };
-    const float *pd[RF], *pg[RF], *pu[RF];       // rows behind the last repeat it: not stored
+    const T* pd[RF];
+    const float *pg[RF], *pu[RF];                // rows behind the last repeat it: not stored
 #pragma unroll
     for (int i = 0; i < RF; ++i) {
         const int64_t r = min(row0 + i * 16 + r16, g.m - 1);
@@ -55,7 +84,7 @@ __global__ __launch_bounds__(256, 2) void k_gated_short_dx(ShortBack g) {
     auto load = [&](Slab& s, int64_t t) {
 #pragma unroll
         for (int i = 0; i < RF; ++i) {
-            __builtin_memcpy(&s.dh[i], pd[i] + t * 16, 16);
+            s.dh[i].load(pd[i] + t * 16);
             __builtin_memcpy(&s.g[i], pg[i] + t * 16, 16);
             __builtin_memcpy(&s.u[i], pu[i] + t * 16, 16);
         }
@@ -76,7 +105,7 @@ __global__ __launch_bounds__(256, 2) void k_gated_short_dx(ShortBack g) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
 #pragma unroll
-                    for (int j = 0; j < CF; ++j) acc[i][j] = mma4(s.w[z][e][j], d[z][e], acc[i][j]);
+                    for (int j = 0; j < CF; ++j) acc[i][j] = mma4(to_float(s.w[z][e][j]), d[z][e], acc[i][j]);
         }
     };
     const int64_t whole = g.h / 16;
@@ -85,13 +114,16 @@ __global__ __launch_bounds__(256, 2) void k_gated_short_dx(ShortBack g) {
         Slab s;
         const int64_t len = g.h - whole * 16 - q * 4;
 #pragma unroll
-        for (int i = 0; i < RF; ++i) s.dh[i] = load4(pd[i] + whole * 16, len), s.g[i] = load4(pg[i] + whole * 16, len), s.u[i] = load4(pu[i] + whole * 16, len);
+        for (int i = 0; i < RF; ++i) {
+            s.dh[i].load(pd[i] + whole * 16, len);
+            s.g[i] = load4(pg[i] + whole * 16, len), s.u[i] = load4(pu[i] + whole * 16, len);
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
             for (int j = 0; j < CF; ++j) {
                 const int64_t at = (whole * 16 + q * 4 + e) * g.ws + col[j];
-                s.w[0][e][j] = e < len ? g.w[0][at] : 0.0f, s.w[1][e][j] = e < len ? g.w[1][at] : 0.0f;
+                s.w[0][e][j] = e < len ? g.w[0][at] : from_float<T>(0.0f), s.w[1][e][j] = e < len ? g.w[1][at] : from_float<T>(0.0f);
             }
         multiply(s);
     }
@@ -119,45 +151,40 @@ __global__ __launch_bounds__(256, 2) void k_gated_short_dx(ShortBack g) {
 #pragma unroll
         for (int j = 0; j < CF; ++j) {
             const int64_t c = j * 16 + q * 4;
-            float* p = g.out[0] + row * g.os + c;
-            if (c + 4 <= g.k) __builtin_memcpy(p, &acc[i][j], 16);
-            else
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (c + r < g.k) p[r] = acc[i][j][r];
+            store4(g.out[0] + row * g.os + c, acc[i][j], g.k - c);
         }
     }
 }
 
 // dwg = dg^T x, dwu = du^T x: a workgroup has 64 hidden units (the last ones end with the row and may repeat some) and a piece of the rows, whose
 // slabs of 4 E rows its waves take in turn.  A lane has four neighbouring hidden units of a row, one for each of four fragments.
-template <int CF>
-__global__ __launch_bounds__(256, 2) void k_gated_short_dw(ShortBack g) {
+template <typename T, int CF>
+__global__ __launch_bounds__(256, 2) void k_gated_short_dw(ShortBack<T> g) {
     constexpr int E = CF <= 2 ? 4 : 2;           // what two slabs and the sums leave of the registers
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, q = lane >> 4;
     const int64_t h0 = min((int64_t)blockIdx.x * 64, g.h - 64);
     const int64_t slabs = (g.m + 4 * E - 1) / (4 * E), per = (slabs + g.splits - 1) / g.splits;
     const int64_t sb = min((int64_t)blockIdx.y * per, slabs), se = min(sb + per, slabs);
     struct Slab {
-        f32x4 dh[E], g[E], u[E];
-        float x[E][CF];
+        Four<T> dh[E];
+        f32x4 g[E], u[E];
+        T x[E][CF];
     };
     int col[CF];
 #pragma unroll
     for (int j = 0; j < CF; ++j) col[j] = min(j * 16 + r16, (int)g.k - 1);
     f32x4 acc[2][4][CF] = {};
-    auto load_rows = [&](Slab& s, int64_t t, int64_t last) {
+    auto load = [&](Slab& s, int64_t t) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int64_t r = min(t * 4 * E + e * 4 + q, last), at = r * g.h + h0 + r16 * 4;
-            __builtin_memcpy(&s.dh[e], g.dh + r * g.dhs + h0 + r16 * 4, 16);
+            const int64_t r = min(t * 4 * E + e * 4 + q, g.m - 1), at = r * g.h + h0 + r16 * 4;
+            s.dh[e].load(g.dh + r * g.dhs + h0 + r16 * 4);
             __builtin_memcpy(&s.g[e], g.kg + at, 16);
             __builtin_memcpy(&s.u[e], g.ku + at, 16);
 #pragma unroll
             for (int j = 0; j < CF; ++j) s.x[e][j] = g.x[r * g.xs + col[j]];
         }
     };
-    auto load = [&](Slab& s, int64_t t) { load_rows(s, t, g.m - 1); };
     auto multiply = [&](const Slab& s) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -168,7 +195,7 @@ __global__ __launch_bounds__(256, 2) void k_gated_short_dw(ShortBack g) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < CF; ++j) acc[z][i][j] = mma4(s.x[e][j], d[z][i], acc[z][i][j]);
+                    for (int j = 0; j < CF; ++j) acc[z][i][j] = mma4(to_float(s.x[e][j]), d[z][i], acc[z][i][j]);
         }
     };
     const int64_t whole = max(sb, min(se, g.m / (4 * E)));
@@ -179,9 +206,10 @@ __global__ __launch_bounds__(256, 2) void k_gated_short_dw(ShortBack g) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
             if (whole * 4 * E + e * 4 + q >= g.m) {
-                s.dh[e] = s.g[e] = s.u[e] = f32x4{};
+                s.dh[e].load(g.dh, 0);
+                s.g[e] = s.u[e] = f32x4{};
 #pragma unroll
-                for (int j = 0; j < CF; ++j) s.x[e][j] = 0.0f;
+                for (int j = 0; j < CF; ++j) s.x[e][j] = from_float<T>(0.0f);
             }
         multiply(s);
     }
@@ -205,15 +233,13 @@ __global__ __launch_bounds__(256, 2) void k_gated_short_dw(ShortBack g) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int64_t row = h0 + r16 * 4 + (i & 3), z = i >> 2;
-        float* p = g.splits > 1 ? g.part + ((z * g.splits + blockIdx.y) * g.h + row) * g.k : (z ? g.out[1] : g.out[0]) + row * g.os;
+        float* const part = g.part + ((z * g.splits + blockIdx.y) * g.h + row) * g.k;
+        T* const out = (z ? g.out[1] : g.out[0]) + row * g.os;
 #pragma unroll
         for (int j = 0; j < CF; ++j) {
             const int64_t c = j * 16 + q * 4;
-            if (c + 4 <= g.k) __builtin_memcpy(p + c, &acc[i >> 2][i & 3][j], 16);
-            else
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (c + r < g.k) p[c + r] = acc[i >> 2][i & 3][j][r];
+            if (g.splits > 1) store4(part + c, acc[i >> 2][i & 3][j], g.k - c);
+            else store4(out + c, acc[i >> 2][i & 3][j], g.k - c);
         }
     }
 }

@@ -198,10 +198,11 @@ def test_gated_unit_many_rows_few_hidden_units(act, rows, cols, hidden):
 
 # many rows, few columns, many hidden units: every number of column fragments, whole and broken slabs on both sides
 @pytest.mark.parametrize('rows,cols,hidden', [(4096, 1, 1025), (4099, 3, 1040), (5001, 16, 1000), (50007, 15, 129), (20011, 17, 300), (9999, 32, 640), (33001, 33, 200),
-                                              (33009, 48, 144), (16501, 49, 333), (40001, 64, 131), (65536, 4, 65)])
+                                              (33009, 48, 144), (16501, 49, 333), (40001, 64, 131), (65536, 4, 65), (131073, 7, 65), (8197, 16, 1100)])
 @pytest.mark.parametrize('act', ['silu', 'gelu'])
-def test_gated_unit_few_columns(act, rows, cols, hidden):
-    check_gated(torch.float32, act, rows, cols, hidden)
+@pytest.mark.parametrize('dtype', TYPES)
+def test_gated_unit_few_columns(dtype, act, rows, cols, hidden):
+    check_gated(dtype, act, rows, cols, hidden)
 
 
 def test_gated_unit_few_columns_strides_infinities_and_parts():
