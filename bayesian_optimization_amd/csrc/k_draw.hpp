@@ -446,10 +446,12 @@ __device__ void draw_decide(DrawLds<T>& s, const DrawRow& p) {
         if (first) goal = p.top_p * (all_m + st.floor_mass);
         spare = first && !(all_m >= goal);                                     // all above the group of the top-k cut is kept
         // the first bin with which the running mass reaches the goal; the last one in use if rounding leaves none
-        if (c1 && above + run_m >= goal) atomicMin(&s.bin, (unsigned)b1);
-        if (c0 && above + (run_m - m1) >= goal) atomicMin(&s.bin, (unsigned)b0);
-        if (c1) atomicMax(&s.any_bin, (unsigned)b1);
-        else if (c0) atomicMax(&s.any_bin, (unsigned)b0);
+        // (one lane a wave asks: a thousand atomics on one address took 8 us)
+        const bool reach0 = c0 && above + (run_m - m1) >= goal, reach1 = c1 && above + run_m >= goal;
+        const unsigned long long reach = __ballot(reach0 || reach1), any = __ballot(c0 || c1);
+        const int lane = tid & 63;
+        if (reach && lane == __ffsll(reach) - 1) atomicMin(&s.bin, (unsigned)(reach0 ? b0 : b1));
+        if (any && lane == 63 - __clzll((long long)any)) atomicMax(&s.any_bin, (unsigned)(c1 ? b1 : b0));
     }
     __syncthreads();
     const unsigned bin = s.bin != 0xffffffffu ? s.bin : s.any_bin;
