@@ -4,8 +4,11 @@
 // Four products' worth of matrix work forward (two projections), eight back.  Both projections of a tile are formed by the
 // same workgroup from one staged tile of x, so the activation and the product are an epilogue on the accumulators and g, u
 // never go to memory unless the caller keeps them for the backward pass.  Sums are held in 32 bits, and so are the kept g and
-// u: rounded to 16 bits they would put two more roundings of the same size under every gradient.  h is rounded once, and dg and
-// du once each, to the type of x: they are operands of the matrix instructions.
+// u: rounded to 16 bits they would put two more roundings of the same size under every gradient.  h is rounded once.  dg and du are
+// operands of the matrix instructions, so of the type of x, rounded once each: in 16 bits, over a gradient's many elements, the error is
+// then 1.4 times that of the gradient's own rounding.  Over few elements, where terms may cancel in all of them, it can be several times
+// (3 with 10 in float16), so that there, and where it costs nothing, the products take a sum of two numbers of 16 bits: the rounded one
+// and what the rounding left.  (The whole-step kernels, whose gradients have 128 elements or more, take one.)
 #pragma once
 
 #include <type_traits>
@@ -89,7 +92,7 @@ constexpr int GATED_SUM = 1;      // a[0] b[0] + a[1] b[1]
 constexpr int GATED_PAIR = 2;     // a[z] b[0] to out[z], z = 0, 1
 
 struct GatedArgs {
-    Operand a[2], b[2];
+    Operand a[2], b[2], rest[2];  // rest: what the rounding of a[0], a[1] left (where that is an operand of two parts)
     int64_t m, n, k;              // out is (m, n), k the contraction (of each part)
     void* out[2];
     int64_t os;                   // row stride of out
@@ -97,6 +100,20 @@ struct GatedArgs {
     int act, splits;
     float* part;                  // splits > 1: [z][split][m][n] sums in 32 bits
 };
+
+// Numbers of type T that make up one element of dg and du where they are not rounded to one.
+template <typename T>
+constexpr int SLOPE_PARTS = sizeof(T) == 2 ? 2 : 1;
+template <int N>
+struct Parts {
+    uint4 v[N];
+};
+// What the rounding of d to hi left; nothing if hi is beyond the type's range.
+template <typename T>
+__device__ __forceinline__ T rounding_rest(float d, T hi) {
+    const float h = to_float(hi);
+    return from_float<T>(fabsf(h) < INFINITY ? d - h : 0.0f);
+}
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Tile kernel for every shape, stride and alignment: 64 x 64 outputs, 4 waves of 32 x 32, 128 bytes of contraction a step,
@@ -146,10 +163,10 @@ struct TileLoad {
     }
 };
 
-template <typename T, int MODE, bool AKC, bool BKC>
+template <typename T, int MODE, bool AKC, bool BKC, int NA>
 __global__ __launch_bounds__(256) void k_gated_tile(GatedArgs g) {
     constexpr int KS = STEP_BYTES / sizeof(T), NB = MODE == GATED_FWD ? 2 : 1;
-    __shared__ uint4 la[TB * 8], lb[NB][TB * 8];
+    __shared__ uint4 la[NA][TB * 8], lb[NB][TB * 8];
     const int64_t nt = (g.n + TB - 1) / TB;
     const int64_t row0 = (int64_t)(blockIdx.x / nt) * TB, col0 = (int64_t)(blockIdx.x % nt) * TB;
     const int z = MODE == GATED_PAIR ? blockIdx.z : 0, split = blockIdx.y;
@@ -165,30 +182,33 @@ __global__ __launch_bounds__(256) void k_gated_tile(GatedArgs g) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) acc[b][i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const int64_t steps1 = (ke - kb + KS - 1) / KS, steps = MODE == GATED_SUM ? 2 * steps1 : steps1;
-    TileLoad<T, AKC> ta;
+    TileLoad<T, AKC> ta[NA];
     TileLoad<T, BKC> tb[NB];
     auto fetch = [&](int64_t s) {
         const int part = MODE == GATED_SUM && s >= steps1;
         const int64_t k0 = kb + (s - (part ? steps1 : 0)) * KS;
-        ta.load(g.a[MODE == GATED_PAIR ? z : part], row0, g.m, k0, ke);
+        ta[0].load(g.a[MODE == GATED_PAIR ? z : part], row0, g.m, k0, ke);
+        if constexpr (NA == 2) ta[1].load(g.rest[MODE == GATED_PAIR ? z : part], row0, g.m, k0, ke);
         tb[0].load(g.b[part], col0, g.n, k0, ke);
         if constexpr (NB == 2) tb[1].load(g.b[1], col0, g.n, k0, ke);
     };
     if (steps > 0) fetch(0);
     for (int64_t s = 0; s < steps; ++s) {
-        ta.store(la);
+#pragma unroll
+        for (int a = 0; a < NA; ++a) ta[a].store(la[a]);
 #pragma unroll
         for (int b = 0; b < NB; ++b) tb[b].store(lb[b]);
         __syncthreads();
         if (s + 1 < steps) fetch(s + 1);
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
-            uint4 fa[2], fb[NB][2];
+            uint4 fa[NA][2], fb[NB][2];
             const int c = kk * 4 + (lane >> 4);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int r = wr + i * 16 + (lane & 15);
-                fa[i] = la[r * 8 + (c ^ (r & 7))];
+#pragma unroll
+                for (int a = 0; a < NA; ++a) fa[a][i] = la[a][r * 8 + (c ^ (r & 7))];
                 const int q = wc + i * 16 + (lane & 15);
 #pragma unroll
                 for (int b = 0; b < NB; ++b) fb[b][i] = lb[b][q * 8 + (c ^ (q & 7))];
@@ -198,7 +218,9 @@ __global__ __launch_bounds__(256) void k_gated_tile(GatedArgs g) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) acc[b][i][j] = mma<T>(fb[b][j], fa[i], acc[b][i][j]);
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int a = 0; a < NA; ++a) acc[b][i][j] = mma<T>(fb[b][j], fa[a][i], acc[b][i][j]);
         }
         __syncthreads();
     }
@@ -248,8 +270,8 @@ __device__ __forceinline__ uint4 small_fragment(const Operand& o, int64_t row, i
     return __builtin_bit_cast(uint4, r);
 }
 
-// What the backward products of a small problem need of dg (which = 0) and du (1), computed where it is used and rounded as
-// k_gated_slopes would: element (row, k) of the operand is element (row, k) of dh, g, u if KC, else (k, row).
+// What the backward products of a small problem need of dg (which = 0) and du (1), computed where it is used, in the parts that
+// k_gated_slopes would write: element (row, k) of the operand is element (row, k) of dh, g, u if KC, else (k, row).
 struct SlopeOperand {
     const void* dh;
     const float *kg, *ku;
@@ -257,9 +279,9 @@ struct SlopeOperand {
     int act;
 };
 template <typename T, bool KC, bool WHOLE>
-__device__ __forceinline__ uint4 slope_fragment(const SlopeOperand& o, int which, int64_t row, int64_t k, int64_t k1) {
+__device__ __forceinline__ Parts<SLOPE_PARTS<T>> slope_fragment(const SlopeOperand& o, int which, int64_t row, int64_t k, int64_t k1) {
     constexpr int V = 16 / sizeof(T);
-    Pack<T> r;
+    Pack<T> r[SLOPE_PARTS<T>];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int64_t i = KC ? row : k + j, c = KC ? k + j : row;
@@ -267,24 +289,31 @@ __device__ __forceinline__ uint4 slope_fragment(const SlopeOperand& o, int which
             float a, da;
             activation<T>(o.kg[i * o.n + c], o.act, a, da);
             const float d = to_float(((const T*)o.dh)[i * o.dhs + c]);
-            r.v[j] = from_float<T>(which ? d * a : d * o.ku[i * o.n + c] * da);
+            const float slope = which ? d * a : d * o.ku[i * o.n + c] * da;
+            r[0].v[j] = from_float<T>(slope);
+            if constexpr (SLOPE_PARTS<T> == 2) r[1].v[j] = rounding_rest(slope, r[0].v[j]);
         } else {
-            r.v[j] = from_float<T>(0.0f);
+#pragma unroll
+            for (int q = 0; q < SLOPE_PARTS<T>; ++q) r[q].v[j] = from_float<T>(0.0f);
         }
     }
-    return __builtin_bit_cast(uint4, r);
+    Parts<SLOPE_PARTS<T>> parts;
+#pragma unroll
+    for (int q = 0; q < SLOPE_PARTS<T>; ++q) parts.v[q] = __builtin_bit_cast(uint4, r[q]);
+    return parts;
 }
 
-// The body: NB products side by side (one first operand, NB second ones), slabs of contraction [kb, ke) dealt to the waves; fa(i, k, whole)
+// The body: NB products side by side (one first operand, of NA parts, NB second ones), slabs of contraction [kb, ke) dealt to the waves; fa(i, k, whole)
 // and fb(b, i, k, whole) give fragments i < FR.
-template <typename T, int NB, int FR, typename FA, typename FB>
+template <typename T, int NA, int NB, int FR, typename FA, typename FB>
 __device__ __forceinline__ void small_sums(f32x4 (&acc)[NB][FR][FR], int64_t kb, int64_t ke, FA&& fa, FB&& fb) {
     constexpr int SLAB = 64 / sizeof(T), V = 16 / sizeof(T);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t slabs = (ke - kb) / SLAB;
     auto slab = [&](int64_t k0, auto whole) {
         const int64_t k = k0 + (lane >> 4) * V;
-        uint4 a[FR], b[NB][FR];
+        Parts<NA> a[FR];
+        uint4 b[NB][FR];
 #pragma unroll
         for (int i = 0; i < FR; ++i) {
             a[i] = fa(i, k, whole);
@@ -296,7 +325,9 @@ __device__ __forceinline__ void small_sums(f32x4 (&acc)[NB][FR][FR], int64_t kb,
 #pragma unroll
             for (int i = 0; i < FR; ++i)
 #pragma unroll
-                for (int j = 0; j < FR; ++j) acc[q][i][j] = mma<T>(b[q][j], a[i], acc[q][i][j]);
+                for (int j = 0; j < FR; ++j)
+#pragma unroll
+                    for (int p = 0; p < NA; ++p) acc[q][i][j] = mma<T>(b[q][j], a[i].v[p], acc[q][i][j]);
     };
 #pragma unroll 4
     for (int64_t s = wave; s < slabs; s += SMALL_WAVES) slab(kb + s * SLAB, std::true_type{});
@@ -322,7 +353,7 @@ __device__ __forceinline__ void small_join(const f32x4 (&acc)[NB][FR][FR], f32x4
     }
 }
 
-template <typename T, int MODE, bool AKC, bool BKC, int FR>
+template <typename T, int MODE, bool AKC, bool BKC, int FR, int NA>
 __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small(GatedArgs g) {
     constexpr int SLAB = 64 / sizeof(T), NB = MODE == GATED_FWD ? 2 : 1, SB = 16 * FR;
     __shared__ f32x4 sums[SMALL_WAVES][NB * FR * FR][64];
@@ -339,7 +370,13 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small(GatedArgs g) {
 #pragma unroll
     for (int part = 0; part < (MODE == GATED_SUM ? 2 : 1); ++part) {
         const Operand oa = MODE == GATED_PAIR && z ? g.a[1] : g.a[part], ob = g.b[part], ob2 = g.b[1];
-        small_sums<T, NB, FR>(acc, kb, ke, [&](int i, int64_t k, auto whole) { return small_fragment<T, AKC, whole.value>(oa, ra[i], k, ke); },
+        const Operand rest = MODE == GATED_PAIR && z ? g.rest[1] : g.rest[part];
+        small_sums<T, NA, NB, FR>(acc, kb, ke, [&](int i, int64_t k, auto whole) {
+                              Parts<NA> r;
+                              r.v[0] = small_fragment<T, AKC, whole.value>(oa, ra[i], k, ke);
+                              if constexpr (NA == 2) r.v[1] = small_fragment<T, AKC, whole.value>(rest, ra[i], k, ke);
+                              return r;
+                          },
                           [&](int b, int i, int64_t k, auto whole) { return small_fragment<T, BKC, whole.value>(b ? ob2 : ob, rb[i], k, ke); });
     }
     f32x4 v[NB];
@@ -386,7 +423,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small_back(SlopeOper
         for (int i = 0; i < 2; ++i) ra[i] = min(row0 + i * 16 + (lane & 15), m - 1);
 #pragma unroll
         for (int which = 0; which < 2; ++which)
-            small_sums<T, 1, 2>(acc, 0, h, [&](int i, int64_t q, auto whole) { return slope_fragment<T, true, whole.value>(s, which, ra[i], q, h); },
+            small_sums<T, SLOPE_PARTS<T>, 1, 2>(acc, 0, h, [&](int i, int64_t q, auto whole) { return slope_fragment<T, true, whole.value>(s, which, ra[i], q, h); },
                              [&](int, int i, int64_t q, auto whole) { return small_fragment<T, false, whole.value>(which ? wu : wg, rb[i], q, h); });
     } else {                                   // dw = d^T x, contraction over the rows
         id -= tiles_x;
@@ -396,7 +433,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small_back(SlopeOper
         int64_t ra[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) ra[i] = min(row0 + i * 16 + (lane & 15), h - 1);
-        small_sums<T, 1, 2>(acc, 0, m, [&](int i, int64_t q, auto whole) { return slope_fragment<T, false, whole.value>(s, which, ra[i], q, m); },
+        small_sums<T, SLOPE_PARTS<T>, 1, 2>(acc, 0, m, [&](int i, int64_t q, auto whole) { return slope_fragment<T, false, whole.value>(s, which, ra[i], q, m); },
                          [&](int, int i, int64_t q, auto whole) { return small_fragment<T, false, whole.value>(x, rb[i], q, m); });
     }
     small_join<1, 2>(acc, v, sums);
@@ -420,11 +457,11 @@ __global__ __launch_bounds__(256) void k_gated_join(GatedArgs g) {
     ((T*)g.out[z])[e / g.n * g.os + e % g.n] = from_float<T>(v);
 }
 
-// dg = dh u act'(g), du = dh act(g).
-template <typename T>
+// dg = dh u act'(g), du = dh act(g), and what their roundings left.
+template <typename T, bool REST>
 __global__ __launch_bounds__(256) void k_gated_slopes(const T* __restrict__ dh, int64_t dhs, const float* __restrict__ kg,
                                                       const float* __restrict__ ku, int64_t m, int64_t n, int act, T* __restrict__ dg,
-                                                      T* __restrict__ du) {
+                                                      T* __restrict__ du, T* __restrict__ dg_rest, T* __restrict__ du_rest) {
     constexpr int V = Pack<T>::N;
     const int64_t packs = (n + V - 1) / V;
     for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < m * packs; id += (int64_t)gridDim.x * 256) {
@@ -432,7 +469,7 @@ __global__ __launch_bounds__(256) void k_gated_slopes(const T* __restrict__ dh, 
         const int64_t e = row * n + c;
         const T* d = dh + row * dhs + c;
         const int len = (int)min((int64_t)V, n - c);
-        Pack<T> pd, og, ou;
+        Pack<T> pd, og, ou, rg, ru;
         float gv[V], uv[V];
         if (len == V) {
             pd = load_pack(d);
@@ -450,16 +487,21 @@ __global__ __launch_bounds__(256) void k_gated_slopes(const T* __restrict__ dh, 
         for (int i = 0; i < V; ++i) {
             float a, da;
             activation<T>(gv[i], act, a, da);
-            og.v[i] = from_float<T>(to_float(pd.v[i]) * uv[i] * da);
-            ou.v[i] = from_float<T>(to_float(pd.v[i]) * a);
+            const float sg = to_float(pd.v[i]) * uv[i] * da, su = to_float(pd.v[i]) * a;
+            og.v[i] = from_float<T>(sg), ou.v[i] = from_float<T>(su);
+            if constexpr (REST) rg.v[i] = rounding_rest(sg, og.v[i]), ru.v[i] = rounding_rest(su, ou.v[i]);
         }
         if (len == V) {
             store_pack(dg + e, og);
             store_pack(du + e, ou);
+            if constexpr (REST) store_pack(dg_rest + e, rg), store_pack(du_rest + e, ru);
         } else {
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (i < len) dg[e + i] = og.v[i], du[e + i] = ou.v[i];
+            for (int i = 0; i < V; ++i) {
+                if (i >= len) continue;
+                dg[e + i] = og.v[i], du[e + i] = ou.v[i];
+                if constexpr (REST) dg_rest[e + i] = rg.v[i], du_rest[e + i] = ru.v[i];
+            }
         }
     }
 }
@@ -480,14 +522,14 @@ AnyPlan any_plan(int64_t m, int64_t n, int64_t k, int zs, bool can_split) {
     if (can_split && tiles > 0 && tiles < 256) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(512, tiles), k / (4 * step)));
     return p;
 }
-template <typename T, int MODE, bool AKC, bool BKC>
+template <typename T, int MODE, bool AKC, bool BKC, int NA>
 void launch_any(hipStream_t st, const GatedArgs& g, const AnyPlan& p) {
     const int64_t b = p.small ? 16 * p.fragments : TB;
     const dim3 grid((unsigned)(ceil_div(g.m, b) * ceil_div(g.n, b)), (unsigned)g.splits, MODE == GATED_PAIR ? 2 : 1);
     if (p.small && MODE == GATED_FWD && p.fragments == 1)
-        hipLaunchKernelGGL((k_gated_small<T, GATED_FWD, true, true, 1>), grid, dim3(64 * SMALL_WAVES), 0, st, g);
-    else if (p.small) hipLaunchKernelGGL((k_gated_small<T, MODE, AKC, BKC, 2>), grid, dim3(64 * SMALL_WAVES), 0, st, g);
-    else hipLaunchKernelGGL((k_gated_tile<T, MODE, AKC, BKC>), grid, dim3(256), 0, st, g);
+        hipLaunchKernelGGL((k_gated_small<T, GATED_FWD, true, true, 1, 1>), grid, dim3(64 * SMALL_WAVES), 0, st, g);
+    else if (p.small) hipLaunchKernelGGL((k_gated_small<T, MODE, AKC, BKC, 2, NA>), grid, dim3(64 * SMALL_WAVES), 0, st, g);
+    else hipLaunchKernelGGL((k_gated_tile<T, MODE, AKC, BKC, NA>), grid, dim3(256), 0, st, g);
 }
 
 }  // namespace gpbo_static

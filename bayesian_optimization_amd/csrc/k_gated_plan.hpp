@@ -126,7 +126,7 @@ hipError_t gated_forward(hipStream_t st, GatedArgs g, char* work) {
         else if (g.m <= 4) hipLaunchKernelGGL((k_gated_few<T, 4>), dim3(hidden, 1), dim3(256), 0, st, g);
         else hipLaunchKernelGGL((k_gated_few<T, 8>), dim3(hidden, (unsigned)ceil_div(g.m, 8)), dim3(256), 0, st, g);
     } else {
-        launch_any<T, GATED_FWD, true, true>(st, g, any_plan<T>(g.m, g.n, g.k, 1, false));
+        launch_any<T, GATED_FWD, true, true, 1>(st, g, any_plan<T>(g.m, g.n, g.k, 1, false));
     }
     return hipGetLastError();
 }
@@ -135,13 +135,14 @@ hipError_t gated_forward(hipStream_t st, GatedArgs g, char* work) {
 // rows; these copies are a few per cent of the products' time.
 struct BackwardPlan {
     bool fast = false, one = false, narrow = false, few_cols = false;      // one: k_gated_small_back
+    bool parts = false;                                                    // dg and du in two parts
     int tile_x = 128, tile_w = 128, splits_x = 1, splits_w = 1;
     AnyPlan any_x, any_w;
     int64_t hp = 0, mp = 0;
-    int64_t d_bytes = 0, dt_bytes = 0, xt_bytes = 0, wt_bytes = 0, part_bytes = 0;
+    int64_t d_bytes = 0, rest_bytes = 0, dt_bytes = 0, xt_bytes = 0, wt_bytes = 0, part_bytes = 0;
     int splits_narrow = 1;
     int64_t narrow_d_bytes = 0, narrow_bytes = 0;
-    int64_t bytes() const { return std::max(narrow_bytes, 2 * d_bytes + 2 * dt_bytes + xt_bytes + 2 * wt_bytes + part_bytes); }
+    int64_t bytes() const { return std::max(narrow_bytes, 2 * d_bytes + 2 * rest_bytes + 2 * dt_bytes + xt_bytes + 2 * wt_bytes + part_bytes); }
 };
 template <typename T>
 BackwardPlan backward_plan(int64_t m, int64_t k, int64_t h) {
@@ -187,7 +188,9 @@ BackwardPlan backward_plan(int64_t m, int64_t k, int64_t h) {
         // (27 to 29 and 30), worse from there on (1000 x 30 -> 24: 44, 20 x 30 -> 1000: 60)
         p.one = m > 0 && 4 * m * h * ceil_div(k, SB) <= (int64_t)1 << 20 && std::max(m, 2 * h) <= 512;
         if (p.one) return p;
-        p.d_bytes = round_up(m * h * B, 256);
+        // in two parts where a gradient has few elements (with the forward pass 20000 x 5 -> 77 bf16 57 us without, 64 with; 1000 x 520 ->
+        // 400, where it would take away less than the gradients' own roundings, 44 and 61)
+        p.d_bytes = round_up(m * h * B, 256), p.parts = SLOPE_PARTS<T> == 2 && std::min(m, h) * k < 4096, p.rest_bytes = p.parts ? p.d_bytes : 0;
         p.any_x = any_plan<T>(m, k, h, 1, true), p.any_w = any_plan<T>(h, k, m, 2, true);
         p.splits_x = p.any_x.splits, p.splits_w = p.any_w.splits;
     }
@@ -264,9 +267,13 @@ hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const voi
     }
     char* at = work;
     auto take = [&](int64_t bytes) { char* r = at; at += bytes; return r; };
-    T *dg = (T*)take(p.d_bytes), *du = (T*)take(p.d_bytes), *dgt = (T*)take(p.dt_bytes), *dut = (T*)take(p.dt_bytes), *xt = (T*)take(p.xt_bytes),
+    T *dg = (T*)take(p.d_bytes), *du = (T*)take(p.d_bytes), *dg_rest = (T*)take(p.rest_bytes), *du_rest = (T*)take(p.rest_bytes), *dgt = (T*)take(p.dt_bytes), *dut = (T*)take(p.dt_bytes), *xt = (T*)take(p.xt_bytes),
       *wgt = (T*)take(p.wt_bytes), *wut = (T*)take(p.wt_bytes);
     float* part = (float*)take(p.part_bytes);
+    auto by_parts = [&](auto&& launch) {
+        if (p.parts) launch(std::integral_constant<int, SLOPE_PARTS<T>>{});
+        else launch(std::integral_constant<int, 1>{});
+    };
     if (p.fast) {
         hipLaunchKernelGGL(k_gated_slopes_both<T>, dim3((unsigned)(p.mp / 64 * (p.hp / 64))), dim3(256), 0, st, (const T*)dh, dhs, kg, ku, m, h, act,
                            dg, du, p.hp, dgt, dut, p.mp);
@@ -281,8 +288,10 @@ hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const voi
         if (blocks) hipLaunchKernelGGL((k_gated_pack<T, true>), dim3((unsigned)blocks), dim3(256), 0, st, a);
     } else if (m > 0) {
         const int64_t packs = m * ceil_div(h, Pack<T>::N);
-        hipLaunchKernelGGL(k_gated_slopes<T>, dim3((unsigned)std::min<int64_t>(ceil_div(packs, 256), 8192)), dim3(256), 0, st, (const T*)dh, dhs,
-                           kg, ku, m, h, act, dg, du);
+        by_parts([&](auto parts) {
+            hipLaunchKernelGGL((k_gated_slopes<T, parts.value == 2>), dim3((unsigned)std::min<int64_t>(ceil_div(packs, 256), 8192)), dim3(256), 0, st,
+                               (const T*)dh, dhs, kg, ku, m, h, act, dg, du, dg_rest, du_rest);
+        });
     }
     if (dx && m > 0) {
         GatedArgs g{};
@@ -292,7 +301,8 @@ hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const voi
             launch_fast<T, GATED_SUM>(st, g, p.tile_x);
         } else {
             g.a[0] = {dg, h, 1}, g.a[1] = {du, h, 1}, g.b[0] = {wg, 1, ws}, g.b[1] = {wu, 1, ws}, g.k = h;
-            launch_any<T, GATED_SUM, true, false>(st, g, p.any_x);
+            g.rest[0] = {dg_rest, h, 1}, g.rest[1] = {du_rest, h, 1};
+            by_parts([&](auto parts) { launch_any<T, GATED_SUM, true, false, parts.value>(st, g, p.any_x); });
         }
         if (g.splits > 1) hipLaunchKernelGGL(k_gated_join<T>, dim3((unsigned)ceil_div(m * k, 256), 1), dim3(256), 0, st, g);
     }
@@ -304,7 +314,8 @@ hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const voi
             launch_fast<T, GATED_PAIR>(st, g, p.tile_w);
         } else {
             g.a[0] = {dg, 1, h}, g.a[1] = {du, 1, h}, g.b[0] = g.b[1] = {x, 1, xs}, g.k = m;
-            launch_any<T, GATED_PAIR, false, false>(st, g, p.any_w);
+            g.rest[0] = {dg_rest, 1, h}, g.rest[1] = {du_rest, 1, h};
+            by_parts([&](auto parts) { launch_any<T, GATED_PAIR, false, false, parts.value>(st, g, p.any_w); });
         }
         if (g.splits > 1) hipLaunchKernelGGL(k_gated_join<T>, dim3((unsigned)ceil_div(h * k, 256), 2), dim3(256), 0, st, g);
     }

@@ -263,7 +263,17 @@ def test_gated_unit_many_rows_strides_infinities_and_parts():
     assert bool(torch.isnan(h2[77]).all()) and torch.equal(torch.cat([h[:77], h[78:]]), torch.cat([h2[:77], h2[78:]]))
 
 
-def check_gated(dtype, act, rows, cols, hidden):
+# Gradients of few elements, where the terms of a sum may cancel in all of them: in 16 bits dg and du enter as two numbers, the rounded one
+# and what the rounding left, itself rounded by at most half of a step, so that they are off by the square of half a step
+@pytest.mark.parametrize('rows,cols,hidden', [(1, 1, 1), (2, 170, 14), (60, 1, 21), (500, 1, 1), (512, 5, 200), (600, 10, 1), (3109, 2, 4), (1000, 3, 600), (311, 56, 1),
+                                              (213819, 10, 1), (20001, 5, 77), (3, 1300, 2000), (1, 4095, 2001), (65, 62, 3001)])
+@pytest.mark.parametrize('act', ['silu', 'gelu'])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_gated_unit_gradients_of_few_elements(dtype, act, rows, cols, hidden):
+    check_gated(dtype, act, rows, cols, hidden, slope=half(dtype) ** 2)
+
+
+def check_gated(dtype, act, rows, cols, hidden, slope=None):
     from bayesian_optimization_amd import features
     x, dh = rand((rows, cols), dtype, 1), rand((rows, hidden), dtype, 2)
     wg, wu = rand((hidden, cols), dtype, 3, cols ** -0.5), rand((hidden, cols), dtype, 4, cols ** -0.5)
@@ -283,8 +293,9 @@ def check_gated(dtype, act, rows, cols, hidden):
     within(h, want, ea * u.abs() + a.abs() * eu + ea * eu + 2 * U * want.abs() + H * want.abs() * 1.01 + tiny, 'h')
     d = dh.double()
     dg, du = d * u * da, d * a
-    edg = d.abs() * (eu * da.abs() + u.abs() * eda + eu * eda) + (H * 1.01 + 4 * U) * dg.abs() + tiny      # rounded once to the type of x
-    edu = d.abs() * ea + (H * 1.01 + 4 * U) * du.abs() + tiny
+    S = H if slope is None else slope
+    edg = d.abs() * (eu * da.abs() + u.abs() * eda + eu * eda) + (S * 1.01 + 4 * U) * dg.abs() + tiny      # rounded once to the type of x
+    edu = d.abs() * ea + (S * 1.01 + 4 * U) * du.abs() + tiny
     wga, wua, xa = wg.double().abs(), wu.double().abs(), x.double().abs()
     want = dg @ wg.double() + du @ wu.double()
     terms = (dg.abs() + edg) @ wga + (du.abs() + edu) @ wua
