@@ -115,13 +115,16 @@ __device__ __forceinline__ double from_fixed(unsigned long long hi, unsigned lon
 }
 
 // Inclusive sums over the workgroup's threads, in thread order; the total comes back too.  Two barriers; red: a place a wave.
+// Every sum is that of the aligned half blocks in front of it, joined from the right, so that the picks can rely on two things in
+// floating point as well: the sums never fall, and one where nothing is added has its predecessor's bits (a scan in which every lane adds up
+// a window that ends with it has neither: of 5000 scores whose last 2000 have no weight, a third of the rows then ended in a step there).
 template <int THREADS = DRAW_THREADS, typename V>
 __device__ __forceinline__ V block_scan(V v, V* red, V& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const V x = __shfl_up(v, o);
-        if (lane >= o) v += x;
+        const V x = __shfl(v, (lane & -2 * o) | (o - 1));      // the sum of the half block in front
+        if (lane & o) v += x;
     }
     __syncthreads();                           // earlier reads of red are done
     if (lane == 63) red[wave] = v;
@@ -135,6 +138,11 @@ __device__ __forceinline__ V block_scan(V v, V* red, V& total) {
     total = all;
     return before + v;
 }
+
+// Mass in front of which a draw lies: u times the whole, u out of range counting as the nearest end.  It is below the whole, whatever that
+// is ((1 - 2^-53) Z rounds to less than Z), and the running sums end at the whole without falling: there is a first sum above it, that
+// sum is above its predecessor, and so its place has a weight.
+__device__ __forceinline__ double draw_goal(double u, double total) { return fmin(fmax(u, 0.0), 1.0 - 0x1p-53) * total; }
 
 // Where the search for the cut stands.  Lives in LDS (one workgroup a row) or in the workspace (many).
 enum { PHASE_TOPK = 0, PHASE_TOPP = 1, PHASE_PICK = 2, PHASE_DONE = 3 };
@@ -634,15 +642,13 @@ __device__ void draw_from_list(DrawLds<T>& s, const DrawArgs& a, const DrawRow& 
     if (tid < (int)kept) s.l.c[tid] = ci;
     __syncthreads();
     for (int64_t q = tid; q < a.draws; q += DRAW_THREADS) {
-        const double at = fmax(a.u[row * a.draws + q], 0.0) * total;
-        int lo = 0, hi = (int)kept - 1;        // the first c > at; the last kept one if rounding leaves none
+        const double at = draw_goal(a.u[row * a.draws + q], total);
+        int lo = 0, hi = (int)kept - 1;        // the first c > at
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
             if (s.l.c[mid] > at) hi = mid;
             else lo = mid + 1;
         }
-        // a weight of zero is never drawn: step back over those at the end
-        while (lo > 0 && s.l.c[lo] == s.l.c[lo - 1]) --lo;
         a.index[row * a.draws + q] = s.l.pick[lo];
         if (a.logp) a.logp[row * a.draws + q] = draw_t<T>(s.l.key[lo], top, p.temperature) - log(total);
     }
@@ -753,14 +759,13 @@ __global__ __launch_bounds__(THREADS) void k_draw_short(DrawArgs a) {
     key_s[tid] = mine;
     __syncthreads();
     for (int64_t q = tid; q < a.draws; q += THREADS) {
-        const double at = fmax(a.u[row * a.draws + q], 0.0) * total;
-        int lo = 0, hi = n - 1;                // the first c > at; the last kept one if rounding leaves none
+        const double at = draw_goal(a.u[row * a.draws + q], total);
+        int lo = 0, hi = n - 1;                // the first c > at
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
             if (c_s[mid] > at) hi = mid;
             else lo = mid + 1;
         }
-        while (lo > 0 && c_s[lo] == c_s[lo - 1]) --lo;
         a.index[row * a.draws + q] = lo;
         if (a.logp) a.logp[row * a.draws + q] = draw_t<T>(key_s[lo], top, p.temperature) - log(total);
     }
@@ -842,14 +847,14 @@ __device__ void draw_tiles_mass(const DrawKept<T>& kw, const T* x, uint32_t begi
 
 // One wave: the pick inside [begin, end), of at most 64 * 64 elements, for mass `goal` with `run` in front of it and `ties` of the
 // cut's ties already met (of which cut_ties are kept).  A lane sums a run of neighbours, the lane that holds the goal is found
-// by a scan over the lanes, and then its run is spread over the lanes.
+// by a scan over the lanes, and then its run is spread over the lanes.  Only lanes with a weight are asked: these sums and those over the
+// tiles differ in their last bits, and where none passes the goal for that it is the last one.  The pick lies in the tile whatever the sums are.
 template <typename T>
 __device__ int64_t draw_in_tile(const DrawKept<T>& kw, const T* x, uint32_t begin, uint32_t end, double run, uint32_t ties, uint32_t cut_ties, double goal) {
     using Key = typename Score<T>::Key;
     constexpr uint32_t V = Pack<T>::N;
     const uint32_t lane = threadIdx.x & 63;
     uint32_t each = (end - begin + 63) / 64;
-    int64_t pick = -1;
     for (int stage = 0; stage < 2; ++stage) {
         const uint32_t b = min(end, begin + lane * each), e = min(end, b + each);
         double m = 0.0;
@@ -882,17 +887,15 @@ __device__ int64_t draw_in_tile(const DrawKept<T>& kw, const T* x, uint32_t begi
             if (lane >= (uint32_t)o) incl += v;
         }
         const unsigned long long any = __ballot(m > 0.0), hit = __ballot(m > 0.0 && run + incl > goal);
-        if (!any) return pick;                 // cannot be: the tile was chosen for its mass
-        const int at = hit ? __ffsll(hit) - 1 : 63 - __clzll((long long)any);      // the last one with weight if rounding leaves none
+        const int at = hit ? __ffsll(hit) - 1 : 63 - __clzll((long long)(any | 1));
         run += __shfl(incl - m, at);
         ties = __shfl(before, at);
-        begin = min(end, begin + at * each);
+        begin = min(end - 1, begin + at * each);
         end = min(end, begin + each);
-        pick = begin;
         if (each == 1) break;
         each = 1;
     }
-    return pick;
+    return begin;
 }
 
 constexpr uint32_t TILE = 4096;
@@ -976,14 +979,13 @@ __global__ __launch_bounds__(DRAW_THREADS) void k_draw_row(DrawArgs a) {
     s.t.c[tid] = incl, s.t.ties[tid] = before;
     __syncthreads();
     for (int64_t q = wave; q < a.draws; q += DRAW_THREADS / 64) {
-        const double goal = fmax(a.u[row * a.draws + q], 0.0) * total;
-        int lo = 0, hi = (int)tiles - 1;       // the first tile whose sum passes the goal, the last with any mass if none does
+        const double goal = draw_goal(a.u[row * a.draws + q], total);
+        int lo = 0, hi = (int)tiles - 1;       // the first tile whose sum passes the goal
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
             if (s.t.c[mid] > goal) hi = mid;
             else lo = mid + 1;
         }
-        while (lo > 0 && s.t.c[lo] == s.t.c[lo - 1]) --lo;
         const int64_t pick = draw_in_tile(kw, x, lo * tile, min(n, (lo + 1) * tile), lo ? s.t.c[lo - 1] : 0.0, s.t.ties[lo], cut_ties, goal);
         if (lane == 0) {
             a.index[row * a.draws + q] = pick;
@@ -1262,14 +1264,13 @@ __global__ __launch_bounds__(256) void k_draw_pick(DrawArgs a, char* work) {
     const uint32_t n = (uint32_t)a.cols, tiles = (n + TILE - 1) / TILE;
     const double total = rw.w->total;
     for (int64_t q = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); q < a.draws; q += (int64_t)gridDim.x * 4) {
-        const double goal = fmax(a.u[row * a.draws + q], 0.0) * total;
+        const double goal = draw_goal(a.u[row * a.draws + q], total);
         int lo = 0, hi = (int)tiles - 1;
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
             if (rw.c[mid] > goal) hi = mid;
             else lo = mid + 1;
         }
-        while (lo > 0 && rw.c[lo] == rw.c[lo - 1]) --lo;
         const int64_t pick = draw_in_tile(kw, x, (uint32_t)lo * TILE, min(n, (uint32_t)(lo + 1) * TILE), lo ? rw.c[lo - 1] : 0.0, rw.ties[lo],
                                           rw.w->st.cut_ties, goal);
         if ((threadIdx.x & 63) == 0) {
