@@ -139,6 +139,19 @@ __device__ __forceinline__ V block_scan(V v, V* red, V& total) {
     return before + v;
 }
 
+// How many threads, from the first on, `in` holds for without a gap.  Two barriers; red: a place a wave.
+template <int THREADS = DRAW_THREADS>
+__device__ __forceinline__ int block_leading(bool in, unsigned long long* red) {
+    const unsigned long long out = __ballot(!in);
+    __syncthreads();                           // earlier reads of red are done
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = out ? threadIdx.x + __ffsll(out) - 1 : THREADS;
+    __syncthreads();
+    unsigned long long first = THREADS;
+#pragma unroll
+    for (int i = 0; i < THREADS / 64; ++i) first = min(first, red[i]);
+    return (int)first;
+}
+
 // Mass in front of which a draw lies: u times the whole, u out of range counting as the nearest end.  It is below the whole, whatever that
 // is ((1 - 2^-53) Z rounds to less than Z), and the running sums end at the whole without falling: there is a first sum above it, that
 // sum is above its predecessor, and so its place has a weight.
@@ -598,10 +611,10 @@ __device__ void draw_cut_from_list(DrawLds<T>& s, const DrawRow& p, int n) {
         const double incl = block_scan(w, s.red, all);
         in = k != 0 && (tid == 0 || st.above + (incl - w) < st.goal);
     }
-    unsigned long long taken, same;
-    block_scan(in ? 1ull : 0ull, s.red_u, taken);
-    const Key cut = s.l.key2[taken ? (int)taken - 1 : 0];
-    block_scan(in && k == cut ? 1ull : 0ull, s.red_u, same);
+    const int taken = block_leading(in, s.red_u);
+    const Key cut = s.l.key2[taken ? taken - 1 : 0];
+    unsigned long long same;
+    block_scan(tid < taken && k == cut ? 1ull : 0ull, s.red_u, same);
     __syncthreads();
     if (tid == 0) {
         st.cut = cut, st.cut_ties = (uint32_t)same;
@@ -628,22 +641,21 @@ __device__ void draw_from_list(DrawLds<T>& s, const DrawArgs& a, const DrawRow& 
         if (goal < 0.0) goal = p.top_p * total;
         keep = keep && (tid == 0 || run - w < goal);
     }
-    // the kept ones are the first `kept` positions; now in index order
-    unsigned long long kept;
-    block_scan(keep ? 1ull : 0ull, s.red_u, kept);
-    Key ki = keep ? kr : 0;
-    uint32_t ii = keep ? s.l.idx2[tid] : 0xffffffffu;
+    // the kept ones are the first `kept` positions, also should an exponential not fall where its argument does; now in index order
+    const int kept = block_leading(keep, s.red_u);
+    Key ki = tid < kept ? kr : 0;
+    uint32_t ii = tid < kept ? s.l.idx2[tid] : 0xffffffffu;
     int few = 64;                              // they stand in front: no more than they need to be sorted
-    while (few < (int)kept) few <<= 1;
+    while (few < kept) few <<= 1;
     block_sort<Key, true>(ki, ii, few, s.l.key, s.l.idx);
-    const double wi = tid < (int)kept ? exp(draw_t<T>(ki, top, p.temperature)) : 0.0;
+    const double wi = tid < kept ? exp(draw_t<T>(ki, top, p.temperature)) : 0.0;
     const double ci = block_scan(wi, s.red, total);      // its barriers stand between the sort's last reads of l.key and this
-    if (tid < (int)kept) s.l.key[tid] = ki, s.l.pick[tid] = ii;
-    if (tid < (int)kept) s.l.c[tid] = ci;
+    if (tid < kept) s.l.key[tid] = ki, s.l.pick[tid] = ii;
+    if (tid < kept) s.l.c[tid] = ci;
     __syncthreads();
     for (int64_t q = tid; q < a.draws; q += DRAW_THREADS) {
         const double at = draw_goal(a.u[row * a.draws + q], total);
-        int lo = 0, hi = (int)kept - 1;        // the first c > at
+        int lo = 0, hi = kept - 1;        // the first c > at
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
             if (s.l.c[mid] > at) hi = mid;
@@ -725,6 +737,7 @@ __global__ __launch_bounds__(THREADS) void k_draw_short(DrawArgs a) {
     __shared__ Key key_s[THREADS], top_s, cut_s;
     __shared__ uint32_t idx_s[THREADS], top_i, cut_i;
     __shared__ double c_s[THREADS], red[16];
+    __shared__ unsigned long long red_u[16];
     const int tid = threadIdx.x, n = (int)a.cols;
     const int64_t row = blockIdx.x;
     const T* x = (const T*)a.scores + row * a.stride;
@@ -747,10 +760,8 @@ __global__ __launch_bounds__(THREADS) void k_draw_short(DrawArgs a) {
         const double run = block_scan<THREADS>(in ? w : 0.0, red, total);
         in = in && (tid == 0 || run - w < p.top_p * total);
     }
-    // the kept ones are the first in rank: the last of them is the one behind which the next position is not kept
-    idx_s[tid] = in;
-    __syncthreads();
-    if (in && (tid == THREADS - 1 || !idx_s[tid + 1])) cut_s = k, cut_i = i;
+    // the kept ones are the first in rank, the best among them
+    if (tid == block_leading<THREADS>(in, red_u) - 1) cut_s = k, cut_i = i;
     __syncthreads();
     const Key cut = cut_s;
     const bool keep = mine != 0 && (mine > cut || (mine == cut && (uint32_t)tid <= cut_i));
