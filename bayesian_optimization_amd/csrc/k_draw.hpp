@@ -1302,8 +1302,19 @@ int64_t draw_work_bytes(int64_t rows, int64_t cols) {
 
 template <typename T>
 hipError_t draw_rows(hipStream_t st, const DrawArgs& a, char* work) {
+    // one workgroup a row; a launch takes fewer than 2^32 threads, so that many rows go in pieces
+    auto launch = [&](auto k, int threads) {
+        const int64_t most = ((int64_t)1 << 31) / threads;
+        for (int64_t r = 0; r < a.rows; r += most) {
+            DrawArgs p = a;
+            p.rows = std::min(most, a.rows - r);
+            p.scores = (const T*)a.scores + r * a.stride, p.u = a.u + r * a.draws, p.index = a.index + r * a.draws;
+            if (a.params) p.params = a.params + r * 4;
+            if (a.logp) p.logp = a.logp + r * a.draws;
+            hipLaunchKernelGGL(k, dim3((unsigned)p.rows), dim3(threads), 0, st, p);
+        }
+    };
     if (a.cols <= LIST) {
-        auto launch = [&](auto k, int threads) { hipLaunchKernelGGL(k, dim3((unsigned)a.rows), dim3(threads), 0, st, a); };
         if (a.cols <= 64) launch(k_draw_short<T, 64>, 64);
         else if (a.cols <= 128) launch(k_draw_short<T, 128>, 128);
         else if (a.cols <= 256) launch(k_draw_short<T, 256>, 256);
@@ -1312,7 +1323,7 @@ hipError_t draw_rows(hipStream_t st, const DrawArgs& a, char* work) {
         return hipGetLastError();
     }
     if (!draw_long(a.rows, a.cols)) {
-        hipLaunchKernelGGL(k_draw_row<T>, dim3((unsigned)a.rows), dim3(DRAW_THREADS), 0, st, a);
+        launch(k_draw_row<T>, DRAW_THREADS);
         return hipGetLastError();
     }
     // a workgroup of 1024 threads a CU over all rows, shares of at least 16 K

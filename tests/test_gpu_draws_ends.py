@@ -83,3 +83,20 @@ def test_members_of_a_list_without_weight():
         for st in (dict(top_k=cols - 3), dict(top_k=min(500, cols - 1)), dict()):
             u = ends_and_borders(s, 1, **st)
             check_ends(s, u, *draws.sample(s, u, **st), **st)
+
+
+@pytest.mark.parametrize('rows,cols,dtype', [((1 << 26) + 3, 2, torch.float16), ((1 << 22) + 5, 513, torch.bfloat16), ((1 << 22) + 5, 1025, torch.bfloat16)])
+def test_more_rows_than_a_launch_takes(rows, cols, dtype):
+    """2^32 threads and more, at 64 or 1024 a row: the rows around the border of two launches, and all of them against smaller calls."""
+    from bayesian_optimization_amd import draws
+    g = torch.Generator(device='cuda').manual_seed(cols)
+    s = torch.empty(rows, cols, dtype=dtype, device='cuda').normal_(generator=g)
+    u = torch.rand(rows, 1, generator=g, device='cuda', dtype=torch.float64)
+    top_k = torch.randint(0, 4, (rows,), generator=g, device='cuda')
+    for st in (dict(top_p=0.9), dict(top_k=top_k, temperature=0.5)):
+        index, logp = draws.sample(s, u, **st)
+        step = (rows + 6) // 7
+        for r in range(0, rows, step):
+            part = dict(st, top_k=top_k[r:r + step]) if 'top_k' in st else st
+            i, lp = draws.sample(s[r:r + step], u[r:r + step], **part)
+            assert torch.equal(i, index[r:r + step]) and torch.equal(lp, logp[r:r + step]), r
