@@ -430,15 +430,16 @@ __global__ __launch_bounds__(256) void k_norm_bwd_long_cols(NormArgs a) {
         }
 }
 
-// dw (blockIdx.y = 0) and db (1): the groups' partial sums, 16 interleaved running sums a column joined in a fixed order.
+// dw (blockIdx.y = 0) and db (1) of the columns from `first` on: the groups' partial sums, 16 interleaved running sums a column joined in a
+// fixed order.
 template <typename T>
-__global__ __launch_bounds__(1024) void k_norm_cols(const float* __restrict__ part, int groups, int64_t cols, T* __restrict__ dw,
+__global__ __launch_bounds__(1024) void k_norm_cols(const float* __restrict__ part, int groups, int64_t cols, int64_t first, T* __restrict__ dw,
                                                     T* __restrict__ db) {
     __shared__ float lds[16][64];
     T* out = blockIdx.y ? db : dw;
     if (!out) return;
     const int cl = threadIdx.x & 63, s = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 64 + cl;
+    const int64_t c = first + (int64_t)blockIdx.x * 64 + cl;
     float v = 0.0f;
     if (c < cols) {
         const float* p = part + (int64_t)blockIdx.y * cols + c;
@@ -540,9 +541,10 @@ hipError_t norm_backward(hipStream_t st, NormArgs a, void* dw, void* db) {
             hipLaunchKernelGGL(k_norm_bwd_long_cols<T>, dim3((unsigned)ceil_div(ceil_div(a.cols, Pack<T>::N), 256), (unsigned)p.groups), dim3(256), 0,
                                st, a);
     }
-    if (dw || db)
-        hipLaunchKernelGGL(k_norm_cols<T>, dim3((unsigned)ceil_div(a.cols, 64), 2), dim3(1024), 0, st, (const float*)a.part,
-                           a.rows > 0 ? (int)p.groups : 0, a.cols, (T*)dw, (T*)db);
+    constexpr int64_t MOST = (int64_t)1 << 27;      // columns of a launch, which takes fewer than 2^32 threads, 16 a column
+    for (int64_t c = 0; (dw || db) && c < a.cols; c += MOST)
+        hipLaunchKernelGGL(k_norm_cols<T>, dim3((unsigned)ceil_div(std::min(MOST, a.cols - c), 64), 2), dim3(1024), 0, st, (const float*)a.part,
+                           a.rows > 0 ? (int)p.groups : 0, a.cols, c, (T*)dw, (T*)db);
     return hipGetLastError();
 }
 
