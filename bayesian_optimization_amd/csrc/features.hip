@@ -15,6 +15,9 @@ bool is_float_type(int32_t t) { return t == GPBO_TYPE_F32 || t == GPBO_TYPE_BF16
 bool matrix_ok(int64_t rows, int64_t cols, int64_t stride) {
     return rows >= 0 && rows <= MOST && cols >= 1 && cols <= MOST && (stride >= cols || rows <= 1);
 }
+bool unit_ok(int64_t rows, int64_t cols, int64_t hidden) {
+    return matrix_ok(rows, cols, cols) && matrix_ok(rows, hidden, hidden) && cols <= MOST_ACROSS && hidden <= MOST_ACROSS;
+}
 bool work_ok(const void* p, int64_t bytes, int64_t need) {
     return need >= 0 && (need == 0 || (p && bytes >= need && (reinterpret_cast<uintptr_t>(p) & 255) == 0));
 }
@@ -71,7 +74,7 @@ int gpbo_layernorm_backward(int32_t device, void* stream, int32_t dtype, const v
 }
 
 int64_t gpbo_gated_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_t hidden) {
-    if (!is_float_type(dtype) || !matrix_ok(rows, cols, cols) || !matrix_ok(rows, hidden, hidden)) return -1;
+    if (!is_float_type(dtype) || !unit_ok(rows, cols, hidden)) return -1;
     return by_type(dtype, [&](auto t) { return forward_plan<decltype(t)>(rows, cols, hidden).bytes(); });
 }
 
@@ -81,7 +84,7 @@ int gpbo_gated(int32_t device, void* stream, int32_t dtype, int32_t act, const v
     if (!is_float_type(dtype) || (act != GPBO_ACT_SILU && act != GPBO_ACT_GELU) || !matrix_ok(rows, cols, x_stride) ||
         !matrix_ok(hidden, cols, w_stride) || !matrix_ok(rows, hidden, h_stride) || device < 0 || device >= MAX_DEVICES)
         return GPBO_ERR_BAD_ARG;
-    if (!!keep_g != !!keep_u || ceil_div(rows, TB) * ceil_div(hidden, TB) > MOST) return GPBO_ERR_BAD_ARG;
+    if (!!keep_g != !!keep_u || !unit_ok(rows, cols, hidden)) return GPBO_ERR_BAD_ARG;
     if (rows == 0) return GPBO_OK;
     if (!x || !wg || !wu || !h || !work_ok(workspace, workspace_bytes, gpbo_gated_workspace(dtype, rows, cols, hidden))) return GPBO_ERR_BAD_ARG;
     DeviceGuard guard(device);
@@ -93,7 +96,7 @@ int gpbo_gated(int32_t device, void* stream, int32_t dtype, int32_t act, const v
 }
 
 int64_t gpbo_gated_backward_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_t hidden) {
-    if (!is_float_type(dtype) || !matrix_ok(rows, cols, cols) || !matrix_ok(rows, hidden, hidden)) return -1;
+    if (!is_float_type(dtype) || !unit_ok(rows, cols, hidden)) return -1;
     return by_type(dtype, [&](auto t) { return backward_plan<decltype(t)>(rows, cols, hidden).bytes(); });
 }
 
@@ -105,7 +108,7 @@ int gpbo_gated_backward(int32_t device, void* stream, int32_t dtype, int32_t act
         !matrix_ok(hidden, cols, w_stride) || !matrix_ok(rows, hidden, dh_stride) || device < 0 || device >= MAX_DEVICES)
         return GPBO_ERR_BAD_ARG;
     if (!!dwg != !!dwu || (dx && !matrix_ok(rows, cols, dx_stride)) || (dwg && !matrix_ok(hidden, cols, dw_stride))) return GPBO_ERR_BAD_ARG;
-    if (ceil_div(rows, TB) * ceil_div(cols, TB) > MOST || ceil_div(hidden, TB) * ceil_div(cols, TB) > MOST) return GPBO_ERR_BAD_ARG;
+    if (!unit_ok(rows, cols, hidden)) return GPBO_ERR_BAD_ARG;
     if (rows > 0 && (!dh || !x || !wg || !wu || !keep_g || !keep_u)) return GPBO_ERR_BAD_ARG;
     if (!work_ok(workspace, workspace_bytes, gpbo_gated_backward_workspace(dtype, rows, cols, hidden))) return GPBO_ERR_BAD_ARG;
     DeviceGuard guard(device);

@@ -431,7 +431,7 @@ template <typename T, int R>
 __global__ __launch_bounds__(256) void k_gated_few(GatedArgs g) {
     constexpr int V = Pack<T>::N;
     const int lane = threadIdx.x & 63;
-    const int64_t h = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), row0 = (int64_t)blockIdx.y * R;
+    const int64_t h = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6), row0 = (int64_t)blockIdx.y * R;
     if (h >= g.n) return;
     const T *wg = (const T*)g.b[0].p + h * g.b[0].sr, *wu = (const T*)g.b[1].p + h * g.b[1].sr;
     const T* x[R];

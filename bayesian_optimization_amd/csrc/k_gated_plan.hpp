@@ -10,6 +10,23 @@ inline bool aligned16(const void* p, int64_t stride, int64_t bytes) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * bytes % 16 == 0 && stride * bytes < (1 << 23);
 }
 
+// A launch takes fewer than 2^32 threads: at 256 for 64 x 64 outputs, 2^23 such tiles at a time.  MOST_ACROSS columns of outputs (also the
+// most that the entry points take) leave 128 rows of them.
+constexpr int64_t MOST_ACROSS = 1 << 28;
+template <typename T, typename L>
+void by_rows(const GatedArgs& g, L&& launch) {
+    const int64_t most = ((int64_t)1 << 23) / ceil_div(g.n, TB) * TB;
+    for (int64_t r = 0; r < g.m; r += most) {
+        GatedArgs p = g;
+        p.m = std::min(most, g.m - r);
+        for (Operand* o : {&p.a[0], &p.a[1], &p.rest[0], &p.rest[1]})
+            if (o->p) o->p = (const T*)o->p + r * o->sr;
+        p.out[0] = (T*)g.out[0] + r * g.os;
+        if (g.keep_g) p.keep_g = g.keep_g + r * g.n, p.keep_u = g.keep_u + r * g.n;
+        launch(p);
+    }
+}
+
 // Few hidden units in 32 bits: a wave has 32 rows, so it takes 16384 of them to give every second SIMD one, and x has to outweigh the
 // rest (20000 x 483 -> 24: forward 20 us, 25 with the small form; with the backward pass 74 and 141; 1 M x 621 -> 24: 0.99 and 2.9 ms,
 // 3.5 and 10.2 with the tiles for large operands).
@@ -41,7 +58,7 @@ inline int better_tile(int64_t t256, int64_t t128) {
 struct ForwardPlan {
     bool narrow = false, fast = false, stream = false;
     int tile = 128;
-    int64_t kp = 0, x_bytes = 0, w_bytes = 0;
+    int64_t kp = 0, rows = 0, x_bytes = 0, w_bytes = 0;      // rows: of x packed at a time
     int64_t bytes() const { return fast ? x_bytes + 2 * w_bytes : 0; }
 };
 // The loads straight into LDS need whole steps and 16-byte rows.  What has neither is packed into the workspace first, which pays from
@@ -59,7 +76,9 @@ ForwardPlan forward_plan(int64_t m, int64_t k, int64_t h) {
     p.stream = sizeof(T) == 2 && p.kp <= STREAM_MOST && m * h >= (int64_t)1 << 21 && ceil_div(m, STREAM_ROWS) * ceil_div(h, 256) >= 512;
     p.fast = p.fast || p.stream;
     if (k >= 8 * KS) p.tile = better_tile(ceil_div(m, 256) * ceil_div(h, 128), ceil_div(m, 128) * ceil_div(h, 64));
-    p.x_bytes = round_up(m * p.kp * (int64_t)sizeof(T), 256);
+    // (8 GB of rows at most: a thousand of the longest, and a few columns are padded to many times their size)
+    p.rows = std::max<int64_t>(1, std::min(m, ((int64_t)1 << 33) / (p.kp * (int64_t)sizeof(T))));
+    p.x_bytes = round_up(p.rows * p.kp * (int64_t)sizeof(T), 256);
     p.w_bytes = round_up(h * p.kp * (int64_t)sizeof(T), 256);
     return p;
 }
@@ -94,8 +113,10 @@ void launch_stream(hipStream_t st, const GatedArgs& g) {
 }
 
 inline void launch_narrow(hipStream_t st, const GatedArgs& g) {
-    by_fragments(narrow_fragments(g.n), [&](auto f) {
-        hipLaunchKernelGGL(k_gated_narrow<f.value>, dim3((unsigned)ceil_div(g.m, 128)), dim3(256), 0, st, g);
+    by_rows<float>(g, [&](const GatedArgs& part) {
+        by_fragments(narrow_fragments(g.n), [&](auto f) {
+            hipLaunchKernelGGL(k_gated_narrow<f.value>, dim3((unsigned)ceil_div(part.m, 128)), dim3(256), 0, st, part);
+        });
     });
 }
 
@@ -107,26 +128,35 @@ hipError_t gated_forward(hipStream_t st, GatedArgs g, char* work) {
     if (p.narrow && std::max(g.a[0].sr, g.b[0].sr) < NARROW_STRIDE) {
         launch_narrow(st, g);
     } else if (p.fast) {
-        if (!direct || g.k % KS != 0) {
-            PackArgs a{};
-            a.count = 3;
-            a.job[0] = {g.a[0].p, g.a[0].sr, g.m, g.k, work, p.kp, ceil_div(g.m, 64) * ceil_div(p.kp, 64)};
-            a.job[1] = {g.b[0].p, g.b[0].sr, g.n, g.k, work + p.x_bytes, p.kp, ceil_div(g.n, 64) * ceil_div(p.kp, 64)};
-            a.job[2] = {g.b[1].p, g.b[1].sr, g.n, g.k, work + p.x_bytes + p.w_bytes, p.kp, ceil_div(g.n, 64) * ceil_div(p.kp, 64)};
-            hipLaunchKernelGGL((k_gated_pack<T, false>), dim3((unsigned)(a.job[0].blocks + a.job[1].blocks + a.job[2].blocks)), dim3(256), 0, st, a);
-            g.a[0] = {a.job[0].dst, p.kp, 1}, g.b[0] = {a.job[1].dst, p.kp, 1}, g.b[1] = {a.job[2].dst, p.kp, 1};
-            g.k = p.kp;
+        auto launch = [&](const GatedArgs& part) { p.stream ? launch_stream<T>(st, part) : launch_fast<T, GATED_FWD>(st, part, p.tile); };
+        if (direct && g.k % KS == 0) {
+            by_rows<T>(g, launch);
+        } else {
+            for (int64_t r = 0; r < g.m; r += p.rows) {      // (weights with the first rows)
+                GatedArgs part = g;
+                part.m = std::min(p.rows, g.m - r);
+                PackArgs a{};
+                a.count = r == 0 ? 3 : 1;
+                a.job[0] = {(const T*)g.a[0].p + r * g.a[0].sr, g.a[0].sr, part.m, g.k, work, p.kp, ceil_div(part.m, 64) * ceil_div(p.kp, 64)};
+                a.job[1] = {g.b[0].p, g.b[0].sr, g.n, g.k, work + p.x_bytes, p.kp, ceil_div(g.n, 64) * ceil_div(p.kp, 64)};
+                a.job[2] = {g.b[1].p, g.b[1].sr, g.n, g.k, work + p.x_bytes + p.w_bytes, p.kp, a.job[1].blocks};
+                hipLaunchKernelGGL((k_gated_pack<T, false>), dim3((unsigned)(a.job[0].blocks + (r == 0 ? 2 * a.job[1].blocks : 0))), dim3(256), 0, st, a);
+                part.a[0] = {work, p.kp, 1}, part.b[0] = {a.job[1].dst, p.kp, 1}, part.b[1] = {a.job[2].dst, p.kp, 1}, part.k = p.kp;
+                part.out[0] = (T*)g.out[0] + r * g.os;
+                if (g.keep_g) part.keep_g = g.keep_g + r * g.n, part.keep_u = g.keep_u + r * g.n;
+                by_rows<T>(part, launch);
+            }
         }
-        if (p.stream) launch_stream<T>(st, g);
-        else launch_fast<T, GATED_FWD>(st, g, p.tile);
     } else if (g.m <= 16) {
-        const unsigned hidden = (unsigned)ceil_div(g.n, 4);
-        if (g.m == 1) hipLaunchKernelGGL((k_gated_few<T, 1>), dim3(hidden, 1), dim3(256), 0, st, g);
-        else if (g.m == 2) hipLaunchKernelGGL((k_gated_few<T, 2>), dim3(hidden, 1), dim3(256), 0, st, g);
-        else if (g.m <= 4) hipLaunchKernelGGL((k_gated_few<T, 4>), dim3(hidden, 1), dim3(256), 0, st, g);
-        else hipLaunchKernelGGL((k_gated_few<T, 8>), dim3(hidden, (unsigned)ceil_div(g.m, 8)), dim3(256), 0, st, g);
+        const int64_t fours = ceil_div(g.n, 4), x = std::min<int64_t>(fours, 1 << 22);
+        const dim3 grid((unsigned)x, (unsigned)ceil_div(g.m, 8), (unsigned)ceil_div(fours, x));
+        if (g.m == 1) hipLaunchKernelGGL((k_gated_few<T, 1>), grid, dim3(256), 0, st, g);
+        else if (g.m == 2) hipLaunchKernelGGL((k_gated_few<T, 2>), grid, dim3(256), 0, st, g);
+        else if (g.m <= 4) hipLaunchKernelGGL((k_gated_few<T, 4>), grid, dim3(256), 0, st, g);
+        else hipLaunchKernelGGL((k_gated_few<T, 8>), grid, dim3(256), 0, st, g);
     } else {
-        launch_any<T, GATED_FWD, true, true, 1>(st, g, any_plan<T>(g.m, g.n, g.k, 1, false));
+        const AnyPlan any = any_plan<T>(g.m, g.n, g.k, 1, false);
+        by_rows<T>(g, [&](const GatedArgs& part) { launch_any<T, GATED_FWD, true, true, 1>(st, part, any); });
     }
     return hipGetLastError();
 }
@@ -212,12 +242,16 @@ hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const voi
         hipLaunchKernelGGL(k_gated_narrow_slopes, dim3((unsigned)std::min<int64_t>(ceil_div(m * g.hp / 4, 256), 8192)), dim3(256), 0, st,
                            (const float*)dh, dhs, kg, ku, m, h, act, (float*)work, g.hp);
         if (dx) {
-            g.out[0] = (float*)dx, g.os = dxs;
+            constexpr int64_t MOST = (int64_t)1 << 29;      // rows of a launch, at 4 threads a row or fewer
             by_fragments(fragments, [&](auto f) {
                 // (a wave of 16 rows, where d takes more registers, has three of its kind on a SIMD as well)
                 constexpr int RF = f.value <= 4 ? 2 : 1;
-                const int64_t walkers = ceil_div(m, 64 * RF), beside = std::max<int64_t>(1, std::min<int64_t>(ceil_div(k, 64), 1024 / walkers));
-                hipLaunchKernelGGL((k_gated_narrow_dx<RF, f.value>), dim3((unsigned)walkers, (unsigned)beside), dim3(256), 0, st, g);
+                for (int64_t r = 0; r < m; r += MOST) {
+                    NarrowBack part = g;
+                    part.m = std::min(MOST, m - r), part.d = g.d + r * 16 * f.value, part.out[0] = (float*)dx + r * dxs, part.os = dxs;
+                    const int64_t walkers = ceil_div(part.m, 64 * RF), beside = std::max<int64_t>(1, std::min<int64_t>(ceil_div(k, 64), 1024 / walkers));
+                    hipLaunchKernelGGL((k_gated_narrow_dx<RF, f.value>), dim3((unsigned)walkers, (unsigned)beside), dim3(256), 0, st, part);
+                }
             });
         }
         if (dwg) {
@@ -302,7 +336,9 @@ hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const voi
         } else {
             g.a[0] = {dg, h, 1}, g.a[1] = {du, h, 1}, g.b[0] = {wg, 1, ws}, g.b[1] = {wu, 1, ws}, g.k = h;
             g.rest[0] = {dg_rest, h, 1}, g.rest[1] = {du_rest, h, 1};
-            by_parts([&](auto parts) { launch_any<T, GATED_SUM, true, false, parts.value>(st, g, p.any_x); });
+            by_parts([&](auto parts) {
+                by_rows<T>(g, [&](const GatedArgs& part) { launch_any<T, GATED_SUM, true, false, parts.value>(st, part, p.any_x); });
+            });
         }
         if (g.splits > 1) hipLaunchKernelGGL(k_gated_join<T>, dim3((unsigned)ceil_div(m * k, 256), 1), dim3(256), 0, st, g);
     }

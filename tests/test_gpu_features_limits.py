@@ -25,3 +25,51 @@ def test_layer_norm_gradients_of_more_columns_than_a_launch_takes():
             want = terms.sum(0)      # three roundings a term and one of the sum in 32 bits, half a step of bfloat16 at the end
             assert bool(((got[at].double() - want).abs() <= 5 * 2.0 ** -24 * terms.abs().sum(0) + 2.0 ** -8 * 1.01 * want.abs()).all()), lo
     assert bool(torch.isfinite(dx).all())
+
+
+@pytest.mark.parametrize('dtype,rows,cols,hidden', [
+    (torch.bfloat16, (1 << 30) + 70, 1, 1),            # 2^24 tiles of 64 rows and more, in both directions
+    (torch.float32, (1 << 29) + 37, 1, 1),             # the kernels for few hidden units
+    (torch.float16, (1 << 27) + 100, 3, 2),            # rows packed into the workspace in pieces: a short contraction,
+    (torch.bfloat16, (1 << 23) + 5000000, 257, 2),     # and a longer one
+    (torch.bfloat16, 3, 1, (1 << 26) + 5)])            # hidden units, a wave each
+def test_gated_unit_of_more_than_a_launch_takes(dtype, rows, cols, hidden):
+    from bayesian_optimization_amd import features
+    U, H = 2.0 ** -24, torch.finfo(dtype).eps / 2
+    tiny = 2.0 ** -24 if dtype == torch.float16 else 1e-37
+    x, dh = rand((rows, cols), dtype, 3), rand((rows, hidden), dtype, 4)
+    wg, wu = rand((hidden, cols), dtype, 5, cols ** -0.5), rand((hidden, cols), dtype, 6, cols ** -0.5)
+    h, kept = features.gated_unit(x, wg, wu, keep=True)
+    dx, dwg, dwu = features.gated_unit_backward(dh, x, wg, wu, kept)
+    wgd, wud = wg.double(), wu.double()
+    sums = [torch.zeros(hidden, cols, dtype=torch.float64, device='cuda') for _ in range(4)]
+    step = max(1, (1 << 27) // (cols + hidden))
+    for lo in range(0, rows, step):
+        at = slice(lo, min(rows, lo + step))
+        xd, d = x[at].double(), dh[at].double()
+        g, u = xd @ wgd.t(), xd @ wud.t()
+        eg, eu = ((cols + 1) * U * (xd.abs() @ w.abs().t()) for w in (wgd, wud))
+        s = torch.sigmoid(g)
+        a, da = g * s, s * (1 + g * torch.sigmoid(-g))
+        assert bool(((kept[0, at].double() - g).abs() <= eg + 1e-37).all()) and bool(((kept[1, at].double() - u).abs() <= eu + 1e-37).all()), lo
+        # as in the tests of smaller sizes: |act'| <= 1.13, |act''| <= 0.8, some 16 roundings in the activation
+        ea = 1.13 * eg + 16 * U * (1 + g.abs()) * torch.minimum(g.abs(), torch.ones_like(g))
+        eda = 0.8 * eg + 16 * U * (1 + g.abs())
+        want = a * u
+        assert bool(((h[at].double() - want).abs() <= ea * u.abs() + a.abs() * eu + ea * eu + 2 * U * want.abs() + H * want.abs() * 1.01 + tiny).all()), lo
+        dg, du = d * u * da, d * a
+        edg = d.abs() * (eu * da.abs() + u.abs() * eda + eu * eda) + (H * 1.01 + 4 * U) * dg.abs() + tiny
+        edu = d.abs() * ea + (H * 1.01 + 4 * U) * du.abs() + tiny
+        if hidden < 1 << 20:       # (a sum over more: beyond what this tolerance says anything about)
+            want = dg @ wgd + du @ wud
+            terms = (dg.abs() + edg) @ wgd.abs() + (du.abs() + edu) @ wud.abs()
+            off = edg @ wgd.abs() + edu @ wud.abs() + (2 * hidden + 1) * U * terms + H * want.abs() * 1.01 + tiny
+            assert bool(((dx[at].double() - want).abs() <= off).all()), lo
+        for i, (v, e) in enumerate(((dg, edg), (du, edu)) if rows > 1000 else ()):
+            for k in range(cols):      # (a library's product over so many rows takes seconds)
+                xk = xd[:, k:k + 1]
+                sums[i][:, k] += (v * xk).sum(0)
+                sums[2 + i][:, k] += ((e + (rows / 2048 / 32 + 300) * U * v.abs()) * xk.abs()).sum(0)      # (256 pieces of 8 waves, 32 rows an instruction)
+    if rows > 1000:
+        for got, want, e in ((dwg, sums[0], sums[2]), (dwu, sums[1], sums[3])):
+            assert bool(((got.double() - want).abs() <= e + H * want.abs() * 1.01).all())
