@@ -122,6 +122,7 @@ SIGNATURES = {
     'gpbo_layernorm_backward': (C.c_int, [C.c_int32, _vp, C.c_int32, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp,
                                           _vp, _i64]),
     'gpbo_gated_workspace': (_i64, [C.c_int32, _i64, _i64, _i64]),
+    'gpbo_gated_workspace_for': (_i64, [C.c_int32, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64]),
     'gpbo_gated': (C.c_int, [C.c_int32, _vp, C.c_int32, C.c_int32, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp,
                              _i64]),
     'gpbo_gated_backward_workspace': (_i64, [C.c_int32, _i64, _i64, _i64]),

@@ -32,6 +32,13 @@ auto by_type(int32_t dtype, F&& f) {
     }
 }
 
+GatedArgs unit_of(const void* x, int64_t x_stride, int64_t rows, int64_t cols, const void* wg, const void* wu, int64_t w_stride, int64_t hidden) {
+    GatedArgs g{};
+    g.a[0] = {x, x_stride, 1}, g.b[0] = {wg, w_stride, 1}, g.b[1] = {wu, w_stride, 1};
+    g.m = rows, g.n = hidden, g.k = cols;
+    return g;
+}
+
 }  // namespace
 
 extern "C" {
@@ -78,6 +85,13 @@ int64_t gpbo_gated_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_t 
     return by_type(dtype, [&](auto t) { return forward_plan<decltype(t)>(rows, cols, hidden).bytes(); });
 }
 
+int64_t gpbo_gated_workspace_for(int32_t dtype, const void* x, int64_t x_stride, int64_t rows, int64_t cols, const void* wg, const void* wu,
+                                 int64_t w_stride, int64_t hidden) {
+    if (!is_float_type(dtype) || !unit_ok(rows, cols, hidden) || !matrix_ok(rows, cols, x_stride) || !matrix_ok(hidden, cols, w_stride)) return -1;
+    const GatedArgs g = unit_of(x, x_stride, rows, cols, wg, wu, w_stride, hidden);
+    return by_type(dtype, [&](auto t) { return forward_bytes<decltype(t)>(g); });
+}
+
 int gpbo_gated(int32_t device, void* stream, int32_t dtype, int32_t act, const void* x, int64_t x_stride, int64_t rows,
                int64_t cols, const void* wg, const void* wu, int64_t w_stride, int64_t hidden, void* h, int64_t h_stride,
                float* keep_g, float* keep_u, void* workspace, int64_t workspace_bytes) {
@@ -86,12 +100,13 @@ int gpbo_gated(int32_t device, void* stream, int32_t dtype, int32_t act, const v
         return GPBO_ERR_BAD_ARG;
     if (!!keep_g != !!keep_u || !unit_ok(rows, cols, hidden)) return GPBO_ERR_BAD_ARG;
     if (rows == 0) return GPBO_OK;
-    if (!x || !wg || !wu || !h || !work_ok(workspace, workspace_bytes, gpbo_gated_workspace(dtype, rows, cols, hidden))) return GPBO_ERR_BAD_ARG;
+    if (!x || !wg || !wu || !h ||
+        !work_ok(workspace, workspace_bytes, gpbo_gated_workspace_for(dtype, x, x_stride, rows, cols, wg, wu, w_stride, hidden)))
+        return GPBO_ERR_BAD_ARG;
     DeviceGuard guard(device);
     if (!guard.ok) return GPBO_ERR_HIP;
-    GatedArgs g{};
-    g.a[0] = {x, x_stride, 1}, g.b[0] = {wg, w_stride, 1}, g.b[1] = {wu, w_stride, 1};
-    g.m = rows, g.n = hidden, g.k = cols, g.out[0] = h, g.os = h_stride, g.keep_g = keep_g, g.keep_u = keep_u, g.act = act, g.splits = 1;
+    GatedArgs g = unit_of(x, x_stride, rows, cols, wg, wu, w_stride, hidden);
+    g.out[0] = h, g.os = h_stride, g.keep_g = keep_g, g.keep_u = keep_u, g.act = act, g.splits = 1;
     return result(by_type(dtype, [&](auto t) { return gated_forward<decltype(t)>((hipStream_t)stream, g, (char*)workspace); }));
 }
 

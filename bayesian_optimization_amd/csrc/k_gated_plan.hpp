@@ -120,16 +120,25 @@ inline void launch_narrow(hipStream_t st, const GatedArgs& g) {
     });
 }
 
+// Whether the loads straight into LDS can take the operands as they are.
+template <typename T>
+bool direct(const GatedArgs& g) {
+    return g.k * (int64_t)sizeof(T) % STEP_BYTES == 0 && aligned16(g.a[0].p, g.a[0].sr, sizeof(T)) && aligned16(g.b[0].p, g.b[0].sr, sizeof(T)) &&
+           aligned16(g.b[1].p, g.b[1].sr, sizeof(T));
+}
+template <typename T>
+int64_t forward_bytes(const GatedArgs& g) {
+    return direct<T>(g) ? 0 : forward_plan<T>(g.m, g.k, g.n).bytes();
+}
+
 template <typename T>
 hipError_t gated_forward(hipStream_t st, GatedArgs g, char* work) {
-    constexpr int KS = STEP_BYTES / sizeof(T);
     const ForwardPlan p = forward_plan<T>(g.m, g.k, g.n);
-    const bool direct = aligned16(g.a[0].p, g.a[0].sr, sizeof(T)) && aligned16(g.b[0].p, g.b[0].sr, sizeof(T)) && aligned16(g.b[1].p, g.b[1].sr, sizeof(T));
     if (p.narrow && std::max(g.a[0].sr, g.b[0].sr) < NARROW_STRIDE) {
         launch_narrow(st, g);
     } else if (p.fast) {
         auto launch = [&](const GatedArgs& part) { p.stream ? launch_stream<T>(st, part) : launch_fast<T, GATED_FWD>(st, part, p.tile); };
-        if (direct && g.k % KS == 0) {
+        if (direct<T>(g)) {
             by_rows<T>(g, launch);
         } else {
             for (int64_t r = 0; r < g.m; r += p.rows) {      // (weights with the first rows)

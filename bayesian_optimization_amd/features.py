@@ -90,6 +90,8 @@ def gated_unit(x, w_gate, w_up, act='silu', keep=False):
         kg = kept.data_ptr()
         ku = kg + 4 * rows * hidden
     nbytes = workspace('gpbo_gated_workspace', code, rows, cols, hidden)
+    if nbytes:      # that is for operands that have to be copied first
+        nbytes = L.load().gpbo_gated_workspace_for(code, x.data_ptr(), stride, rows, cols, w_gate.data_ptr(), w_up.data_ptr(), ws, hidden)
     work = scratch(nbytes, x.device)
     st = L.load().gpbo_gated(at, stream_of(at), code, a, x.data_ptr(), stride, rows, cols, w_gate.data_ptr(), w_up.data_ptr(), ws, hidden,
                              h.data_ptr(), hidden, kg, ku, pointer(work), nbytes)

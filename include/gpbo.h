@@ -387,6 +387,9 @@ int gpbo_layernorm_backward(int32_t device, void* stream, int32_t dtype, const v
  * dtype: GPBO_TYPE_F32, _BF16 or _F16 for all of these; sums in 32 bits.  keep_g, keep_u (rows, hidden; contiguous float32;
  * both or neither): x wg^T and x wu^T, for the backward pass.  cols and hidden are at most 2^28 (268,435,456). */
 int64_t gpbo_gated_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_t hidden);
+/* What a call on these very operands needs: nothing where they are read in place, whatever the function above says. */
+int64_t gpbo_gated_workspace_for(int32_t dtype, const void* x, int64_t x_stride, int64_t rows, int64_t cols, const void* wg, const void* wu,
+                                 int64_t w_stride, int64_t hidden);
 int gpbo_gated(int32_t device, void* stream, int32_t dtype, int32_t act, const void* x, int64_t x_stride, int64_t rows,
                int64_t cols, const void* wg, const void* wu, int64_t w_stride, int64_t hidden, void* h, int64_t h_stride,
                float* keep_g, float* keep_u, void* workspace, int64_t workspace_bytes);

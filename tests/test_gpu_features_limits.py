@@ -73,3 +73,21 @@ def test_gated_unit_of_more_than_a_launch_takes(dtype, rows, cols, hidden):
     if rows > 1000:
         for got, want, e in ((dwg, sums[0], sums[2]), (dwu, sums[1], sums[3])):
             assert bool(((got.double() - want).abs() <= e + H * want.abs() * 1.01).all())
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+def test_operands_read_in_place_are_not_copied(dtype):
+    """Memory that a call takes beside its result: none where rows are aligned and whole steps long, a copy of x and the weights else."""
+    from bayesian_optimization_amd import features
+    rows, cols, hidden = 1 << 17, 256, 512
+    x, w = rand((rows, cols + 8), dtype, 7), rand((hidden, cols + 8), dtype, 8, 0.1)
+    result = rows * hidden * x.element_size()
+    for a, b, copy in ((x[:, :cols], w[:, :cols], 0), (x[:, :cols].contiguous(), w[:, :cols].contiguous(), 0), (x[:, 1:cols + 1], w[:, 1:cols + 1], rows * cols * x.element_size())):
+        want = features.gated_unit(a, b, b)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        h = features.gated_unit(a, b, b)
+        assert copy <= torch.cuda.max_memory_allocated() - before - result <= copy * 1.02 + (1 << 20)
+        assert torch.equal(h, want)
+        del h, want
