@@ -7,8 +7,8 @@
 // u: rounded to 16 bits they would put two more roundings of the same size under every gradient.  h is rounded once.  dg and du are
 // operands of the matrix instructions, so of the type of x, rounded once each: in 16 bits, over a gradient's many elements, the error is
 // then 1.4 times that of the gradient's own rounding.  Over few elements, where terms may cancel in all of them, it can be several times
-// (3 with 10 in float16), so that there, and where it costs nothing, the products take a sum of two numbers of 16 bits: the rounded one
-// and what the rounding left.  (The whole-step kernels, whose gradients have 128 elements or more, take one.)
+// (3 with 10 in float16), so that there (under 4096 elements), and where it costs nothing, the products take a sum of two numbers of 16
+// bits: the rounded one and what the rounding left.
 #pragma once
 
 #include <type_traits>

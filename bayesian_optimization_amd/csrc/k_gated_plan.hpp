@@ -209,7 +209,12 @@ BackwardPlan backward_plan(int64_t m, int64_t k, int64_t h) {
     // bits 1.9 (1000 x 520 -> 1000, 4.2: 98 without, 66 with; 1000 x 520 -> 400, 1.7: 44 and 57) or, over many rows, 1 (2000 x 520 -> 200: 59
     // and 53); or two million elements over many rows.
     const int64_t enough = B == 4 ? (int64_t)1 << 32 : m >= 2000 ? (int64_t)1 << 30 : (int64_t)7 << 28;
-    p.fast = !p.narrow && m >= 128 && (8 * m * h * k >= enough || (m >= 4096 && std::max(h, k) >= 128 && m * std::max(h, k) >= (int64_t)1 << 21)) && m * B < (1 << 23) && h * B < (1 << 23);
+    // In two parts where a gradient has few elements (with the forward pass 20000 x 5 -> 77 bf16 57 us without, 64 with; 1000 x 520 ->
+    // 400, where it would take away less than the gradients' own roundings, 44 and 61).  The any-shape kernels do that, whatever the size: the
+    // whole-step kernels with a second part are slower still (backward 8192 x 1 -> 256 28 us, 88 with them, 35 with one part; 1 M x 60 -> 64
+    // 924, 1215 and 564).
+    const bool few_elements = SLOPE_PARTS<T> == 2 && std::min(m, h) * k < 4096;
+    p.fast = !p.narrow && !few_elements && m >= 128 && (8 * m * h * k >= enough || (m >= 4096 && std::max(h, k) >= 128 && m * std::max(h, k) >= (int64_t)1 << 21)) && m * B < (1 << 23) && h * B < (1 << 23);
     if (p.fast) {
         p.hp = round_up(h, 64), p.mp = round_up(m, 64);
         auto choose = [&](int64_t rows, int64_t cols, int64_t zs, int64_t steps, int& tile, int& splits) {
@@ -227,9 +232,7 @@ BackwardPlan backward_plan(int64_t m, int64_t k, int64_t h) {
         // (27 to 29 and 30), worse from there on (1000 x 30 -> 24: 44, 20 x 30 -> 1000: 60)
         p.one = m > 0 && 4 * m * h * ceil_div(k, SB) <= (int64_t)1 << 20 && std::max(m, 2 * h) <= 512;
         if (p.one) return p;
-        // in two parts where a gradient has few elements (with the forward pass 20000 x 5 -> 77 bf16 57 us without, 64 with; 1000 x 520 ->
-        // 400, where it would take away less than the gradients' own roundings, 44 and 61)
-        p.d_bytes = round_up(m * h * B, 256), p.parts = SLOPE_PARTS<T> == 2 && std::min(m, h) * k < 4096, p.rest_bytes = p.parts ? p.d_bytes : 0;
+        p.d_bytes = round_up(m * h * B, 256), p.parts = few_elements, p.rest_bytes = p.parts ? p.d_bytes : 0;
         p.any_x = any_plan<T>(m, k, h, 1, true), p.any_w = any_plan<T>(h, k, m, 2, true);
         p.splits_x = p.any_x.splits, p.splits_w = p.any_w.splits;
     }

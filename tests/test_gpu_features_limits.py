@@ -3,6 +3,8 @@ import numpy as np
 import pytest
 import torch
 
+from test_gpu_features import check_gated, half
+
 pytestmark = pytest.mark.gpu
 
 
@@ -91,3 +93,12 @@ def test_operands_read_in_place_are_not_copied(dtype):
         assert copy <= torch.cuda.max_memory_allocated() - before - result <= copy * 1.02 + (1 << 20)
         assert torch.equal(h, want)
         del h, want
+
+
+# Gradients of few elements among many rows or hidden units, which the kernels for large operands take: split contractions, both products
+@pytest.mark.parametrize('rows,cols,hidden', [(8192, 1, 256), (4096, 512, 1), (300000, 60, 64), (100003, 31, 128), (70000, 128, 16), (40001, 1000, 4), (131072, 25, 150), (128, 30, 100000)])
+@pytest.mark.parametrize('act', ['silu', 'gelu'])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_gradients_of_few_elements_among_many_rows(dtype, act, rows, cols, hidden):
+    """dg and du as two numbers there too: off by the square of half a step, not by half a step."""
+    check_gated(dtype, act, rows, cols, hidden, slope=half(dtype) ** 2)
