@@ -5,10 +5,10 @@
 // same workgroup from one staged tile of x, so the activation and the product are an epilogue on the accumulators and g, u
 // never go to memory unless the caller keeps them for the backward pass.  Sums are held in 32 bits, and so are the kept g and
 // u: rounded to 16 bits they would put two more roundings of the same size under every gradient.  h is rounded once.  dg and du are
-// operands of the matrix instructions, so of the type of x, rounded once each: in 16 bits, over a gradient's many elements, the error is
-// then 1.4 times that of the gradient's own rounding.  Over few elements, where terms may cancel in all of them, it can be several times
-// (3 with 10 in float16), so that there (under 4096 elements), and where it costs nothing, the products take a sum of two numbers of 16
-// bits: the rounded one and what the rounding left.
+// operands of the matrix instructions, so of the type of x, rounded once each (in float16 scaled into its range): in 16 bits, over a gradient's
+// many elements, the error is then 1.4 times that of the gradient's own rounding.  Over few elements, where terms may cancel in all of
+// them, it can be several times (3 with 10 in float16), so that there (under 4096 elements) the products take a sum of two numbers of 16
+// bits: the rounded one and what the rounding left.  The kernels for small problems and for few columns take them in 32 bits.
 #pragma once
 
 #include <type_traits>
@@ -99,7 +99,39 @@ struct GatedArgs {
     float *keep_g, *keep_u;       // (m, n) contiguous, or null
     int act, splits;
     float* part;                  // splits > 1: [z][split][m][n] sums in 32 bits
+    const float* range;           // float16: the range of a, or null
 };
+
+// Float16 holds 40 powers of two, of which dg and du, products of three numbers, leave any one part: below 6e-8 they would be nothing and beyond
+// 65504 infinite where the gradients themselves are neither.  So in float16 they are multiplied by the power of two that puts the largest
+// of both next to the upper end, and the products by its inverse: exact, and what is lost at the lower end is 2^-39 of the largest.
+// k_gated_range leaves the largest in 256 pieces, which every wave that needs the factor puts together.
+template <typename T>
+constexpr bool RANGED = std::is_same_v<T, f16>;
+constexpr int RANGE_PIECES = 256;
+constexpr int64_t RANGE_BYTES = RANGE_PIECES * 4;
+// The exponent of the factor; all lanes of the wave take part.
+__device__ __forceinline__ int range_exponent(const float* range) {
+    if (!range) return 0;
+    f32x4 v;
+    __builtin_memcpy(&v, range + (threadIdx.x & 63) * 4, 16);
+    float most = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+    if (!(most > 0.0f)) return 0;
+    return min(100, 14 + 127 - (int)(__float_as_uint(most) >> 23));      // the largest comes to 2^14 .. 2^15
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+template <typename T>
+__device__ __forceinline__ float range_up(const float* range) {
+    if constexpr (RANGED<T>) return power_of_two(range_exponent(range));
+    return 1.0f;
+}
+template <typename T>
+__device__ __forceinline__ float range_down(const float* range) {
+    if constexpr (RANGED<T>) return power_of_two(-range_exponent(range));
+    return 1.0f;
+}
 
 // Numbers of type T that make up one element of dg and du where they are not rounded to one.
 template <typename T>
@@ -224,6 +256,8 @@ __global__ __launch_bounds__(256) void k_gated_tile(GatedArgs g) {
         }
         __syncthreads();
     }
+    float down = 1.0f;
+    if constexpr (MODE != GATED_FWD) down = range_down<T>(g.range);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -243,7 +277,7 @@ __global__ __launch_bounds__(256) void k_gated_tile(GatedArgs g) {
                 } else {
                     const float v = acc[0][i][j][r];
                     if (g.splits > 1) g.part[(((int64_t)z * g.splits + split) * g.m + row) * g.n + col + r] = v;
-                    else ((T*)g.out[z])[row * g.os + col + r] = from_float<T>(v);
+                    else ((T*)g.out[z])[row * g.os + col + r] = from_float<T>(v * down);
                 }
             }
         }
@@ -270,49 +304,61 @@ __device__ __forceinline__ uint4 small_fragment(const Operand& o, int64_t row, i
     return __builtin_bit_cast(uint4, r);
 }
 
-// What the backward products of a small problem need of dg (which = 0) and du (1), computed where it is used, in the parts that
-// k_gated_slopes would write: element (row, k) of the operand is element (row, k) of dh, g, u if KC, else (k, row).
+// What the backward products of a small problem need of dg (which = 0) and du (1), computed where it is used, in 32 bits: element (row, k)
+// of the operand is element (row, k) of dh, g, u if KC, else (k, row).
 struct SlopeOperand {
     const void* dh;
     const float *kg, *ku;
     int64_t dhs, n;               // row strides of dh; of kg and ku
     int act;
 };
+template <typename T>
+struct Slopes {
+    float v[Pack<T>::N];
+};
 template <typename T, bool KC, bool WHOLE>
-__device__ __forceinline__ Parts<SLOPE_PARTS<T>> slope_fragment(const SlopeOperand& o, int which, int64_t row, int64_t k, int64_t k1) {
-    constexpr int V = 16 / sizeof(T);
-    Pack<T> r[SLOPE_PARTS<T>];
+__device__ __forceinline__ Slopes<T> slope_fragment(const SlopeOperand& o, int which, int64_t row, int64_t k, int64_t k1) {
+    Slopes<T> r;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
+    for (int j = 0; j < Pack<T>::N; ++j) {
         const int64_t i = KC ? row : k + j, c = KC ? k + j : row;
+        r.v[j] = 0.0f;
         if (WHOLE || k + j < k1) {
             float a, da;
             activation<T>(o.kg[i * o.n + c], o.act, a, da);
             const float d = to_float(((const T*)o.dh)[i * o.dhs + c]);
-            const float slope = which ? d * a : d * o.ku[i * o.n + c] * da;
-            r[0].v[j] = from_float<T>(slope);
-            if constexpr (SLOPE_PARTS<T> == 2) r[1].v[j] = rounding_rest(slope, r[0].v[j]);
-        } else {
-#pragma unroll
-            for (int q = 0; q < SLOPE_PARTS<T>; ++q) r[q].v[j] = from_float<T>(0.0f);
+            r.v[j] = which ? d * a : d * o.ku[i * o.n + c] * da;
         }
     }
-    Parts<SLOPE_PARTS<T>> parts;
-#pragma unroll
-    for (int q = 0; q < SLOPE_PARTS<T>; ++q) parts.v[q] = __builtin_bit_cast(uint4, r[q]);
-    return parts;
+    return r;
 }
 
-// The body: NB products side by side (one first operand, of NA parts, NB second ones), slabs of contraction [kb, ke) dealt to the waves; fa(i, k, whole)
+// A fragment of the second operand against one of the first, in parts of the same type or in 32 bits (instructions of 32 bits then, which take
+// element j of every lane: a sixteenth of the speed, over a contraction of a few hundred).
+template <typename T, int NA>
+__device__ __forceinline__ f32x4 product(const uint4& b, const Parts<NA>& a, f32x4 c) {
+#pragma unroll
+    for (int p = 0; p < NA; ++p) c = mma<T>(b, a.v[p], c);
+    return c;
+}
+template <typename T>
+__device__ __forceinline__ f32x4 product(const uint4& b, const Slopes<T>& a, f32x4 c) {
+    const Pack<T> v = __builtin_bit_cast(Pack<T>, b);
+#pragma unroll
+    for (int j = 0; j < Pack<T>::N; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(to_float(v.v[j]), a.v[j], c, 0, 0, 0);
+    return c;
+}
+
+// The body: NB products side by side (one first operand, in fragments of type A, NB second ones), slabs of contraction [kb, ke) dealt to the waves; fa(i, k, whole)
 // and fb(b, i, k, whole) give fragments i < FR.
-template <typename T, int NA, int NB, int FR, typename FA, typename FB>
+template <typename T, typename A, int NB, int FR, typename FA, typename FB>
 __device__ __forceinline__ void small_sums(f32x4 (&acc)[NB][FR][FR], int64_t kb, int64_t ke, FA&& fa, FB&& fb) {
     constexpr int SLAB = 64 / sizeof(T), V = 16 / sizeof(T);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t slabs = (ke - kb) / SLAB;
     auto slab = [&](int64_t k0, auto whole) {
         const int64_t k = k0 + (lane >> 4) * V;
-        Parts<NA> a[FR];
+        A a[FR];
         uint4 b[NB][FR];
 #pragma unroll
         for (int i = 0; i < FR; ++i) {
@@ -325,9 +371,7 @@ __device__ __forceinline__ void small_sums(f32x4 (&acc)[NB][FR][FR], int64_t kb,
 #pragma unroll
             for (int i = 0; i < FR; ++i)
 #pragma unroll
-                for (int j = 0; j < FR; ++j)
-#pragma unroll
-                    for (int p = 0; p < NA; ++p) acc[q][i][j] = mma<T>(b[q][j], a[i].v[p], acc[q][i][j]);
+                for (int j = 0; j < FR; ++j) acc[q][i][j] = product<T>(b[q][j], a[i], acc[q][i][j]);
     };
 #pragma unroll 4
     for (int64_t s = wave; s < slabs; s += SMALL_WAVES) slab(kb + s * SLAB, std::true_type{});
@@ -371,7 +415,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small(GatedArgs g) {
     for (int part = 0; part < (MODE == GATED_SUM ? 2 : 1); ++part) {
         const Operand oa = MODE == GATED_PAIR && z ? g.a[1] : g.a[part], ob = g.b[part], ob2 = g.b[1];
         const Operand rest = MODE == GATED_PAIR && z ? g.rest[1] : g.rest[part];
-        small_sums<T, NA, NB, FR>(acc, kb, ke, [&](int i, int64_t k, auto whole) {
+        small_sums<T, Parts<NA>, NB, FR>(acc, kb, ke, [&](int i, int64_t k, auto whole) {
                               Parts<NA> r;
                               r.v[0] = small_fragment<T, AKC, whole.value>(oa, ra[i], k, ke);
                               if constexpr (NA == 2) r.v[1] = small_fragment<T, AKC, whole.value>(rest, ra[i], k, ke);
@@ -382,6 +426,8 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small(GatedArgs g) {
     f32x4 v[NB];
     small_join<NB, FR>(acc, v, sums);
     if (wave >= FR * FR) return;
+    float down = 1.0f;
+    if constexpr (MODE != GATED_FWD) down = range_down<T>(g.range);
     const int64_t row = row0 + wave / FR * 16 + (lane & 15), col = col0 + wave % FR * 16 + (lane >> 4) * 4;
     if (row >= g.m) return;
 #pragma unroll
@@ -393,14 +439,15 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small(GatedArgs g) {
         } else if (g.splits > 1) {
             g.part[(((int64_t)z * g.splits + split) * g.m + row) * g.n + col + r] = v[0][r];
         } else {
-            ((T*)(z ? g.out[1] : g.out[0]))[row * g.os + col + r] = from_float<T>(v[0][r]);
+            ((T*)(z ? g.out[1] : g.out[0]))[row * g.os + col + r] = from_float<T>(v[0][r] * down);
         }
     }
 }
 
 // The whole backward pass of a small problem in one launch: the tiles of dx, then those of dwg and of dwu, each with its part of dg
 // and du computed on the way into the matrix instructions (every tile column again, which is why it has to be small; 95 x 621 -> 128 in
-// 32 bits: 14 us, bound by the chain of loads and erfc; forward + backward 25 us, 31 with three launches).
+// 32 bits: 14 us, bound by the chain of loads and erfc; forward + backward 25 us, 31 with three launches).  dg and du stay in 32 bits, and
+// so do the products: as two numbers of 16 bits they took as long, and in float16 a launch more for their range.
 template <typename T>
 __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small_back(SlopeOperand s, Operand x, Operand wg, Operand wu, int64_t m, int64_t k, int64_t h,
                                                                        void* dx, int64_t dxs, void* dwg, void* dwu, int64_t dws) {
@@ -423,7 +470,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small_back(SlopeOper
         for (int i = 0; i < 2; ++i) ra[i] = min(row0 + i * 16 + (lane & 15), m - 1);
 #pragma unroll
         for (int which = 0; which < 2; ++which)
-            small_sums<T, SLOPE_PARTS<T>, 1, 2>(acc, 0, h, [&](int i, int64_t q, auto whole) { return slope_fragment<T, true, whole.value>(s, which, ra[i], q, h); },
+            small_sums<T, Slopes<T>, 1, 2>(acc, 0, h, [&](int i, int64_t q, auto whole) { return slope_fragment<T, true, whole.value>(s, which, ra[i], q, h); },
                              [&](int, int i, int64_t q, auto whole) { return small_fragment<T, false, whole.value>(which ? wu : wg, rb[i], q, h); });
     } else {                                   // dw = d^T x, contraction over the rows
         id -= tiles_x;
@@ -433,7 +480,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small_back(SlopeOper
         int64_t ra[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) ra[i] = min(row0 + i * 16 + (lane & 15), h - 1);
-        small_sums<T, SLOPE_PARTS<T>, 1, 2>(acc, 0, m, [&](int i, int64_t q, auto whole) { return slope_fragment<T, false, whole.value>(s, which, ra[i], q, m); },
+        small_sums<T, Slopes<T>, 1, 2>(acc, 0, m, [&](int i, int64_t q, auto whole) { return slope_fragment<T, false, whole.value>(s, which, ra[i], q, m); },
                          [&](int, int i, int64_t q, auto whole) { return small_fragment<T, false, whole.value>(x, rb[i], q, m); });
     }
     small_join<1, 2>(acc, v, sums);
@@ -449,21 +496,67 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small_back(SlopeOper
 template <typename T>
 __global__ __launch_bounds__(256) void k_gated_join(GatedArgs g) {
     const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, z = blockIdx.y;
+    const float down = range_down<T>(g.range);
     if (e >= g.m * g.n) return;
     const float* p = g.part + z * g.splits * g.m * g.n + e;
     float v = 0.0f;
 #pragma unroll 8
     for (int s = 0; s < g.splits; ++s) v += p[(int64_t)s * g.m * g.n];
-    ((T*)g.out[z])[e / g.n * g.os + e % g.n] = from_float<T>(v);
+    ((T*)g.out[z])[e / g.n * g.os + e % g.n] = from_float<T>(v * down);
+}
+
+// The largest finite |dg| and |du|, in pieces.  One more pass over dh and the kept products (16384 x 8192: 0.3 ms).
+constexpr int RANGE_THREADS = 1024;
+template <typename T>
+__global__ __launch_bounds__(RANGE_THREADS) void k_gated_range(const T* __restrict__ dh, int64_t dhs, const float* __restrict__ kg, const float* __restrict__ ku,
+                                                     int64_t m, int64_t n, int act, float* __restrict__ range) {
+    constexpr int V = 4;
+    const int64_t packs = (n + V - 1) / V;
+    float most = 0.0f;
+    auto look = [&](float d, float gv, float uv) {
+        float a, da;
+        activation<T>(gv, act, a, da);
+        const float g = fabsf(d * uv * da), u = fabsf(d * a);
+        most = fmaxf(most, g < INFINITY ? g : 0.0f);
+        most = fmaxf(most, u < INFINITY ? u : 0.0f);
+    };
+    for (int64_t id = (int64_t)blockIdx.x * RANGE_THREADS + threadIdx.x; id < m * packs; id += (int64_t)gridDim.x * RANGE_THREADS) {
+        const int64_t row = id / packs, c = (id % packs) * V, e = row * n + c;
+        const T* d = dh + row * dhs + c;
+        if (c + V <= n) {
+            T pd[V];
+            float gv[V], uv[V];
+            __builtin_memcpy(pd, d, sizeof(pd));
+            __builtin_memcpy(gv, kg + e, sizeof(gv));
+            __builtin_memcpy(uv, ku + e, sizeof(uv));
+#pragma unroll
+            for (int i = 0; i < V; ++i) look(to_float(pd[i]), gv[i], uv[i]);
+        } else {
+            for (int i = 0; c + i < n; ++i) look(to_float(d[i]), kg[e + i], ku[e + i]);
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+    __shared__ float waves[RANGE_THREADS / 64];
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = most;
+    __syncthreads();
+    // a piece a workgroup; the first one clears those that no workgroup has
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int i = 0; i < RANGE_THREADS / 64; ++i) most = fmaxf(most, waves[i]);
+        range[blockIdx.x] = most;
+    }
+    if (blockIdx.x == 0 && threadIdx.x >= gridDim.x && threadIdx.x < RANGE_PIECES) range[threadIdx.x] = 0.0f;
 }
 
 // dg = dh u act'(g), du = dh act(g), and what their roundings left.
 template <typename T, bool REST>
 __global__ __launch_bounds__(256) void k_gated_slopes(const T* __restrict__ dh, int64_t dhs, const float* __restrict__ kg,
-                                                      const float* __restrict__ ku, int64_t m, int64_t n, int act, T* __restrict__ dg,
-                                                      T* __restrict__ du, T* __restrict__ dg_rest, T* __restrict__ du_rest) {
+                                                      const float* __restrict__ ku, int64_t m, int64_t n, int act, const float* range,
+                                                      T* __restrict__ dg, T* __restrict__ du, T* __restrict__ dg_rest, T* __restrict__ du_rest) {
     constexpr int V = Pack<T>::N;
     const int64_t packs = (n + V - 1) / V;
+    const float up = range_up<T>(range);
     for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < m * packs; id += (int64_t)gridDim.x * 256) {
         const int64_t row = id / packs, c = (id % packs) * V;
         const int64_t e = row * n + c;
@@ -487,7 +580,7 @@ __global__ __launch_bounds__(256) void k_gated_slopes(const T* __restrict__ dh, 
         for (int i = 0; i < V; ++i) {
             float a, da;
             activation<T>(gv[i], act, a, da);
-            const float sg = to_float(pd.v[i]) * uv[i] * da, su = to_float(pd.v[i]) * a;
+            const float sg = to_float(pd.v[i]) * uv[i] * da * up, su = to_float(pd.v[i]) * a * up;
             og.v[i] = from_float<T>(sg), ou.v[i] = from_float<T>(su);
             if constexpr (REST) rg.v[i] = rounding_rest(sg, og.v[i]), ru.v[i] = rounding_rest(su, ou.v[i]);
         }

@@ -137,6 +137,8 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 256 ? 1 : 2) void k_gated_fast(
 
     // lane: row lane % 16 of a fragment, eight neighbouring columns of a pair of them
     static_assert(FN % 4 == 0, "fragments come in pairs, of both weight matrices");
+    float down = 1.0f;
+    if constexpr (MODE != GATED_FWD) down = range_down<T>(g.splits > 1 ? nullptr : g.range);
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
         const int64_t row = row0 + wm * FM * 16 + i * 16 + (lane & 15);
@@ -151,7 +153,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 256 ? 1 : 2) void k_gated_fast(
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
                 if constexpr (MODE == GATED_FWD) v[r] = activate<T>(acc[i][j + (r >> 2)][r & 3], g.act) * acc[i][j + (r >> 2) + UP][r & 3];
-                else v[r] = acc[i][j + (r >> 2)][r & 3];
+                else v[r] = acc[i][j + (r >> 2)][r & 3] * down;
             }
             if (MODE != GATED_FWD && g.splits > 1) {
                 float* p = g.part + (((int64_t)z * g.splits + split) * g.m + row) * g.n + col;
@@ -252,9 +254,10 @@ __global__ __launch_bounds__(256) void k_gated_pack(PackArgs a) {
 // 0.53 ms for 2.4 GB).
 template <typename T>
 __global__ __launch_bounds__(256) void k_gated_slopes_both(const T* __restrict__ dh, int64_t dhs, const float* __restrict__ kg,
-                                                           const float* __restrict__ ku, int64_t m, int64_t n, int act, T* __restrict__ dg,
-                                                           T* __restrict__ du, int64_t hp, T* __restrict__ dgt, T* __restrict__ dut, int64_t mp) {
+                                                           const float* __restrict__ ku, int64_t m, int64_t n, int act, const float* range,
+                                                           T* __restrict__ dg, T* __restrict__ du, int64_t hp, T* __restrict__ dgt, T* __restrict__ dut, int64_t mp) {
     __shared__ T tg[64][66], tu[64][66];
+    const float up = range_up<T>(range);
     const int64_t tiles_c = hp / 64, r0 = blockIdx.x / tiles_c * 64, c0 = blockIdx.x % tiles_c * 64;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;      // four columns a thread, 16 rows a pass
 #pragma unroll
@@ -278,8 +281,8 @@ __global__ __launch_bounds__(256) void k_gated_slopes_both(const T* __restrict__
         for (int k = 0; k < 4; ++k) {
             float a, da;
             activation<T>(gv[k], act, a, da);
-            og[k] = from_float<T>(k < len ? to_float(dv[k]) * uv[k] * da : 0.0f);
-            ou[k] = from_float<T>(k < len ? to_float(dv[k]) * a : 0.0f);
+            og[k] = from_float<T>(k < len ? to_float(dv[k]) * uv[k] * da * up : 0.0f);
+            ou[k] = from_float<T>(k < len ? to_float(dv[k]) * a * up : 0.0f);
             tg[ty + i * 16][tx * 4 + k] = og[k];
             tu[ty + i * 16][tx * 4 + k] = ou[k];
         }

@@ -178,10 +178,10 @@ struct BackwardPlan {
     int tile_x = 128, tile_w = 128, splits_x = 1, splits_w = 1;
     AnyPlan any_x, any_w;
     int64_t hp = 0, mp = 0;
-    int64_t d_bytes = 0, rest_bytes = 0, dt_bytes = 0, xt_bytes = 0, wt_bytes = 0, part_bytes = 0;
+    int64_t range_bytes = 0, d_bytes = 0, rest_bytes = 0, dt_bytes = 0, xt_bytes = 0, wt_bytes = 0, part_bytes = 0;
     int splits_narrow = 1;
     int64_t narrow_d_bytes = 0, narrow_bytes = 0;
-    int64_t bytes() const { return std::max(narrow_bytes, 2 * d_bytes + 2 * rest_bytes + 2 * dt_bytes + xt_bytes + 2 * wt_bytes + part_bytes); }
+    int64_t bytes() const { return std::max(narrow_bytes, range_bytes + 2 * d_bytes + 2 * rest_bytes + 2 * dt_bytes + xt_bytes + 2 * wt_bytes + part_bytes); }
 };
 template <typename T>
 BackwardPlan backward_plan(int64_t m, int64_t k, int64_t h) {
@@ -236,6 +236,7 @@ BackwardPlan backward_plan(int64_t m, int64_t k, int64_t h) {
         p.any_x = any_plan<T>(m, k, h, 1, true), p.any_w = any_plan<T>(h, k, m, 2, true);
         p.splits_x = p.any_x.splits, p.splits_w = p.any_w.splits;
     }
+    p.range_bytes = RANGED<T> && m > 0 ? RANGE_BYTES : 0;
     p.part_bytes = std::max<int64_t>(p.splits_x > 1 ? p.splits_x * m * k * 4 : 0, p.splits_w > 1 ? 2 * p.splits_w * h * k * 4 : 0);
     return p;
 }
@@ -311,7 +312,11 @@ hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const voi
         }
         return hipGetLastError();
     }
-    char* at = work;
+    float* const range = p.range_bytes ? (float*)work : nullptr;
+    if (range)
+        hipLaunchKernelGGL(k_gated_range<T>, dim3((unsigned)std::min<int64_t>(ceil_div(m * ceil_div(h, 4), RANGE_THREADS), RANGE_PIECES)), dim3(RANGE_THREADS),
+                           0, st, (const T*)dh, dhs, kg, ku, m, h, act, range);
+    char* at = work + p.range_bytes;
     auto take = [&](int64_t bytes) { char* r = at; at += bytes; return r; };
     T *dg = (T*)take(p.d_bytes), *du = (T*)take(p.d_bytes), *dg_rest = (T*)take(p.rest_bytes), *du_rest = (T*)take(p.rest_bytes), *dgt = (T*)take(p.dt_bytes), *dut = (T*)take(p.dt_bytes), *xt = (T*)take(p.xt_bytes),
       *wgt = (T*)take(p.wt_bytes), *wut = (T*)take(p.wt_bytes);
@@ -322,7 +327,7 @@ hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const voi
     };
     if (p.fast) {
         hipLaunchKernelGGL(k_gated_slopes_both<T>, dim3((unsigned)(p.mp / 64 * (p.hp / 64))), dim3(256), 0, st, (const T*)dh, dhs, kg, ku, m, h, act,
-                           dg, du, p.hp, dgt, dut, p.mp);
+                           range, dg, du, p.hp, dgt, dut, p.mp);
         PackArgs a{};
         if (dwg) a.job[a.count++] = {x, xs, m, k, xt, p.mp, p.mp / 64 * ceil_div(k, 64)};
         if (dx) {
@@ -336,12 +341,12 @@ hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const voi
         const int64_t packs = m * ceil_div(h, Pack<T>::N);
         by_parts([&](auto parts) {
             hipLaunchKernelGGL((k_gated_slopes<T, parts.value == 2>), dim3((unsigned)std::min<int64_t>(ceil_div(packs, 256), 8192)), dim3(256), 0, st,
-                               (const T*)dh, dhs, kg, ku, m, h, act, dg, du, dg_rest, du_rest);
+                               (const T*)dh, dhs, kg, ku, m, h, act, range, dg, du, dg_rest, du_rest);
         });
     }
     if (dx && m > 0) {
         GatedArgs g{};
-        g.m = m, g.n = k, g.out[0] = dx, g.os = dxs, g.splits = p.splits_x, g.part = part;
+        g.m = m, g.n = k, g.out[0] = dx, g.os = dxs, g.splits = p.splits_x, g.part = part, g.range = range;
         if (p.fast) {
             g.a[0] = {dg, p.hp, 1}, g.a[1] = {du, p.hp, 1}, g.b[0] = {wgt, p.hp, 1}, g.b[1] = {wut, p.hp, 1}, g.k = p.hp;
             launch_fast<T, GATED_SUM>(st, g, p.tile_x);
@@ -356,7 +361,7 @@ hipError_t gated_backward(hipStream_t st, const void* dh, int64_t dhs, const voi
     }
     if (dwg) {
         GatedArgs g{};
-        g.m = h, g.n = k, g.out[0] = dwg, g.out[1] = dwu, g.os = dws, g.splits = p.splits_w, g.part = part;
+        g.m = h, g.n = k, g.out[0] = dwg, g.out[1] = dwu, g.os = dws, g.splits = p.splits_w, g.part = part, g.range = range;
         if (p.fast) {
             g.a[0] = {dgt, p.mp, 1}, g.a[1] = {dut, p.mp, 1}, g.b[0] = g.b[1] = {xt, p.mp, 1}, g.k = p.mp;
             launch_fast<T, GATED_PAIR>(st, g, p.tile_w);

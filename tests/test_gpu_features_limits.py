@@ -102,3 +102,63 @@ def test_operands_read_in_place_are_not_copied(dtype):
 def test_gradients_of_few_elements_among_many_rows(dtype, act, rows, cols, hidden):
     """dg and du as two numbers there too: off by the square of half a step, not by half a step."""
     check_gated(dtype, act, rows, cols, hidden, slope=half(dtype) ** 2)
+
+
+# Every backward kernel: one launch, fragments into registers with one part and two, 64 x 64 tiles, both tiles for large operands, few columns
+RANGES = [(95, 621, 128), (60, 1, 21), (600, 10, 1), (1000, 520, 200), (3000, 400, 100), (2050, 621, 777), (8200, 1024, 1100), (50007, 15, 300), (1, 40, 7)]
+
+
+@pytest.mark.parametrize('rows,cols,hidden', RANGES)
+# scales of x, of the weights and of dh; which gradients are then numbers of float16's range
+@pytest.mark.parametrize('sx,sw,sd,what', [(1.0, 0.1, 1e-4, 'xw'), (300.0, 3e-4, 1e-6, 'w'), (3e-4, 300.0, 1e-6, 'x'), (3000.0, 0.002, 1e4, 'x'), (5e-4, 1.2e4, 1e4, 'w')])
+def test_float16_gradients_whose_slopes_leave_its_range(rows, cols, hidden, sx, sw, sd, what):
+    """dg and du around 1e-7, or beyond 65504, with gradients in between: off by their rounding relative to themselves, and by 2^-39 of the
+    largest of them, wherever that lies."""
+    from bayesian_optimization_amd import features
+    from test_gpu_features import gated_ref, rand as normal, within
+    U, H, f16 = 2.0 ** -24, 2.0 ** -11, torch.float16
+    x, dh = normal((rows, cols), f16, 1, sx), normal((rows, hidden), f16, 2, sd)
+    wg, wu = normal((hidden, cols), f16, 3, sw * cols ** -0.5), normal((hidden, cols), f16, 4, sw * cols ** -0.5)
+    h, kept = features.gated_unit(x, wg, wu, keep=True)
+    dx, dwg, dwu = features.gated_unit_backward(dh, x, wg, wu, kept)
+    g, u, a, da = gated_ref(x, wg, wu, 'silu')
+    eg, eu = ((cols + 1) * U * (x.double().abs() @ w.double().abs().t()) for w in (wg, wu))
+    ea = 1.13 * eg + 16 * U * (1 + g.abs()) * torch.minimum(g.abs(), torch.ones_like(g))
+    eda = 0.8 * eg + 16 * U * (1 + g.abs())
+    d = dh.double()
+    dg, du = d * u * da, d * a
+    low = 2.0 ** -39 * max(float(dg.abs().max()), float(du.abs().max()))
+    edg = d.abs() * (eu * da.abs() + u.abs() * eda + eu * eda) + (H * 1.01 + 4 * U) * dg.abs() + low
+    edu = d.abs() * ea + (H * 1.01 + 4 * U) * du.abs() + low
+    wga, wua, xa, tiny = wg.double().abs(), wu.double().abs(), x.double().abs(), 2.0 ** -25
+
+    def check(got, want, off, name):
+        inside = want.abs() + off < 65504
+        assert int(inside.sum()) > 0.9 * want.numel()
+        within(torch.where(inside, got.double(), want), want, off + H * want.abs() * 1.01 + tiny, name)
+    if 'x' in what:
+        want = dg @ wg.double() + du @ wu.double()
+        check(dx, want, edg @ wga + edu @ wua + (2 * hidden + 1) * U * ((dg.abs() + edg) @ wga + (du.abs() + edu) @ wua), 'dx')
+    if 'w' in what:
+        for got, v, e in ((dwg, dg, edg), (dwu, du, edu)):
+            check(got, v.t() @ x.double(), e.t() @ xa + (rows + 1) * U * ((v.abs() + e).t() @ xa), 'dw')
+
+
+@pytest.mark.parametrize('rows,cols,hidden', RANGES[:7])
+def test_float16_gradients_around_an_infinity(rows, cols, hidden):
+    """An infinite or NaN gradient that comes in enters what depends on it, and does not count as the largest of the others."""
+    from bayesian_optimization_amd import features
+    x, dh = rand((rows, cols), torch.float16, 1), rand((rows, hidden), torch.float16, 2, 1e-4)
+    wg, wu = rand((hidden, cols), torch.float16, 3, 0.1 * cols ** -0.5), rand((hidden, cols), torch.float16, 4, 0.1 * cols ** -0.5)
+    _, kept = features.gated_unit(x, wg, wu, keep=True)
+    want = features.gated_unit_backward(dh, x, wg, wu, kept)
+    for bad in (float('inf'), float('nan')):
+        d = dh.clone()
+        d[rows // 2, 0] = bad
+        dx, dwg, dwu = features.gated_unit_backward(d, x, wg, wu, kept)
+        assert not bool(torch.isfinite(dx[rows // 2]).any()) and not bool(torch.isfinite(dwu[0]).any())
+        others = torch.arange(rows, device='cuda') != rows // 2
+        assert bool(((dx[others].double() - want[0][others].double()).abs() <= 2.0 ** -10 * want[0][others].double().abs() + 2.0 ** -24).all())
+        assert torch.isfinite(dwg[1:]).all() and torch.isfinite(dwu[1:]).all()
+    zero = features.gated_unit_backward(torch.zeros_like(dh), x, wg, wu, kept)
+    assert all(float(v.abs().max()) == 0 for v in zero)
