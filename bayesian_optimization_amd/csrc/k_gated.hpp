@@ -45,9 +45,10 @@ __device__ __forceinline__ f32x4 mma<float>(const uint4& a, const uint4& b, f32x
 
 // act(g) and act'(g), with the hardware's exponential and reciprocal (one unit in the last place each).  silu through the logistic
 // function, whose exponential saturates to 0 or infinity with the right limit; gelu through q = Phi(-|g|) = 1/2 erfc(|g| / sqrt 2) = exp(-g^2 / 2)
-// t R(t), t = 1 / (1 + c |g|), which keeps the far negative tail that 1 + erf loses: for results of 16 bits the five terms of Abramowitz and Stegun
-// 7.1.26 (1.5e-7 in erf), for 32 bits ten (a least-squares fit, reweighted to even out its relative error, of erfcx(z) / t with c = 0.45 / sqrt 2:
-// 3.2e-8, half a rounding).  With all roundings a result is within 3 units of 2^-24 (1 + |g|) min(|g|, 1).  The activation of every output is as much
+// t R(t), t = 1 / (1 + c |g|), which keeps the far negative tail that 1 + erf loses: R has six terms for results of 16 bits (relative error
+// 4.9e-5, a tenth of half a step of float16, and 1.7e-7 in q) and ten for 32 bits (2e-8; scripts/gelu_tail_fit.py has the fit).  With all
+// roundings a result of 32 bits is within 3 units of 2^-24 (1 + |g|) min(|g|, 1); relative to itself it is off by the rounding of the
+// exponent as well, g^2 units of 2^-24, which is less than what the roundings of g, a sum, do to it.  The activation of every output is as much
 // vector work as a short contraction is matrix work (1 M x 256 -> 512 in 16 bits, with tiles: 1.27 -> 0.83 ms against expf and erfcf).
 template <typename T>
 __device__ __forceinline__ void activation(float g, int act, float& a, float& da) {
@@ -59,16 +60,13 @@ __device__ __forceinline__ void activation(float g, int act, float& a, float& da
     }
     constexpr bool WIDE = sizeof(T) == 4;
     const float e = __builtin_amdgcn_exp2f(-0.72134752044448170f * g * g);      // exp(-g^2 / 2)
-    const float t = __builtin_amdgcn_rcpf(1.0f + ((WIDE ? 0.45f : 0.3275911f) * 0.70710678118654752f) * fabsf(g));
-    float r;
-    if constexpr (WIDE) {
-        constexpr float R[10] = {0.253885329f, 0.253883153f, 0.228271648f, 0.175252140f, 0.119950369f, -0.0223577060f, 0.142400503f, -0.300581962f, 0.190687597f, -0.0413910411f};
-        r = R[9];
+    const float t = __builtin_amdgcn_rcpf(1.0f + ((WIDE ? 0.3354f : 0.6014f) * 0.70710678118654752f) * fabsf(g));
+    constexpr int TERMS = WIDE ? 10 : 6;
+    constexpr float R[2][10] = {{0.338197976f, 0.357509732f, 0.166214883f, 0.482815653f, -0.461610645f, 0.116872713f},
+                                {0.18920809f, 0.189721197f, 0.173563048f, 0.186824769f, 0.016709242f, 0.365303278f, -0.393553346f, 0.497524679f, -0.279960424f, 0.0546594486f}};
+    float r = R[WIDE][TERMS - 1];
 #pragma unroll
-        for (int i = 8; i >= 0; --i) r = fmaf(r, t, R[i]);
-    } else {
-        r = 0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)));
-    }
+    for (int i = TERMS - 2; i >= 0; --i) r = fmaf(r, t, R[WIDE][i]);
     const float q = 0.5f * e * t * r;
     const float cdf = g < 0.0f ? q : 1.0f - q;
     a = g * cdf;

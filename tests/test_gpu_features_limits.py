@@ -1,5 +1,6 @@
 """GPU: layer norm and gated unit at sizes where a launch of a thread or more an element does not take them, and other limits."""
-import numpy as np
+import math
+
 import pytest
 import torch
 
@@ -162,3 +163,27 @@ def test_float16_gradients_around_an_infinity(rows, cols, hidden):
         assert torch.isfinite(dwg[1:]).all() and torch.isfinite(dwu[1:]).all()
     zero = features.gated_unit_backward(torch.zeros_like(dh), x, wg, wu, kept)
     assert all(float(v.abs().max()) == 0 for v in zero)
+
+
+# a few rows, fragments into registers, 64 x 64 tiles, rows streamed through LDS, tiles for large operands
+@pytest.mark.parametrize('rows,cols,hidden', [(5, 2, 7), (100, 2, 9), (3000, 2, 600), (70001, 2, 40), (2100, 300, 1000)])
+@pytest.mark.parametrize('dtype,big,least', [(torch.float32, 1e18, -12.0), (torch.bfloat16, 1e18, -12.0), (torch.float16, 6e4, -7.0)])
+def test_gelu_keeps_its_lower_tail(dtype, big, least, rows, cols, hidden):
+    """Far below zero gelu is next to nothing, and times a large factor a number again: off relative to itself by half a step, by the fit
+    (6e-5 for 16 bits, 4e-7 for 32) and by the rounding of the exponent g^2 / 2, three roundings of 2^-24 of it, with a dozen others."""
+    from bayesian_optimization_amd import features
+    U = 2.0 ** -24
+    x = torch.zeros((rows, cols), dtype=dtype, device='cuda')
+    x[:, 0] = torch.linspace(least, -0.5, rows, device='cuda').to(dtype)      # g and u are products of two numbers, without a sum
+    x[:, 1] = big
+    w = torch.zeros((2, hidden, cols), dtype=dtype, device='cuda')
+    w[0, :, 0], w[1, :, 1] = 1.0, big
+    h, kept = features.gated_unit(x, w[0], w[1], 'gelu', keep=True)
+    g, u = x[:, :1].double(), x[:, 1:2].double() * w[1, 0, 1].double()
+    assert torch.equal(kept[0, :, 0], x[:, 0].float()) and bool(((kept[1, :, :1].double() - u).abs() <= U * u).all())
+    want = 0.5 * g * torch.erfc(-g / math.sqrt(2)) * u
+    rel = half(dtype) * 1.01 + (4e-7 if dtype == torch.float32 else 6e-5) + (2 * g * g + 16) * U
+    assert bool((want.abs() > 1e-3).all())
+    inside = want.abs() * 1.01 < torch.finfo(dtype).max
+    off = (h.double() - want).abs() / want.abs()
+    assert bool(((off <= rel) | ~inside).all()), (off - rel).max()
