@@ -4,6 +4,8 @@ A call on a few rows takes less time on the GPU than its checks take here, so th
 device numbers, and results are allocated one by one rather than sliced out of each other."""
 from __future__ import annotations
 
+import warnings
+
 import torch
 
 from . import _lib as L
@@ -20,12 +22,21 @@ def stream_of(device: int):
     return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
+def off_tape(name, t):
+    """These calls are not part of torch's graph of gradients: says so where one would be expected."""
+    if t.requires_grad and torch.is_grad_enabled():
+        warnings.warn('%s requires a gradient, but this call is not recorded: backward() will not reach %s through it (call the operator\'s own '
+                      'backward pass, under torch.no_grad())' % (name, name), stacklevel=4)
+
+
 def tensor(name, t, device=None):
     """The number of the GPU that t is on; it must be `device` if one is given."""
     if not isinstance(t, Tensor):
         raise TypeError('%s must be a torch tensor, got %s' % (name, type(t).__name__))
     if not t.is_cuda:
         raise ValueError('%s is on %s, expected a GPU (there is no CPU path)' % (name, t.device))
+    if t.requires_grad:
+        off_tape(name, t)
     at = t.get_device()
     if device is not None and at != device:
         raise ValueError('%s is on %s, expected cuda:%d' % (name, t.device, device))

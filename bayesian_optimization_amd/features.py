@@ -2,7 +2,8 @@
 measured spectra have 621 channels, BayesOpt/BayesOpt_v4.ipynb:681-697; gradients are supported up to 16 input columns).
 
 ``layer_norm`` and ``gated_unit`` and their backward passes run on torch tensors on a GPU, on the current stream, without
-waiting for it.  ``FeatureMap`` puts them together: normalise a row, one gated unit, a few features.
+waiting for it.  They are not recorded by torch's autograd: a tensor that requires a gradient is taken with a warning, unless gradients
+are off, and the backward passes are called by hand.  ``FeatureMap`` puts them together: normalise a row, one gated unit, a few features.
 ``hyperopt.lml_features`` differentiates the likelihood through it."""
 from __future__ import annotations
 
@@ -10,7 +11,7 @@ import numpy as np
 import torch
 
 from . import _lib as L
-from ._device import TYPES, check_status, pointer, rows_of, scratch, stream_of, tensor, vector_of, workspace
+from ._device import TYPES, check_status, off_tape, pointer, rows_of, scratch, stream_of, tensor, vector_of, workspace
 
 ACTIVATIONS = {'silu': L.ACT_SILU, 'gelu': L.ACT_GELU}
 _like, _f32 = torch.empty_like, torch.float32
@@ -128,7 +129,8 @@ def gated_unit_backward(dh, x, w_gate, w_up, kept, act='silu', need_dx=True, nee
 
 class FeatureMap:
     """z = gated_unit(layer_norm(x)) @ w_out^T: the inputs of a GP as a learned function of raw ones.  ``params`` holds the five
-    tensors (norm_weight, norm_bias, w_gate, w_up, w_out); an optimiser of the caller's choice updates them in place."""
+    tensors (norm_weight, norm_bias, w_gate, w_up, w_out), which may be parameters; an optimiser of the caller's choice updates them in
+    place, with the gradients that backward() returns."""
 
     def __init__(self, cols, hidden, features, dtype=torch.float32, device='cuda', act='silu', eps=1e-5, seed=0):
         if min(cols, hidden, features) < 1:
@@ -145,12 +147,15 @@ class FeatureMap:
     def forward(self, x, keep=False):
         """z (rows, features) float32; keep: also what backward() needs."""
         p = self.params
-        y, mean, rstd = layer_norm(x, p['norm_weight'], p['norm_bias'], self.eps)
-        h = gated_unit(y, p['w_gate'], p['w_up'], self.act, keep=keep)
-        h, kept = h if keep else (h, None)
-        z = h.float() @ p['w_out'].float().t()
+        off_tape('x', x)
+        with torch.no_grad():
+            y, mean, rstd = layer_norm(x, p['norm_weight'], p['norm_bias'], self.eps)
+            h = gated_unit(y, p['w_gate'], p['w_up'], self.act, keep=keep)
+            h, kept = h if keep else (h, None)
+            z = h.float() @ p['w_out'].float().t()
         return (z, (x, mean, rstd, y, kept, h)) if keep else z
 
+    @torch.no_grad()
     def backward(self, dz, saved):
         """Gradients of the parameters, by name, and of x, under 'x'; dz (rows, features) float32."""
         p = self.params
