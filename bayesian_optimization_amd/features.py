@@ -127,6 +127,14 @@ def gated_unit_backward(dh, x, w_gate, w_up, kept, act='silu', need_dx=True, nee
     return dx, dwg, dwu
 
 
+def _exponent(dh):
+    """The power of two, as a tensor, that brings the largest finite element between 2^-11 and 2^14, where float16 holds it and most of what is
+    smaller; 0 if it lies there."""
+    most = torch.where(torch.isfinite(dh), dh, 0.0).abs().amax() if dh.numel() else dh.new_zeros(())
+    at = torch.frexp(most).exponent
+    return torch.where(most > 0, at.clamp(-10, 14) - at, 0)
+
+
 class FeatureMap:
     """z = gated_unit(layer_norm(x)) @ w_out^T: the inputs of a GP as a learned function of raw ones.  ``params`` holds the five
     tensors (norm_weight, norm_bias, w_gate, w_up, w_out), which may be parameters; an optimiser of the caller's choice updates them in
@@ -161,10 +169,18 @@ class FeatureMap:
         p = self.params
         x, mean, rstd, y, kept, h = saved
         dz = dz.float()
-        dh = (dz @ p['w_out'].float()).to(h.dtype)
-        dy, dwg, dwu = gated_unit_backward(dh, y, p['w_gate'], p['w_up'], kept, self.act)
+        dh = dz @ p['w_out'].float()
+        ranged = h.dtype == torch.float16      # a likelihood's gradient knows no bounds: the passes through float16 are taken on a multiple of it
+        if ranged:
+            e = _exponent(dh)
+            dh = torch.ldexp(dh, e)
+        dy, dwg, dwu = gated_unit_backward(dh.to(h.dtype), y, p['w_gate'], p['w_up'], kept, self.act)
         dx, dw, db = layer_norm_backward(dy, x, p['norm_weight'], mean, rstd)
-        return {'norm_weight': dw, 'norm_bias': db, 'w_gate': dwg, 'w_up': dwu, 'w_out': (dz.t() @ h.float()).to(h.dtype), 'x': dx}
+        grads = {'norm_weight': dw, 'norm_bias': db, 'w_gate': dwg, 'w_up': dwu, 'x': dx}
+        if ranged:
+            grads = {k: torch.ldexp(v.float(), -e).to(v.dtype) for k, v in grads.items()}
+        grads['w_out'] = (dz.t() @ h.float()).to(h.dtype)
+        return grads
 
     def numpy(self, x):
         """Features of host rows as the float64 array GP.fit and GP.set_candidates take."""
