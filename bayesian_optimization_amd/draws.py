@@ -17,24 +17,27 @@ _f64 = torch.float64
 _NAMES, _NEUTRAL = ('temperature', 'top_k', 'top_p', 'min_p'), (1.0, 0, 1.0, 0.0)
 
 
-def _numbers(settings):
-    """The four settings as plain numbers, checked; the neutral one for a tensor that is not on the host, which cannot be looked at
-    without waiting for it."""
-    temperature, top_k, top_p, min_p = (
-        v if not isinstance(v, Tensor) else v.item() if v.dim() == 0 and not v.is_cuda else neutral for v, neutral in zip(settings, _NEUTRAL))
+def _check(temperature, top_k, top_p, min_p):
     if not (temperature >= 0.0 and math.isfinite(temperature)):
         raise ValueError('temperature must be finite and >= 0; got %r' % (temperature,))
     if not (0 <= top_k < math.inf and top_k == int(top_k)):
         raise ValueError('top_k must be a whole number >= 0; got %r' % (top_k,))
     if not (0.0 <= top_p <= 1.0 and 0.0 <= min_p <= 1.0):
         raise ValueError('top_p and min_p must lie in [0, 1]; got %r and %r' % (top_p, min_p))
-    return temperature, top_k, top_p, min_p
 
 
-def _per_row(settings, numbers, rows, device, at):
+def _numbers(settings):
+    """The four settings as plain numbers, checked; the neutral one for a tensor that is not on the host, which cannot be looked at
+    without waiting for it."""
+    numbers = tuple(v if not isinstance(v, Tensor) else v.item() if v.dim() == 0 and not v.is_cuda else neutral for v, neutral in zip(settings, _NEUTRAL))
+    _check(*numbers)
+    return numbers
+
+
+def _per_row(settings, rows, device, at):
     """(rows, 4) float64 on the GPU from four settings, each a number or a tensor there of one number, or one per row."""
     columns = []
-    for name, v, number in zip(_NAMES, settings, numbers):
+    for name, v, number in zip(_NAMES, settings, _numbers(settings)):
         if isinstance(v, Tensor) and (v.is_cuda or v.dim() > 0):
             tensor(name, v, at)
             if v.dim() > 0 and tuple(v.shape) != (rows,):
@@ -61,11 +64,11 @@ def sample(scores, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if u.dim() != 2 or u.shape[0] != rows or u.dtype != _f64:
         raise ValueError('u must be (%d, draws) float64; got %s %s' % (rows, tuple(u.shape), u.dtype))
     device, params = scores.device, None
-    settings = (temperature, top_k, top_p, min_p)
-    temperature, top_k, top_p, min_p = numbers = _numbers(settings)
-    if any(isinstance(v, Tensor) for v in settings):
-        params = _per_row(settings, numbers, rows, device, at)
+    if isinstance(temperature, Tensor) or isinstance(top_k, Tensor) or isinstance(top_p, Tensor) or isinstance(min_p, Tensor):
+        params = _per_row((temperature, top_k, top_p, min_p), rows, device, at)
         temperature, top_k, top_p, min_p = _NEUTRAL
+    else:
+        _check(temperature, top_k, top_p, min_p)
     if not u.is_contiguous():
         u = u.contiguous()
     draws, code = u.shape[1], _TYPES[scores.dtype]
