@@ -138,6 +138,19 @@ template <int N>
 struct Parts {
     uint4 v[N];
 };
+// The sums of a product's parts; what the roundings left is left out where it met an infinity (zero times it is no number, and the rounded
+// part alone says what becomes of it).
+template <int N>
+struct Sums {
+    f32x4 v[N] = {};
+    __device__ __forceinline__ f32x4 all() const {
+        if constexpr (N == 1) return v[0];
+        f32x4 r = v[0];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] += fabsf(v[N - 1][i]) < INFINITY ? v[N - 1][i] : 0.0f;
+        return r;
+    }
+};
 // What the rounding of d to hi left; nothing if hi is beyond the type's range.
 template <typename T>
 __device__ __forceinline__ T rounding_rest(float d, T hi) {
@@ -204,13 +217,7 @@ __global__ __launch_bounds__(256) void k_gated_tile(GatedArgs g) {
     const int64_t kb = min(split * per, g.k), ke = min(kb + per, g.k);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wr = (wave >> 1) * 32, wc = (wave & 1) * 32;
-    f32x4 acc[NB][2][2];
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) acc[b][i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    Sums<NA> acc[NB][2][2];
     const int64_t steps1 = (ke - kb + KS - 1) / KS, steps = MODE == GATED_SUM ? 2 * steps1 : steps1;
     TileLoad<T, AKC> ta[NA];
     TileLoad<T, BKC> tb[NB];
@@ -250,7 +257,7 @@ __global__ __launch_bounds__(256) void k_gated_tile(GatedArgs g) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
 #pragma unroll
-                        for (int a = 0; a < NA; ++a) acc[b][i][j] = mma<T>(fb[b][j], fa[a][i], acc[b][i][j]);
+                        for (int a = 0; a < NA; ++a) acc[b][i][j].v[a] = mma<T>(fb[b][j], fa[a][i], acc[b][i][j].v[a]);
         }
         __syncthreads();
     }
@@ -262,18 +269,19 @@ __global__ __launch_bounds__(256) void k_gated_tile(GatedArgs g) {
         for (int j = 0; j < 2; ++j) {
             const int64_t row = row0 + wr + i * 16 + (lane & 15), col = col0 + wc + j * 16 + (lane >> 4) * 4;
             if (row >= g.m) continue;
+            const f32x4 first = acc[0][i][j].all(), second = acc[NB - 1][i][j].all();
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 if (col + r >= g.n) continue;
                 if constexpr (MODE == GATED_FWD) {
-                    const float gv = acc[0][i][j][r], uv = acc[NB - 1][i][j][r];
+                    const float gv = first[r], uv = second[r];
                     ((T*)g.out[0])[row * g.os + col + r] = from_float<T>(activate<T>(gv, g.act) * uv);
                     if (g.keep_g) {
                         g.keep_g[row * g.n + col + r] = gv;
                         g.keep_u[row * g.n + col + r] = uv;
                     }
                 } else {
-                    const float v = acc[0][i][j][r];
+                    const float v = first[r];
                     if (g.splits > 1) g.part[(((int64_t)z * g.splits + split) * g.m + row) * g.n + col + r] = v;
                     else ((T*)g.out[z])[row * g.os + col + r] = from_float<T>(v * down);
                 }
@@ -334,23 +342,21 @@ __device__ __forceinline__ Slopes<T> slope_fragment(const SlopeOperand& o, int w
 // A fragment of the second operand against one of the first, in parts of the same type or in 32 bits (instructions of 32 bits then, which take
 // element j of every lane: a sixteenth of the speed, over a contraction of a few hundred).
 template <typename T, int NA>
-__device__ __forceinline__ f32x4 product(const uint4& b, const Parts<NA>& a, f32x4 c) {
+__device__ __forceinline__ void product(const uint4& b, const Parts<NA>& a, Sums<NA>& c) {
 #pragma unroll
-    for (int p = 0; p < NA; ++p) c = mma<T>(b, a.v[p], c);
-    return c;
+    for (int p = 0; p < NA; ++p) c.v[p] = mma<T>(b, a.v[p], c.v[p]);
 }
 template <typename T>
-__device__ __forceinline__ f32x4 product(const uint4& b, const Slopes<T>& a, f32x4 c) {
+__device__ __forceinline__ void product(const uint4& b, const Slopes<T>& a, Sums<1>& c) {
     const Pack<T> v = __builtin_bit_cast(Pack<T>, b);
 #pragma unroll
-    for (int j = 0; j < Pack<T>::N; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(to_float(v.v[j]), a.v[j], c, 0, 0, 0);
-    return c;
+    for (int j = 0; j < Pack<T>::N; ++j) c.v[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(to_float(v.v[j]), a.v[j], c.v[0], 0, 0, 0);
 }
 
 // The body: NB products side by side (one first operand, in fragments of type A, NB second ones), slabs of contraction [kb, ke) dealt to the waves; fa(i, k, whole)
 // and fb(b, i, k, whole) give fragments i < FR.
-template <typename T, typename A, int NB, int FR, typename FA, typename FB>
-__device__ __forceinline__ void small_sums(f32x4 (&acc)[NB][FR][FR], int64_t kb, int64_t ke, FA&& fa, FB&& fb) {
+template <typename T, typename A, int NA, int NB, int FR, typename FA, typename FB>
+__device__ __forceinline__ void small_sums(Sums<NA> (&acc)[NB][FR][FR], int64_t kb, int64_t ke, FA&& fa, FB&& fb) {
     constexpr int SLAB = 64 / sizeof(T), V = 16 / sizeof(T);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t slabs = (ke - kb) / SLAB;
@@ -369,15 +375,15 @@ __device__ __forceinline__ void small_sums(f32x4 (&acc)[NB][FR][FR], int64_t kb,
 #pragma unroll
             for (int i = 0; i < FR; ++i)
 #pragma unroll
-                for (int j = 0; j < FR; ++j) acc[q][i][j] = product<T>(b[q][j], a[i], acc[q][i][j]);
+                for (int j = 0; j < FR; ++j) product<T>(b[q][j], a[i], acc[q][i][j]);
     };
 #pragma unroll 4
     for (int64_t s = wave; s < slabs; s += SMALL_WAVES) slab(kb + s * SLAB, std::true_type{});
     if (kb + slabs * SLAB < ke && slabs % SMALL_WAVES == wave) slab(kb + slabs * SLAB, std::false_type{});      // the broken last one
 }
 // The waves' sums, in wave order: fragment `wave` of the FR * FR in v of the first waves.
-template <int NB, int FR>
-__device__ __forceinline__ void small_join(const f32x4 (&acc)[NB][FR][FR], f32x4 (&v)[NB], f32x4 (*sums)[NB * FR * FR][64]) {
+template <int NA, int NB, int FR>
+__device__ __forceinline__ void small_join(const Sums<NA> (&acc)[NB][FR][FR], f32x4 (&v)[NB], f32x4 (*sums)[NB * FR * FR][64]) {
     constexpr int F = FR * FR;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -385,7 +391,7 @@ __device__ __forceinline__ void small_join(const f32x4 (&acc)[NB][FR][FR], f32x4
 #pragma unroll
         for (int i = 0; i < FR; ++i)
 #pragma unroll
-            for (int j = 0; j < FR; ++j) sums[wave][b * F + i * FR + j][lane] = acc[b][i][j];
+            for (int j = 0; j < FR; ++j) sums[wave][b * F + i * FR + j][lane] = acc[b][i][j].all();
     __syncthreads();
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -405,7 +411,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small(GatedArgs g) {
     const int64_t per = ((g.k + g.splits - 1) / g.splits + SLAB - 1) / SLAB * SLAB;
     const int64_t kb = min(split * per, g.k), ke = min(kb + per, g.k);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    f32x4 acc[NB][FR][FR] = {};
+    Sums<NA> acc[NB][FR][FR];
     int64_t ra[FR], rb[FR];                      // rows behind the last repeat it: their outputs are not stored
 #pragma unroll
     for (int i = 0; i < FR; ++i) ra[i] = min(row0 + i * 16 + (lane & 15), g.m - 1), rb[i] = min(col0 + i * 16 + (lane & 15), g.n - 1);
@@ -413,7 +419,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small(GatedArgs g) {
     for (int part = 0; part < (MODE == GATED_SUM ? 2 : 1); ++part) {
         const Operand oa = MODE == GATED_PAIR && z ? g.a[1] : g.a[part], ob = g.b[part], ob2 = g.b[1];
         const Operand rest = MODE == GATED_PAIR && z ? g.rest[1] : g.rest[part];
-        small_sums<T, Parts<NA>, NB, FR>(acc, kb, ke, [&](int i, int64_t k, auto whole) {
+        small_sums<T, Parts<NA>>(acc, kb, ke, [&](int i, int64_t k, auto whole) {
                               Parts<NA> r;
                               r.v[0] = small_fragment<T, AKC, whole.value>(oa, ra[i], k, ke);
                               if constexpr (NA == 2) r.v[1] = small_fragment<T, AKC, whole.value>(rest, ra[i], k, ke);
@@ -422,7 +428,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small(GatedArgs g) {
                           [&](int b, int i, int64_t k, auto whole) { return small_fragment<T, BKC, whole.value>(b ? ob2 : ob, rb[i], k, ke); });
     }
     f32x4 v[NB];
-    small_join<NB, FR>(acc, v, sums);
+    small_join(acc, v, sums);
     if (wave >= FR * FR) return;
     float down = 1.0f;
     if constexpr (MODE != GATED_FWD) down = range_down<T>(g.range);
@@ -453,7 +459,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small_back(SlopeOper
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t nt = (k + SB - 1) / SB, tiles_x = dx ? (m + SB - 1) / SB * nt : 0, tiles_w = (h + SB - 1) / SB * nt;
     int64_t id = blockIdx.x;
-    f32x4 acc[1][2][2] = {};
+    Sums<1> acc[1][2][2];
     f32x4 v[1];
     const int64_t col0 = id < tiles_x ? id % nt * SB : (id - tiles_x) % nt * SB;
     int64_t rb[2];
@@ -468,7 +474,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small_back(SlopeOper
         for (int i = 0; i < 2; ++i) ra[i] = min(row0 + i * 16 + (lane & 15), m - 1);
 #pragma unroll
         for (int which = 0; which < 2; ++which)
-            small_sums<T, Slopes<T>, 1, 2>(acc, 0, h, [&](int i, int64_t q, auto whole) { return slope_fragment<T, true, whole.value>(s, which, ra[i], q, h); },
+            small_sums<T, Slopes<T>>(acc, 0, h, [&](int i, int64_t q, auto whole) { return slope_fragment<T, true, whole.value>(s, which, ra[i], q, h); },
                              [&](int, int i, int64_t q, auto whole) { return small_fragment<T, false, whole.value>(which ? wu : wg, rb[i], q, h); });
     } else {                                   // dw = d^T x, contraction over the rows
         id -= tiles_x;
@@ -478,10 +484,10 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void k_gated_small_back(SlopeOper
         int64_t ra[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) ra[i] = min(row0 + i * 16 + (lane & 15), h - 1);
-        small_sums<T, Slopes<T>, 1, 2>(acc, 0, m, [&](int i, int64_t q, auto whole) { return slope_fragment<T, false, whole.value>(s, which, ra[i], q, m); },
+        small_sums<T, Slopes<T>>(acc, 0, m, [&](int i, int64_t q, auto whole) { return slope_fragment<T, false, whole.value>(s, which, ra[i], q, m); },
                          [&](int, int i, int64_t q, auto whole) { return small_fragment<T, false, whole.value>(x, rb[i], q, m); });
     }
-    small_join<1, 2>(acc, v, sums);
+    small_join(acc, v, sums);
     if (wave >= 4) return;
     const int64_t row = row0 + (wave >> 1) * 16 + (lane & 15), col = col0 + (wave & 1) * 16 + (lane >> 4) * 4;
     if (row >= rows) return;

@@ -212,7 +212,7 @@ BackwardPlan backward_plan(int64_t m, int64_t k, int64_t h) {
     // In two parts where a gradient has few elements (with the forward pass 20000 x 5 -> 77 bf16 57 us without, 64 with; 1000 x 520 ->
     // 400, where it would take away less than the gradients' own roundings, 44 and 61).  The any-shape kernels do that, whatever the size: the
     // whole-step kernels with a second part are slower still (backward 8192 x 1 -> 256 28 us, 88 with them, 35 with one part; 1 M x 60 -> 64
-    // 924, 1215 and 564).
+    // 992, 1215 and 564).
     const bool few_elements = SLOPE_PARTS<T> == 2 && std::min(m, h) * k < 4096;
     p.fast = !p.narrow && !few_elements && m >= 128 && (8 * m * h * k >= enough || (m >= 4096 && std::max(h, k) >= 128 && m * std::max(h, k) >= (int64_t)1 << 21)) && m * B < (1 << 23) && h * B < (1 << 23);
     if (p.fast) {

@@ -187,3 +187,21 @@ def test_gelu_keeps_its_lower_tail(dtype, big, least, rows, cols, hidden):
     inside = want.abs() * 1.01 < torch.finfo(dtype).max
     off = (h.double() - want).abs() / want.abs()
     assert bool(((off <= rel) | ~inside).all()), (off - rel).max()
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('rows,cols,hidden', [(30, 11, 9), (600, 10, 1), (4096, 512, 1), (70000, 7, 20), (1000, 3, 600), (130, 31, 3000), (1000, 520, 200), (2050, 621, 777)])
+def test_an_infinite_weight_enters_its_column_alone(dtype, rows, cols, hidden):
+    """Whatever dg and du enter the products as: the gradient of that column is infinite with the sign of its term, the others are as without."""
+    from bayesian_optimization_amd import features
+    x = rand((rows, cols), dtype, 1)
+    wg, wu = rand((hidden, cols), dtype, 3, 0.1 * cols ** -0.5), rand((hidden, cols), dtype, 4, 0.1 * cols ** -0.5)
+    _, kept = features.gated_unit(x, wg, wu, keep=True)
+    dh = torch.ones((rows, hidden), dtype=dtype, device='cuda')
+    want, _, _ = features.gated_unit_backward(dh, x, wg, wu, kept)
+    wu[hidden - 1, cols - 1] = float('inf')
+    dx, _, _ = features.gated_unit_backward(dh, x, wg, wu, kept)
+    assert torch.equal(dx[:, :-1], want[:, :-1])
+    du = torch.nn.functional.silu(kept[0, :, -1].double())
+    sure = du.abs() > 1e-4             # (a factor that float16 holds)
+    assert bool((dx[:, -1].double() == torch.where(du > 0, float('inf'), -float('inf')))[sure].all()) and int(sure.sum()) > 0.9 * rows
