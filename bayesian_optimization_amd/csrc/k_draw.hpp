@@ -14,9 +14,10 @@
 // Bound by memory: a pass over the row per step, two to five of them, and by the exponential of the scores of a top-p step.
 // Short rows: one workgroup a row does everything (k_draw_row).  Long rows: the same steps with many workgroups a row, one
 // launch a step, the state of a row in the workspace; the last workgroup to arrive at a step takes its decision.
-// Measured: 256 rows of 65537 scores of 16 bits with top_k and top_p 37 us (a pass over them 7 at the rate of a copy; what is left is
-// one workgroup's chain of small steps), 16.8 M float64 scores with min_p and top_p 97 us where 1024 of them or fewer
-// pass min_p, else 111 (two passes of 30, launches with nothing to do 2 to 4 each, the cut and the picks 20 or 35 in one workgroup).
+// Measured: 256 rows of 65537 scores of 16 bits with top_k and top_p 35 us (a pass over them 7 at the rate of a copy; what is left is
+// one workgroup's chain of small steps, whose kernel spills 17 to 28 of its 128 registers), 16.8 M float64 scores with min_p and top_p 88
+// to 94 us where 1024 of them or fewer pass min_p, else 108, 97 to 123 with scores that no cache holds (two passes of 30, launches with
+// nothing to do 2 to 4 each, the cut and the picks 20 or 35 in one workgroup).
 #pragma once
 
 #include <hip/hip_runtime.h>

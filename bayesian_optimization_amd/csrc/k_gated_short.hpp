@@ -157,7 +157,8 @@ __global__ __launch_bounds__(256, 2) void k_gated_short_dx(ShortBack<T> g) {
 }
 
 // dwg = dg^T x, dwu = du^T x: a workgroup has 64 hidden units (the last ones end with the row and may repeat some) and a piece of the rows, whose
-// slabs of 4 E rows its waves take in turn.  A lane has four neighbouring hidden units of a row, one for each of four fragments.
+// slabs of 4 E rows its waves take in turn.  A lane has four neighbouring hidden units of a row, one for each of four fragments.  (With more than
+// 48 columns 28 registers are spilled.)
 template <typename T, int CF>
 __global__ __launch_bounds__(256, 2) void k_gated_short_dw(ShortBack<T> g) {
     constexpr int E = CF <= 2 ? 4 : 2;           // what two slabs and the sums leave of the registers

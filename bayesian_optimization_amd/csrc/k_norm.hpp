@@ -6,6 +6,7 @@
 // in 32 bits), TPR threads share a row in 16-byte packs, and a workgroup walks over rows with weight and bias (and, going
 // back, the column sums of dw and db) in registers too.  The column sums of every row group go to the workspace and are
 // added by a second launch in a fixed order: no atomics, the same bits every time.
+// (Backward at 16384 elements a row spills 7 registers in float32 and float16.)
 // Measured: 1 M x 621 bf16 forward 516 us, 5.0 TB/s; 16384 x 4096 bf16 forward + backward 152 us, 4.4 TB/s with x read in both.
 #pragma once
 

@@ -394,7 +394,8 @@ int gpbo_gated(int32_t device, void* stream, int32_t dtype, int32_t act, const v
                int64_t cols, const void* wg, const void* wu, int64_t w_stride, int64_t hidden, void* h, int64_t h_stride,
                float* keep_g, float* keep_u, void* workspace, int64_t workspace_bytes);
 /* Its backward pass from dh (rows, hidden) and the kept products: dx (rows, cols) and dwg, dwu (hidden, cols; one row
- * stride).  dx may be NULL, and so may dwg and dwu together. */
+ * stride).  dx may be NULL, and so may dwg and dwu together.  Sums in 32 bits; in 16 bits dh u act'(g) and dh act(g) are operands of type
+ * dtype in large problems (in float16 scaled into its range), rounded once, or, for gradients of under 4096 elements, in two parts. */
 int64_t gpbo_gated_backward_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_t hidden);
 int gpbo_gated_backward(int32_t device, void* stream, int32_t dtype, int32_t act, const void* dh, int64_t dh_stride, const void* x,
                         int64_t x_stride, int64_t rows, int64_t cols, const void* wg, const void* wu, int64_t w_stride,
