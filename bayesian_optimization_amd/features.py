@@ -156,7 +156,8 @@ class FeatureMap:
     def forward(self, x, keep=False):
         """z (rows, features) float32; keep: also what backward() needs."""
         p = self.params
-        off_tape('x', x)
+        if getattr(x, 'requires_grad', False):
+            off_tape('x', x)
         with torch.no_grad():
             y, mean, rstd = layer_norm(x, p['norm_weight'], p['norm_bias'], self.eps)
             h = gated_unit(y, p['w_gate'], p['w_up'], self.act, keep=keep)

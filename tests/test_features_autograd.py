@@ -71,6 +71,8 @@ def test_a_feature_map_of_parameters():
     assert hyperopt.lml_features(fmap, x, y, theta, 0.3)[0] < nll
     with pytest.warns(UserWarning, match='x requires a gradient'):
         fmap.forward(x.clone().requires_grad_())
+    with pytest.raises(TypeError, match='x must be a torch tensor'):
+        fmap.forward(raw)
 
 
 @pytest.mark.gpu
